@@ -455,7 +455,7 @@ def _exact_verify(case, s):
                 r = (torch.arange(V, device=DEV) == int((lg == lg.max()).nonzero()[0])).double()
             else:
                 r = torch.exp(lg / T - torch.logsumexp(lg / T, 0))
-            p = r
+            p, mass = r, 1.0
             if s["draft"] is not None and T > 0:
                 d = s["draft"][b, node].double() / T
                 q = torch.exp(d - torch.logsumexp(d, 0))
@@ -470,7 +470,8 @@ def _exact_verify(case, s):
                     break
                 left = (r - q).clamp(min=0)
                 if T > 0:
-                    if float(left.sum()) <= TINY:
+                    mass *= float(left.sum())
+                    if mass <= TINY:
                         r = p
                         break
                     r = left / left.sum()
