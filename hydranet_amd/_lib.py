@@ -49,6 +49,14 @@ SIGNATURES: dict[str, list] = {
     "hn_hbm_read_probe": [P, L, L, P, P],
     "hn_attn_decode_rope": [P, L, P, P, P, P, P, L, L, L, L, L, L, P, F, P, L, P],
     "hn_rope_append": [P, L, P, L, P, L, P, P, P, L, L, L, L, L, P, P, P, L, P],
+    "hn_tree_plan": [P, L, L, L, P, P, P, P],
+    "hn_tree_append": [P, L, P, P, L, P, L, P, L, L, L, L, L, P, P, P, L, P],
+    "hn_tree_attention_workspace_bytes": [L, L, L, L, L],
+    "hn_tree_attention": [P, P, P, L, P, P, L, L, L, L, L, L, L, F, P, L, P, L, P],
+    "hn_verify_tree_workspace_bytes": [L, L, L, I],
+    "hn_verify_tree": [P, L, L, P, L, L, I, P, P, L, P, P, F, L, L, L, P, P, P, P, L, P],
+    "hn_kv_keep": [P, P, L, L, L, L, L, P, P, L, P, L, P, P],
+    "hn_kv_fork": [P, P, L, L, L, L, L, P, P, L, L, P],
     "hn_grouped_expert_mlp_int4": [P, P, P, P, P, L, L, L, L, L, L, P, P, P, L, P],
     "hn_set_decode_path": [I],
     "hn_gemm_workspace_bytes": [],
@@ -75,7 +83,9 @@ ROUTE_MAX_LOGITS = 8192   # T * E
 ROUTE_MAX_ASSIGN = 1024   # T * k
 
 RESTYPES = {"hn_skinny_workspace_bytes": ctypes.c_long,
-            "hn_attn_prefill_workspace_bytes": ctypes.c_long, "hn_gemm_workspace_bytes": ctypes.c_long,
+            "hn_attn_prefill_workspace_bytes": ctypes.c_long,
+            "hn_tree_attention_workspace_bytes": ctypes.c_long,
+            "hn_verify_tree_workspace_bytes": ctypes.c_long, "hn_gemm_workspace_bytes": ctypes.c_long,
             "hn_moe_decode_layer_partials": ctypes.c_long}
 
 # Tokens per weight matrix up to which the decode (skinny / streaming) kernels run
@@ -109,6 +119,15 @@ def call(name: str, *args) -> None:
     if rc != 0:
         msg = lib().hn_last_error_string().decode(errors="replace")
         raise RuntimeError(f"{name} failed (rc={rc}): {msg}")
+
+
+def call_on(device: torch.device, name: str, *args) -> None:
+    """call() with `device` as the current device, where its stream launches."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        call(name, *args)
+    else:
+        with torch.cuda.device(device):
+            call(name, *args)
 
 
 _DECODE_PATH = threading.local()

@@ -19,6 +19,7 @@ ARCH = os.environ.get("HN_OFFLOAD_ARCH", "gfx950")
 
 SOURCES = ["hn_abi.cpp", "hn_quant.hip", "hn_gemv.hip", "hn_route.hip", "hn_stream.hip",
            "hn_mid.hip", "hn_gemm.hip", "hn_decoder.hip", "hn_attn.hip",
+           "hn_tree.hip", "hn_verify.hip", "hn_cache.hip",
            "hn_noalloc.hip", "hn_probe.hip"]
 
 

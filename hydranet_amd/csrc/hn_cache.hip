@@ -1,0 +1,135 @@
+// The KV cache's positions compacted after drafted tokens were verified, and
+// copied to further sequences, in every layer by one launch (up to 64 layers,
+// whose addresses travel in the kernel's arguments).  Keys are cached
+// [B][nkv][hd][max_len], values [B][nkv][max_len][hd], fp16.
+#include "hn_common.h"
+
+namespace {
+
+constexpr int kLayers = 64;  // layers per launch
+constexpr int kPairs = 128;  // copies per launch
+
+struct Layers {
+  h16* kt[kLayers];
+  h16* v[kLayers];
+};
+
+// Grid (B * nkv, layers), a thread per element of a position.  Positions go in
+// ascending order, kStep at a time: the sources of a step are read before its
+// destinations are written, and path[j] >= j, so a later source (at or past its
+// own j) is never an earlier destination.
+constexpr int kStep = 8;
+__global__ __launch_bounds__(256) void keep_kernel(Layers L, long max_len, int nkv, int hd,
+                                                   const long* __restrict__ lens,
+                                                   const int* __restrict__ path, long ld_p,
+                                                   const int* __restrict__ count, int S,
+                                                   long* __restrict__ lens_out) {
+  const int bg = blockIdx.x, b = bg / nkv, layer = blockIdx.y;
+  const long C = lens[b];
+  int n = count[b];
+  n = n < 0 ? 0 : n > S ? S : n;
+  if (lens_out && layer == 0 && bg == b * nkv && threadIdx.x == 0)
+    lens_out[b] = C < 0 ? C : C + n;
+  if (C < 0) return;
+  h16* kt = L.kt[layer] + (long)bg * hd * max_len + C;
+  h16* v = L.v[layer] + ((long)bg * max_len + C) * hd;
+  const int* p = path + (long)b * ld_p;
+  for (int d = threadIdx.x; d < hd; d += blockDim.x)
+    for (int j0 = 0; j0 < n; j0 += kStep) {
+      h16 kr[kStep], vr[kStep];
+      int at[kStep];
+#pragma unroll
+      for (int j = 0; j < kStep; ++j) {
+        at[j] = j0 + j < n ? p[j0 + j] : 0;
+        if (at[j] > j0 + j && C + at[j] < max_len) {
+          kr[j] = kt[(long)d * max_len + at[j]];
+          vr[j] = v[(long)at[j] * hd + d];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kStep; ++j)
+        if (at[j] > j0 + j && C + at[j] < max_len) {
+          kt[(long)d * max_len + j0 + j] = kr[j];
+          v[(long)(j0 + j) * hd + d] = vr[j];
+        }
+    }
+}
+
+struct Pairs {
+  int src[kPairs];
+  int dst[kPairs];
+};
+
+// Grid (nkv * hd, pairs, layers): the positions of one row of keys, and as many
+// elements of the values.
+__global__ __launch_bounds__(256) void fork_kernel(Layers L, Pairs P, long max_len, int nkv, int hd,
+                                                   long n) {
+  const int g = blockIdx.x / hd, d = blockIdx.x - g * hd, layer = blockIdx.z;
+  const long a = (long)P.src[blockIdx.y] * nkv + g, b = (long)P.dst[blockIdx.y] * nkv + g;
+  h16* kt = L.kt[layer];
+  h16* v = L.v[layer];
+  for (long p = threadIdx.x; p < n; p += blockDim.x) {
+    kt[(b * hd + d) * max_len + p] = kt[(a * hd + d) * max_len + p];
+    v[b * max_len * hd + d * n + p] = v[a * max_len * hd + d * n + p];
+  }
+}
+
+}  // namespace
+
+// See include/hn_int4.h.
+extern "C" int hn_kv_keep(void* const* kt, void* const* v, long layers, long max_len, long B,
+                          long nkv, long hd, const long* lens, const int* path, long ld_path,
+                          const int* count, long S, long* lens_out, void* stream) {
+  const char* who = "hn_kv_keep";
+  HN_ARG_CHECK(layers >= 1 && B >= 0 && nkv > 0 && hd > 0 && max_len > 0 && S >= 1 && ld_path >= S,
+               "%s: need layers, heads, positions and nodes > 0, ld_path >= nodes", who);
+  HN_ARG_CHECK(B * nkv < (1L << 31), "%s: too many heads", who);
+  if (B == 0) return 0;
+  HN_ARG_CHECK(kt && v && lens && path && count, "%s: null operand", who);
+  HN_ARG_CHECK(lens_out != lens, "%s: lens_out must not be lens (other workgroups read it)", who);
+  for (long l = 0; l < layers; ++l) HN_ARG_CHECK(kt[l] && v[l], "%s: null layer %ld", who, l);
+  for (long l0 = 0; l0 < layers; l0 += kLayers) {
+    const int m = (int)(layers - l0 < kLayers ? layers - l0 : kLayers);
+    Layers L = {};
+    for (int l = 0; l < m; ++l) L.kt[l] = (h16*)kt[l0 + l], L.v[l] = (h16*)v[l0 + l];
+    hipLaunchKernelGGL(keep_kernel, dim3((unsigned)(B * nkv), (unsigned)m),
+                       dim3(hd <= 128 ? 128 : 256), 0, (hipStream_t)stream, L, max_len, (int)nkv,
+                       (int)hd, lens, path, ld_path, count, (int)S, l0 ? nullptr : lens_out);
+    HN_LAUNCH_CHECK(who);
+  }
+  return 0;
+}
+
+// See include/hn_int4.h.
+extern "C" int hn_kv_fork(void* const* kt, void* const* v, long layers, long max_len, long B,
+                          long nkv, long hd, const int* src, const int* dst, long pairs, long n,
+                          void* stream) {
+  const char* who = "hn_kv_fork";
+  HN_ARG_CHECK(layers >= 1 && B >= 0 && nkv > 0 && hd > 0 && max_len > 0 && pairs >= 0,
+               "%s: need layers, heads and positions > 0", who);
+  HN_ARG_CHECK(n >= 0 && n <= max_len, "%s: need 0 <= positions <= max_len", who);
+  if (pairs == 0 || n == 0) return 0;
+  HN_ARG_CHECK(nkv * hd < (1L << 31), "%s: too many heads", who);
+  HN_ARG_CHECK(kt && v && src && dst, "%s: null operand", who);
+  for (long l = 0; l < layers; ++l) HN_ARG_CHECK(kt[l] && v[l], "%s: null layer %ld", who, l);
+  for (long i = 0; i < pairs; ++i) {
+    HN_ARG_CHECK(src[i] >= 0 && src[i] < B && dst[i] >= 0 && dst[i] < B,
+                 "%s: sequence out of range", who);
+    for (long j = 0; j < pairs; ++j)
+      HN_ARG_CHECK(dst[i] != src[j] && (i == j || dst[i] != dst[j]),
+                   "%s: a destination is a source or given twice", who);
+  }
+  for (long l0 = 0; l0 < layers; l0 += kLayers)
+    for (long p0 = 0; p0 < pairs; p0 += kPairs) {
+      const int m = (int)(layers - l0 < kLayers ? layers - l0 : kLayers);
+      const int np = (int)(pairs - p0 < kPairs ? pairs - p0 : kPairs);
+      Layers L = {};
+      Pairs P = {};
+      for (int l = 0; l < m; ++l) L.kt[l] = (h16*)kt[l0 + l], L.v[l] = (h16*)v[l0 + l];
+      for (int p = 0; p < np; ++p) P.src[p] = src[p0 + p], P.dst[p] = dst[p0 + p];
+      hipLaunchKernelGGL(fork_kernel, dim3((unsigned)(nkv * hd), (unsigned)np, (unsigned)m),
+                         dim3(256), 0, (hipStream_t)stream, L, P, max_len, (int)nkv, (int)hd, n);
+      HN_LAUNCH_CHECK(who);
+    }
+  return 0;
+}

@@ -20,6 +20,7 @@ reference:
 """
 from __future__ import annotations
 
+import ctypes
 import math
 from dataclasses import dataclass
 from typing import List, Optional
@@ -102,6 +103,81 @@ class KVCache:
                               dtype=dtype) for _ in range(num_layers)]
         self.max_len = max_len
         self.cur_len = 0
+
+    @classmethod
+    def wrap(cls, kt: List[torch.Tensor], v: List[torch.Tensor]) -> "KVCache":
+        """A cache over given tensors, one of each kind per layer."""
+        assert len(kt) == len(v) > 0 and kt[0].dim() == 4, "kt, v: a tensor per layer"
+        c = cls.__new__(cls)
+        c.kt, c.v = list(kt), list(v)
+        c.max_len, c.cur_len = kt[0].shape[3], 0
+        return c
+
+    def _layers(self):
+        """The layers' addresses for the kernels over the whole cache, the layers checked."""
+        B, nkv, hd, n = self.kt[0].shape
+        dev, want, wv = self.kt[0].device, (B, nkv, hd, n), (B, nkv, n, hd)
+        for t, w in [(t, want) for t in self.kt] + [(t, wv) for t in self.v]:
+            assert t.shape == w and t.dtype == torch.float16 and t.device == dev \
+                and t.is_contiguous(), "contiguous fp16 layers of one shape on one device"
+        arr = ctypes.c_void_p * len(self.kt)
+        return arr(*[t.data_ptr() for t in self.kt]), arr(*[t.data_ptr() for t in self.v])
+
+    def keep(self, lens: torch.Tensor, path: torch.Tensor, count: torch.Tensor) -> torch.Tensor:
+        """After a verification (model/speculative.py), the accepted nodes' entries
+        in every layer go from positions lens + path[:, j] to lens + j, j < count,
+        in place; returns lens + count (int64 [B]; sequences with a negative length
+        are left alone and keep it).  path int32 [B, S] with path[:, j] >= j, as
+        verify_tree gives it; entries that break this leave their position as it was."""
+        B, nkv, hd, n = self.kt[0].shape
+        dev = self.kt[0].device
+        assert lens.dtype == torch.int64 and tuple(lens.shape) == (B,) and lens.device == dev \
+            and lens.is_contiguous(), f"lens: int64 [{B}] on {dev}"
+        assert path.dtype == torch.int32 and path.dim() == 2 and path.shape[0] == B \
+            and path.shape[1] >= 1 and path.device == dev, f"path: int32 [{B}, nodes] on {dev}"
+        assert count.dtype == torch.int32 and tuple(count.shape) == (B,) \
+            and count.device == dev and count.is_contiguous(), f"count: int32 [{B}] on {dev}"
+        if path.stride(1) != 1 or path.stride(0) < path.shape[1]:
+            path = path.contiguous()
+        S = path.shape[1]
+        if lens.is_cuda:
+            from .. import _lib
+            kt, v = self._layers()
+            out = torch.empty_like(lens)
+            _lib.call_on(dev, "hn_kv_keep", kt, v, len(self.kt), n, B, nkv, hd, lens.data_ptr(),
+                         path.data_ptr(), max(path.stride(0), S), count.data_ptr(), S,
+                         out.data_ptr(), _lib.stream(dev))
+            return out
+        j = torch.arange(S)
+        c = count.clamp(0, S)
+        src = lens[:, None] + path
+        ok = (j < c[:, None]) & (path >= j) & (lens >= 0)[:, None] & (src < n)
+        b, j = ok.nonzero(as_tuple=True)
+        for kt, v in zip(self.kt, self.v):
+            kt[b, :, :, lens[b] + j] = kt[b, :, :, src[b, j]]
+            v[b, :, lens[b] + j] = v[b, :, src[b, j]]
+        return torch.where(lens >= 0, lens + c, lens)
+
+    def fork(self, src: List[int], dst: List[int], length: int) -> None:
+        """Positions [0, length) of sequence src[i] copied to sequence dst[i] in
+        every layer.  A source may be given several times, a destination once, and
+        no sequence as both."""
+        B, nkv, hd, n = self.kt[0].shape
+        assert len(src) == len(dst) and len(set(dst)) == len(dst) and not set(src) & set(dst), \
+            "as many sources as destinations, each destination once and no source"
+        assert all(0 <= b < B for b in (*src, *dst)), f"sequences 0 to {B - 1}"
+        assert 0 <= length <= n, f"length {length} of a cache of {n}"
+        if self.kt[0].is_cuda:
+            from .. import _lib
+            kt, v = self._layers()
+            ints = ctypes.c_int * max(1, len(src))
+            dev = self.kt[0].device
+            _lib.call_on(dev, "hn_kv_fork", kt, v, len(self.kt), n, B, nkv, hd, ints(*src),
+                         ints(*dst), len(src), length, _lib.stream(dev))
+            return
+        for kt, v in zip(self.kt, self.v):
+            kt[dst, :, :, :length] = kt[src, :, :, :length]
+            v[dst, :, :length] = v[src, :, :length]
 
     def update(self, layer: int, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor) -> None:
         """k, v [B, kv_heads, S, head_dim] at positions pos [S] (int64, on the device)."""

@@ -439,6 +439,94 @@ int hn_rope_append(const void* q, long ld_q, const void* k, long ld_k, const voi
                    long nh, long nkv, long hd, void* q_out, void* kt, void* vc, long max_len,
                    void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Trees of drafted tokens (speculative decoding; the reference's
+ * spec/verifier.py:216-330 and inference/speculative.py:331-405 verify chains).
+ * A tree of S <= 256 nodes is a row of parents, node i below parents[i] < i,
+ * -1: directly below the cached positions.  A node with any other parent, and
+ * every node below it, is padding.  lens [B] int64 (device): cached positions
+ * C_b of each sequence, negative for a sequence that takes no part.  Node i of
+ * sequence b sits at cache position C_b + i; its rotary position is C_b +
+ * depth(i); it sees positions [0, C_b) and those of itself and its ancestors.
+ *
+ * hn_tree_plan: of parents [B][ld_p] int32, the checked parents up [B][S]
+ *   int32 (-2: padding), depth [B][S] int32 (-1: padding) and seen [B][S][4]
+ *   u64, bit j of a node's 256: node j is itself or an ancestor (none of a
+ *   padding node's).  The calls below take one such tree for all sequences
+ *   (trees = 1) or one per sequence (trees = B). */
+int hn_tree_plan(const int* parents, long ld_p, long B, long S, int* up, int* depth,
+                 unsigned long long* seen, void* stream);
+
+/* hn_tree_append: qkv [B * S][ld_qkv] fp16 (query heads, keys, values, as
+ *   hn_attn_decode_rope takes them); the queries, rotated with cos_t / sin_t
+ *   [table_rows][hd] fp32, go to q_out [B][nkv][rep][S][hd], the rotated keys to
+ *   kt[b][g][:][C_b + i] and the values to v[b][g][C_b + i][:].  Rotation in
+ *   fp32, rounded once to fp16.  Padding nodes and sequences with a negative
+ *   length write no cache position and zero queries; a node whose position is
+ *   past the table or the cache writes no cache position and NaN queries.
+ *   hd 128. */
+int hn_tree_append(const void* qkv, long ld_qkv, const float* cos_t, const float* sin_t,
+                   long table_rows, const int* depth, long trees, const long* lens, long B, long S,
+                   long nkv, long rep, long hd, void* q_out, void* kt, void* v, long max_len,
+                   void* stream);
+
+/* hn_tree_attention: out[(b * S + i) * ld_o + (g * rep + r) * hd + d] = softmax(
+ *   scale * q k) v over the positions node i sees, fp32 scores, statistics and
+ *   sums.  q [B][nkv][rep][S][hd] (hn_tree_append's q_out), seen of
+ *   hn_tree_plan.  bound: at least C_b + S of every sequence (it sizes the
+ *   launch; a sequence past it gives NaN).  Rows of padding nodes and of
+ *   sequences with a negative length are zero.  A position that a row does not
+ *   see has no effect on it, whatever it holds.  hd 128, max_len a multiple of 8
+ *   below 2^23, 16-byte aligned operands, ld_o a multiple of 8.  work:
+ *   hn_tree_attention_workspace_bytes(...) bytes, any contents. */
+long hn_tree_attention_workspace_bytes(long B, long nkv, long rep, long S, long bound);
+int hn_tree_attention(const void* q, const void* kt, const void* v, long max_len, const long* lens,
+                      const unsigned long long* seen, long trees, long B, long nkv, long rep,
+                      long hd, long S, long bound, float scale, void* out, long ld_o, void* work,
+                      long work_bytes, void* stream);
+
+/* hn_verify_tree: accepts drafted tokens so that what is kept is distributed as
+ *   drawn from the target.  logits: the target's after each node, rows of V at
+ *   b * ld_b + i * ld_s (dtype 0 fp16, 1 bf16, 2 fp32); draft: the drafter's
+ *   after each node, its children drawn from them (NULL: certain proposals);
+ *   tokens [B][S] int64, node i's token; up of hn_tree_plan; u [B][S] fp32
+ *   uniforms in [0, 1): u[b][i] tests node i, u[b][0] draws the last token.
+ *   Probabilities are softmax(logits / T), T = temps[b] (device) or, with temps
+ *   NULL, temperature; T <= 0 takes the largest logit, the lowest index of
+ *   equals.  From node 0 on, the current node's children are tested in order of
+ *   index: accepted with probability min(1, r(x) / q(x)), r = p at first, r =
+ *   norm(max(r - q, 0)) after a rejection (of a certain proposal: r without x).
+ *   path [B][S] int32: node 0 and the accepted nodes, then -1; count [B] int32:
+ *   how many those are; token [B] int64: drawn from r after the last of them,
+ *   the lowest t whose sum of r up to t exceeds u[b][0].  Where at most
+ *   2^-40 of p's mass is left, the other children are rejected and the token is
+ *   drawn from p.  A NaN logit counts as -inf, +inf as the largest finite number; a row
+ *   without a finite logit gives token -1.  A token outside [0, V) is rejected.
+ *   work: hn_verify_tree_workspace_bytes(...) bytes, 16-byte aligned, any
+ *   contents. */
+long hn_verify_tree_workspace_bytes(long B, long S, long V, int soft);
+int hn_verify_tree(const void* logits, long ld_b, long ld_s, const void* draft, long ld_db,
+                   long ld_ds, int dtype, const long* tokens, const int* up, long trees,
+                   const float* u, const float* temps, float temperature, long B, long S, long V,
+                   int* path, int* count, long* token, void* work, long work_bytes, void* stream);
+
+/* hn_kv_keep: after a verification, positions C_b + path[b][j] of every layer's
+ *   cache go to C_b + j, j < count[b] (clamped to [0, S]), and lens_out[b] = C_b
+ *   + count[b] (NULL: not written; not lens itself).  kt, v: HOST arrays of the
+ *   layers' device pointers, kt[l] [B][nkv][hd][max_len], v[l]
+ *   [B][nkv][max_len][hd] fp16.  An entry with path[b][j] < j or past the cache
+ *   leaves its position as it was; a sequence with a negative length is left
+ *   alone.  Any alignment. */
+int hn_kv_keep(void* const* kt, void* const* v, long layers, long max_len, long B, long nkv,
+               long hd, const long* lens, const int* path, long ld_path, const int* count, long S,
+               long* lens_out, void* stream);
+
+/* hn_kv_fork: positions [0, n) of sequence src[i] copied to sequence dst[i], i <
+ *   pairs, in every layer.  kt, v, src, dst: HOST arrays.  A source may be given
+ *   several times, a destination once, and no sequence as both. */
+int hn_kv_fork(void* const* kt, void* const* v, long layers, long max_len, long B, long nkv,
+               long hd, const int* src, const int* dst, long pairs, long n, void* stream);
+
 /* Decode kernel family for hn_int4_linear, hn_int4_gate_up_silu,
  * hn_expert_mlp_int4 and hn_grouped_expert_mlp_int4, for the calling thread
  * only (each thread starts at 0; a switch never affects another thread):

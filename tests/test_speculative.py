@@ -1,0 +1,220 @@
+"""CPU checks of the tree-speculation operators (hydranet_amd/model/speculative.py,
+KVCache.keep / fork): the torch forms against node-by-node 64-bit ones, what is
+refused, and that verification keeps the target's distribution."""
+import random
+
+import pytest
+import torch
+
+from hydranet_amd.model.decoder import KVCache
+from hydranet_amd.model.speculative import (PADDING, DraftTree, tree_append, tree_attention,
+                                            verify_tree)
+from tests import _tree_ref as ref
+
+
+def _tree(rows):
+    return DraftTree(torch.tensor(rows, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("S,kind", [(1, "chain"), (2, "chain"), (70, "chain"), (9, "star"),
+                                    (33, "random"), (40, "padded"), (65, "roots"),
+                                    (256, "random"), (256, "chain")])
+def test_plan(S, kind):
+    rng = random.Random(S)
+    rows = [ref.random_tree(rng, S, kind) for _ in range(3)]
+    t = _tree(rows)
+    see = t.visible()
+    for b, row in enumerate(rows):
+        for i in range(S):
+            way = ref.way_up(row, i)
+            assert t.depth[b, i] == len(way) - 1
+            assert t.up[b, i] == (row[i] if way else PADDING)
+            assert see[b, i].nonzero().flatten().tolist() == way
+
+
+def _cache(B, nkv, hd, n, dtype=torch.float64):
+    return KVCache.wrap([torch.randn(B, nkv, hd, n, dtype=dtype)],
+                        [torch.randn(B, nkv, n, hd, dtype=dtype)])
+
+
+@pytest.mark.parametrize("kind", ["chain", "random", "padded", "roots"])
+@pytest.mark.parametrize("shared", [False, True])
+def test_append_and_attention(kind, shared):
+    torch.manual_seed(3)
+    rng = random.Random(5)
+    B, nkv, rep, S, hd, n = 4, 2, 3, 7, 16, 40
+    rows = [ref.random_tree(rng, S, kind)] * B if shared else \
+        [ref.random_tree(rng, S, kind) for _ in range(B)]
+    tree = _tree(rows[0] if shared else rows)
+    lens = torch.tensor([0, 20, -1, n - S])
+    c = _cache(B, nkv, hd, n)
+    a = torch.outer(torch.arange(n).float(), 0.3 ** torch.arange(hd // 2).float()).repeat(1, 2)
+    cos, sin = a.cos(), a.sin()
+    qkv = torch.randn(B * S, (nkv * rep + 2 * nkv) * hd, dtype=torch.float64)
+    want = ref.append(qkv, cos, sin, rows, lens, nkv * rep, c.kt[0], c.v[0])
+    q = tree_append(qkv, cos, sin, tree, lens, c, 0, nkv * rep)
+    for got, w in zip((q, c.kt[0], c.v[0]), want):
+        torch.testing.assert_close(got, w, rtol=1e-12, atol=1e-12)
+    c.v[0][1, :, 20 + S:] = float("nan")  # positions nobody sees
+    c.kt[0][1, :, :, 20 + S:] = float("nan")
+    o = tree_attention(q, tree, lens, c, 0, n)
+    w, _, _ = ref.attention(q, c.kt[0], c.v[0], rows, lens)
+    torch.testing.assert_close(o.view(B, S, nkv * rep, hd), w, rtol=1e-10, atol=1e-12)
+    short = tree_attention(q, tree, lens, c, 0, 20 + S)
+    assert torch.equal(short[:3], o[:3])
+    live = tree.depth.expand(B, S)[3] >= 0
+    assert short[3, live].isnan().all() and bool((short[3, ~live] == 0).all())
+
+
+@pytest.mark.parametrize("kind", ["chain", "random", "padded", "star"])
+@pytest.mark.parametrize("soft", [True, False])
+def test_verify_against_the_definition(kind, soft):
+    rng = random.Random(11)
+    g = torch.Generator().manual_seed(2)
+    B, S, V = 40, 9, 23
+    rows = [ref.random_tree(rng, S, kind) for _ in range(B)]
+    logits = torch.randn(B, S, V, generator=g) * 2
+    draft = logits + torch.randn(B, S, V, generator=g) if soft else None
+    logits[3, :, 5:9] = -float("inf")
+    logits[4, 0] = float("nan")
+    tokens = torch.randint(0, V, (B, S), generator=g)
+    up = torch.tensor(rows).clamp(0, S - 1)
+    likely = logits.nan_to_num(0).gather(1, up[..., None].expand(B, S, V)).argmax(-1)
+    tokens = torch.where(torch.rand(B, S, generator=g) < 0.6, likely, tokens)
+    tokens[5, 1], tokens[6, 2] = -1, V
+    u = torch.rand(B, S, generator=g)
+    temps = torch.rand(B, generator=g)
+    temps[::4] = 0
+    got = verify_tree(logits, tokens, _tree(rows), u, draft, temps)
+    paths, toks, _ = ref.verify(logits, tokens, rows, u, draft, temps)
+    for b in range(B):
+        assert got.path[b].tolist() == paths[b] + [-1] * (S - len(paths[b]))
+        assert got.count[b] == len(paths[b])
+    assert got.token.tolist() == toks
+    assert int((got.count > 1).sum()) > 4
+
+
+@pytest.mark.parametrize("soft", [True, False])
+def test_verify_keeps_the_targets_distribution(soft):
+    """One root with three children drawn from q (or certain): the first token after the root
+    (the accepted child's, else the drawn one) is distributed as p.  N draws; a frequency's
+    deviation sqrt(p (1 - p) / N) is at most 0.5 / sqrt(N); 5 deviations of it."""
+    g = torch.Generator().manual_seed(8)
+    N, V = 20000, 4
+    p = torch.tensor([0.5, 0.3, 0.15, 0.05]).log()
+    q = torch.tensor([0.1, 0.2, 0.3, 0.4]).log()
+    logits = p.expand(N, 4, V).contiguous()
+    draft = q.expand(N, 4, V).contiguous()
+    tokens = torch.multinomial(q.exp().expand(N, V), 4, replacement=True, generator=g)
+    if not soft:
+        tokens[:] = torch.tensor([0, 3, 1, 3])
+    got = verify_tree(logits, tokens, _tree([-1, 0, 0, 0]), torch.rand(N, 4, generator=g),
+                      draft if soft else None)
+    first = torch.where(got.count > 1, tokens.gather(1, got.path[:, 1:2].clamp(min=0).long())[:, 0],
+                        got.token)
+    freq = torch.bincount(first, minlength=V).double() / N
+    assert (freq - p.double().exp()).abs().max() < 5 * 0.5 / N ** 0.5
+
+
+def test_keep_and_fork():
+    torch.manual_seed(1)
+    B, n, S = 4, 30, 6
+    c = KVCache.wrap([torch.randn(B, 2, 4, n) for _ in range(3)],
+                     [torch.randn(B, 2, n, 4) for _ in range(3)])
+    old = [t.clone() for t in c.kt], [t.clone() for t in c.v]
+    lens = torch.tensor([5, 0, -1, n - S])
+    path = torch.tensor([[0, 2, 5, -1, -1, -1], [0, 1, 2, 3, 4, 5], [0, 3, 4, -1, -1, -1],
+                         [0, 0, 4, 5, -1, -1]], dtype=torch.int32)
+    count = torch.tensor([3, 9, 2, 4], dtype=torch.int32)
+    got = c.keep(lens, path, count)
+    assert got.tolist() == [8, 6, -1, n - S + 4]
+    for l in range(3):
+        k, v = old[0][l].clone(), old[1][l].clone()
+        for b, moves in ((0, [(1, 2), (2, 5)]), (3, [(2, 4), (3, 5)])):
+            for j, i in moves:
+                k[b, :, :, lens[b] + j] = old[0][l][b, :, :, lens[b] + i]
+                v[b, :, lens[b] + j] = old[1][l][b, :, lens[b] + i]
+        assert torch.equal(c.kt[l], k) and torch.equal(c.v[l], v)
+    old = [t.clone() for t in c.kt], [t.clone() for t in c.v]
+    c.fork([0, 0], [1, 2], 7)
+    for l in range(3):
+        assert torch.equal(c.kt[l][1, :, :, :7], old[0][l][0, :, :, :7])
+        assert torch.equal(c.v[l][2, :, :7], old[1][l][0, :, :7])
+        assert torch.equal(c.kt[l][1:, :, :, 7:], old[0][l][1:, :, :, 7:])
+        assert torch.equal(c.v[l][3], old[1][l][3]) and torch.equal(c.v[l][0], old[1][l][0])
+
+
+def test_refusals():
+    c = _cache(2, 2, 8, 16)
+    t = _tree([-1, 0, 1])
+    lens = torch.zeros(2, dtype=torch.int64)
+    qkv, tab = torch.zeros(6, 8 * 8, dtype=torch.float64), torch.zeros(16, 8)
+    q = torch.zeros(2, 2, 6, 8, dtype=torch.float64)
+    lg, tok, u = torch.zeros(2, 3, 5), torch.zeros(2, 3, dtype=torch.int64), torch.zeros(2, 3)
+    one = torch.ones(2, dtype=torch.int32)
+    path = torch.zeros(2, 3, dtype=torch.int32)
+    for bad in (
+            lambda: DraftTree(torch.zeros(3)),
+            lambda: DraftTree(torch.zeros(257, dtype=torch.int32)),
+            lambda: DraftTree(torch.zeros(0, dtype=torch.int32)),
+            lambda: tree_append(qkv, tab, tab, t, lens.int(), c, 0, 4),
+            lambda: tree_append(qkv, tab, tab, t, lens[:1], c, 0, 4),
+            lambda: tree_append(qkv, tab, tab, t, lens, c, 0, 5),
+            lambda: tree_append(qkv[:5], tab, tab, t, lens, c, 0, 4),
+            lambda: tree_append(qkv, tab.half(), tab, t, lens, c, 0, 4),
+            lambda: tree_append(qkv, tab, tab, _tree([[-1, 0, 1]] * 3), lens, c, 0, 4),
+            lambda: tree_attention(q[:, :1], t, lens, c, 0, 16),
+            lambda: tree_attention(q[:, :, :5], t, lens, c, 0, 16),
+            lambda: tree_attention(q, t, lens, c, 0, 2),
+            lambda: tree_attention(q, t, lens, c, 0, 17),
+            lambda: verify_tree(lg.double(), tok, t, u),
+            lambda: verify_tree(lg[:, :2], tok, t, u),
+            lambda: verify_tree(lg, tok.int(), t, u),
+            lambda: verify_tree(lg, tok, t, u[:, :2]),
+            lambda: verify_tree(lg, tok, t, u, lg.half()),
+            lambda: verify_tree(lg, tok, t, u, temperature=-1.0),
+            lambda: verify_tree(lg, tok, t, u, temperature=torch.ones(3)),
+            lambda: c.keep(lens, path.long(), one),
+            lambda: c.keep(lens, path[:1], one),
+            lambda: c.keep(lens, path, one[:1]),
+            lambda: c.fork([0], [0], 4), lambda: c.fork([0, 0], [1, 1], 4),
+            lambda: c.fork([0], [2], 4), lambda: c.fork([0], [1], 17),
+            lambda: c.fork([0, 1], [1], 4)):
+        with pytest.raises(AssertionError):
+            bad()
+
+
+def test_library_refusals_without_gpu():
+    """Rejected arguments return before any HIP call."""
+    import ctypes
+    from hydranet_amd import _lib
+    P = ctypes.c_void_p(16)
+    two = (ctypes.c_void_p * 2)(16, 16)
+    i0, i1 = (ctypes.c_int * 2)(0, 0), (ctypes.c_int * 2)(1, 1)
+    for name, args in [
+            ("hn_tree_plan", (P, 257, 1, 257, P, P, P, None)),
+            ("hn_tree_plan", (P, 2, 1, 3, P, P, P, None)),
+            ("hn_tree_plan", (None, 3, 1, 3, P, P, P, None)),
+            ("hn_tree_append", (P, 1024, P, P, 8, P, 1, P, 1, 1, 2, 4, 64, P, P, P, 8, None)),
+            ("hn_tree_append", (P, 1024, P, P, 8, P, 1, P, 1, 1, 2, 4, 128, P, P, P, 8, None)),
+            ("hn_tree_append", (P, 1536, P, P, 8, P, 2, P, 3, 1, 2, 4, 128, P, P, P, 8, None)),
+            ("hn_tree_append", (P, 1536, P, P, 8, P, 1, None, 3, 1, 2, 4, 128, P, P, P, 8, None)),
+            ("hn_tree_attention", (P, P, P, 12, P, P, 1, 1, 1, 1, 128, 1, 9, 1.0, P, 128, P, 1 << 30, None)),
+            ("hn_tree_attention", (P, P, P, 16, P, P, 1, 1, 1, 1, 128, 1, 17, 1.0, P, 128, P, 1 << 30, None)),
+            ("hn_tree_attention", (P, P, P, 16, P, P, 1, 1, 1, 1, 128, 4, 3, 1.0, P, 128, P, 1 << 30, None)),
+            ("hn_tree_attention", (P, P, P, 16, P, P, 1, 1, 2, 1, 128, 1, 9, 1.0, P, 128, P, 1 << 30, None)),
+            ("hn_tree_attention", (P, P, ctypes.c_void_p(8), 16, P, P, 1, 1, 1, 1, 128, 1, 9, 1.0, P, 128, P, 1 << 30, None)),
+            ("hn_verify_tree", (P, 9, 3, None, 0, 0, 3, P, P, 1, P, None, 1.0, 1, 3, 3, P, P, P, P, 1 << 30, None)),
+            ("hn_verify_tree", (P, 9, 2, None, 0, 0, 0, P, P, 1, P, None, 1.0, 1, 3, 3, P, P, P, P, 1 << 30, None)),
+            ("hn_verify_tree", (P, 9, 3, P, 9, 2, 0, P, P, 1, P, None, 1.0, 1, 3, 3, P, P, P, P, 1 << 30, None)),
+            ("hn_verify_tree", (P, 9, 3, None, 0, 0, 0, P, P, 1, P, None, -1.0, 1, 3, 3, P, P, P, P, 1 << 30, None)),
+            ("hn_verify_tree", (P, 9, 3, None, 0, 0, 0, P, P, 1, None, None, 1.0, 1, 3, 3, P, P, P, P, 1 << 30, None)),
+            ("hn_kv_keep", (two, two, 2, 8, 1, 1, 4, P, P, 2, P, 3, None, None)),
+            ("hn_kv_keep", (two, two, 2, 8, 1, 1, 4, P, P, 3, P, 3, P, None)),
+            ("hn_kv_keep", ((ctypes.c_void_p * 2)(16, None), two, 2, 8, 1, 1, 4, P, P, 3, P, 3, None, None)),
+            ("hn_kv_fork", (two, two, 2, 8, 4, 1, 4, i0, i0, 1, 4, None)),
+            ("hn_kv_fork", (two, two, 2, 8, 4, 1, 4, i0, i1, 2, 4, None)),
+            ("hn_kv_fork", (two, two, 2, 8, 1, 1, 4, i0, i1, 1, 4, None)),
+            ("hn_kv_fork", (two, two, 2, 8, 4, 1, 4, i0, i1, 1, 9, None))]:
+        with pytest.raises(RuntimeError, match=name):
+            _lib.call(name, *args)
