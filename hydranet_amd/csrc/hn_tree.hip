@@ -93,57 +93,436 @@ __global__ __launch_bounds__(kHd) void append_kernel(
   }
 }
 
-// One wave per (sequence, query head, node): 64 positions at a time, a lane per
-// position for the scores, then a lane per two elements of the output.
-__global__ __launch_bounds__(256) void attend_kernel(
-    const h16* __restrict__ q, const h16* __restrict__ ktc, const h16* __restrict__ vc,
-    long max_len, const long* __restrict__ lens, const u64* __restrict__ seen, int trees, long rows,
-    int nkv, int rep, int S, long bound, float scale, h16* __restrict__ out, long ld_o) {
-  const int lane = threadIdx.x & 63;
-  const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);  // (b, g, r, i)
-  if (row >= rows) return;
-  const int i = (int)(row % S);
-  const long bh = row / S, bg = bh / rep, b = bg / nkv;
-  const int head = (int)(bh - b * nkv * rep);
-  const u64* see = seen + ((trees > 1 ? b * S : 0) + i) * kWords;
-  const long C = lens[b], L = C + S;
-  h16* o = out + (b * S + i) * ld_o + (long)head * kHd + 2 * lane;
-  const bool live = C >= 0 && ((see[i >> 6] >> (i & 63)) & 1);
-  if (!live || L > bound) {
-    const h16 v = live ? (h16)__builtin_nanf("") : (h16)0.f;
-    o[0] = v, o[1] = v;
-    return;
-  }
-  const h16* kt = ktc + bg * kHd * max_len;
-  const h16* v = vc + bg * max_len * kHd;
-  const h16* qr = q + row * kHd;
-  float mx = -__builtin_inff(), sum = 0.f, o0 = 0.f, o1 = 0.f;
-  for (long p0 = 0; p0 < L; p0 += 64) {
-    const long p = p0 + lane;
-    bool vis = p < C;
-    if (p >= C && p < L) vis = (see[(p - C) >> 6] >> ((p - C) & 63)) & 1;
-    float s = -__builtin_inff();
-    if (vis) {
-      s = 0.f;
-      for (int d = 0; d < kHd; ++d) s += (float)qr[d] * (float)kt[(long)d * max_len + p];
-      s *= scale;
+// ---------------------------------------------------------------------------
+// Attention.  One workgroup of 4 waves takes RT tiles of 16 rows of one
+// (sequence, KV head), a row being a (query head of the group, node) pair, and a
+// range of the positions; each wave walks its own tiles of 128 positions:
+//   S^T = K Q^T    v_mfma_f32_16x16x32_f16, A = K, B = Q;
+//   softmax        a lane holds 32 consecutive positions of one row, 32 * (lane /
+//                  16) on, of row lane % 16;
+//   O^T += V^T P   the lane's probabilities are the B operand as they are.
+// K is cached as [hd][position] and V as [position][hd], so both products
+// contract over the axis that is not dense in memory.  A lane loads 8 vectors of
+// 8 halves, an 8 x 8 block, and v_perm takes pairs of its rows apart: 32 of them
+// make the 8 operands of the block's 8 products, product j holding every lane's
+// column j.  Which positions (of K) or columns (of V) a product holds is a
+// permutation that the sums do not see, and it makes a lane's scores
+// consecutive.  So neither K nor V passes through LDS, each element is loaded
+// once per workgroup, and a wave keeps 3 to 4 blocks of 8 KB in flight: block s
+// of a tile (4 of K, then 4 of V) is replaced by block s + 4 once it is used.
+constexpr int kPos = 128;     // positions per tile
+constexpr int kOPad = kHd + 4;
+constexpr float kLog2e = 1.4426950408889634f;
+// Probabilities are 2^8 times the softmax's, relative to a maximum that follows
+// the true one only when it lags by 2^6: below 2^14, so fp16 holds them, and
+// those down to 2^-22 of the largest are normal numbers.
+constexpr float kUp = 8.f, kLag = 6.f;
+
+typedef float float4v __attribute__((ext_vector_type(4)));
+
+template <bool B>
+struct Bool {
+  static constexpr bool value = B;
+};
+
+struct Attend {
+  const h16 *q, *kt, *v;
+  const long* lens;
+  const u64* seen;
+  h16* out;
+  float* part;
+  long max_len, bound, ld_o;
+  int trees, nkv, rep, S, R, blocks, splits, tps, units;
+  float scale;
+};
+
+__device__ __forceinline__ uint32_t perm_lo(uint32_t a, uint32_t b) {  // (a.lo, b.lo)
+  return __builtin_amdgcn_perm(b, a, 0x05040100u);
+}
+__device__ __forceinline__ uint32_t perm_hi(uint32_t a, uint32_t b) {  // (a.hi, b.hi)
+  return __builtin_amdgcn_perm(b, a, 0x07060302u);
+}
+// column c of an 8 x 8 block
+template <int C>
+__device__ __forceinline__ half8_t column(const u32x4 r[8]) {
+  u32x4 w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w[i] = C & 1 ? perm_hi(r[2 * i][C >> 1], r[2 * i + 1][C >> 1])
+                 : perm_lo(r[2 * i][C >> 1], r[2 * i + 1][C >> 1]);
+  return __builtin_bit_cast(half8_t, w);
+}
+
+// max without the canonicalising multiply that fmaxf has on a product's result
+__device__ __forceinline__ float larger(float a, float b) {
+  return __builtin_amdgcn_fmed3f(a, b, __builtin_inff());
+}
+
+// Bits [at, at + 32) of what a node sees, positions before its tree (at < 0) all
+// seen.
+__device__ __forceinline__ uint32_t window(const u64* see, long at) {
+  if (at <= -32) return ~0u;
+  if (at >= kMaxNodes) return 0u;
+  if (at < 0) return (uint32_t)(see[0] << -at) | ((1u << -at) - 1u);
+  const int w = (int)(at >> 6), s = (int)(at & 63);
+  u64 x = see[w] >> s;
+  if (s > 32 && w + 1 < kWords) x |= see[w + 1] << (64 - s);
+  return (uint32_t)x;
+}
+
+// The halves of w that are NaN or infinite, as a mask.
+__device__ __forceinline__ uint32_t odd_mask(uint32_t w) {
+  return ((w & 0x7c00u) == 0x7c00u ? 0xffffu : 0u) |
+         ((w & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u);
+}
+
+template <int RT>
+__global__ __launch_bounds__(256, 1) void attend_kernel(Attend A) {
+  constexpr int kRows = 16 * RT;
+  __shared__ __align__(16) float s_o[4][16][kOPad];
+  __shared__ float s_m[4][kRows], s_l[4][kRows];
+  __shared__ u32x4 s_q[RT][4][64];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = lane & 15, kg = lane >> 4;
+  // the row blocks of one (head, range) follow each other on one XCD, whose L2
+  // then serves all but the first
+  const int id = blockIdx.x, grp = id / (8 * A.blocks), in = id - grp * 8 * A.blocks;
+  const int unit = 8 * grp + (in & 7), block = in >> 3;
+  if (unit >= A.units) return;
+  const int bg = unit / A.splits, split = unit - bg * A.splits;
+  const int b = bg / A.nkv, g = bg - b * A.nkv;
+  const int row0 = block * kRows;
+  const long C = A.lens[b], L = C + A.S;
+  const int tree = A.trees > 1 ? b : 0;
+  const bool run = C >= 0 && L <= A.bound;
+  const int tiles = run ? (int)((L + kPos - 1) / kPos) : 0;
+  const int first = split * A.tps, end = first + A.tps < tiles ? first + A.tps : tiles;
+  if (run ? first >= tiles : split > 0) return;
+
+  // queries, as each lane's operands: rows past the last are zero
+  for (int t = wave; t < RT; t += 4) {
+    const int row = row0 + 16 * t + n;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      u32x4 w = {0, 0, 0, 0};
+      if (row < A.R && run)
+        w = *reinterpret_cast<const u32x4*>(A.q + ((long)bg * A.R + row) * kHd + 32 * u + 8 * kg);
+      s_q[t][u][lane] = w;
     }
-    float tm = s;
-    for (int off = 32; off; off >>= 1) tm = fmaxf(tm, __shfl_xor(tm, off, 64));
-    const float nm = fmaxf(mx, tm), ref = nm == -__builtin_inff() ? 0.f : nm;
-    const float al = expf(mx - ref), e = vis ? expf(s - ref) : 0.f;
-    sum = sum * al + e, o0 *= al, o1 *= al, mx = nm;
-    u64 todo = __ballot(vis);
-    while (todo) {
-      const int j = __builtin_ctzll(todo);
-      todo &= todo - 1;
-      const float pj = __shfl(e, j, 64);
-      const h16* vr = v + (p0 + j) * kHd + 2 * lane;
-      o0 += pj * (float)vr[0], o1 += pj * (float)vr[1];
+  }
+  __syncthreads();
+
+  const long slab = (long)bg * kHd * A.max_len;
+  const uint32_t pitch = (uint32_t)A.max_len * 2;  // bytes of a row of keys
+  const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
+      (void*)(A.kt + slab), (short)0, (int)(pitch * kHd), 0x00020000);
+  const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
+      (void*)(A.v + slab), (short)0, (int)(pitch * kHd), 0x00020000);
+  constexpr uint32_t kNone = 0xfffff000u;  // past both: reads zero, without an access
+
+  u32x4 ring[4][8];
+  // keys 32 u + 8 kg + r at positions p0 + 8 n on; a vector past the row's end
+  // (its positions are past the sequence) reads the row's last instead.  The
+  // lane's part of the address is one register, the rest a scalar that is
+  // stepped from load to load (32 of them, kept, would spill).
+  auto load_k = [&](u32x4 (&x)[8], int tile, int u) {
+    const int p0 = tile * kPos, last = (int)A.max_len - 8 - p0;
+    const uint32_t at =
+        tile < end ? (uint32_t)(8 * kg) * pitch + 2u * (uint32_t)(8 * n < last ? 8 * n : last) : kNone;
+    uint32_t step = pitch;
+    asm volatile("" : "+s"(step));
+    uint32_t so = 2u * (uint32_t)p0 + (uint32_t)(32 * u) * step;
+#pragma unroll
+    for (int r = 0; r < 8; ++r, so += step)
+      x[r] = __builtin_bit_cast(
+          u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, (int)at, (int)so, 0));
+  };
+  // values of positions p0 + 32 kg + 8 t + j at elements 8 n on.  The lane's
+  // part, j and t share no bit, so j is the instruction's own offset.
+  auto load_v = [&](u32x4 (&x)[8], int tile, int t) {
+    const int so = tile * (kPos * kHd * 2) + t * (8 * kHd * 2);
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      x[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
+                                           rv, (kg << 13) | (n << 4) | (j << 8), so, 0));
+  };
+  // the same of a sequence's last tiles: past its end, zero (their probabilities
+  // are, and what a longer sequence left there may be anything)
+  auto load_v_end = [&](u32x4 (&x)[8], int tile, int t) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const long p = (long)tile * kPos + 32 * kg + 8 * t + j;
+      const uint32_t at = p < L ? (uint32_t)p * (kHd * 2) + 16 * n : kNone;
+      x[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, (int)at, 0, 0));
+    }
+  };
+
+  float4v o[RT][8], l[RT];
+  float mx[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    mx[t] = -__builtin_inff();
+    l[t] = (float4v)(0.f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[t][e] = (float4v)(0.f);
+  }
+  const float scale = A.scale * kLog2e;
+  half8_t ones;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ones[i] = (h16)1.f;
+
+  int tile = first + wave;
+#pragma unroll
+  for (int u = 0; u < 4; ++u) load_k(ring[u], tile, u);
+  // EDGE: a tile that holds nodes, or positions past the sequence
+  auto walk = [&](auto edge_tile) {
+    constexpr bool EDGE = decltype(edge_tile)::value;
+    float4v s[RT][8];
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[t][j] = (float4v)(0.f);
+#define HN_QK(J)                                                                                 \
+  {                                                                                              \
+    const half8_t a = column<J>(ring[u]);                                                        \
+    _Pragma("unroll") for (int t = 0; t < RT; ++t) s[t][J] =                                     \
+        __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q[t], s[t][J], 0, 0, 0);                       \
+  }
+    int ql = lane;
+    asm volatile("" : "+v"(ql));  // queries are read again for each tile, not kept in registers
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      half8_t q[RT];
+#pragma unroll
+      for (int t = 0; t < RT; ++t) q[t] = __builtin_bit_cast(half8_t, s_q[t][u][ql]);
+      HN_QK(0) HN_QK(1)
+      __builtin_amdgcn_sched_barrier(0);
+      HN_QK(2) HN_QK(3)
+      __builtin_amdgcn_sched_barrier(0);
+      HN_QK(4) HN_QK(5)
+      __builtin_amdgcn_sched_barrier(0);
+      HN_QK(6) HN_QK(7)
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (EDGE)
+        load_v_end(ring[u], tile, u);
+      else
+        load_v(ring[u], tile, u);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#undef HN_QK
+    const int p0 = tile * kPos;
+    half8_t p[RT][4];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      if constexpr (EDGE) {
+        const int row = row0 + 16 * t + n;
+        const int node = row < A.R ? row % A.S : 0;
+        const uint32_t w = window(A.seen + ((long)tree * A.S + node) * kWords, p0 + 32 * kg - C);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (!((w >> (8 * r + j)) & 1u)) s[t][j][r] = -__builtin_inff();
+      }
+      float tm = s[t][0][0];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) tm = larger(tm, s[t][j][r]);
+      tm = fmaxf(tm, __shfl_xor(tm, 16, 64));
+      tm = fmaxf(tm, __shfl_xor(tm, 32, 64)) * scale;
+      if (__any(tm > mx[t] + kLag)) {
+        const float nm = fmaxf(mx[t], tm);
+        const float al = nm == mx[t] ? 1.f : __builtin_amdgcn_exp2f(mx[t] - nm);
+        l[t] *= al;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[t][e] *= al;
+        mx[t] = nm;
+      }
+      // a row that has seen nothing yet: every score is -inf
+      const float ref = mx[t] == -__builtin_inff() ? 0.f : mx[t] - kUp;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          p[t][r][j] = (h16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j][r], scale, -ref));
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#define HN_PV(E)                                                                                 \
+  {                                                                                              \
+    const half8_t a = column<E>(ring[u]);                                                        \
+    _Pragma("unroll") for (int t = 0; t < RT; ++t) o[t][E] =                                     \
+        __builtin_amdgcn_mfma_f32_16x16x32_f16(a, p[t][u], o[t][E], 0, 0, 0);                    \
+  }
+    uint32_t any_odd = 0;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if constexpr (EDGE) {
+        // a node's value that is no number must not reach, as 0 times it, the
+        // rows that do not see it: taken out here, added to the others below
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const bool node = p0 + 32 * kg + 8 * u + j >= C;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t w = ring[u][j][i], m = node ? odd_mask(w) : 0u;
+            any_odd |= m;
+            ring[u][j][i] = w & ~m;
+          }
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+        l[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, p[t][u], l[t], 0, 0, 0);
+      HN_PV(0) HN_PV(1)
+      __builtin_amdgcn_sched_barrier(0);
+      HN_PV(2) HN_PV(3)
+      __builtin_amdgcn_sched_barrier(0);
+      HN_PV(4) HN_PV(5)
+      __builtin_amdgcn_sched_barrier(0);
+      HN_PV(6) HN_PV(7)
+      __builtin_amdgcn_sched_barrier(0);
+      load_k(ring[u], tile + 4, u);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#undef HN_PV
+    if (EDGE && __any(any_odd != 0)) {
+      const long a0 = p0 > C ? p0 - C : 0, a1 = p0 + kPos - C < A.S ? p0 + kPos - C : A.S;
+      for (long a = a0; a < a1; ++a) {
+        const h16* vr = A.v + slab + (C + a) * kHd + 32 * kg;
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+          const int row = row0 + 16 * t + n;
+          const int node = row < A.R ? row % A.S : 0;
+          const bool vis = (A.seen[((long)tree * A.S + node) * kWords + (a >> 6)] >> (a & 63)) & 1;
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float x = (float)vr[8 * r + e];
+              if (vis && !(__builtin_fabsf(x) < __builtin_inff())) o[t][e][r] += x;
+            }
+        }
+      }
+    }
+  };
+  const int inner = (int)(C / kPos) < end ? (int)(C / kPos) : end;  // tiles all rows see whole
+  for (; tile < inner; tile += 4) walk(Bool<false>{});
+  for (; tile < end; tile += 4) walk(Bool<true>{});
+
+  // The waves' sums joined, 16 rows at a time; then the rows themselves where
+  // this is the sequence's only range, else this range's sums.
+  if (kg == 0)
+#pragma unroll
+    for (int t = 0; t < RT; ++t) s_m[wave][16 * t + n] = mx[t], s_l[wave][16 * t + n] = l[t][0];
+  const bool whole = tiles <= A.tps;
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    if (t) __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float4v w = {o[t][4 * h][r], o[t][4 * h + 1][r], o[t][4 * h + 2][r],
+                           o[t][4 * h + 3][r]};
+        *reinterpret_cast<float4v*>(&s_o[wave][n][32 * kg + 8 * r + 4 * h]) = w;
+      }
+    __syncthreads();
+    const int rr = tid >> 4, d = 8 * (tid & 15), row = row0 + 16 * t + rr;
+    if (row < A.R) {
+      float m = s_m[0][16 * t + rr];
+#pragma unroll
+      for (int w = 1; w < 4; ++w) m = fmaxf(m, s_m[w][16 * t + rr]);
+      const float ref = m == -__builtin_inff() ? 0.f : m;
+      float sum = 0.f, x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float mw = s_m[w][16 * t + rr];
+        // a wave without tiles has sums of zero and weight exp2(-inf) = 0
+        const float al = __builtin_amdgcn_exp2f(mw - ref);
+        sum += al * s_l[w][16 * t + rr];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] += al * s_o[w][rr][d + i];
+      }
+      const int head = row / A.S, node = row - head * A.S;
+      if (whole) {
+        const bool live = C >= 0 && ((A.seen[((long)tree * A.S + node) * kWords + (node >> 6)] >>
+                                      (node & 63)) & 1);
+        const float is = !run ? __builtin_nanf("") : 1.f / sum;
+        half8_t y;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = live ? (h16)(x[i] * is) : (h16)0.f;
+        *reinterpret_cast<half8_t*>(A.out + ((long)b * A.S + node) * A.ld_o +
+                                    (long)(g * A.rep + head) * kHd + d) = y;
+      } else {
+        float* po = A.part + (((long)bg * A.splits + split) * A.R + row) * kHd + d;
+        float* pm = A.part + (long)A.units * A.R * kHd + (((long)bg * A.splits + split) * A.R + row) * 2;
+#pragma unroll
+        for (int i = 0; i < 8; i += 4)
+          *reinterpret_cast<float4v*>(po + i) = float4v{x[i], x[i + 1], x[i + 2], x[i + 3]};
+        if ((tid & 15) == 0) pm[0] = m, pm[1] = sum;
+      }
     }
   }
-  for (int off = 32; off; off >>= 1) sum += __shfl_xor(sum, off, 64);
-  o[0] = (h16)(o0 / sum), o[1] = (h16)(o1 / sum);
+}
+
+// The ranges' sums joined: 16 threads per row, 8 elements each.
+__global__ __launch_bounds__(256) void join_kernel(Attend A, long rows) {
+  const long at = (long)blockIdx.x * 16 + (threadIdx.x >> 4);  // bg * R + row
+  if (at >= rows) return;
+  const int d = 8 * (threadIdx.x & 15);
+  const int bg = (int)(at / A.R), row = (int)(at - (long)bg * A.R);
+  const int b = bg / A.nkv, g = bg - b * A.nkv, head = row / A.S, node = row - head * A.S;
+  const long C = A.lens[b], L = C + A.S;
+  if (C < 0 || L > A.bound) return;
+  const int tiles = (int)((L + kPos - 1) / kPos), ns = (tiles + A.tps - 1) / A.tps;
+  if (ns == 1) return;
+  const float* po = A.part + ((long)bg * A.splits * A.R + row) * kHd + d;
+  const float* pm = A.part + (long)A.units * A.R * kHd + ((long)bg * A.splits * A.R + row) * 2;
+  float m = -__builtin_inff();
+  for (int i = 0; i < ns; ++i) m = fmaxf(m, pm[(long)i * A.R * 2]);
+  const float ref = m == -__builtin_inff() ? 0.f : m;
+  float sum = 0.f, x[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) x[i] = 0.f;
+#pragma unroll 4
+  for (int i = 0; i < ns; ++i) {
+    const float al = __builtin_amdgcn_exp2f(pm[(long)i * A.R * 2] - ref);
+    sum += al * pm[(long)i * A.R * 2 + 1];
+    const float4v lo = *reinterpret_cast<const float4v*>(po + (long)i * A.R * kHd);
+    const float4v hi = *reinterpret_cast<const float4v*>(po + (long)i * A.R * kHd + 4);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] += al * lo[k], x[4 + k] += al * hi[k];
+  }
+  const u64* see = A.seen + ((A.trees > 1 ? (long)b * A.S : 0) + node) * kWords;
+  const bool live = (see[node >> 6] >> (node & 63)) & 1;
+  const float is = 1.f / sum;
+  half8_t y;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = live ? (h16)(x[i] * is) : (h16)0.f;
+  *reinterpret_cast<half8_t*>(A.out + ((long)b * A.S + node) * A.ld_o +
+                              (long)(g * A.rep + head) * kHd + d) = y;
+}
+
+// Row tiles per workgroup, and how the positions are split so that about two
+// rounds of workgroups fill the chip.
+struct Plan {
+  int rt, blocks, splits, tps;
+};
+Plan plan_of(long B, long nkv, long rep, long S, long bound) {
+  const long R = rep * S, tiles = (bound + kPos - 1) / kPos;
+  Plan p;
+  p.rt = R <= 16 ? 1 : 2;
+  p.blocks = (int)((R + 16 * p.rt - 1) / (16 * p.rt));
+  const long heads = B * nkv * p.blocks, want = 512;
+  long splits = (want + heads - 1) / heads;
+  splits = splits < 1 ? 1 : splits;
+  p.tps = (int)((tiles + splits - 1) / splits + 3) / 4 * 4;
+  p.splits = (int)((tiles + p.tps - 1) / p.tps);
+  return p;
 }
 
 bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -187,7 +566,9 @@ extern "C" int hn_tree_append(const void* qkv, long ld_qkv, const float* cos_t, 
 
 // See include/hn_int4.h.
 extern "C" long hn_tree_attention_workspace_bytes(long B, long nkv, long rep, long S, long bound) {
-  return 0;
+  if (B <= 0 || nkv <= 0 || rep <= 0 || S <= 0 || bound <= 0) return 0;
+  const Plan p = plan_of(B, nkv, rep, S, bound);
+  return p.splits == 1 ? 0 : B * nkv * p.splits * rep * S * (kHd + 2) * 4;
 }
 
 // See include/hn_int4.h.
@@ -206,12 +587,27 @@ extern "C" int hn_tree_attention(const void* q, const void* kt, const void* v, l
   HN_ARG_CHECK(al16(q) && al16(kt) && al16(v) && al16(out) && ld_o % 8 == 0 &&
                    ld_o >= nkv * rep * hd && lens && seen,
                "%s: operands must be 16-byte aligned, ld_o >= heads * %d", who, kHd);
-  const long rows = B * nkv * rep * S;
-  HN_ARG_CHECK(rows < (1L << 31), "%s: too many rows", who);
-  hipLaunchKernelGGL(attend_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0,
-                     (hipStream_t)stream, (const h16*)q, (const h16*)kt, (const h16*)v, max_len, lens,
-                     seen, (int)trees, rows, (int)nkv, (int)rep, (int)S, bound, scale, (h16*)out,
-                     ld_o);
+  const Plan p = plan_of(B, nkv, rep, S, bound);
+  const long units = B * nkv * p.splits, rows = B * nkv * rep * S;
+  HN_ARG_CHECK(rows < (1L << 31) && (units + 7) / 8 * 8 * p.blocks < (1L << 31),
+               "%s: too many rows", who);
+  const long need = hn_tree_attention_workspace_bytes(B, nkv, rep, S, bound);
+  HN_ARG_CHECK(need == 0 || (work && al16(work) && work_bytes >= need),
+               "%s: needs a 16-byte aligned workspace of %ld bytes (got %ld)", who, need,
+               work_bytes);
+  const Attend A = {(const h16*)q, (const h16*)kt, (const h16*)v, lens, seen, (h16*)out,
+                    (float*)work, max_len, bound, ld_o, (int)trees, (int)nkv, (int)rep, (int)S,
+                    (int)(rep * S), p.blocks, p.splits, p.tps, (int)units, scale};
+  const dim3 grid((unsigned)((units + 7) / 8 * 8 * p.blocks));
+  hipStream_t st = (hipStream_t)stream;
+  if (p.rt == 1)
+    hipLaunchKernelGGL(attend_kernel<1>, grid, dim3(256), 0, st, A);
+  else
+    hipLaunchKernelGGL(attend_kernel<2>, grid, dim3(256), 0, st, A);
   HN_LAUNCH_CHECK(who);
+  if (p.splits > 1) {
+    hipLaunchKernelGGL(join_kernel, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, A, rows);
+    HN_LAUNCH_CHECK(who);
+  }
   return 0;
 }
