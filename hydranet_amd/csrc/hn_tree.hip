@@ -7,6 +7,7 @@
 // at cache position C + i, its rotary position is C + depth(i), and it sees
 // positions [0, C) and those of itself and its ancestors.
 #include "hn_common.h"
+#include "hn_lds_dma.h"
 
 namespace {
 
@@ -112,6 +113,7 @@ __global__ __launch_bounds__(kHd) void append_kernel(
 // of a tile (4 of K, then 4 of V) is replaced by block s + 4 once it is used.
 constexpr int kPos = 128;     // positions per tile
 constexpr int kOPad = kHd + 4;
+constexpr uint32_t kNone = 0xfffff000u;  // an offset past any descriptor: reads zero, no access
 constexpr float kLog2e = 1.4426950408889634f;
 // Probabilities are 2^8 times the softmax's, relative to a maximum that follows
 // the true one only when it lags by 2^6: below 2^14, so fp16 holds them, and
@@ -153,9 +155,17 @@ __device__ __forceinline__ half8_t column(const u32x4 r[8]) {
   return __builtin_bit_cast(half8_t, w);
 }
 
-// max without the canonicalising multiply that fmaxf has on a product's result
-__device__ __forceinline__ float larger(float a, float b) {
-  return __builtin_amdgcn_fmed3f(a, b, __builtin_inff());
+// max over the four lanes, 16 apart, that hold one row.  (The swapped pair goes
+// through scalars: a bit cast of a vector's element takes element 0.)
+__device__ __forceinline__ float row_max(float x) {
+  const uint32_t w = __builtin_bit_cast(uint32_t, x);
+  const auto a = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+  const uint32_t a0 = a[0], a1 = a[1];
+  x = fmaxf(__builtin_bit_cast(float, a0), __builtin_bit_cast(float, a1));
+  const uint32_t v = __builtin_bit_cast(uint32_t, x);
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  const uint32_t b0 = b[0], b1 = b[1];
+  return fmaxf(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
 }
 
 // Bits [at, at + 32) of what a node sees, positions before its tree (at < 0) all
@@ -176,29 +186,120 @@ __device__ __forceinline__ uint32_t odd_mask(uint32_t w) {
          ((w & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u);
 }
 
-template <int RT>
-__global__ __launch_bounds__(256, 1) void attend_kernel(Attend A) {
+// A workgroup's share of the work.  The row blocks of one (head, range) follow
+// each other on one XCD, whose L2 then serves all but the first.
+struct Where {
+  int bg, b, g, split, row0, tree, tiles, first, end;
+  long C, L;
+  bool run;   // the sequence takes part and is within the bound
+  bool none;  // nothing to do, nothing to write
+};
+__device__ __forceinline__ Where where_of(const Attend& A, int rows) {
+  Where W;
+  const int id = blockIdx.x, grp = id / (8 * A.blocks), in = id - grp * 8 * A.blocks;
+  const int unit = 8 * grp + (in & 7);
+  W.bg = unit / A.splits, W.split = unit - W.bg * A.splits;
+  W.b = W.bg / A.nkv, W.g = W.bg - W.b * A.nkv;
+  W.row0 = (in >> 3) * rows;
+  W.none = unit >= A.units;
+  if (W.none) return W;
+  W.C = A.lens[W.b], W.L = W.C + A.S;
+  W.tree = A.trees > 1 ? W.b : 0;
+  W.run = W.C >= 0 && W.L <= A.bound;
+  W.tiles = W.run ? (int)((W.L + kPos - 1) / kPos) : 0;
+  W.first = W.split * A.tps;
+  W.end = W.first + A.tps < W.tiles ? W.first + A.tps : W.tiles;
+  W.none = W.run ? W.first >= W.tiles : W.split > 0;
+  return W;
+}
+
+// The sums of 16 rows of each of RG row groups, PG waves each, joined: wave rg *
+// PG + pg has left them in s_o, s_m and s_l.  Then the rows themselves where the
+// sequence has this one range, else the range's sums.  `t`: which 16 of a
+// group's `per` rows.
+template <int RG, int PG>
+__device__ __forceinline__ void finish(const Attend& A, const Where& W, const float* s_o,
+                                       const float* s_m, const float* s_l, int t, int per) {
+  const bool whole = W.tiles <= A.tps;
+  for (int i = threadIdx.x; i < RG * 256; i += 64 * RG * PG) {
+    const int rr = (i >> 4) & 15, w0 = (i >> 8) * PG, d = 8 * (i & 15);
+    const int row = W.row0 + (i >> 8) * per + 16 * t + rr;
+    if (row >= A.R) continue;
+    float m = -__builtin_inff();
+#pragma unroll
+    for (int w = 0; w < PG; ++w) m = fmaxf(m, s_m[(w0 + w) * per + 16 * t + rr]);
+    const float ref = m == -__builtin_inff() ? 0.f : m;
+    float sum = 0.f, x[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x[k] = 0.f;
+#pragma unroll
+    for (int w = 0; w < PG; ++w) {
+      // a wave without tiles has sums of zero and weight exp2(-inf) = 0
+      const float al = __builtin_amdgcn_exp2f(s_m[(w0 + w) * per + 16 * t + rr] - ref);
+      const float* ow = s_o + ((w0 + w) * 16 + rr) * kOPad + d;
+      sum += al * s_l[(w0 + w) * per + 16 * t + rr];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] += al * ow[k];
+    }
+    const int head = row / A.S, node = row - head * A.S;
+    if (whole) {
+      const bool live = W.C >= 0 && ((A.seen[((long)W.tree * A.S + node) * kWords + (node >> 6)] >>
+                                      (node & 63)) & 1);
+      const float is = !W.run ? __builtin_nanf("") : 1.f / sum;
+      half8_t y;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) y[k] = live ? (h16)(x[k] * is) : (h16)0.f;
+      *reinterpret_cast<half8_t*>(A.out + ((long)W.b * A.S + node) * A.ld_o +
+                                  (long)(W.g * A.rep + head) * kHd + d) = y;
+    } else {
+      const long at = ((long)W.bg * A.splits + W.split) * A.R + row;
+      float* pm = A.part + (long)A.units * A.R * kHd + at * 2;
+#pragma unroll
+      for (int k = 0; k < 8; k += 4)
+        *reinterpret_cast<float4v*>(A.part + at * kHd + d + k) =
+            float4v{x[k], x[k + 1], x[k + 2], x[k + 3]};
+      if ((i & 15) == 0) pm[0] = m, pm[1] = sum;
+    }
+  }
+}
+
+// NaN and infinities among the nodes' values, which the products leave out, added
+// to the rows that see them.  hd(k, r): the element that o[t][k][r] holds.
+template <int RT, typename F, typename G>
+__device__ __forceinline__ void add_odd(const Attend& A, const Where& W, int row0, int n,
+                                        float4v (&o)[RT][8], F hd, G mine) {
+  const h16* v = A.v + ((long)W.bg * A.max_len + W.C) * kHd;
+  for (int a = 0; a < A.S; ++a) {
+    if (!mine(W.C + a)) continue;
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      const int row = row0 + 16 * t + n;
+      const int node = row < A.R ? row % A.S : 0;
+      const bool vis = (A.seen[((long)W.tree * A.S + node) * kWords + (a >> 6)] >> (a & 63)) & 1;
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float x = (float)v[(long)a * kHd + hd(k, r)];
+          if (vis && !(__builtin_fabsf(x) < __builtin_inff())) o[t][k][r] += x;
+        }
+    }
+  }
+}
+
+template <int RT, int D, int OCC>
+__global__ __launch_bounds__(256, OCC) void attend_kernel(Attend A) {
   constexpr int kRows = 16 * RT;
-  __shared__ __align__(16) float s_o[4][16][kOPad];
-  __shared__ float s_m[4][kRows], s_l[4][kRows];
+  __shared__ __align__(16) float s_o[4 * 16 * kOPad];
+  __shared__ float s_m[4 * kRows], s_l[4 * kRows];
   __shared__ u32x4 s_q[RT][4][64];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, kg = lane >> 4;
-  // the row blocks of one (head, range) follow each other on one XCD, whose L2
-  // then serves all but the first
-  const int id = blockIdx.x, grp = id / (8 * A.blocks), in = id - grp * 8 * A.blocks;
-  const int unit = 8 * grp + (in & 7), block = in >> 3;
-  if (unit >= A.units) return;
-  const int bg = unit / A.splits, split = unit - bg * A.splits;
-  const int b = bg / A.nkv, g = bg - b * A.nkv;
-  const int row0 = block * kRows;
-  const long C = A.lens[b], L = C + A.S;
-  const int tree = A.trees > 1 ? b : 0;
-  const bool run = C >= 0 && L <= A.bound;
-  const int tiles = run ? (int)((L + kPos - 1) / kPos) : 0;
-  const int first = split * A.tps, end = first + A.tps < tiles ? first + A.tps : tiles;
-  if (run ? first >= tiles : split > 0) return;
+  const Where W = where_of(A, kRows);
+  if (W.none) return;
+  const int bg = W.bg, tree = W.tree, end = W.end, row0 = W.row0;
+  const long C = W.C, L = W.L;
 
   // queries, as each lane's operands: rows past the last are zero
   for (int t = wave; t < RT; t += 4) {
@@ -206,7 +307,7 @@ __global__ __launch_bounds__(256, 1) void attend_kernel(Attend A) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       u32x4 w = {0, 0, 0, 0};
-      if (row < A.R && run)
+      if (row < A.R && W.run)
         w = *reinterpret_cast<const u32x4*>(A.q + ((long)bg * A.R + row) * kHd + 32 * u + 8 * kg);
       s_q[t][u][lane] = w;
     }
@@ -215,13 +316,10 @@ __global__ __launch_bounds__(256, 1) void attend_kernel(Attend A) {
 
   const long slab = (long)bg * kHd * A.max_len;
   const uint32_t pitch = (uint32_t)A.max_len * 2;  // bytes of a row of keys
-  const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc(
-      (void*)(A.kt + slab), (short)0, (int)(pitch * kHd), 0x00020000);
-  const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc(
-      (void*)(A.v + slab), (short)0, (int)(pitch * kHd), 0x00020000);
-  constexpr uint32_t kNone = 0xfffff000u;  // past both: reads zero, without an access
+  const __amdgpu_buffer_rsrc_t rk = rsrc(A.kt + slab, (int)(pitch * kHd));
+  const __amdgpu_buffer_rsrc_t rv = rsrc(A.v + slab, (int)(pitch * kHd));
 
-  u32x4 ring[4][8];
+  u32x4 ring[D][8];
   // keys 32 u + 8 kg + r at positions p0 + 8 n on; a vector past the row's end
   // (its positions are past the sequence) reads the row's last instead.  The
   // lane's part of the address is one register, the rest a scalar that is
@@ -238,14 +336,18 @@ __global__ __launch_bounds__(256, 1) void attend_kernel(Attend A) {
       x[r] = __builtin_bit_cast(
           u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, (int)at, (int)so, 0));
   };
-  // values of positions p0 + 32 kg + 8 t + j at elements 8 n on.  The lane's
-  // part, j and t share no bit, so j is the instruction's own offset.
+  // values of positions p0 + 32 kg + 8 t + j at elements 8 n on.  j has bits of
+  // its own in the lane's part of the address, so it is the instruction's offset.
+  const int vlane = (kg << 13) | (n << 4);
   auto load_v = [&](u32x4 (&x)[8], int tile, int t) {
     const int so = tile * (kPos * kHd * 2) + t * (8 * kHd * 2);
+    int at = vlane;
+    asm volatile("" : "+v"(at));
+    at &= ~0x700;
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      x[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(
-                                           rv, (kg << 13) | (n << 4) | (j << 8), so, 0));
+      x[j] = __builtin_bit_cast(
+          u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, at | (j << 8), so, 0));
   };
   // the same of a sequence's last tiles: past its end, zero (their probabilities
   // are, and what a longer sequence left there may be anything)
@@ -272,12 +374,25 @@ __global__ __launch_bounds__(256, 1) void attend_kernel(Attend A) {
 #pragma unroll
   for (int i = 0; i < 8; ++i) ones[i] = (h16)1.f;
 
-  int tile = first + wave;
+  int tile = W.first + wave;
 #pragma unroll
-  for (int u = 0; u < 4; ++u) load_k(ring[u], tile, u);
+  for (int u = 0; u < D; ++u) load_k(ring[u], tile, u);
+  uint32_t any_odd = 0;
   // EDGE: a tile that holds nodes, or positions past the sequence
   auto walk = [&](auto edge_tile) {
     constexpr bool EDGE = decltype(edge_tile)::value;
+    // block c of the tile is used: block c + D, of the next tile's keys past 8
+    auto next = [&](int c) {
+      const int a = c + D;
+      if (a < 4)
+        load_k(ring[c % D], tile, a);
+      else if (a >= 8)
+        load_k(ring[c % D], tile + 4, a - 8);
+      else if constexpr (EDGE)
+        load_v_end(ring[c % D], tile, a - 4);
+      else
+        load_v(ring[c % D], tile, a - 4);
+    };
     float4v s[RT][8];
 #pragma unroll
     for (int t = 0; t < RT; ++t)
@@ -285,7 +400,7 @@ __global__ __launch_bounds__(256, 1) void attend_kernel(Attend A) {
       for (int j = 0; j < 8; ++j) s[t][j] = (float4v)(0.f);
 #define HN_QK(J)                                                                                 \
   {                                                                                              \
-    const half8_t a = column<J>(ring[u]);                                                        \
+    const half8_t a = column<J>(ring[u % D]);                                                        \
     _Pragma("unroll") for (int t = 0; t < RT; ++t) s[t][J] =                                     \
         __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q[t], s[t][J], 0, 0, 0);                       \
   }
@@ -304,10 +419,7 @@ __global__ __launch_bounds__(256, 1) void attend_kernel(Attend A) {
       __builtin_amdgcn_sched_barrier(0);
       HN_QK(6) HN_QK(7)
       __builtin_amdgcn_sched_barrier(0);
-      if constexpr (EDGE)
-        load_v_end(ring[u], tile, u);
-      else
-        load_v(ring[u], tile, u);
+      next(u);
       __builtin_amdgcn_sched_barrier(0);
     }
 #undef HN_QK
@@ -329,9 +441,8 @@ __global__ __launch_bounds__(256, 1) void attend_kernel(Attend A) {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) tm = larger(tm, s[t][j][r]);
-      tm = fmaxf(tm, __shfl_xor(tm, 16, 64));
-      tm = fmaxf(tm, __shfl_xor(tm, 32, 64)) * scale;
+        for (int r = 0; r < 4; ++r) tm = fmaxf(tm, s[t][j][r]);
+      tm = row_max(tm) * scale;
       if (__any(tm > mx[t] + kLag)) {
         const float nm = fmaxf(mx[t], tm);
         const float al = nm == mx[t] ? 1.f : __builtin_amdgcn_exp2f(mx[t] - nm);
@@ -351,25 +462,25 @@ __global__ __launch_bounds__(256, 1) void attend_kernel(Attend A) {
     }
 #define HN_PV(E)                                                                                 \
   {                                                                                              \
-    const half8_t a = column<E>(ring[u]);                                                        \
+    const half8_t a = column<E>(ring[u % D]);                                                        \
     _Pragma("unroll") for (int t = 0; t < RT; ++t) o[t][E] =                                     \
         __builtin_amdgcn_mfma_f32_16x16x32_f16(a, p[t][u], o[t][E], 0, 0, 0);                    \
   }
-    uint32_t any_odd = 0;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       if constexpr (EDGE) {
         // a node's value that is no number must not reach, as 0 times it, the
-        // rows that do not see it: taken out here, added to the others below
+        // rows that do not see it: taken out here, added to the others at the end
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const bool node = p0 + 32 * kg + 8 * u + j >= C;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const uint32_t w = ring[u][j][i], m = node ? odd_mask(w) : 0u;
+            const uint32_t w = ring[u % D][j][i], m = node ? odd_mask(w) : 0u;
             any_odd |= m;
-            ring[u][j][i] = w & ~m;
+            ring[u % D][j][i] = w & ~m;
           }
+          asm volatile("" : "+v"(any_odd));  // now, not from kept masks at the end
         }
       }
 #pragma unroll
@@ -383,89 +494,276 @@ __global__ __launch_bounds__(256, 1) void attend_kernel(Attend A) {
       __builtin_amdgcn_sched_barrier(0);
       HN_PV(6) HN_PV(7)
       __builtin_amdgcn_sched_barrier(0);
-      load_k(ring[u], tile + 4, u);
+      next(4 + u);
       __builtin_amdgcn_sched_barrier(0);
     }
 #undef HN_PV
-    if (EDGE && __any(any_odd != 0)) {
-      const long a0 = p0 > C ? p0 - C : 0, a1 = p0 + kPos - C < A.S ? p0 + kPos - C : A.S;
-      for (long a = a0; a < a1; ++a) {
-        const h16* vr = A.v + slab + (C + a) * kHd + 32 * kg;
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-          const int row = row0 + 16 * t + n;
-          const int node = row < A.R ? row % A.S : 0;
-          const bool vis = (A.seen[((long)tree * A.S + node) * kWords + (a >> 6)] >> (a & 63)) & 1;
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float x = (float)vr[8 * r + e];
-              if (vis && !(__builtin_fabsf(x) < __builtin_inff())) o[t][e][r] += x;
-            }
-        }
-      }
-    }
   };
   const int inner = (int)(C / kPos) < end ? (int)(C / kPos) : end;  // tiles all rows see whole
   for (; tile < inner; tile += 4) walk(Bool<false>{});
   for (; tile < end; tile += 4) walk(Bool<true>{});
+  if (__any(any_odd != 0))  // rare
+    add_odd<RT>(A, W, row0, n, o, [&](int e, int r) { return 32 * kg + 8 * r + e; },
+                [&](long p) {
+                  const int at = (int)(p / kPos);
+                  return at >= W.first && at < end && ((at - W.first) & 3) == wave;
+                });
 
-  // The waves' sums joined, 16 rows at a time; then the rows themselves where
-  // this is the sequence's only range, else this range's sums.
   if (kg == 0)
 #pragma unroll
-    for (int t = 0; t < RT; ++t) s_m[wave][16 * t + n] = mx[t], s_l[wave][16 * t + n] = l[t][0];
-  const bool whole = tiles <= A.tps;
+    for (int t = 0; t < RT; ++t)
+      s_m[wave * kRows + 16 * t + n] = mx[t], s_l[wave * kRows + 16 * t + n] = l[t][0];
 #pragma unroll
   for (int t = 0; t < RT; ++t) {
     if (t) __syncthreads();
 #pragma unroll
     for (int r = 0; r < 4; ++r)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float4v w = {o[t][4 * h][r], o[t][4 * h + 1][r], o[t][4 * h + 2][r],
-                           o[t][4 * h + 3][r]};
-        *reinterpret_cast<float4v*>(&s_o[wave][n][32 * kg + 8 * r + 4 * h]) = w;
-      }
+      for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<float4v*>(s_o + (wave * 16 + n) * kOPad + 32 * kg + 8 * r + 4 * h) =
+            float4v{o[t][4 * h][r], o[t][4 * h + 1][r], o[t][4 * h + 2][r], o[t][4 * h + 3][r]};
     __syncthreads();
-    const int rr = tid >> 4, d = 8 * (tid & 15), row = row0 + 16 * t + rr;
-    if (row < A.R) {
-      float m = s_m[0][16 * t + rr];
+    finish<1, 4>(A, W, s_o, s_m, s_l, t, kRows);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Many rows per KV head: the tiles of K and V shared through LDS.  8 waves, RG
+// groups of 32 rows by PG parts of a stage of SP = WP * PG positions.  A stage
+// of keys [128 hd][SP] and values [SP][128 hd] goes from memory to LDS as it lies
+// (buffer_load ... lds), D - 1 stages ahead, and ds_read_b64_tr_b16 turns it on
+// the way to the registers: 16 lanes read 4 rows of 16 halves, and lane i gets
+// column i.  The operands' layouts are the MFMA's own: a lane's scores are
+// positions 16 j + 4 kg + r of its part, of row lane % 16, and with the values'
+// rows taken as {4 kg + r, 16 + 4 kg + r} they are the second product's operand
+// as they are.
+//
+// Both transposing reads take 32 bytes of each of 16 rows; a row's 16-byte chunks
+// are stored at chunk ^ (2 * key(row)), so that the 8 rows that half a wave reads
+// cover the 64 banks once.
+template <int SP>
+__device__ __forceinline__ int key_of_k(int hd) {
+  return SP == 64 ? ((hd >> 1) & 1) | ((hd >> 2) & 2) : (hd & 3) | ((hd >> 1) & 4);
+}
+
+typedef short short4v __attribute__((ext_vector_type(4)));
+
+// Two transposing reads: columns of 4 rows each, 8 halves of one column per lane.
+__device__ __forceinline__ half8_t read_tr(uint32_t at, int lo, int hi) {
+  typedef __attribute__((address_space(3))) short4v* P;
+  __attribute__((address_space(3))) char* base = (__attribute__((address_space(3))) char*)nullptr + at;
+  const short4v a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(base + lo));
+  const short4v b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(base + hi));
+  return __builtin_bit_cast(
+      half8_t, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+template <int RG, int PG, int WP, int D>
+__global__ __launch_bounds__(512, 2) void share_kernel(Attend A) {
+  constexpr int RT = 2, SP = WP * PG, JB = WP / 16;
+  constexpr int kKBytes = SP * kHd * 2, kStage = 2 * kKBytes;
+  constexpr int kDma = SP / 4 / 8;  // DMA instructions per wave and operand of a stage
+  static_assert(RG * PG == 8 && (SP == 64 || SP == 128), "");
+  constexpr int kSum = 8 * 16 * kOPad * 4;
+  __shared__ __align__(1024) unsigned char s_buf[D * kStage > kSum ? D * kStage : kSum];
+  __shared__ float s_m[8 * 16 * RT], s_l[8 * 16 * RT];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = lane & 15, kg = lane >> 4, rg = wave / PG, pg = wave - rg * PG;
+  const Where W = where_of(A, 32 * RG);
+  if (W.none) return;
+  const int row0 = W.row0 + 32 * rg;  // this wave's rows
+
+  half8_t q[RT][4];
 #pragma unroll
-      for (int w = 1; w < 4; ++w) m = fmaxf(m, s_m[w][16 * t + rr]);
-      const float ref = m == -__builtin_inff() ? 0.f : m;
-      float sum = 0.f, x[8];
+  for (int t = 0; t < RT; ++t) {
+    const int row = row0 + 16 * t + n;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = 0.f;
+    for (int u = 0; u < 4; ++u) {
+      u32x4 w = {0, 0, 0, 0};
+      if (row < A.R && W.run)
+        w = *reinterpret_cast<const u32x4*>(A.q + ((long)W.bg * A.R + row) * kHd + 32 * u + 8 * kg);
+      q[t][u] = __builtin_bit_cast(half8_t, w);
+    }
+  }
+
+  const long slab = (long)W.bg * kHd * A.max_len;
+  const uint32_t pitch = (uint32_t)A.max_len * 2;
+  const __amdgpu_buffer_rsrc_t rk = rsrc(A.kt + slab, (int)(pitch * kHd));
+  const __amdgpu_buffer_rsrc_t rv = rsrc(A.v + slab, (int)(pitch * kHd));
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)s_buf;
+
+  // DMA: instruction i of wave w moves bytes 1024 (w + 8 i) on of a stage's keys
+  // and of its values; the lane's part of the addresses is the same for all i
+  constexpr int kRowK = 1024 / (2 * SP), kChunks = SP / 8;  // rows of keys per instruction
+  const int kr = lane / kChunks, vr = lane >> 4;
+  const int kc = (lane % kChunks) ^ (2 * key_of_k<SP>(kRowK * wave + kr));
+  const uint32_t kat = (uint32_t)kr * pitch + 16 * kc;
+  const uint32_t vat = vr * (kHd * 2) + 16 * ((lane & 15) ^ (2 * ((4 * wave + vr) & 7)));
+  const int stages = kPos / SP * (W.end - W.first);
+  // positions past the sequence read as zero: their probabilities are, and what a
+  // longer sequence left there may be anything
+  auto issue = [&](int st) {
+    const long p0 = (long)W.first * kPos + (long)st * SP;
+    const uint32_t at = lds0 + (uint32_t)(st % D) * kStage + wave * 1024;
+    const uint32_t ka = st < stages && p0 + 8 * kc < W.L ? kat : kNone;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float mw = s_m[w][16 * t + rr];
-        // a wave without tiles has sums of zero and weight exp2(-inf) = 0
-        const float al = __builtin_amdgcn_exp2f(mw - ref);
-        sum += al * s_l[w][16 * t + rr];
+    for (int i = 0; i < kDma; ++i) {
+      const int qi = wave + 8 * i;
+      dma_b128(rk, ka, (uint32_t)(kRowK * qi) * pitch + 2 * (uint32_t)p0, at + i * 8192);
+    }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] += al * s_o[w][rr][d + i];
-      }
-      const int head = row / A.S, node = row - head * A.S;
-      if (whole) {
-        const bool live = C >= 0 && ((A.seen[((long)tree * A.S + node) * kWords + (node >> 6)] >>
-                                      (node & 63)) & 1);
-        const float is = !run ? __builtin_nanf("") : 1.f / sum;
-        half8_t y;
+    for (int i = 0; i < kDma; ++i) {
+      const int qi = wave + 8 * i;
+      const uint32_t va = st < stages && p0 + 4 * qi + vr < W.L ? vat : kNone;
+      dma_b128(rv, va, ((uint32_t)p0 + 4 * qi) * (kHd * 2), at + kKBytes + i * 8192);
+    }
+  };
+
+  // this lane's part of the reads: 8 bytes of row (lane % 16) / 4 of a group's 4
+  const int rr = n >> 2, half = 16 * ((n & 3) >> 1) + 8 * (n & 1);
+  uint32_t k_at[JB], v_at[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = live ? (h16)(x[i] * is) : (h16)0.f;
-        *reinterpret_cast<half8_t*>(A.out + ((long)b * A.S + node) * A.ld_o +
-                                    (long)(g * A.rep + head) * kHd + d) = y;
-      } else {
-        float* po = A.part + (((long)bg * A.splits + split) * A.R + row) * kHd + d;
-        float* pm = A.part + (long)A.units * A.R * kHd + (((long)bg * A.splits + split) * A.R + row) * 2;
+  for (int j = 0; j < JB; ++j)
+    k_at[j] = lds0 + (8 * kg + rr) * (2 * SP) + half +
+              32 * ((pg * JB + j) ^ key_of_k<SP>(8 * kg + rr));
 #pragma unroll
-        for (int i = 0; i < 8; i += 4)
-          *reinterpret_cast<float4v*>(po + i) = float4v{x[i], x[i + 1], x[i + 2], x[i + 3]};
-        if ((tid & 15) == 0) pm[0] = m, pm[1] = sum;
+  for (int e = 0; e < 8; ++e)
+    v_at[e] = lds0 + kKBytes + (pg * WP + 4 * kg + rr) * (kHd * 2) + half +
+              32 * (e ^ ((4 * kg + rr) & 7));
+
+  float4v o[RT][8], l[RT];
+  float mx[RT];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    mx[t] = -__builtin_inff();
+    l[t] = (float4v)(0.f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[t][e] = (float4v)(0.f);
+  }
+  const float scale = A.scale * kLog2e;
+  half8_t ones;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ones[i] = (h16)1.f;
+  uint32_t any_odd = 0;
+
+  auto walk = [&](auto edge_stage, long p0, uint32_t at) {
+    constexpr bool EDGE = decltype(edge_stage)::value;
+    float4v s[RT][JB];
+#pragma unroll
+    for (int j = 0; j < JB; ++j) {
+#pragma unroll
+      for (int t = 0; t < RT; ++t) s[t][j] = (float4v)(0.f);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const half8_t a = read_tr(k_at[j] + at, u * 32 * 2 * SP, u * 32 * 2 * SP + 4 * 2 * SP);
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+          s[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q[t][u], s[t][j], 0, 0, 0);
       }
     }
+    half8_t p[RT][JB / 2];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+      if constexpr (EDGE) {
+        const int row = row0 + 16 * t + n;
+        const int node = row < A.R ? row % A.S : 0;
+        const u64* see = A.seen + ((long)W.tree * A.S + node) * kWords;
+#pragma unroll
+        for (int x = 0; x < JB / 2; ++x) {
+          const uint32_t w = window(see, p0 + 32 * x + 4 * kg - W.C);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if (!((w >> r) & 1u)) s[t][2 * x][r] = -__builtin_inff();
+            if (!((w >> (16 + r)) & 1u)) s[t][2 * x + 1][r] = -__builtin_inff();
+          }
+        }
+      }
+      float tm = s[t][0][0];
+#pragma unroll
+      for (int j = 0; j < JB; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) tm = fmaxf(tm, s[t][j][r]);
+      tm = row_max(tm) * scale;
+      if (__any(tm > mx[t] + kLag)) {
+        const float nm = fmaxf(mx[t], tm);
+        const float al = nm == mx[t] ? 1.f : __builtin_amdgcn_exp2f(mx[t] - nm);
+        l[t] *= al;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[t][e] *= al;
+        mx[t] = nm;
+      }
+      const float ref = mx[t] == -__builtin_inff() ? 0.f : mx[t] - kUp;
+#pragma unroll
+      for (int j = 0; j < JB; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          p[t][j >> 1][4 * (j & 1) + r] =
+              (h16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j][r], scale, -ref));
+    }
+#pragma unroll
+    for (int x = 0; x < JB / 2; ++x) {
+#pragma unroll
+      for (int t = 0; t < RT; ++t)
+        l[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, p[t][x], l[t], 0, 0, 0);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        half8_t a = read_tr(v_at[e] + at, x * 32 * kHd * 2, x * 32 * kHd * 2 + 16 * kHd * 2);
+        if constexpr (EDGE) {
+          // nodes' values that are no numbers: see add_odd
+          u32x4 w = __builtin_bit_cast(u32x4, a);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const long pos = p0 + 32 * x + 16 * (i >> 1) + 4 * kg + 2 * (i & 1);
+            const uint32_t node = (pos >= W.C ? 0xffffu : 0u) | (pos + 1 >= W.C ? 0xffff0000u : 0u);
+            const uint32_t m = odd_mask(w[i]) & node;
+            any_odd |= m;
+            w[i] &= ~m;
+          }
+          asm volatile("" : "+v"(any_odd));
+          a = __builtin_bit_cast(half8_t, w);
+        }
+#pragma unroll
+        for (int t = 0; t < RT; ++t)
+          o[t][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, p[t][x], o[t][e], 0, 0, 0);
+      }
+    }
+  };
+
+#pragma unroll
+  for (int st = 0; st < D - 1; ++st) issue(st);
+  for (int st = 0; st < stages; ++st) {
+    wait_vmcnt<2 * kDma*(D - 2)>();  // this wave's part of the stage has landed
+    stage_barrier();                 // everyone's, and the stage before is used
+    issue(st + D - 1);
+    const long p0 = (long)W.first * kPos + (long)st * SP;
+    const uint32_t at = (uint32_t)(st % D) * kStage;
+    if (p0 + SP <= W.C)
+      walk(Bool<false>{}, p0 + pg * WP, at);
+    else
+      walk(Bool<true>{}, p0 + pg * WP, at);
+  }
+  wait_vmcnt<0>();  // the reads past the end have written their zeros
+  __syncthreads();
+  if (__any(any_odd != 0))
+    add_odd<RT>(A, W, row0, n, o, [&](int e, int r) { return 16 * e + 4 * kg + r; },
+                [&](long p) {
+                  const int at = (int)(p / kPos);
+                  return at >= W.first && at < W.end && (int)(p / WP) % PG == pg;
+                });
+  float* s_o = reinterpret_cast<float*>(s_buf);
+  if (kg == 0)
+#pragma unroll
+    for (int t = 0; t < RT; ++t)
+      s_m[wave * 16 * RT + 16 * t + n] = mx[t], s_l[wave * 16 * RT + 16 * t + n] = l[t][0];
+#pragma unroll
+  for (int t = 0; t < RT; ++t) {
+    if (t) __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      *reinterpret_cast<float4v*>(s_o + (wave * 16 + n) * kOPad + 16 * e + 4 * kg) = o[t][e];
+    __syncthreads();
+    finish<RG, PG>(A, W, s_o, s_m, s_l, t, 16 * RT);
   }
 }
 
@@ -507,16 +805,16 @@ __global__ __launch_bounds__(256) void join_kernel(Attend A, long rows) {
                               (long)(g * A.rep + head) * kHd + d) = y;
 }
 
-// Row tiles per workgroup, and how the positions are split so that about two
-// rounds of workgroups fill the chip.
+// Which kernel, its rows per workgroup, and how the positions are split so that
+// about two rounds of workgroups fill the chip.
 struct Plan {
-  int rt, blocks, splits, tps;
+  int rows, blocks, splits, tps;
 };
 Plan plan_of(long B, long nkv, long rep, long S, long bound) {
   const long R = rep * S, tiles = (bound + kPos - 1) / kPos;
   Plan p;
-  p.rt = R <= 16 ? 1 : 2;
-  p.blocks = (int)((R + 16 * p.rt - 1) / (16 * p.rt));
+  p.rows = R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : R <= 128 ? 128 : 256;
+  p.blocks = (int)((R + p.rows - 1) / p.rows);
   const long heads = B * nkv * p.blocks, want = 512;
   long splits = (want + heads - 1) / heads;
   splits = splits < 1 ? 1 : splits;
@@ -600,10 +898,13 @@ extern "C" int hn_tree_attention(const void* q, const void* kt, const void* v, l
                     (int)(rep * S), p.blocks, p.splits, p.tps, (int)units, scale};
   const dim3 grid((unsigned)((units + 7) / 8 * 8 * p.blocks));
   hipStream_t st = (hipStream_t)stream;
-  if (p.rt == 1)
-    hipLaunchKernelGGL(attend_kernel<1>, grid, dim3(256), 0, st, A);
-  else
-    hipLaunchKernelGGL(attend_kernel<2>, grid, dim3(256), 0, st, A);
+  switch (p.rows) {
+    case 16: hipLaunchKernelGGL((attend_kernel<1, 4, 2>), grid, dim3(256), 0, st, A); break;
+    case 32: hipLaunchKernelGGL((attend_kernel<2, 4, 1>), grid, dim3(256), 0, st, A); break;
+    case 64: hipLaunchKernelGGL((share_kernel<2, 4, 32, 2>), grid, dim3(512), 0, st, A); break;
+    case 128: hipLaunchKernelGGL((share_kernel<4, 2, 64, 2>), grid, dim3(512), 0, st, A); break;
+    default: hipLaunchKernelGGL((share_kernel<8, 1, 64, 4>), grid, dim3(512), 0, st, A);
+  }
   HN_LAUNCH_CHECK(who);
   if (p.splits > 1) {
     hipLaunchKernelGGL(join_kernel, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, A, rows);
