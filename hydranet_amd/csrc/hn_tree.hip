@@ -170,11 +170,11 @@ __device__ __forceinline__ float row_max(float x) {
 
 // Bits [at, at + 32) of what a node sees, positions before its tree (at < 0) all
 // seen.
-__device__ __forceinline__ uint32_t window(const u64* see, long at) {
+__device__ __forceinline__ uint32_t window(const u64* see, int at) {
   if (at <= -32) return ~0u;
   if (at >= kMaxNodes) return 0u;
   if (at < 0) return (uint32_t)(see[0] << -at) | ((1u << -at) - 1u);
-  const int w = (int)(at >> 6), s = (int)(at & 63);
+  const int w = at >> 6, s = at & 63;
   u64 x = see[w] >> s;
   if (s > 32 && w + 1 < kWords) x |= see[w + 1] << (64 - s);
   return (uint32_t)x;
@@ -190,7 +190,7 @@ __device__ __forceinline__ uint32_t odd_mask(uint32_t w) {
 // each other on one XCD, whose L2 then serves all but the first.
 struct Where {
   int bg, b, g, split, row0, tree, tiles, first, end;
-  long C, L;
+  int C, L;   // cached positions (-1: none take part), and with the nodes
   bool run;   // the sequence takes part and is within the bound
   bool none;  // nothing to do, nothing to write
 };
@@ -203,10 +203,11 @@ __device__ __forceinline__ Where where_of(const Attend& A, int rows) {
   W.row0 = (in >> 3) * rows;
   W.none = unit >= A.units;
   if (W.none) return W;
-  W.C = A.lens[W.b], W.L = W.C + A.S;
+  const long C = A.lens[W.b];
+  W.run = C >= 0 && C + A.S <= A.bound;
+  W.C = C < 0 ? -1 : W.run ? (int)C : 0, W.L = W.C + A.S;
   W.tree = A.trees > 1 ? W.b : 0;
-  W.run = W.C >= 0 && W.L <= A.bound;
-  W.tiles = W.run ? (int)((W.L + kPos - 1) / kPos) : 0;
+  W.tiles = W.run ? (W.L + kPos - 1) / kPos : 0;
   W.first = W.split * A.tps;
   W.end = W.first + A.tps < W.tiles ? W.first + A.tps : W.tiles;
   W.none = W.run ? W.first >= W.tiles : W.split > 0;
@@ -299,7 +300,7 @@ __global__ __launch_bounds__(256, OCC) void attend_kernel(Attend A) {
   const Where W = where_of(A, kRows);
   if (W.none) return;
   const int bg = W.bg, tree = W.tree, end = W.end, row0 = W.row0;
-  const long C = W.C, L = W.L;
+  const int C = W.C, L = W.L;
 
   // queries, as each lane's operands: rows past the last are zero
   for (int t = wave; t < RT; t += 4) {
@@ -354,7 +355,7 @@ __global__ __launch_bounds__(256, OCC) void attend_kernel(Attend A) {
   auto load_v_end = [&](u32x4 (&x)[8], int tile, int t) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const long p = (long)tile * kPos + 32 * kg + 8 * t + j;
+      const int p = tile * kPos + 32 * kg + 8 * t + j;
       const uint32_t at = p < L ? (uint32_t)p * (kHd * 2) + 16 * n : kNone;
       x[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, (int)at, 0, 0));
     }
@@ -499,13 +500,13 @@ __global__ __launch_bounds__(256, OCC) void attend_kernel(Attend A) {
     }
 #undef HN_PV
   };
-  const int inner = (int)(C / kPos) < end ? (int)(C / kPos) : end;  // tiles all rows see whole
+  const int inner = C / kPos < end ? C / kPos : end;  // tiles all rows see whole
   for (; tile < inner; tile += 4) walk(Bool<false>{});
   for (; tile < end; tile += 4) walk(Bool<true>{});
   if (__any(any_odd != 0))  // rare
     add_odd<RT>(A, W, row0, n, o, [&](int e, int r) { return 32 * kg + 8 * r + e; },
-                [&](long p) {
-                  const int at = (int)(p / kPos);
+                [&](int p) {
+                  const int at = p / kPos;
                   return at >= W.first && at < end && ((at - W.first) & 3) == wave;
                 });
 
@@ -604,7 +605,7 @@ __global__ __launch_bounds__(512, 2) void share_kernel(Attend A) {
   // positions past the sequence read as zero: their probabilities are, and what a
   // longer sequence left there may be anything
   auto issue = [&](int st) {
-    const long p0 = (long)W.first * kPos + (long)st * SP;
+    const int p0 = W.first * kPos + st * SP;
     const uint32_t at = lds0 + (uint32_t)(st % D) * kStage + wave * 1024;
     const uint32_t ka = st < stages && p0 + 8 * kc < W.L ? kat : kNone;
 #pragma unroll
@@ -647,20 +648,29 @@ __global__ __launch_bounds__(512, 2) void share_kernel(Attend A) {
   for (int i = 0; i < 8; ++i) ones[i] = (h16)1.f;
   uint32_t any_odd = 0;
 
-  auto walk = [&](auto edge_stage, long p0, uint32_t at) {
+  auto walk = [&](auto edge_stage, int p0, uint32_t at) {
     constexpr bool EDGE = decltype(edge_stage)::value;
+    // operands are read one group of products ahead, no further: the scheduler
+    // would else fill the registers with them
     float4v s[RT][JB];
+    half8_t ka[2][4];
+    auto keys = [&](int j) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        ka[j & 1][u] = read_tr(k_at[j] + at, u * 32 * 2 * SP, u * 32 * 2 * SP + 4 * 2 * SP);
+    };
+    keys(0);
 #pragma unroll
     for (int j = 0; j < JB; ++j) {
+      if (j + 1 < JB) keys(j + 1);
 #pragma unroll
       for (int t = 0; t < RT; ++t) s[t][j] = (float4v)(0.f);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const half8_t a = read_tr(k_at[j] + at, u * 32 * 2 * SP, u * 32 * 2 * SP + 4 * 2 * SP);
+      for (int u = 0; u < 4; ++u)
 #pragma unroll
         for (int t = 0; t < RT; ++t)
-          s[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q[t][u], s[t][j], 0, 0, 0);
-      }
+          s[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[j & 1][u], q[t][u], s[t][j], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
     }
     half8_t p[RT][JB / 2];
 #pragma unroll
@@ -701,55 +711,68 @@ __global__ __launch_bounds__(512, 2) void share_kernel(Attend A) {
           p[t][j >> 1][4 * (j & 1) + r] =
               (h16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j][r], scale, -ref));
     }
+    constexpr int EB = 4;  // operands per group
+    half8_t va[2][EB];
+    auto values = [&](int i) {
+      const int x = i * EB / 8, e0 = i * EB % 8;
 #pragma unroll
-    for (int x = 0; x < JB / 2; ++x) {
+      for (int e = 0; e < EB; ++e)
+        va[i & 1][e] = read_tr(v_at[e0 + e] + at, x * 32 * kHd * 2, x * 32 * kHd * 2 + 16 * kHd * 2);
+    };
+    values(0);
 #pragma unroll
-      for (int t = 0; t < RT; ++t)
-        l[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, p[t][x], l[t], 0, 0, 0);
+    for (int i = 0; i < JB / 2 * 8 / EB; ++i) {
+      const int x = i * EB / 8, e0 = i * EB % 8;
+      if (i + 1 < JB / 2 * 8 / EB) values(i + 1);
+      if (e0 == 0)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        half8_t a = read_tr(v_at[e] + at, x * 32 * kHd * 2, x * 32 * kHd * 2 + 16 * kHd * 2);
+        for (int t = 0; t < RT; ++t)
+          l[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, p[t][x], l[t], 0, 0, 0);
+#pragma unroll
+      for (int e = 0; e < EB; ++e) {
+        half8_t a = va[i & 1][e];
         if constexpr (EDGE) {
           // nodes' values that are no numbers: see add_odd
           u32x4 w = __builtin_bit_cast(u32x4, a);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const long pos = p0 + 32 * x + 16 * (i >> 1) + 4 * kg + 2 * (i & 1);
+          for (int k = 0; k < 4; ++k) {
+            const int pos = p0 + 32 * x + 16 * (k >> 1) + 4 * kg + 2 * (k & 1);
             const uint32_t node = (pos >= W.C ? 0xffffu : 0u) | (pos + 1 >= W.C ? 0xffff0000u : 0u);
-            const uint32_t m = odd_mask(w[i]) & node;
+            const uint32_t m = odd_mask(w[k]) & node;
             any_odd |= m;
-            w[i] &= ~m;
+            w[k] &= ~m;
           }
           asm volatile("" : "+v"(any_odd));
           a = __builtin_bit_cast(half8_t, w);
         }
 #pragma unroll
         for (int t = 0; t < RT; ++t)
-          o[t][e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, p[t][x], o[t][e], 0, 0, 0);
+          o[t][e0 + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, p[t][x], o[t][e0 + e], 0, 0, 0);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
 
 #pragma unroll
   for (int st = 0; st < D - 1; ++st) issue(st);
-  for (int st = 0; st < stages; ++st) {
+  int st = 0;
+  auto stage = [&](auto edge_stage) {
     wait_vmcnt<2 * kDma*(D - 2)>();  // this wave's part of the stage has landed
     stage_barrier();                 // everyone's, and the stage before is used
     issue(st + D - 1);
-    const long p0 = (long)W.first * kPos + (long)st * SP;
-    const uint32_t at = (uint32_t)(st % D) * kStage;
-    if (p0 + SP <= W.C)
-      walk(Bool<false>{}, p0 + pg * WP, at);
-    else
-      walk(Bool<true>{}, p0 + pg * WP, at);
-  }
+    walk(edge_stage, W.first * kPos + st * SP + pg * WP, (uint32_t)(st % D) * kStage);
+  };
+  const int seen_whole = W.C / SP - W.first * (kPos / SP);  // stages before the nodes
+  const int inner = seen_whole < stages ? seen_whole : stages;
+  for (; st < inner; ++st) stage(Bool<false>{});
+  for (; st < stages; ++st) stage(Bool<true>{});
   wait_vmcnt<0>();  // the reads past the end have written their zeros
   __syncthreads();
   if (__any(any_odd != 0))
     add_odd<RT>(A, W, row0, n, o, [&](int e, int r) { return 16 * e + 4 * kg + r; },
-                [&](long p) {
-                  const int at = (int)(p / kPos);
-                  return at >= W.first && at < W.end && (int)(p / WP) % PG == pg;
+                [&](int p) {
+                  const int at = p / kPos;
+                  return at >= W.first && at < W.end && p / WP % PG == pg;
                 });
   float* s_o = reinterpret_cast<float*>(s_buf);
   if (kg == 0)
