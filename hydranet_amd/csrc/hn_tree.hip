@@ -134,7 +134,7 @@ struct Attend {
   h16* out;
   float* part;
   long max_len, bound, ld_o;
-  int trees, nkv, rep, S, R, blocks, splits, tps, units;
+  int trees, B, nkv, rep, S, R, blocks, grain, wgs;
   float scale;
 };
 
@@ -186,42 +186,123 @@ __device__ __forceinline__ uint32_t odd_mask(uint32_t w) {
          ((w & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u);
 }
 
-// A workgroup's share of the work.  The row blocks of one (head, range) follow
-// each other on one XCD, whose L2 then serves all but the first.
-struct Where {
-  int bg, b, g, split, row0, tree, tiles, first, end;
-  int C, L;   // cached positions (-1: none take part), and with the nodes
-  bool run;   // the sequence takes part and is within the bound
-  bool none;  // nothing to do, nothing to write
-};
-__device__ __forceinline__ Where where_of(const Attend& A, int rows) {
-  Where W;
-  const int id = blockIdx.x, grp = id / (8 * A.blocks), in = id - grp * 8 * A.blocks;
-  const int unit = 8 * grp + (in & 7);
-  W.bg = unit / A.splits, W.split = unit - W.bg * A.splits;
-  W.b = W.bg / A.nkv, W.g = W.bg - W.b * A.nkv;
-  W.row0 = (in >> 3) * rows;
-  W.none = unit >= A.units;
-  if (W.none) return W;
-  const long C = A.lens[W.b];
-  W.run = C >= 0 && C + A.S <= A.bound;
-  W.C = C < 0 ? -1 : W.run ? (int)C : 0, W.L = W.C + A.S;
-  W.tree = A.trees > 1 ? W.b : 0;
-  W.tiles = W.run ? (W.L + kPos - 1) / kPos : 0;
-  W.first = W.split * A.tps;
-  W.end = W.first + A.tps < W.tiles ? W.first + A.tps : W.tiles;
-  W.none = W.run ? W.first >= W.tiles : W.split > 0;
-  return W;
+// The work is cut into grains of `grain` positions of one (sequence, KV head), in
+// order, and workgroup w of wgs (A.wgs, or T if that is less) takes grains [w T /
+// wgs, (w + 1) T / wgs) of the T there are: each the same share whatever the sequences' lengths, which
+// only the device knows.  A share is one range of positions of one head or
+// several; a head's range that is not whole leaves its sums in the workspace,
+// in entry 2 w, or 2 w + 1 if it is not w's first, for join_kernel.  The row
+// blocks of a share follow each other on one XCD, whose L2 then serves all but
+// the first.
+__device__ __forceinline__ int grains_of(const Attend& A, int b) {
+  const long C = A.lens[b];
+  return C < 0 || C + A.S > A.bound ? 0 : (int)((C + A.S + A.grain - 1) / A.grain);
 }
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// Grains of one head of the sequences below `to`, by a wave.
+__device__ __forceinline__ int grains_below(const Attend& A, int to) {
+  int n = 0;
+  for (int b = threadIdx.x & 63; b < to; b += 64) n += grains_of(A, b);
+  for (int off = 32; off; off >>= 1) n += __shfl_xor(n, off, 64);
+  return uniform(n);
+}
+
+// A range of positions of one KV head: tiles [first, end).
+struct Where {
+  int bg, b, g, row0, tree, first, end;
+  int C, L;     // cached positions, and with the nodes
+  bool whole;   // all of the head's
+  long part;    // else its entry of the workspace
+};
+
+struct Share {
+  int w, block, b, g, at, n;  // next: grain `at` of the n of head g of sequence b
+  int left;                   // grains left
+  bool first;
+
+  __device__ bool begin(const Attend& A) {
+    const int id = blockIdx.x, grp = id / (8 * A.blocks), in = id - grp * 8 * A.blocks;
+    w = 8 * grp + (in & 7), block = in >> 3;
+    if (w >= A.wgs) return false;
+    const long T = (long)grains_below(A, A.B) * A.nkv;
+    const int wgs = T < A.wgs ? (int)T : A.wgs;  // each of these has a grain
+    first = true, b = 0, g = 0, at = 0, n = 0, left = 0;
+    if (w >= wgs) return true;
+    const int from = (int)(w * T / wgs);
+    left = (int)((w + 1) * T / wgs) - from;
+    const int lane = threadIdx.x & 63;
+    int base = 0;  // grains of one head of the sequences before
+    for (int c = 0; c < A.B; c += 64) {
+      const int t = c + lane < A.B ? grains_of(A, c + lane) : 0;
+      int sum = t;
+      for (int off = 1; off < 64; off <<= 1) {
+        const int x = __shfl_up(sum, off, 64);
+        if (lane >= off) sum += x;
+      }
+      const u64 past = __ballot((base + sum) * A.nkv > from);
+      if (past) {
+        const int l = __builtin_ctzll(past);
+        b = c + l;
+        n = __builtin_amdgcn_readlane(t, l);
+        const int in_b = from - (base + __builtin_amdgcn_readlane(sum, l) - n) * A.nkv;
+        g = in_b / n, at = in_b - g * n;
+        break;
+      }
+      base += __builtin_amdgcn_readlane(sum, 63);
+    }
+    return true;
+  }
+
+  __device__ bool next(const Attend& A, int rows, Where& W) {
+    if (left <= 0) return false;
+    while (at >= n) {  // the next head that has grains
+      at = 0;
+      if (n > 0 && ++g < A.nkv) break;
+      g = 0;
+      n = uniform(grains_of(A, ++b));
+    }
+    const int m = n - at < left ? n - at : left;
+    W.b = b, W.g = g, W.bg = b * A.nkv + g, W.row0 = block * rows;
+    W.tree = A.trees > 1 ? b : 0;
+    W.C = uniform((int)A.lens[b]), W.L = W.C + A.S;
+    const int per = A.grain / kPos, tiles = (W.L + kPos - 1) / kPos;
+    W.first = at * per;
+    W.end = W.first + m * per < tiles ? W.first + m * per : tiles;
+    W.whole = m == n;
+    W.part = 2 * (long)w + !first;
+    at += m, left -= m, first = false;
+    return true;
+  }
+
+  // Rows of the sequences that have no grains: zero, or NaN past the bound.
+  __device__ void rest(const Attend& A, int rows) {
+    for (int e = w; e < A.B; e += A.wgs) {
+      if (grains_of(A, e)) continue;
+      const u64* seen = A.seen + (A.trees > 1 ? (long)e * A.S : 0) * kWords;
+      const int cols = A.nkv * A.rep * (kHd / 8);
+      for (long i = (long)block * blockDim.x + threadIdx.x; i < (long)A.S * cols;
+           i += (long)A.blocks * blockDim.x) {
+        const int node = (int)(i / cols), col = (int)(i - (long)node * cols);
+        const bool live =
+            A.lens[e] >= 0 && ((seen[(long)node * kWords + (node >> 6)] >> (node & 63)) & 1);
+        half8_t y;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) y[k] = live ? (h16)__builtin_nanf("") : (h16)0.f;
+        *reinterpret_cast<half8_t*>(A.out + ((long)e * A.S + node) * A.ld_o + 8 * col) = y;
+      }
+    }
+  }
+};
 
 // The sums of 16 rows of each of RG row groups, PG waves each, joined: wave rg *
 // PG + pg has left them in s_o, s_m and s_l.  Then the rows themselves where the
-// sequence has this one range, else the range's sums.  `t`: which 16 of a
+// range is whole, else the range's sums.  `t`: which 16 of a
 // group's `per` rows.
 template <int RG, int PG>
 __device__ __forceinline__ void finish(const Attend& A, const Where& W, const float* s_o,
                                        const float* s_m, const float* s_l, int t, int per) {
-  const bool whole = W.tiles <= A.tps;
   for (int i = threadIdx.x; i < RG * 256; i += 64 * RG * PG) {
     const int rr = (i >> 4) & 15, w0 = (i >> 8) * PG, d = 8 * (i & 15);
     const int row = W.row0 + (i >> 8) * per + 16 * t + rr;
@@ -243,18 +324,18 @@ __device__ __forceinline__ void finish(const Attend& A, const Where& W, const fl
       for (int k = 0; k < 8; ++k) x[k] += al * ow[k];
     }
     const int head = row / A.S, node = row - head * A.S;
-    if (whole) {
-      const bool live = W.C >= 0 && ((A.seen[((long)W.tree * A.S + node) * kWords + (node >> 6)] >>
+    if (W.whole) {
+      const bool live = ((A.seen[((long)W.tree * A.S + node) * kWords + (node >> 6)] >>
                                       (node & 63)) & 1);
-      const float is = !W.run ? __builtin_nanf("") : 1.f / sum;
+      const float is = 1.f / sum;
       half8_t y;
 #pragma unroll
       for (int k = 0; k < 8; ++k) y[k] = live ? (h16)(x[k] * is) : (h16)0.f;
       *reinterpret_cast<half8_t*>(A.out + ((long)W.b * A.S + node) * A.ld_o +
                                   (long)(W.g * A.rep + head) * kHd + d) = y;
     } else {
-      const long at = ((long)W.bg * A.splits + W.split) * A.R + row;
-      float* pm = A.part + (long)A.units * A.R * kHd + at * 2;
+      const long at = W.part * A.R + row;
+      float* pm = A.part + 2 * (long)A.wgs * A.R * kHd + at * 2;
 #pragma unroll
       for (int k = 0; k < 8; k += 4)
         *reinterpret_cast<float4v*>(A.part + at * kHd + d + k) =
@@ -297,8 +378,9 @@ __global__ __launch_bounds__(256, OCC) void attend_kernel(Attend A) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, kg = lane >> 4;
-  const Where W = where_of(A, kRows);
-  if (W.none) return;
+  Share share;
+  if (!share.begin(A)) return;
+  for (Where W; share.next(A, kRows, W);) {
   const int bg = W.bg, tree = W.tree, end = W.end, row0 = W.row0;
   const int C = W.C, L = W.L;
 
@@ -308,7 +390,7 @@ __global__ __launch_bounds__(256, OCC) void attend_kernel(Attend A) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       u32x4 w = {0, 0, 0, 0};
-      if (row < A.R && W.run)
+      if (row < A.R)
         w = *reinterpret_cast<const u32x4*>(A.q + ((long)bg * A.R + row) * kHd + 32 * u + 8 * kg);
       s_q[t][u][lane] = w;
     }
@@ -526,13 +608,16 @@ __global__ __launch_bounds__(256, OCC) void attend_kernel(Attend A) {
     __syncthreads();
     finish<1, 4>(A, W, s_o, s_m, s_l, t, kRows);
   }
+  __syncthreads();  // the next range's waves write what the rows are read from
+  }
+  share.rest(A, kRows);
 }
 
 // ---------------------------------------------------------------------------
 // Many rows per KV head: the tiles of K and V shared through LDS.  8 waves, RG
 // groups of 32 rows by PG parts of a stage of SP = WP * PG positions.  A stage
 // of keys [128 hd][SP] and values [SP][128 hd] goes from memory to LDS as it lies
-// (buffer_load ... lds), D - 1 stages ahead, and ds_read_b64_tr_b16 turns it on
+// (buffer_load ... lds), two stages ahead, and ds_read_b64_tr_b16 turns it on
 // the way to the registers: 16 lanes read 4 rows of 16 halves, and lane i gets
 // column i.  The operands' layouts are the MFMA's own: a lane's scores are
 // positions 16 j + 4 kg + r of its part, of row lane % 16, and with the values'
@@ -571,8 +656,9 @@ __global__ __launch_bounds__(512, 2) void share_kernel(Attend A) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, kg = lane >> 4, rg = wave / PG, pg = wave - rg * PG;
-  const Where W = where_of(A, 32 * RG);
-  if (W.none) return;
+  Share share;
+  if (!share.begin(A)) return;
+  for (Where W; share.next(A, 32 * RG, W);) {
   const int row0 = W.row0 + 32 * rg;  // this wave's rows
 
   half8_t q[RT][4];
@@ -582,7 +668,7 @@ __global__ __launch_bounds__(512, 2) void share_kernel(Attend A) {
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       u32x4 w = {0, 0, 0, 0};
-      if (row < A.R && W.run)
+      if (row < A.R)
         w = *reinterpret_cast<const u32x4*>(A.q + ((long)W.bg * A.R + row) * kHd + 32 * u + 8 * kg);
       q[t][u] = __builtin_bit_cast(half8_t, w);
     }
@@ -648,8 +734,12 @@ __global__ __launch_bounds__(512, 2) void share_kernel(Attend A) {
   for (int i = 0; i < 8; ++i) ones[i] = (h16)1.f;
   uint32_t any_odd = 0;
 
-  auto walk = [&](auto edge_stage, int p0, uint32_t at) {
+  half8_t p[RT][JB / 2];
+  // scores and probabilities of a stage
+  auto scores = [&](auto edge_stage, int st) __attribute__((always_inline)) {
     constexpr bool EDGE = decltype(edge_stage)::value;
+    const int p0 = W.first * kPos + st * SP + pg * WP;
+    const uint32_t at = (uint32_t)(st % D) * kStage;
     // operands are read one group of products ahead, no further: the scheduler
     // would else fill the registers with them
     float4v s[RT][JB];
@@ -672,7 +762,6 @@ __global__ __launch_bounds__(512, 2) void share_kernel(Attend A) {
           s[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[j & 1][u], q[t][u], s[t][j], 0, 0, 0);
       __builtin_amdgcn_sched_barrier(0);
     }
-    half8_t p[RT][JB / 2];
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
       if constexpr (EDGE) {
@@ -711,19 +800,25 @@ __global__ __launch_bounds__(512, 2) void share_kernel(Attend A) {
           p[t][j >> 1][4 * (j & 1) + r] =
               (h16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j][r], scale, -ref));
     }
+  };
+  // its values, by those probabilities
+  auto values = [&](auto edge_stage, int st) __attribute__((always_inline)) {
+    constexpr bool EDGE = decltype(edge_stage)::value;
+    const int p0 = W.first * kPos + st * SP + pg * WP;
+    const uint32_t at = (uint32_t)(st % D) * kStage;
     constexpr int EB = 4;  // operands per group
     half8_t va[2][EB];
-    auto values = [&](int i) {
+    auto read = [&](int i) {
       const int x = i * EB / 8, e0 = i * EB % 8;
 #pragma unroll
       for (int e = 0; e < EB; ++e)
         va[i & 1][e] = read_tr(v_at[e0 + e] + at, x * 32 * kHd * 2, x * 32 * kHd * 2 + 16 * kHd * 2);
     };
-    values(0);
+    read(0);
 #pragma unroll
     for (int i = 0; i < JB / 2 * 8 / EB; ++i) {
       const int x = i * EB / 8, e0 = i * EB % 8;
-      if (i + 1 < JB / 2 * 8 / EB) values(i + 1);
+      if (i + 1 < JB / 2 * 8 / EB) read(i + 1);
       if (e0 == 0)
 #pragma unroll
         for (int t = 0; t < RT; ++t)
@@ -753,19 +848,27 @@ __global__ __launch_bounds__(512, 2) void share_kernel(Attend A) {
     }
   };
 
-#pragma unroll
-  for (int st = 0; st < D - 1; ++st) issue(st);
+  // The two waves of a SIMD (w and w + 4) are a phase apart: the later four take a
+  // stage's values after the next barrier, so that one's products run under the
+  // other's exponentials.  Two stages are in flight, one is in use, and one is
+  // kept for those values.
+  static_assert(D == 4, "");
+  const bool late = wave >= 4;
+  issue(0), issue(1);
   int st = 0;
-  auto stage = [&](auto edge_stage) {
-    wait_vmcnt<2 * kDma*(D - 2)>();  // this wave's part of the stage has landed
-    stage_barrier();                 // everyone's, and the stage before is used
-    issue(st + D - 1);
-    walk(edge_stage, W.first * kPos + st * SP + pg * WP, (uint32_t)(st % D) * kStage);
+  auto stage = [&](auto edge_stage) __attribute__((always_inline)) {
+    wait_vmcnt<2 * kDma>();  // this wave's part of the stage has landed
+    stage_barrier();         // everyone's, and stage st - 2 is used
+    issue(st + 2);
+    if (late && st > 0) values(edge_stage, st - 1);
+    scores(edge_stage, st);
+    if (!late) values(edge_stage, st);
   };
   const int seen_whole = W.C / SP - W.first * (kPos / SP);  // stages before the nodes
   const int inner = seen_whole < stages ? seen_whole : stages;
   for (; st < inner; ++st) stage(Bool<false>{});
   for (; st < stages; ++st) stage(Bool<true>{});
+  if (late && stages > 0) values(Bool<true>{}, stages - 1);
   wait_vmcnt<0>();  // the reads past the end have written their zeros
   __syncthreads();
   if (__any(any_odd != 0))
@@ -788,61 +891,68 @@ __global__ __launch_bounds__(512, 2) void share_kernel(Attend A) {
     __syncthreads();
     finish<RG, PG>(A, W, s_o, s_m, s_l, t, 16 * RT);
   }
+  __syncthreads();  // the next range's stages go where the rows are read from
+  }
+  share.rest(A, 32 * RG);
 }
 
-// The ranges' sums joined: 16 threads per row, 8 elements each.
-__global__ __launch_bounds__(256) void join_kernel(Attend A, long rows) {
-  const long at = (long)blockIdx.x * 16 + (threadIdx.x >> 4);  // bg * R + row
-  if (at >= rows) return;
-  const int d = 8 * (threadIdx.x & 15);
-  const int bg = (int)(at / A.R), row = (int)(at - (long)bg * A.R);
-  const int b = bg / A.nkv, g = bg - b * A.nkv, head = row / A.S, node = row - head * A.S;
-  const long C = A.lens[b], L = C + A.S;
-  if (C < 0 || L > A.bound) return;
-  const int tiles = (int)((L + kPos - 1) / kPos), ns = (tiles + A.tps - 1) / A.tps;
-  if (ns == 1) return;
-  const float* po = A.part + ((long)bg * A.splits * A.R + row) * kHd + d;
-  const float* pm = A.part + (long)A.units * A.R * kHd + ((long)bg * A.splits * A.R + row) * 2;
+// The ranges' sums joined: 32 threads per row, 4 elements each, of a head that
+// several workgroups share; a workgroup takes 8 rows of one head.
+__global__ __launch_bounds__(256) void join_kernel(Attend A, int per_head) {
+  const int bg = blockIdx.x / per_head, row = 8 * (blockIdx.x - bg * per_head) + (threadIdx.x >> 5);
+  const int b = bg / A.nkv, g = bg - b * A.nkv, n = grains_of(A, b);
+  if (n == 0) return;
+  const long T = (long)grains_below(A, A.B) * A.nkv;
+  const long from = (long)grains_below(A, b) * A.nkv + (long)g * n;
+  // the workgroup that has grain x is the first w with (w + 1) T / wgs > x
+  const long wgs = T < A.wgs ? T : A.wgs;
+  auto owner = [&](long x) { return (int)(((x + 1) * wgs + T - 1) / T) - 1; };
+  const int w0 = owner(from), w1 = owner(from + n - 1);
+  if (w0 == w1 || row >= A.R) return;
+  // the first range is its workgroup's second unless the head starts its share
+  const long e0 = 2L * w0 + ((long)w0 * T / wgs < from);
+  const int d = 4 * (threadIdx.x & 31), k = w1 - w0 + 1;
+  const float* po = A.part + (long)row * kHd + d;
+  const float* pm = A.part + 2 * (long)A.wgs * A.R * kHd + (long)row * 2;
+  auto entry = [&](int i) { return (i == 0 ? e0 : 2L * (w0 + i)) * A.R; };
   float m = -__builtin_inff();
-  for (int i = 0; i < ns; ++i) m = fmaxf(m, pm[(long)i * A.R * 2]);
-  const float ref = m == -__builtin_inff() ? 0.f : m;
-  float sum = 0.f, x[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = 0.f;
 #pragma unroll 4
-  for (int i = 0; i < ns; ++i) {
-    const float al = __builtin_amdgcn_exp2f(pm[(long)i * A.R * 2] - ref);
-    sum += al * pm[(long)i * A.R * 2 + 1];
-    const float4v lo = *reinterpret_cast<const float4v*>(po + (long)i * A.R * kHd);
-    const float4v hi = *reinterpret_cast<const float4v*>(po + (long)i * A.R * kHd + 4);
-#pragma unroll
-    for (int k = 0; k < 4; ++k) x[k] += al * lo[k], x[4 + k] += al * hi[k];
+  for (int i = 0; i < k; ++i) m = fmaxf(m, pm[entry(i) * 2]);
+  const float ref = m == -__builtin_inff() ? 0.f : m;
+  float sum = 0.f;
+  float4v x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int i = 0; i < k; ++i) {
+    const float al = __builtin_amdgcn_exp2f(pm[entry(i) * 2] - ref);
+    sum += al * pm[entry(i) * 2 + 1];
+    x += al * *reinterpret_cast<const float4v*>(po + entry(i) * kHd);
   }
+  const int head = row / A.S, node = row - head * A.S;
   const u64* see = A.seen + ((A.trees > 1 ? (long)b * A.S : 0) + node) * kWords;
   const bool live = (see[node >> 6] >> (node & 63)) & 1;
   const float is = 1.f / sum;
-  half8_t y;
+  typedef h16 half4v __attribute__((ext_vector_type(4)));
+  half4v y;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = live ? (h16)(x[i] * is) : (h16)0.f;
-  *reinterpret_cast<half8_t*>(A.out + ((long)b * A.S + node) * A.ld_o +
-                              (long)(g * A.rep + head) * kHd + d) = y;
+  for (int i = 0; i < 4; ++i) y[i] = live ? (h16)(x[i] * is) : (h16)0.f;
+  *reinterpret_cast<half4v*>(A.out + ((long)b * A.S + node) * A.ld_o +
+                             (long)(g * A.rep + head) * kHd + d) = y;
 }
 
-// Which kernel, its rows per workgroup, and how the positions are split so that
-// about two rounds of workgroups fill the chip.
+// Which kernel, its rows per workgroup, and its workgroups: one for each that the
+// chip holds at a time (they share the work evenly), or for each grain there can be.
 struct Plan {
-  int rows, blocks, splits, tps;
+  int rows, blocks, grain, wgs;
 };
 Plan plan_of(long B, long nkv, long rep, long S, long bound) {
-  const long R = rep * S, tiles = (bound + kPos - 1) / kPos;
+  const long R = rep * S;
   Plan p;
-  p.rows = R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : R <= 128 ? 128 : 256;
+  p.rows = R <= 16 ? 16 : R <= 32 ? 32 : R <= 128 ? 128 : 256;
   p.blocks = (int)((R + p.rows - 1) / p.rows);
-  const long heads = B * nkv * p.blocks, want = 512;
-  long splits = (want + heads - 1) / heads;
-  splits = splits < 1 ? 1 : splits;
-  p.tps = (int)((tiles + splits - 1) / splits + 3) / 4 * 4;
-  p.splits = (int)((tiles + p.tps - 1) / p.tps);
+  p.grain = p.rows <= 32 ? 4 * kPos : kPos;
+  const long most = B * nkv * ((bound + p.grain - 1) / p.grain);
+  const long fill = (long)hn_device_cus() * (p.rows == 16 ? 2 : 1) / p.blocks;
+  p.wgs = (int)(most < fill ? most : fill < 1 ? 1 : fill);
   return p;
 }
 
@@ -889,7 +999,7 @@ extern "C" int hn_tree_append(const void* qkv, long ld_qkv, const float* cos_t, 
 extern "C" long hn_tree_attention_workspace_bytes(long B, long nkv, long rep, long S, long bound) {
   if (B <= 0 || nkv <= 0 || rep <= 0 || S <= 0 || bound <= 0) return 0;
   const Plan p = plan_of(B, nkv, rep, S, bound);
-  return p.splits == 1 ? 0 : B * nkv * p.splits * rep * S * (kHd + 2) * 4;
+  return bound <= p.grain ? 0 : 2L * p.wgs * rep * S * (kHd + 2) * 4;
 }
 
 // See include/hn_int4.h.
@@ -909,28 +1019,29 @@ extern "C" int hn_tree_attention(const void* q, const void* kt, const void* v, l
                    ld_o >= nkv * rep * hd && lens && seen,
                "%s: operands must be 16-byte aligned, ld_o >= heads * %d", who, kHd);
   const Plan p = plan_of(B, nkv, rep, S, bound);
-  const long units = B * nkv * p.splits, rows = B * nkv * rep * S;
-  HN_ARG_CHECK(rows < (1L << 31) && (units + 7) / 8 * 8 * p.blocks < (1L << 31),
+  const long R = rep * S, per_head = (R + 7) / 8;
+  HN_ARG_CHECK(B * nkv * ((bound + kPos - 1) / kPos) < (1L << 31) &&
+                   B * nkv * per_head < (1L << 31) && (p.wgs + 7L) / 8 * 8 * p.blocks < (1L << 31),
                "%s: too many rows", who);
   const long need = hn_tree_attention_workspace_bytes(B, nkv, rep, S, bound);
   HN_ARG_CHECK(need == 0 || (work && al16(work) && work_bytes >= need),
                "%s: needs a 16-byte aligned workspace of %ld bytes (got %ld)", who, need,
                work_bytes);
   const Attend A = {(const h16*)q, (const h16*)kt, (const h16*)v, lens, seen, (h16*)out,
-                    (float*)work, max_len, bound, ld_o, (int)trees, (int)nkv, (int)rep, (int)S,
-                    (int)(rep * S), p.blocks, p.splits, p.tps, (int)units, scale};
-  const dim3 grid((unsigned)((units + 7) / 8 * 8 * p.blocks));
+                    (float*)work, max_len, bound, ld_o, (int)trees, (int)B, (int)nkv, (int)rep,
+                    (int)S, (int)R, p.blocks, p.grain, p.wgs, scale};
+  const dim3 grid((unsigned)((p.wgs + 7) / 8 * 8 * p.blocks));
   hipStream_t st = (hipStream_t)stream;
   switch (p.rows) {
     case 16: hipLaunchKernelGGL((attend_kernel<1, 4, 2>), grid, dim3(256), 0, st, A); break;
     case 32: hipLaunchKernelGGL((attend_kernel<2, 4, 1>), grid, dim3(256), 0, st, A); break;
-    case 64: hipLaunchKernelGGL((share_kernel<2, 4, 32, 2>), grid, dim3(512), 0, st, A); break;
-    case 128: hipLaunchKernelGGL((share_kernel<4, 2, 64, 2>), grid, dim3(512), 0, st, A); break;
+    case 128: hipLaunchKernelGGL((share_kernel<4, 2, 32, 4>), grid, dim3(512), 0, st, A); break;
     default: hipLaunchKernelGGL((share_kernel<8, 1, 64, 4>), grid, dim3(512), 0, st, A);
   }
   HN_LAUNCH_CHECK(who);
-  if (p.splits > 1) {
-    hipLaunchKernelGGL(join_kernel, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, st, A, rows);
+  if (need) {  // a head of several grains may be shared
+    hipLaunchKernelGGL(join_kernel, dim3((unsigned)(B * nkv * per_head)), dim3(256), 0, st, A,
+                       (int)per_head);
     HN_LAUNCH_CHECK(who);
   }
   return 0;
