@@ -614,23 +614,21 @@ __global__ __launch_bounds__(256, OCC) void attend_kernel(Attend A) {
 }
 
 // ---------------------------------------------------------------------------
-// Many rows per KV head: the tiles of K and V shared through LDS.  8 waves, RG
-// groups of 32 rows by PG parts of a stage of SP = WP * PG positions.  A stage
-// of keys [128 hd][SP] and values [SP][128 hd] goes from memory to LDS as it lies
-// (buffer_load ... lds), two stages ahead, and ds_read_b64_tr_b16 turns it on
-// the way to the registers: 16 lanes read 4 rows of 16 halves, and lane i gets
-// column i.  The operands' layouts are the MFMA's own: a lane's scores are
-// positions 16 j + 4 kg + r of its part, of row lane % 16, and with the values'
-// rows taken as {4 kg + r, 16 + 4 kg + r} they are the second product's operand
-// as they are.
+// Many rows per KV head: the tiles of K and V shared through LDS.  4 waves, RG
+// groups of 32 rows by PG parts of a stage of SP = 64 positions.  A stage of keys
+// [128 hd][SP] and values [SP][128 hd] goes from memory to LDS as it lies
+// (buffer_load ... lds), one stage ahead, and ds_read_b64_tr_b16 turns it on the
+// way to the registers: 16 lanes read 4 rows of 16 halves, and lane i gets column
+// i.  The operands' layouts are the MFMA's own: a lane's scores are positions 16 j
+// + 4 kg + r of its part, of row lane % 16, and with the values' rows taken as {4
+// kg + r, 16 + 4 kg + r} they are the second product's operand as they are.
+// Two workgroups per CU: one's loads and barriers under the other's arithmetic.
 //
 // Both transposing reads take 32 bytes of each of 16 rows; a row's 16-byte chunks
 // are stored at chunk ^ (2 * key(row)), so that the 8 rows that half a wave reads
 // cover the 64 banks once.
-template <int SP>
-__device__ __forceinline__ int key_of_k(int hd) {
-  return SP == 64 ? ((hd >> 1) & 1) | ((hd >> 2) & 2) : (hd & 3) | ((hd >> 1) & 4);
-}
+constexpr int kSP = 64;
+__device__ __forceinline__ int key_of_k(int hd) { return ((hd >> 1) & 1) | ((hd >> 2) & 2); }
 
 typedef short short4v __attribute__((ext_vector_type(4)));
 
@@ -644,15 +642,14 @@ __device__ __forceinline__ half8_t read_tr(uint32_t at, int lo, int hi) {
       half8_t, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-template <int RG, int PG, int WP, int D>
-__global__ __launch_bounds__(512, 2) void share_kernel(Attend A) {
-  constexpr int RT = 2, SP = WP * PG, JB = WP / 16;
+template <int RG, int PG>
+__global__ __launch_bounds__(256, 2) void share_kernel(Attend A) {
+  constexpr int RT = 2, SP = kSP, WP = SP / PG, JB = WP / 16, D = 2;
   constexpr int kKBytes = SP * kHd * 2, kStage = 2 * kKBytes;
-  constexpr int kDma = SP / 4 / 8;  // DMA instructions per wave and operand of a stage
-  static_assert(RG * PG == 8 && (SP == 64 || SP == 128), "");
-  constexpr int kSum = 8 * 16 * kOPad * 4;
-  __shared__ __align__(1024) unsigned char s_buf[D * kStage > kSum ? D * kStage : kSum];
-  __shared__ float s_m[8 * 16 * RT], s_l[8 * 16 * RT];
+  constexpr int kDma = SP / 4 / 4;  // DMA instructions per wave and operand of a stage
+  static_assert(RG * PG == 4 && D * kStage >= 4 * 16 * kOPad * 4, "");
+  __shared__ __align__(1024) unsigned char s_buf[D * kStage];
+  __shared__ float s_m[4 * 16 * RT], s_l[4 * 16 * RT];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 15, kg = lane >> 4, rg = wave / PG, pg = wave - rg * PG;
@@ -680,11 +677,11 @@ __global__ __launch_bounds__(512, 2) void share_kernel(Attend A) {
   const __amdgpu_buffer_rsrc_t rv = rsrc(A.v + slab, (int)(pitch * kHd));
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)s_buf;
 
-  // DMA: instruction i of wave w moves bytes 1024 (w + 8 i) on of a stage's keys
+  // DMA: instruction i of wave w moves bytes 1024 (w + 4 i) on of a stage's keys
   // and of its values; the lane's part of the addresses is the same for all i
   constexpr int kRowK = 1024 / (2 * SP), kChunks = SP / 8;  // rows of keys per instruction
   const int kr = lane / kChunks, vr = lane >> 4;
-  const int kc = (lane % kChunks) ^ (2 * key_of_k<SP>(kRowK * wave + kr));
+  const int kc = (lane % kChunks) ^ (2 * key_of_k(kRowK * wave + kr));
   const uint32_t kat = (uint32_t)kr * pitch + 16 * kc;
   const uint32_t vat = vr * (kHd * 2) + 16 * ((lane & 15) ^ (2 * ((4 * wave + vr) & 7)));
   const int stages = kPos / SP * (W.end - W.first);
@@ -696,14 +693,14 @@ __global__ __launch_bounds__(512, 2) void share_kernel(Attend A) {
     const uint32_t ka = st < stages && p0 + 8 * kc < W.L ? kat : kNone;
 #pragma unroll
     for (int i = 0; i < kDma; ++i) {
-      const int qi = wave + 8 * i;
-      dma_b128(rk, ka, (uint32_t)(kRowK * qi) * pitch + 2 * (uint32_t)p0, at + i * 8192);
+      const int qi = wave + 4 * i;
+      dma_b128(rk, ka, (uint32_t)(kRowK * qi) * pitch + 2 * (uint32_t)p0, at + i * 4096);
     }
 #pragma unroll
     for (int i = 0; i < kDma; ++i) {
-      const int qi = wave + 8 * i;
+      const int qi = wave + 4 * i;
       const uint32_t va = st < stages && p0 + 4 * qi + vr < W.L ? vat : kNone;
-      dma_b128(rv, va, ((uint32_t)p0 + 4 * qi) * (kHd * 2), at + kKBytes + i * 8192);
+      dma_b128(rv, va, ((uint32_t)p0 + 4 * qi) * (kHd * 2), at + kKBytes + i * 4096);
     }
   };
 
@@ -713,7 +710,7 @@ __global__ __launch_bounds__(512, 2) void share_kernel(Attend A) {
 #pragma unroll
   for (int j = 0; j < JB; ++j)
     k_at[j] = lds0 + (8 * kg + rr) * (2 * SP) + half +
-              32 * ((pg * JB + j) ^ key_of_k<SP>(8 * kg + rr));
+              32 * ((pg * JB + j) ^ key_of_k(8 * kg + rr));
 #pragma unroll
   for (int e = 0; e < 8; ++e)
     v_at[e] = lds0 + kKBytes + (pg * WP + 4 * kg + rr) * (kHd * 2) + half +
@@ -848,27 +845,19 @@ __global__ __launch_bounds__(512, 2) void share_kernel(Attend A) {
     }
   };
 
-  // The two waves of a SIMD (w and w + 4) are a phase apart: the later four take a
-  // stage's values after the next barrier, so that one's products run under the
-  // other's exponentials.  Two stages are in flight, one is in use, and one is
-  // kept for those values.
-  static_assert(D == 4, "");
-  const bool late = wave >= 4;
-  issue(0), issue(1);
+  issue(0);
   int st = 0;
   auto stage = [&](auto edge_stage) __attribute__((always_inline)) {
-    wait_vmcnt<2 * kDma>();  // this wave's part of the stage has landed
-    stage_barrier();         // everyone's, and stage st - 2 is used
-    issue(st + 2);
-    if (late && st > 0) values(edge_stage, st - 1);
+    wait_vmcnt<0>();  // this wave's part of the stage has landed
+    stage_barrier();  // everyone's, and the stage before is used
+    issue(st + 1);
     scores(edge_stage, st);
-    if (!late) values(edge_stage, st);
+    values(edge_stage, st);
   };
   const int seen_whole = W.C / SP - W.first * (kPos / SP);  // stages before the nodes
   const int inner = seen_whole < stages ? seen_whole : stages;
   for (; st < inner; ++st) stage(Bool<false>{});
   for (; st < stages; ++st) stage(Bool<true>{});
-  if (late && stages > 0) values(Bool<true>{}, stages - 1);
   wait_vmcnt<0>();  // the reads past the end have written their zeros
   __syncthreads();
   if (__any(any_odd != 0))
@@ -947,11 +936,11 @@ struct Plan {
 Plan plan_of(long B, long nkv, long rep, long S, long bound) {
   const long R = rep * S;
   Plan p;
-  p.rows = R <= 16 ? 16 : R <= 32 ? 32 : R <= 128 ? 128 : 256;
+  p.rows = R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128;
   p.blocks = (int)((R + p.rows - 1) / p.rows);
   p.grain = p.rows <= 32 ? 4 * kPos : kPos;
   const long most = B * nkv * ((bound + p.grain - 1) / p.grain);
-  const long fill = (long)hn_device_cus() * (p.rows == 16 ? 2 : 1) / p.blocks;
+  const long fill = (long)hn_device_cus() * (p.rows == 32 ? 1 : 2) / p.blocks;
   p.wgs = (int)(most < fill ? most : fill < 1 ? 1 : fill);
   return p;
 }
@@ -1035,8 +1024,8 @@ extern "C" int hn_tree_attention(const void* q, const void* kt, const void* v, l
   switch (p.rows) {
     case 16: hipLaunchKernelGGL((attend_kernel<1, 4, 2>), grid, dim3(256), 0, st, A); break;
     case 32: hipLaunchKernelGGL((attend_kernel<2, 4, 1>), grid, dim3(256), 0, st, A); break;
-    case 128: hipLaunchKernelGGL((share_kernel<4, 2, 32, 4>), grid, dim3(512), 0, st, A); break;
-    default: hipLaunchKernelGGL((share_kernel<8, 1, 64, 4>), grid, dim3(512), 0, st, A);
+    case 64: hipLaunchKernelGGL((share_kernel<2, 2>), grid, dim3(256), 0, st, A); break;
+    default: hipLaunchKernelGGL((share_kernel<4, 1>), grid, dim3(256), 0, st, A);
   }
   HN_LAUNCH_CHECK(who);
   if (need) {  // a head of several grains may be shared
