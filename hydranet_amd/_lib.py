@@ -53,7 +53,7 @@ SIGNATURES: dict[str, list] = {
     "hn_tree_append": [P, L, P, P, L, P, L, P, L, L, L, L, L, P, P, P, L, P],
     "hn_tree_attention_workspace_bytes": [L, L, L, L, L],
     "hn_tree_attention": [P, P, P, L, P, P, L, L, L, L, L, L, L, F, P, L, P, L, P],
-    "hn_verify_tree_workspace_bytes": [L, L, L, I],
+    "hn_verify_tree_workspace_bytes": [L, L, L],
     "hn_verify_tree": [P, L, L, P, L, L, I, P, P, L, P, P, F, L, L, L, P, P, P, P, L, P],
     "hn_kv_keep": [P, P, L, L, L, L, L, P, P, L, P, L, P, P],
     "hn_kv_fork": [P, P, L, L, L, L, L, P, P, L, L, P],

@@ -17,6 +17,13 @@
 // Sums and probabilities are held in 64 bits: a token's border in the
 // cumulative sum over V tokens is off by V times a term's error, which in 32
 // bits would exceed the width of unlikely tokens.
+//
+// Two launches.  stats_kernel reads every row once, over the whole chip: per
+// row and chunk of tokens the largest logit, its index and the sum of
+// exponentials.  walk_kernel, one workgroup per sequence, has every row's sum
+// and every node's two probabilities from that with one round of loads, walks
+// the tree in LDS, and reads a row again only where it must: both rows of a
+// node per rejection (S(c)), and one chunk for the draw.
 #include <float.h>
 
 #include "hn_common.h"
@@ -24,199 +31,427 @@
 namespace {
 
 constexpr int kMaxNodes = 256;
-constexpr int kThreads = 1024;
 constexpr double kTiny = 0x1p-40;  // residual mass below which nothing is left
 
 typedef __bf16 b16;
 
-template <typename T>
-__device__ __forceinline__ float logit(const T* p) {
-  const float x = (float)*p;
+// exp(d) for d <= 0 in 64 bits: 2^(k / 32) from a table (32 entries: 64 lanes
+// read them without a bank conflict), the rest, at most ln 2 / 64, by four terms
+// of its series: relative error 2e-12.  About a dozen instructions, so a row's sum
+// costs no more than reading it.
+constexpr double kLn2 = 0.693147180559945309417;
+constexpr int kTab = 32;
+
+__device__ __forceinline__ void fill_table(double* tab) {  // by a workgroup; a barrier follows
+  if (threadIdx.x < kTab) {
+    const double x = threadIdx.x * (kLn2 / kTab);
+    double y = 1.;
+#pragma unroll
+    for (int i = 20; i > 0; --i) y = 1. + y * x * (1. / i);
+    tab[threadIdx.x] = y;
+  }
+}
+
+// k: kTab / (T ln 2); of (l - m) / T
+__device__ __forceinline__ double exp_of(const double* tab, float l, double m, double k) {
+  constexpr double a = kLn2 / kTab, magic = 0x1.8p52;
+  // -40000 / 32 is past the smallest double: 0, as for -inf
+  const double x = fmax(((double)l - m) * k, -40000.);
+  const double t = x + magic;
+  const int i = (int)__builtin_bit_cast(unsigned long long, t);
+  const double r = x - (t - magic);
+  const double y =
+      1. + r * (a + r * (a * a / 2. + r * (a * a * a / 6. + r * (a * a * a * a / 24.))));
+  return __builtin_ldexp(y * tab[i & (kTab - 1)], i >> 5);
+}
+
+// A NaN logit counts as -inf, +inf as the largest finite number.
+__device__ __forceinline__ float sane(float x) {
   return x == x ? fminf(x, FLT_MAX) : -__builtin_inff();
 }
 
-struct Row {
-  double m;   // largest logit
-  double iz;  // 1 / sum exp((l - m) / T); 0: no token has a probability
+// 8 logits from any address, -inf past the end
+template <typename T>
+__device__ __forceinline__ void load8(float x[8], const T* p, int left) {
+  typedef T vec __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+  if (left >= 8) {
+    const vec v = *reinterpret_cast<const vec*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = sane((float)v[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = i < left ? sane((float)p[i]) : -__builtin_inff();
+  }
+}
+
+__device__ __forceinline__ double wave_sum(double x) {
+  for (int off = 32; off; off >>= 1) x += __shfl_xor(x, off, 64);
+  return x;
+}
+
+// What a chunk of a row comes to.
+struct Part {
+  float m;   // largest logit
+  int at;    // its lowest index
+  double s;  // sum of exp((l - m) / T)
 };
 
-template <typename T>
-struct Walk {
-  double it;  // 1 / T
-  int V;
-  double* red;  // [kThreads / 64]
+// Chunks: a multiple of kBlock tokens, at most 64 of them.
+constexpr int kBlock = 8192;
+constexpr int kMaxChunks = 64;
+struct Chunks {
+  int n, size;
+};
+__host__ __device__ inline Chunks chunks_of(long V) {
+  const long blocks = (V + kBlock - 1) / kBlock, per = (blocks + kMaxChunks - 1) / kMaxChunks;
+  return Chunks{(int)((blocks + per - 1) / per), (int)(per * kBlock)};
+}
 
-  __device__ double sum(double x) {
-    for (int off = 32; off; off >>= 1) x += __shfl_xor(x, off, 64);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
-    __syncthreads();
-    double t = 0.;
-    for (int w = 0; w < kThreads / 64; ++w) t += red[w];
-    return t;
+struct Verify {
+  const void *logits, *draft;
+  long sb, ss, db, ds;
+  const long* tokens;
+  const int* up;
+  const float *u, *temps;
+  float temp;
+  int trees, S, V;
+  int* path;
+  int* count;
+  long* token;
+  Part* part;  // [B][2][S][chunks]: the target's rows, the drafter's
+};
+
+constexpr int kStat = 256;
+
+// Grid (chunks, rows, B): the target's rows of the tree's nodes, then the
+// drafter's rows of nodes that have children.
+template <typename T>
+__global__ __launch_bounds__(kStat) void stats_kernel(Verify A) {
+  constexpr int kVec = kBlock / kStat / 8;  // vectors of 8 per thread and block
+  __shared__ double tab[kTab], s_s[kStat / 64];
+  __shared__ float s_m[kStat / 64];
+  __shared__ int s_at[kStat / 64];
+  const int b = blockIdx.z, tid = threadIdx.x, wave = tid >> 6;
+  const bool dr = (int)blockIdx.y >= A.S;
+  const int node = blockIdx.y - (dr ? A.S : 0);
+  const int* up = A.up + (A.trees > 1 ? (long)b * A.S : 0);
+  const float t = A.temps ? A.temps[b] : A.temp;
+  const bool greedy = !(t > 0.f);
+  if (dr && greedy) return;
+  if (node && up[node] == -2) return;
+  if (dr) {
+    bool inner = false;
+    for (int i = node + 1 + tid; i < A.S; i += kStat) inner |= up[i] == node;
+    if (!__syncthreads_or(inner)) return;
   }
-  __device__ double largest(double x) {
-    for (int off = 32; off; off >>= 1) x = fmax(x, __shfl_xor(x, off, 64));
+  fill_table(tab);
+  const double k = greedy ? 0. : kTab / ((double)t * kLn2);
+  const T* row = (const T*)(dr ? A.draft : A.logits) +
+                 (dr ? b * A.db + node * A.ds : b * A.sb + node * A.ss);
+  const Chunks C = chunks_of(A.V);
+  const int t0 = blockIdx.x * C.size, t1 = t0 + C.size < A.V ? t0 + C.size : A.V;
+  Part P = {-__builtin_inff(), A.V, 0.};
+  for (int o = t0; o < t1; o += kBlock) {
+    float x[kVec][8];
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) {
+      const int e = o + (j * kStat + tid) * 8;
+      load8(x[j], row + e, e < t1 ? t1 - e : 0);
+    }
+    float m = -__builtin_inff();
+#pragma unroll
+    for (int j = 0; j < kVec; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = fmaxf(m, x[j][i]);
+    const float mine = m;
+    for (int off = 32; off; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+    __syncthreads();  // also the table, and the last block's reads of s_*
+    if ((tid & 63) == 0) s_m[wave] = m;
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
-    __syncthreads();
-    double t = red[0];
-    for (int w = 1; w < kThreads / 64; ++w) t = fmax(t, red[w]);
-    return t;
-  }
-  __device__ Row row(const T* p) {
-    double m = -__builtin_inf();
-    for (int t = threadIdx.x; t < V; t += kThreads) m = fmax(m, (double)logit(p + t));
-    m = largest(m);
+#pragma unroll
+    for (int w = 0; w < kStat / 64; ++w) m = fmaxf(m, s_m[w]);
+    int at = A.V;
     double s = 0.;
-    if (m > -__builtin_inf())
-      for (int t = threadIdx.x; t < V; t += kThreads) s += exp(((double)logit(p + t) - m) * it);
-    s = sum(s);
-    return Row{m, s > 0. ? 1. / s : 0.};
+    if (greedy) {
+      if (mine == m && m > -__builtin_inff())
+#pragma unroll
+        for (int j = kVec - 1; j >= 0; --j)
+#pragma unroll
+          for (int i = 7; i >= 0; --i)
+            if (x[j][i] == m) at = o + (j * kStat + tid) * 8 + i;
+      for (int off = 32; off; off >>= 1) {
+        const int q = __shfl_xor(at, off, 64);
+        at = q < at ? q : at;
+      }
+    } else if (m > -__builtin_inff()) {
+#pragma unroll
+      for (int j = 0; j < kVec; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += exp_of(tab, x[j][i], m, k);
+      s = wave_sum(s);
+    }
+    if ((tid & 63) == 0) s_at[wave] = at, s_s[wave] = s;
+    __syncthreads();
+    if (tid == 0) {
+      s = 0.;
+#pragma unroll
+      for (int w = 0; w < kStat / 64; ++w) {
+        s += s_s[w];
+        at = s_at[w] < at ? s_at[w] : at;
+      }
+      if (m > P.m) {
+        if (!greedy) P.s = P.s * exp_of(tab, P.m, m, k) + s;
+        P.m = m, P.at = at;
+      } else if (!greedy && m > -__builtin_inff()) {
+        P.s += s * exp_of(tab, m, P.m, k);
+      }
+    }
   }
-  __device__ double prob(const T* p, const Row& r, int t) const {
-    return r.iz > 0. ? exp(((double)logit(p + t) - r.m) * it) * r.iz : 0.;
-  }
-};
+  if (tid == 0) A.part[(((long)b * 2 + dr) * A.S + node) * C.n + blockIdx.x] = P;
+}
+
+constexpr int kWalk = 1024, kWaves = kWalk / 64;
 
 template <typename T>
-__global__ __launch_bounds__(kThreads) void verify_kernel(
-    const T* __restrict__ logits, long sb, long ss, const T* __restrict__ draft, long db, long ds,
-    const long* __restrict__ tokens, const int* __restrict__ up, int trees,
-    const float* __restrict__ u, const float* __restrict__ temp, float temp0, int S, int V,
-    int* __restrict__ path, int* __restrict__ count, long* __restrict__ token) {
-  __shared__ double red[kThreads / 64];
-  __shared__ int s_up[kMaxNodes];
-  __shared__ long s_tok[kMaxNodes];
+__global__ __launch_bounds__(kWalk) void walk_kernel(Verify A) {
+  __shared__ double tab[kTab];
+  __shared__ double s_z[2][kMaxNodes];      // 1 / sum of a row's exponentials, 0: no token
+  __shared__ float s_m[2][kMaxNodes];       // its largest logit
+  __shared__ double s_px[kMaxNodes], s_qx[kMaxNodes];  // p, q (of the parent) of a node's token
+  __shared__ int s_up[kMaxNodes], s_tok[kMaxNodes], s_gone[kMaxNodes], s_top[kMaxNodes];
   __shared__ float s_u[kMaxNodes];
-  __shared__ long gone[kMaxNodes];
-  __shared__ double s_part[kThreads];
-  __shared__ int s_pick;
-  const int b = blockIdx.x, tid = threadIdx.x;
-  for (int i = tid; i < S; i += kThreads) {
-    s_up[i] = up[(trees > 1 ? (long)b * S : 0) + i];
-    s_tok[i] = tokens[(long)b * S + i];
-    s_u[i] = u[(long)b * S + i];
-    path[(long)b * S + i] = i ? -1 : 0;
+  __shared__ double s_sum[kMaxChunks][kWaves];
+  __shared__ double s_scan[kWaves];
+  __shared__ int s_pick, s_last;
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int S = A.S, V = A.V;
+  const Chunks C = chunks_of(V);
+  const float tb = A.temps ? A.temps[b] : A.temp;
+  const bool greedy = !(tb > 0.f), soft = A.draft && !greedy;
+  const double k = greedy ? 0. : kTab / ((double)tb * kLn2);
+  const T* lg = (const T*)A.logits + b * A.sb;
+  const T* dl = soft ? (const T*)A.draft + b * A.db : nullptr;
+  fill_table(tab);
+  if (tid < S) {
+    const int up = A.up[(A.trees > 1 ? (long)b * S : 0) + tid];
+    const long x = A.tokens[(long)b * S + tid];
+    s_up[tid] = tid ? up : -1;
+    s_tok[tid] = x >= 0 && x < V ? (int)x : -1;
+    s_u[tid] = A.u[(long)b * S + tid];
+    A.path[(long)b * S + tid] = tid ? -1 : 0;
+    // (rows that stats_kernel left out have neither a probability nor a use)
+    s_z[0][tid] = s_z[1][tid] = 0., s_m[0][tid] = s_m[1][tid] = -__builtin_inff();
+    s_px[tid] = s_qx[tid] = 0., s_top[tid] = -1;
   }
   __syncthreads();
-  const float tb = temp ? temp[b] : temp0;
-  const bool greedy = !(tb > 0.f), soft = draft && !greedy;
-  Walk<T> W = {greedy ? 1. : 1. / (double)tb, V, red};
-  logits += b * sb;
-  if (draft) draft += b * db;
+  // every row's largest logit and sum, a wave per row, a lane per chunk
+  for (int r = wave; r < (soft ? 2 : 1) * S; r += kWaves) {
+    const int dr = r >= S, node = r - (dr ? S : 0);
+    if (s_up[node] == -2) continue;
+    if (dr) {
+      bool inner = false;
+      for (int i = lane; i < S; i += 64) inner |= s_up[i] == node;
+      if (!__any(inner)) continue;
+    }
+    Part P = {-__builtin_inff(), V, 0.};
+    if (lane < C.n) P = A.part[(((long)b * 2 + dr) * S + node) * C.n + lane];
+    float m = P.m;
+    for (int off = 32; off; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+    if (greedy) {
+      int at = P.m == m && m > -__builtin_inff() ? P.at : V;
+      for (int off = 32; off; off >>= 1) {
+        const int q = __shfl_xor(at, off, 64);
+        at = q < at ? q : at;
+      }
+      if (lane == 0) s_top[node] = at < V ? at : -1;
+    } else {
+      const double s =
+          wave_sum(m > -__builtin_inff() ? P.s * exp_of(tab, P.m, m, k) : 0.);
+      if (lane == 0) s_m[dr][node] = m, s_z[dr][node] = s > 0. ? 1. / s : 0.;
+    }
+  }
+  __syncthreads();
+  auto prob = [&](int dr, int node, float l) {
+    const double z = s_z[dr][node];
+    return z > 0. ? exp_of(tab, l, s_m[dr][node], k) * z : 0.;
+  };
+  if (!greedy && tid < S && s_up[tid] >= 0 && s_tok[tid] >= 0) {
+    const int n = s_up[tid];
+    s_px[tid] = prob(0, n, sane((float)lg[n * A.ss + s_tok[tid]]));
+    if (soft) s_qx[tid] = prob(1, n, sane((float)dl[n * A.ds + s_tok[tid]]));
+  }
+  __syncthreads();
 
   int cur = 0, n = 1, ngone = 0;
   double c = 0., mass = 1.;
-  Row P = {}, Q = {};
-  int top = -1;
-  auto enter = [&]() {
-    const T* p = logits + cur * ss;
-    if (greedy) {
-      double m = -__builtin_inf();
-      for (int t = tid; t < V; t += kThreads) m = fmax(m, (double)logit(p + t));
-      m = W.largest(m);
-      int at = V;
-      if (m > -__builtin_inf())
-        for (int t = tid; t < V; t += kThreads)
-          if ((double)logit(p + t) == m) at = at < t ? at : t;
-      at = (int)-W.largest(-(double)at);
-      top = at < V ? at : -1;
-    } else {
-      P = W.row(p);
-      if (soft) Q = W.row(draft + cur * ds);
+  // max(p - c q, 0) of 8 tokens of the current node, less those gone
+  auto left8 = [&](double r[8], int e, int end) {
+    float x[8];
+    load8(x, lg + cur * A.ss + e, end - e);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = prob(0, cur, x[i]);
+    if (c > 0.) {
+      load8(x, dl + cur * A.ds + e, end - e);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r[i] = fmax(r[i] - c * prob(1, cur, x[i]), 0.);
     }
-    c = 0., mass = 1., ngone = 0;
+    for (int j = 0; j < ngone; ++j) {
+      const int g = s_gone[j] - e;
+      if (g >= 0 && g < 8)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i == g) r[i] = 0.;
+    }
   };
-  auto left = [&](int t) -> double {
-    const double p = W.prob(logits + cur * ss, P, t);
-    return soft && c > 0. ? fmax(p - c * W.prob(draft + cur * ds, Q, t), 0.) : p;
+  // a chunk's mass, each wave's part of it into s_sum
+  auto sum_chunk = [&](int ch) {
+    const int t0 = ch * C.size, t1 = t0 + C.size < V ? t0 + C.size : V;
+    double s = 0.;
+    for (int e = t0 + tid * 8; e < t1; e += kWalk * 8) {
+      double r[8];
+      left8(r, e, t1);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) s += r[i];
+    }
+    s = wave_sum(s);
+    if (lane == 0) s_sum[ch][wave] = s;
   };
-  enter();
+  auto chunk = [&](int ch) {
+    double s = 0.;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) s += s_sum[ch][w];
+    return s;
+  };
   for (int i = 1; i < S; ++i) {
     if (s_up[i] != cur) continue;
-    const long x = s_tok[i];
-    const bool in = x >= 0 && x < V;
+    const int x = s_tok[i];
     bool take = false;
     if (greedy) {
-      take = in && x == top;
-    } else if (in && mass > kTiny) {
-      const double px = W.prob(logits + cur * ss, P, (int)x);
+      take = x >= 0 && x == s_top[cur];
+    } else if (x >= 0 && mass > kTiny) {
       if (soft) {
-        const double qx = W.prob(draft + cur * ds, Q, (int)x);
-        take = (double)s_u[i] * qx * mass < px - c * qx;
+        take = (double)s_u[i] * s_qx[i] * mass < s_px[i] - c * s_qx[i];
+        if (!take) {
+          c += mass;
+          __syncthreads();  // the last sums are read
+          for (int ch = 0; ch < C.n; ++ch) sum_chunk(ch);
+          __syncthreads();
+          mass = 0.;
+          for (int ch = 0; ch < C.n; ++ch) mass += chunk(ch);
+        }
       } else {
         bool was = false;
-        for (int j = 0; j < ngone; ++j) was |= gone[j] == x;
-        take = !was && (double)s_u[i] * mass < px;
+        for (int j = 0; j < ngone; ++j) was |= s_gone[j] == x;
+        take = !was && (double)s_u[i] * mass < s_px[i];
         if (!take && !was) {
-          mass -= px;
+          mass -= s_px[i];
           __syncthreads();
-          if (tid == 0) gone[ngone] = x;
+          if (tid == 0) s_gone[ngone] = x;
           __syncthreads();
           ++ngone;
         }
       }
     }
     if (take) {
-      cur = i;
-      if (tid == 0) path[(long)b * S + n] = i;
+      cur = i, c = 0., mass = 1., ngone = 0;
+      if (tid == 0) A.path[(long)b * S + n] = i;
       ++n;
-      enter();
-    } else if (soft && in && mass > kTiny) {
-      c += mass;
-      double s = 0.;
-      for (int t = tid; t < V; t += kThreads) s += left(t);
-      mass = W.sum(s);
     }
   }
-  if (tid == 0) count[b] = n;
+  if (tid == 0) A.count[b] = n;
   if (greedy) {
-    if (tid == 0) token[b] = top;
+    if (tid == 0) A.token[b] = s_top[cur];
     return;
   }
   if (!(mass > kTiny)) c = 0., ngone = 0;  // nothing left: the target itself
-  // inversion: a run of tokens per thread, then the run that holds the target
-  const int per = (V + kThreads - 1) / kThreads, t0 = tid * per;
-  const int t1 = t0 + per < V ? t0 + per : V;
-  auto value = [&](int t) -> double {
-    for (int j = 0; j < ngone; ++j)
-      if (gone[j] == t) return 0.;
-    return left(t);
-  };
-  double s = 0.;
-  int last = -1;
-  for (int t = t0; t < t1; ++t) {
-    const double r = value(t);
-    s += r;
-    if (r > 0.) last = t;
-  }
-  s_part[tid] = s;
-  if (tid == 0) s_pick = V;
-  __syncthreads();
-  double before = 0., all = 0.;
-  for (int j = 0; j < kThreads; ++j) {
-    if (j < tid) before += s_part[j];
-    all += s_part[j];
-  }
-  last = (int)W.largest((double)last);
-  const double target = (double)s_u[0] * all;
-  for (int t = t0; t < t1; ++t) {
-    const double r = value(t);
-    before += r;
-    if (r > 0. && before > target) {
-      atomicMin(&s_pick, t);
-      break;
+
+  // The draw: the chunk that the target falls into, then the token.  The chunks'
+  // masses are those of the last rejection, or the row's own sums, where a token
+  // is gone anew.
+  if (c == 0.) {
+    __syncthreads();
+    if (tid < C.n) {
+      const Part P = A.part[((long)b * 2 * S + cur) * C.n + tid];
+      s_sum[tid][0] = P.m > -__builtin_inff() ? P.s * prob(0, cur, P.m) : 0.;
+#pragma unroll
+      for (int w = 1; w < kWaves; ++w) s_sum[tid][w] = 0.;
     }
+    __syncthreads();
+    for (int j = 0; j < ngone; ++j) {
+      const int ch = s_gone[j] / C.size;
+      bool done = false;
+      for (int q = 0; q < j; ++q) done |= s_gone[q] / C.size == ch;
+      if (!done) sum_chunk(ch);
+    }
+    __syncthreads();
   }
+  double all = 0.;
+  for (int ch = 0; ch < C.n; ++ch) all += chunk(ch);
+  const double target = (double)s_u[0] * all;
+  int pick = -1;
+  double before = 0., cum = 0.;
+  for (int ch = 0; ch < C.n; ++ch) {
+    const double s = chunk(ch);
+    if (s > 0.) pick = ch, before = cum;  // the last that has any, if none exceeds
+    cum += s;
+    if (s > 0. && cum > target) break;
+  }
+  if (pick < 0) {  // no logit is finite
+    if (tid == 0) A.token[b] = -1;
+    return;
+  }
+  const int t0 = pick * C.size, t1 = t0 + C.size < V ? t0 + C.size : V;
+  if (tid == 0) s_pick = V, s_last = -1;
   __syncthreads();
-  if (tid == 0) token[b] = s_pick < V ? s_pick : last;
+  for (int o = t0; o < t1; o += kBlock) {
+    const int e = o + tid * 8;
+    double r[8], sum = 0.;
+    if (e < t1)
+      left8(r, e, t1);
+    else
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r[i] = 0.;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += r[i];
+    double run = sum;  // inclusive over the wave
+    for (int off = 1; off < 64; off <<= 1) {
+      const double y = __shfl_up(run, off, 64);
+      if (lane >= off) run += y;
+    }
+    if (lane == 63) s_scan[wave] = run;
+    __syncthreads();
+    double base = before, total = before;
+    for (int w = 0; w < kWaves; ++w) {
+      if (w < wave) base += s_scan[w];
+      total += s_scan[w];
+    }
+    run = base + run - sum;
+    int hit = V, last = -1;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      run += r[i];
+      if (r[i] > 0.) {
+        last = e + i;
+        if (hit == V && run > target) hit = e + i;
+      }
+    }
+    if (hit < V) atomicMin(&s_pick, hit);
+    if (last >= 0) atomicMax(&s_last, last);
+    before = total;
+    __syncthreads();
+    if (s_pick < V) break;
+  }
+  if (tid == 0) A.token[b] = s_pick < V ? s_pick : s_last;
 }
 
 }  // namespace
 
 // See include/hn_int4.h.
-extern "C" long hn_verify_tree_workspace_bytes(long B, long S, long V, int soft) { return 0; }
+extern "C" long hn_verify_tree_workspace_bytes(long B, long S, long V) {
+  if (B <= 0 || S <= 0 || V <= 0) return 0;
+  return B * 2 * S * chunks_of(V).n * (long)sizeof(Part);
+}
 
 // See include/hn_int4.h.
 extern "C" int hn_verify_tree(const void* logits, long ld_b, long ld_s, const void* draft,
@@ -234,11 +469,23 @@ extern "C" int hn_verify_tree(const void* logits, long ld_b, long ld_s, const vo
                "%s: row strides below the vocabulary", who);
   if (B == 0) return 0;
   HN_ARG_CHECK(logits && tokens && up && u && path && count && token, "%s: null operand", who);
-  HN_ARG_CHECK(B < (1L << 31), "%s: too many sequences", who);
-#define HN_VERIFY(T)                                                                            \
-  hipLaunchKernelGGL(verify_kernel<T>, dim3((unsigned)B), dim3(kThreads), 0, (hipStream_t)stream, \
-                     (const T*)logits, ld_b, ld_s, (const T*)draft, ld_db, ld_ds, tokens, up,   \
-                     (int)trees, u, temps, temperature, (int)S, (int)V, path, count, token)
+  HN_ARG_CHECK(B <= 65535, "%s: at most 65535 sequences", who);
+  const long need = hn_verify_tree_workspace_bytes(B, S, V);
+  HN_ARG_CHECK(work && ((uintptr_t)work & 15) == 0 && work_bytes >= need,
+               "%s: needs a 16-byte aligned workspace of %ld bytes (got %ld)", who, need,
+               work_bytes);
+  const bool soft = draft && (temps || temperature > 0.f);
+  const Verify A = {logits, draft, ld_b,  ld_s,   ld_db,  ld_ds,  tokens, up,
+                    u,      temps, temperature, (int)trees, (int)S, (int)V, path, count,
+                    token,  (Part*)work};
+  const dim3 grid((unsigned)chunks_of(V).n, (unsigned)(soft ? 2 * S : S), (unsigned)B);
+  hipStream_t st = (hipStream_t)stream;
+#define HN_VERIFY(T)                                                            \
+  do {                                                                          \
+    hipLaunchKernelGGL(stats_kernel<T>, grid, dim3(kStat), 0, st, A);           \
+    HN_LAUNCH_CHECK(who);                                                       \
+    hipLaunchKernelGGL(walk_kernel<T>, dim3((unsigned)B), dim3(kWalk), 0, st, A); \
+  } while (0)
   if (dtype == 0)
     HN_VERIFY(h16);
   else if (dtype == 1)

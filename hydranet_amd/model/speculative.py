@@ -245,15 +245,14 @@ def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, tree: DraftTree,
     path = torch.empty((B, S), dtype=torch.int32, device=dev)
     count = torch.empty(B, dtype=torch.int32, device=dev)
     token = torch.empty(B, dtype=torch.int64, device=dev)
-    soft = int(draft is not None)
-    n = _lib.lib().hn_verify_tree_workspace_bytes(B, S, V, soft)
-    work = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    n = _lib.lib().hn_verify_tree_workspace_bytes(B, S, V)
+    work = torch.empty(n, dtype=torch.uint8, device=dev)
     d = (None, 0, 0) if draft is None else (draft.data_ptr(), draft.stride(0), draft.stride(1))
     _lib.call_on(dev, "hn_verify_tree", logits.data_ptr(), logits.stride(0), logits.stride(1), *d,
                  _DTYPES[logits.dtype], tokens.data_ptr(), tree.up.data_ptr(), tree.trees,
                  uniforms.data_ptr(), None if temps is None else temps.data_ptr(), temp, B, S, V,
-                 path.data_ptr(), count.data_ptr(), token.data_ptr(),
-                 None if work is None else work.data_ptr(), n, _lib.stream(dev))
+                 path.data_ptr(), count.data_ptr(), token.data_ptr(), work.data_ptr(), n,
+                 _lib.stream(dev))
     return Verified(path, count, token)
 
 

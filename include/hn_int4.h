@@ -504,7 +504,7 @@ int hn_tree_attention(const void* q, const void* kt, const void* v, long max_len
  *   without a finite logit gives token -1.  A token outside [0, V) is rejected.
  *   work: hn_verify_tree_workspace_bytes(...) bytes, 16-byte aligned, any
  *   contents. */
-long hn_verify_tree_workspace_bytes(long B, long S, long V, int soft);
+long hn_verify_tree_workspace_bytes(long B, long S, long V);
 int hn_verify_tree(const void* logits, long ld_b, long ld_s, const void* draft, long ld_db,
                    long ld_ds, int dtype, const long* tokens, const int* up, long trees,
                    const float* u, const float* temps, float temperature, long B, long S, long V,
