@@ -56,7 +56,8 @@ __device__ __forceinline__ void fill_table(double* tab) {  // by a workgroup; a 
 __device__ __forceinline__ double exp_of(const double* tab, float l, double m, double k) {
   constexpr double a = kLn2 / kTab, magic = 0x1.8p52;
   // -40000 / 32 is past the smallest double: 0, as for -inf
-  const double x = fmax(((double)l - m) * k, -40000.);
+  double x = ((double)l - m) * k;
+  x = x > -40000. ? x : -40000.;
   const double t = x + magic;
   const int i = (int)__builtin_bit_cast(unsigned long long, t);
   const double r = x - (t - magic);
@@ -67,7 +68,7 @@ __device__ __forceinline__ double exp_of(const double* tab, float l, double m, d
 
 // A NaN logit counts as -inf, +inf as the largest finite number.
 __device__ __forceinline__ float sane(float x) {
-  return x == x ? fminf(x, FLT_MAX) : -__builtin_inff();
+  return fminf(fmaxf(x, -__builtin_inff()), FLT_MAX);
 }
 
 // 8 logits from any address, -inf past the end
@@ -84,8 +85,22 @@ __device__ __forceinline__ void load8(float x[8], const T* p, int left) {
   }
 }
 
-__device__ __forceinline__ double wave_sum(double x) {
-  for (int off = 32; off; off >>= 1) x += __shfl_xor(x, off, 64);
+// x of another lane by a data-parallel-primitive move, 0 where there is none
+template <int CTL>
+__device__ __forceinline__ double moved(double x) {
+  const unsigned long long w = __builtin_bit_cast(unsigned long long, x);
+  const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)w, CTL, 0xf, 0xf, false);
+  const unsigned hi = __builtin_amdgcn_update_dpp(0, (int)(w >> 32), CTL, 0xf, 0xf, false);
+  return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+// Sum over the wave, in lane 63: within rows of 16, then over the rows.
+__device__ __forceinline__ double sum_in_63(double x) {
+  x += moved<0x111>(x);  // row_shr:1, 2, 4, 8
+  x += moved<0x112>(x);
+  x += moved<0x114>(x);
+  x += moved<0x118>(x);
+  x += moved<0x142>(x);  // row_bcast:15
+  x += moved<0x143>(x);  // row_bcast:31
   return x;
 }
 
@@ -188,9 +203,9 @@ __global__ __launch_bounds__(kStat) void stats_kernel(Verify A) {
       for (int j = 0; j < kVec; ++j)
 #pragma unroll
         for (int i = 0; i < 8; ++i) s += exp_of(tab, x[j][i], m, k);
-      s = wave_sum(s);
+      s = sum_in_63(s);
     }
-    if ((tid & 63) == 0) s_at[wave] = at, s_s[wave] = s;
+    if ((tid & 63) == 63) s_at[wave] = at, s_s[wave] = s;
     __syncthreads();
     if (tid == 0) {
       s = 0.;
@@ -267,8 +282,8 @@ __global__ __launch_bounds__(kWalk) void walk_kernel(Verify A) {
       if (lane == 0) s_top[node] = at < V ? at : -1;
     } else {
       const double s =
-          wave_sum(m > -__builtin_inff() ? P.s * exp_of(tab, P.m, m, k) : 0.);
-      if (lane == 0) s_m[dr][node] = m, s_z[dr][node] = s > 0. ? 1. / s : 0.;
+          sum_in_63(m > -__builtin_inff() ? P.s * exp_of(tab, P.m, m, k) : 0.);
+      if (lane == 63) s_m[dr][node] = m, s_z[dr][node] = s > 0. ? 1. / s : 0.;
     }
   }
   __syncthreads();
@@ -286,15 +301,30 @@ __global__ __launch_bounds__(kWalk) void walk_kernel(Verify A) {
   int cur = 0, n = 1, ngone = 0;
   double c = 0., mass = 1.;
   // max(p - c q, 0) of 8 tokens of the current node, less those gone
-  auto left8 = [&](double r[8], int e, int end) {
-    float x[8];
-    load8(x, lg + cur * A.ss + e, end - e);
+  struct Rows {
+    const T *p, *q;
+    double pm, pz, qm, qz;  // largest logits, 1 / sums (c's factor in the drafter's)
+    bool both;
+  };
+  auto rows_of = [&]() {
+    Rows R = {lg + cur * A.ss, soft ? dl + cur * A.ds : nullptr, s_m[0][cur], s_z[0][cur],
+              s_m[1][cur], c * s_z[1][cur], c > 0.};
+    if (!(R.pz > 0.)) R.pm = 0.;  // no finite logit: exponents of -inf, sums of 0
+    if (!(s_z[1][cur] > 0.)) R.qm = 0.;
+    return R;
+  };
+  auto left8 = [&](double r[8], const Rows& R, int e, int end) {
+    float x[8], y[8];
+    load8(x, R.p + e, end - e);
+    if (R.both) load8(y, R.q + e, end - e);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = prob(0, cur, x[i]);
-    if (c > 0.) {
-      load8(x, dl + cur * A.ds + e, end - e);
+    for (int i = 0; i < 8; ++i) r[i] = exp_of(tab, x[i], R.pm, k) * R.pz;
+    if (R.both) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) r[i] = fmax(r[i] - c * prob(1, cur, x[i]), 0.);
+      for (int i = 0; i < 8; ++i) {
+        const double d = r[i] - exp_of(tab, y[i], R.qm, k) * R.qz;
+        r[i] = d > 0. ? d : 0.;
+      }
     }
     for (int j = 0; j < ngone; ++j) {
       const int g = s_gone[j] - e;
@@ -305,17 +335,17 @@ __global__ __launch_bounds__(kWalk) void walk_kernel(Verify A) {
     }
   };
   // a chunk's mass, each wave's part of it into s_sum
-  auto sum_chunk = [&](int ch) {
+  auto sum_chunk = [&](const Rows& R, int ch) {
     const int t0 = ch * C.size, t1 = t0 + C.size < V ? t0 + C.size : V;
     double s = 0.;
     for (int e = t0 + tid * 8; e < t1; e += kWalk * 8) {
       double r[8];
-      left8(r, e, t1);
+      left8(r, R, e, t1);
 #pragma unroll
       for (int i = 0; i < 8; ++i) s += r[i];
     }
-    s = wave_sum(s);
-    if (lane == 0) s_sum[ch][wave] = s;
+    s = sum_in_63(s);
+    if (lane == 63) s_sum[ch][wave] = s;
   };
   auto chunk = [&](int ch) {
     double s = 0.;
@@ -335,7 +365,8 @@ __global__ __launch_bounds__(kWalk) void walk_kernel(Verify A) {
         if (!take) {
           c += mass;
           __syncthreads();  // the last sums are read
-          for (int ch = 0; ch < C.n; ++ch) sum_chunk(ch);
+          const Rows R = rows_of();
+          for (int ch = 0; ch < C.n; ++ch) sum_chunk(R, ch);
           __syncthreads();
           mass = 0.;
           for (int ch = 0; ch < C.n; ++ch) mass += chunk(ch);
@@ -366,6 +397,7 @@ __global__ __launch_bounds__(kWalk) void walk_kernel(Verify A) {
   }
   if (!(mass > kTiny)) c = 0., ngone = 0;  // nothing left: the target itself
 
+  const Rows R = rows_of();
   // The draw: the chunk that the target falls into, then the token.  The chunks'
   // masses are those of the last rejection, or the row's own sums, where a token
   // is gone anew.
@@ -382,7 +414,7 @@ __global__ __launch_bounds__(kWalk) void walk_kernel(Verify A) {
       const int ch = s_gone[j] / C.size;
       bool done = false;
       for (int q = 0; q < j; ++q) done |= s_gone[q] / C.size == ch;
-      if (!done) sum_chunk(ch);
+      if (!done) sum_chunk(R, ch);
     }
     __syncthreads();
   }
@@ -408,7 +440,7 @@ __global__ __launch_bounds__(kWalk) void walk_kernel(Verify A) {
     const int e = o + tid * 8;
     double r[8], sum = 0.;
     if (e < t1)
-      left8(r, e, t1);
+      left8(r, R, e, t1);
     else
 #pragma unroll
       for (int i = 0; i < 8; ++i) r[i] = 0.;
