@@ -18,12 +18,13 @@
 // cumulative sum over V tokens is off by V times a term's error, which in 32
 // bits would exceed the width of unlikely tokens.
 //
-// Two launches.  stats_kernel reads every row once, over the whole chip: per
-// row and chunk of tokens the largest logit, its index and the sum of
-// exponentials.  walk_kernel, one workgroup per sequence, has every row's sum
-// and every node's two probabilities from that with one round of loads, walks
-// the tree in LDS, and reads a row again only where it must: both rows of a
-// node per rejection (S(c)), and one chunk for the draw.
+// stats_kernel reads every row once, over the whole chip: per row and chunk of
+// tokens the largest logit, its index and the sum of exponentials.  With a
+// drafter's logits, first_kernel has S(1) of the nodes whose first child is
+// rejected in the same way.  walk_kernel, one workgroup per sequence, has every
+// row's sum and every node's two probabilities from that with one round of
+// loads, walks the tree in LDS, and reads a row again only where it must: both
+// rows of a node per further rejection (S(c)), and one chunk for the draw.
 #include <float.h>
 
 #include "hn_common.h"
@@ -133,7 +134,8 @@ struct Verify {
   int* path;
   int* count;
   long* token;
-  Part* part;  // [B][2][S][chunks]: the target's rows, the drafter's
+  Part* part;     // [B][2][S][chunks]: the target's rows, the drafter's
+  double* first;  // [B][S][chunks]: S(1) of a node whose first child is rejected
 };
 
 constexpr int kStat = 256;
@@ -225,13 +227,129 @@ __global__ __launch_bounds__(kStat) void stats_kernel(Verify A) {
   if (tid == 0) A.part[(((long)b * 2 + dr) * A.S + node) * C.n + blockIdx.x] = P;
 }
 
+// A row's largest logit and 1 / its sum of exponentials (0: no finite logit), by a
+// wave, a lane per chunk; every lane has them.
+struct RowStat {
+  float m;
+  double z;
+};
+// Whether a first child is accepted: u q(x) < p(x).  (first_kernel and the walk
+// decide alike.)
+__device__ __forceinline__ bool first_accepted(float u, double px, double qx) {
+#pragma clang fp contract(off)
+  return (double)u * qx < px;
+}
+__device__ __forceinline__ double from_63(double x) {
+  const unsigned long long w = __builtin_bit_cast(unsigned long long, x);
+  const unsigned lo = __builtin_amdgcn_readlane((int)w, 63);
+  const unsigned hi = __builtin_amdgcn_readlane((int)(w >> 32), 63);
+  return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
+}
+__device__ __forceinline__ RowStat row_stat(const Part* p, int chunks, const double* tab, double k) {
+  const int lane = threadIdx.x & 63;
+  Part P = {-__builtin_inff(), 0, 0.};
+  if (lane < chunks) P = p[lane];
+  float m = P.m;
+  for (int off = 32; off; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+  const bool any = m > -__builtin_inff();
+  const double s = from_63(sum_in_63(any ? P.s * exp_of(tab, P.m, m, k) : 0.));
+  return RowStat{m, s > 0. ? 1. / s : 0.};
+}
+__device__ __forceinline__ double prob_of(const double* tab, const RowStat& r, float l, double k) {
+  return r.z > 0. ? exp_of(tab, l, r.m, k) * r.z : 0.;
+}
+
+// max(p - c q, 0) of 8 tokens
+template <typename T>
+struct Rows {
+  const T *p, *q;
+  double pm, pz, qm, qz;  // largest logits, 1 / sums (c's factor in the drafter's)
+  bool both;              // c > 0
+
+  __device__ Rows(const T* p_, const T* q_, RowStat P, RowStat Q, double c)
+      : p(p_), q(q_), pm(P.z > 0. ? P.m : 0.), pz(P.z), qm(Q.z > 0. ? Q.m : 0.), qz(c * Q.z),
+        both(c > 0.) {}  // without a finite logit: exponents of -inf, sums of 0
+  __device__ __forceinline__ void left8(double r[8], const double* tab, double k, int e,
+                                        int end) const {
+    float x[8], y[8];
+    load8(x, p + e, end - e);
+    if (both) load8(y, q + e, end - e);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = exp_of(tab, x[i], pm, k) * pz;
+    if (both) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const double d = r[i] - exp_of(tab, y[i], qm, k) * qz;
+        r[i] = d > 0. ? d : 0.;
+      }
+    }
+  }
+};
+
+// The mass that a node's first rejection leaves, S(1), by chunks over the whole
+// chip: the walk needs it at each node whose first child is rejected, and most
+// trees need little more.  (A node that the walk does not come to is summed for
+// nothing.)  Grid (chunks, S, B).
+template <typename T>
+__global__ __launch_bounds__(kStat) void first_kernel(Verify A) {
+  __shared__ double tab[kTab], s_s[kStat / 64];
+  __shared__ int s_child;
+  __shared__ bool s_need;
+  const int b = blockIdx.z, node = blockIdx.y, tid = threadIdx.x;
+  const int* up = A.up + (A.trees > 1 ? (long)b * A.S : 0);
+  const long* tok = A.tokens + (long)b * A.S;
+  const float t = A.temps ? A.temps[b] : A.temp;
+  if (!(t > 0.f)) return;
+  if (tid == 0) s_child = A.S;
+  fill_table(tab);
+  __syncthreads();
+  for (int i = node + 1 + tid; i < A.S; i += kStat)
+    if (up[i] == node && tok[i] >= 0 && tok[i] < A.V) {
+      atomicMin(&s_child, i);
+      break;
+    }
+  __syncthreads();
+  const int child = s_child;
+  if (child == A.S) return;
+  const double k = kTab / ((double)t * kLn2);
+  const Chunks C = chunks_of(A.V);
+  const T* p = (const T*)A.logits + b * A.sb + node * A.ss;
+  const T* q = (const T*)A.draft + b * A.db + node * A.ds;
+  const RowStat P = row_stat(A.part + (((long)b * 2) * A.S + node) * C.n, C.n, tab, k);
+  const RowStat Q = row_stat(A.part + (((long)b * 2 + 1) * A.S + node) * C.n, C.n, tab, k);
+  if (tid == 0) {
+    const double px = prob_of(tab, P, sane((float)p[tok[child]]), k);
+    const double qx = prob_of(tab, Q, sane((float)q[tok[child]]), k);
+    s_need = !first_accepted(A.u[(long)b * A.S + child], px, qx);
+  }
+  __syncthreads();
+  if (!s_need) return;
+  const Rows<T> R(p, q, P, Q, 1.);
+  const int t0 = blockIdx.x * C.size, t1 = t0 + C.size < A.V ? t0 + C.size : A.V;
+  double s = 0.;
+  for (int e = t0 + tid * 8; e < t1; e += kStat * 8) {
+    double r[8];
+    R.left8(r, tab, k, e, t1);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += r[i];
+  }
+  s = sum_in_63(s);
+  if ((tid & 63) == 63) s_s[tid >> 6] = s;
+  __syncthreads();
+  if (tid == 0) {
+    s = 0.;
+#pragma unroll
+    for (int w = 0; w < kStat / 64; ++w) s += s_s[w];
+    A.first[((long)b * A.S + node) * C.n + blockIdx.x] = s;
+  }
+}
+
 constexpr int kWalk = 1024, kWaves = kWalk / 64;
 
 template <typename T>
 __global__ __launch_bounds__(kWalk) void walk_kernel(Verify A) {
   __shared__ double tab[kTab];
-  __shared__ double s_z[2][kMaxNodes];      // 1 / sum of a row's exponentials, 0: no token
-  __shared__ float s_m[2][kMaxNodes];       // its largest logit
+  __shared__ RowStat s_stat[2][kMaxNodes];
   __shared__ double s_px[kMaxNodes], s_qx[kMaxNodes];  // p, q (of the parent) of a node's token
   __shared__ int s_up[kMaxNodes], s_tok[kMaxNodes], s_gone[kMaxNodes], s_top[kMaxNodes];
   __shared__ float s_u[kMaxNodes];
@@ -256,7 +374,7 @@ __global__ __launch_bounds__(kWalk) void walk_kernel(Verify A) {
     s_u[tid] = A.u[(long)b * S + tid];
     A.path[(long)b * S + tid] = tid ? -1 : 0;
     // (rows that stats_kernel left out have neither a probability nor a use)
-    s_z[0][tid] = s_z[1][tid] = 0., s_m[0][tid] = s_m[1][tid] = -__builtin_inff();
+    s_stat[0][tid] = s_stat[1][tid] = RowStat{-__builtin_inff(), 0.};
     s_px[tid] = s_qx[tid] = 0., s_top[tid] = -1;
   }
   __syncthreads();
@@ -269,11 +387,12 @@ __global__ __launch_bounds__(kWalk) void walk_kernel(Verify A) {
       for (int i = lane; i < S; i += 64) inner |= s_up[i] == node;
       if (!__any(inner)) continue;
     }
-    Part P = {-__builtin_inff(), V, 0.};
-    if (lane < C.n) P = A.part[(((long)b * 2 + dr) * S + node) * C.n + lane];
-    float m = P.m;
-    for (int off = 32; off; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+    const Part* p = A.part + (((long)b * 2 + dr) * S + node) * C.n;
     if (greedy) {
+      Part P = {-__builtin_inff(), V, 0.};
+      if (lane < C.n) P = p[lane];
+      float m = P.m;
+      for (int off = 32; off; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
       int at = P.m == m && m > -__builtin_inff() ? P.at : V;
       for (int off = 32; off; off >>= 1) {
         const int q = __shfl_xor(at, off, 64);
@@ -281,51 +400,27 @@ __global__ __launch_bounds__(kWalk) void walk_kernel(Verify A) {
       }
       if (lane == 0) s_top[node] = at < V ? at : -1;
     } else {
-      const double s =
-          sum_in_63(m > -__builtin_inff() ? P.s * exp_of(tab, P.m, m, k) : 0.);
-      if (lane == 63) s_m[dr][node] = m, s_z[dr][node] = s > 0. ? 1. / s : 0.;
+      const RowStat R = row_stat(p, C.n, tab, k);
+      if (lane == 0) s_stat[dr][node] = R;
     }
   }
   __syncthreads();
-  auto prob = [&](int dr, int node, float l) {
-    const double z = s_z[dr][node];
-    return z > 0. ? exp_of(tab, l, s_m[dr][node], k) * z : 0.;
-  };
   if (!greedy && tid < S && s_up[tid] >= 0 && s_tok[tid] >= 0) {
     const int n = s_up[tid];
-    s_px[tid] = prob(0, n, sane((float)lg[n * A.ss + s_tok[tid]]));
-    if (soft) s_qx[tid] = prob(1, n, sane((float)dl[n * A.ds + s_tok[tid]]));
+    s_px[tid] = prob_of(tab, s_stat[0][n], sane((float)lg[n * A.ss + s_tok[tid]]), k);
+    if (soft) s_qx[tid] = prob_of(tab, s_stat[1][n], sane((float)dl[n * A.ds + s_tok[tid]]), k);
   }
   __syncthreads();
 
   int cur = 0, n = 1, ngone = 0;
   double c = 0., mass = 1.;
-  // max(p - c q, 0) of 8 tokens of the current node, less those gone
-  struct Rows {
-    const T *p, *q;
-    double pm, pz, qm, qz;  // largest logits, 1 / sums (c's factor in the drafter's)
-    bool both;
-  };
   auto rows_of = [&]() {
-    Rows R = {lg + cur * A.ss, soft ? dl + cur * A.ds : nullptr, s_m[0][cur], s_z[0][cur],
-              s_m[1][cur], c * s_z[1][cur], c > 0.};
-    if (!(R.pz > 0.)) R.pm = 0.;  // no finite logit: exponents of -inf, sums of 0
-    if (!(s_z[1][cur] > 0.)) R.qm = 0.;
-    return R;
+    return Rows<T>(lg + cur * A.ss, soft ? dl + cur * A.ds : nullptr, s_stat[0][cur],
+                   s_stat[1][cur], c);
   };
-  auto left8 = [&](double r[8], const Rows& R, int e, int end) {
-    float x[8], y[8];
-    load8(x, R.p + e, end - e);
-    if (R.both) load8(y, R.q + e, end - e);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r[i] = exp_of(tab, x[i], R.pm, k) * R.pz;
-    if (R.both) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const double d = r[i] - exp_of(tab, y[i], R.qm, k) * R.qz;
-        r[i] = d > 0. ? d : 0.;
-      }
-    }
+  // 8 tokens of the current node's residual, less those gone
+  auto left8 = [&](double r[8], const Rows<T>& R, int e, int end) {
+    R.left8(r, tab, k, e, end);
     for (int j = 0; j < ngone; ++j) {
       const int g = s_gone[j] - e;
       if (g >= 0 && g < 8)
@@ -335,7 +430,7 @@ __global__ __launch_bounds__(kWalk) void walk_kernel(Verify A) {
     }
   };
   // a chunk's mass, each wave's part of it into s_sum
-  auto sum_chunk = [&](const Rows& R, int ch) {
+  auto sum_chunk = [&](const Rows<T>& R, int ch) {
     const int t0 = ch * C.size, t1 = t0 + C.size < V ? t0 + C.size : V;
     double s = 0.;
     for (int e = t0 + tid * 8; e < t1; e += kWalk * 8) {
@@ -353,6 +448,12 @@ __global__ __launch_bounds__(kWalk) void walk_kernel(Verify A) {
     for (int w = 0; w < kWaves; ++w) s += s_sum[ch][w];
     return s;
   };
+  // all chunks' masses, by every wave
+  auto sum_all = [&]() {
+    double s = 0.;
+    for (int j = lane; j < C.n * kWaves; j += 64) s += s_sum[j / kWaves][j % kWaves];
+    return from_63(sum_in_63(s));
+  };
   for (int i = 1; i < S; ++i) {
     if (s_up[i] != cur) continue;
     const int x = s_tok[i];
@@ -361,15 +462,22 @@ __global__ __launch_bounds__(kWalk) void walk_kernel(Verify A) {
       take = x >= 0 && x == s_top[cur];
     } else if (x >= 0 && mass > kTiny) {
       if (soft) {
-        take = (double)s_u[i] * s_qx[i] * mass < s_px[i] - c * s_qx[i];
+        take = c > 0. ? (double)s_u[i] * s_qx[i] * mass < s_px[i] - c * s_qx[i]
+                      : first_accepted(s_u[i], s_px[i], s_qx[i]);
         if (!take) {
-          c += mass;
           __syncthreads();  // the last sums are read
-          const Rows R = rows_of();
-          for (int ch = 0; ch < C.n; ++ch) sum_chunk(R, ch);
+          if (c > 0.) {
+            c += mass;
+            const Rows<T> R = rows_of();
+            for (int ch = 0; ch < C.n; ++ch) sum_chunk(R, ch);
+          } else {
+            c = 1.;
+            for (int j = tid; j < C.n * kWaves; j += kWalk)
+              s_sum[j / kWaves][j % kWaves] =
+                  j % kWaves ? 0. : A.first[((long)b * S + cur) * C.n + j / kWaves];
+          }
           __syncthreads();
-          mass = 0.;
-          for (int ch = 0; ch < C.n; ++ch) mass += chunk(ch);
+          mass = sum_all();
         }
       } else {
         bool was = false;
@@ -397,7 +505,7 @@ __global__ __launch_bounds__(kWalk) void walk_kernel(Verify A) {
   }
   if (!(mass > kTiny)) c = 0., ngone = 0;  // nothing left: the target itself
 
-  const Rows R = rows_of();
+  const Rows<T> R = rows_of();
   // The draw: the chunk that the target falls into, then the token.  The chunks'
   // masses are those of the last rejection, or the row's own sums, where a token
   // is gone anew.
@@ -405,7 +513,8 @@ __global__ __launch_bounds__(kWalk) void walk_kernel(Verify A) {
     __syncthreads();
     if (tid < C.n) {
       const Part P = A.part[((long)b * 2 * S + cur) * C.n + tid];
-      s_sum[tid][0] = P.m > -__builtin_inff() ? P.s * prob(0, cur, P.m) : 0.;
+      s_sum[tid][0] =
+          P.m > -__builtin_inff() ? P.s * prob_of(tab, s_stat[0][cur], P.m, k) : 0.;
 #pragma unroll
       for (int w = 1; w < kWaves; ++w) s_sum[tid][w] = 0.;
     }
@@ -418,9 +527,7 @@ __global__ __launch_bounds__(kWalk) void walk_kernel(Verify A) {
     }
     __syncthreads();
   }
-  double all = 0.;
-  for (int ch = 0; ch < C.n; ++ch) all += chunk(ch);
-  const double target = (double)s_u[0] * all;
+  const double target = (double)s_u[0] * sum_all();
   int pick = -1;
   double before = 0., cum = 0.;
   for (int ch = 0; ch < C.n; ++ch) {
@@ -482,7 +589,7 @@ __global__ __launch_bounds__(kWalk) void walk_kernel(Verify A) {
 // See include/hn_int4.h.
 extern "C" long hn_verify_tree_workspace_bytes(long B, long S, long V) {
   if (B <= 0 || S <= 0 || V <= 0) return 0;
-  return B * 2 * S * chunks_of(V).n * (long)sizeof(Part);
+  return B * S * chunks_of(V).n * (long)(2 * sizeof(Part) + sizeof(double));
 }
 
 // See include/hn_int4.h.
@@ -509,13 +616,19 @@ extern "C" int hn_verify_tree(const void* logits, long ld_b, long ld_s, const vo
   const bool soft = draft && (temps || temperature > 0.f);
   const Verify A = {logits, draft, ld_b,  ld_s,   ld_db,  ld_ds,  tokens, up,
                     u,      temps, temperature, (int)trees, (int)S, (int)V, path, count,
-                    token,  (Part*)work};
+                    token,  (Part*)work,
+                    (double*)((Part*)work + B * 2 * S * chunks_of(V).n)};
   const dim3 grid((unsigned)chunks_of(V).n, (unsigned)(soft ? 2 * S : S), (unsigned)B);
+  const dim3 nodes((unsigned)chunks_of(V).n, (unsigned)(S - 1), (unsigned)B);
   hipStream_t st = (hipStream_t)stream;
 #define HN_VERIFY(T)                                                            \
   do {                                                                          \
     hipLaunchKernelGGL(stats_kernel<T>, grid, dim3(kStat), 0, st, A);           \
     HN_LAUNCH_CHECK(who);                                                       \
+    if (soft && S > 1) {                                                        \
+      hipLaunchKernelGGL(first_kernel<T>, nodes, dim3(kStat), 0, st, A);        \
+      HN_LAUNCH_CHECK(who);                                                     \
+    }                                                                           \
     hipLaunchKernelGGL(walk_kernel<T>, dim3((unsigned)B), dim3(kWalk), 0, st, A); \
   } while (0)
   if (dtype == 0)
