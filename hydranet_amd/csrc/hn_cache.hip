@@ -55,24 +55,75 @@ __global__ __launch_bounds__(256) void keep_kernel(Layers L, long max_len, int n
     }
 }
 
-struct Pairs {
-  int src[kPairs];
-  int dst[kPairs];
+// Copies, those of one source next to each other: sources src[g], destinations
+// dst[first[g] .. first[g + 1]).
+struct Copies {
+  int src[kPairs], first[kPairs + 1], dst[kPairs];
 };
 
-// Grid (nkv * hd, pairs, layers): the positions of one row of keys, and as many
-// elements of the values.
-__global__ __launch_bounds__(256) void fork_kernel(Layers L, Pairs P, long max_len, int nkv, int hd,
+// By elements, for layers of any alignment: grid (nkv * hd, sources, layers), the
+// positions of one row of keys and as many elements of the values.
+__global__ __launch_bounds__(256) void fork_kernel(Layers L, Copies P, long max_len, int nkv, int hd,
                                                    long n) {
   const int g = blockIdx.x / hd, d = blockIdx.x - g * hd, layer = blockIdx.z;
-  const long a = (long)P.src[blockIdx.y] * nkv + g, b = (long)P.dst[blockIdx.y] * nkv + g;
+  const long a = (long)P.src[blockIdx.y] * nkv + g;
   h16* kt = L.kt[layer];
   h16* v = L.v[layer];
   for (long p = threadIdx.x; p < n; p += blockDim.x) {
-    kt[(b * hd + d) * max_len + p] = kt[(a * hd + d) * max_len + p];
-    v[b * max_len * hd + d * n + p] = v[a * max_len * hd + d * n + p];
+    const h16 kx = kt[(a * hd + d) * max_len + p], vx = v[a * max_len * hd + d * n + p];
+    for (int i = P.first[blockIdx.y]; i < P.first[blockIdx.y + 1]; ++i) {
+      const long b = (long)P.dst[i] * nkv + g;
+      kt[(b * hd + d) * max_len + p] = kx;
+      v[b * max_len * hd + d * n + p] = vx;
+    }
   }
 }
+
+// By vectors of 16 bytes: kVecs of them per thread, all loaded before the first
+// is stored, then stored to every destination.  Grid (chunks of keys, then of
+// values, sources, layers).  The last vector of a row of keys may hold positions
+// past n, which stay as they are in the destination.
+constexpr int kVecs = 8;
+__global__ __launch_bounds__(256) void fork_vec_kernel(Layers L, Copies P, long max_len, int nkv,
+                                                       int hd, int n, int key_chunks) {
+  const int layer = blockIdx.z, sg = blockIdx.y;
+  const bool keys = (int)blockIdx.x < key_chunks;
+  const int nv = keys ? (n + 7) / 8 : n * (hd / 8);  // vectors of a row
+  const int rows = keys ? nkv * hd : nkv;
+  const long pitch = keys ? max_len : max_len * hd;
+  h16* base = keys ? L.kt[layer] : L.v[layer];
+  const long seq = (long)nkv * hd * max_len;
+  const long first = (long)(blockIdx.x - (keys ? 0 : key_chunks)) * (256 * kVecs) + threadIdx.x;
+  const long all = (long)rows * nv;
+  u32x4 x[kVecs];
+  long at[kVecs];
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) {
+    const long idx = first + i * 256;
+    const long row = idx / nv;
+    at[i] = idx < all ? row * pitch + 8 * (idx - row * nv) : -1;
+    if (at[i] >= 0) x[i] = *reinterpret_cast<const u32x4*>(base + P.src[sg] * seq + at[i]);
+  }
+  const int tail = keys && n % 8 ? n % 8 : 8;
+  for (int k = P.first[sg]; k < P.first[sg + 1]; ++k) {
+    h16* out = base + P.dst[k] * seq;
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      if (at[i] < 0) continue;
+      const long idx = first + i * 256;
+      if (tail == 8 || (idx + 1) % nv) {
+        *reinterpret_cast<u32x4*>(out + at[i]) = x[i];
+      } else {
+        const half8_t h = __builtin_bit_cast(half8_t, x[i]);
+#pragma unroll
+        for (int e = 0; e < 7; ++e)
+          if (e < tail) out[at[i] + e] = h[e];
+      }
+    }
+  }
+}
+
+bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 }  // namespace
 
@@ -119,17 +170,36 @@ extern "C" int hn_kv_fork(void* const* kt, void* const* v, long layers, long max
       HN_ARG_CHECK(dst[i] != src[j] && (i == j || dst[i] != dst[j]),
                    "%s: a destination is a source or given twice", who);
   }
-  for (long l0 = 0; l0 < layers; l0 += kLayers)
-    for (long p0 = 0; p0 < pairs; p0 += kPairs) {
+  bool vec = max_len % 8 == 0 && hd % 8 == 0 && n < (1L << 31) / hd;
+  for (long l = 0; l < layers; ++l) vec = vec && al16(kt[l]) && al16(v[l]);
+  for (long p0 = 0; p0 < pairs; p0 += kPairs) {
+    const int np = (int)(pairs - p0 < kPairs ? pairs - p0 : kPairs);
+    Copies P = {};
+    int ns = 0, nd = 0;
+    bool done[kPairs] = {};
+    for (int p = 0; p < np; ++p) {
+      if (done[p]) continue;
+      P.src[ns] = src[p0 + p], P.first[ns] = nd;
+      for (int r = p; r < np; ++r)
+        if (!done[r] && src[p0 + r] == src[p0 + p]) P.dst[nd++] = dst[p0 + r], done[r] = true;
+      P.first[++ns] = nd;
+    }
+    for (long l0 = 0; l0 < layers; l0 += kLayers) {
       const int m = (int)(layers - l0 < kLayers ? layers - l0 : kLayers);
-      const int np = (int)(pairs - p0 < kPairs ? pairs - p0 : kPairs);
       Layers L = {};
-      Pairs P = {};
       for (int l = 0; l < m; ++l) L.kt[l] = (h16*)kt[l0 + l], L.v[l] = (h16*)v[l0 + l];
-      for (int p = 0; p < np; ++p) P.src[p] = src[p0 + p], P.dst[p] = dst[p0 + p];
-      hipLaunchKernelGGL(fork_kernel, dim3((unsigned)(nkv * hd), (unsigned)np, (unsigned)m),
-                         dim3(256), 0, (hipStream_t)stream, L, P, max_len, (int)nkv, (int)hd, n);
+      if (vec) {
+        const long per = 256 * kVecs, kc = (nkv * hd * ((n + 7) / 8) + per - 1) / per,
+                   vc = (nkv * n * (hd / 8) + per - 1) / per;
+        hipLaunchKernelGGL(fork_vec_kernel, dim3((unsigned)(kc + vc), (unsigned)ns, (unsigned)m),
+                           dim3(256), 0, (hipStream_t)stream, L, P, max_len, (int)nkv, (int)hd,
+                           (int)n, (int)kc);
+      } else {
+        hipLaunchKernelGGL(fork_kernel, dim3((unsigned)(nkv * hd), (unsigned)ns, (unsigned)m),
+                           dim3(256), 0, (hipStream_t)stream, L, P, max_len, (int)nkv, (int)hd, n);
+      }
       HN_LAUNCH_CHECK(who);
     }
+  }
   return 0;
 }

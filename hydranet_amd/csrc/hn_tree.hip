@@ -64,7 +64,22 @@ __global__ __launch_bounds__(kMaxNodes) void plan_kernel(const int* __restrict__
   depth[o] = n;
 }
 
-// Grid (B * S, nh + nkv), a thread per element of a head.
+// Where a node goes.  in: its position is in the table and the cache; live: it
+// takes part.
+struct Place {
+  long pos, slot;
+  bool live, in;
+};
+__device__ __forceinline__ Place place(const int* depth, int trees, const long* lens, int b, int i,
+                                       int S, long table_rows, long max_len) {
+  const int dep = depth[(trees > 1 ? (long)b * S : 0) + i];
+  const long C = lens[b];
+  Place p = {C + dep, C + i, C >= 0 && dep >= 0, false};
+  p.in = p.live && p.pos < table_rows && p.slot < max_len;
+  return p;
+}
+
+// A thread per element of a head, grid (B * S, nh + nkv): rows of any alignment.
 __global__ __launch_bounds__(kHd) void append_kernel(
     const h16* __restrict__ qkv, long ld, const float* __restrict__ cos_t,
     const float* __restrict__ sin_t, long table_rows, const int* __restrict__ depth, int trees,
@@ -72,10 +87,9 @@ __global__ __launch_bounds__(kHd) void append_kernel(
     h16* __restrict__ kt, h16* __restrict__ vc, long max_len) {
   const int row = blockIdx.x, head = blockIdx.y, d = threadIdx.x;
   const int b = row / S, i = row - b * S, nh = nkv * rep;
-  const int dep = depth[(trees > 1 ? (long)b * S : 0) + i];
-  const long C = lens[b], pos = C + dep, slot = C + i;
-  const bool live = C >= 0 && dep >= 0;
-  const bool in = live && pos < table_rows && slot < max_len;
+  const Place at = place(depth, trees, lens, b, i, S, table_rows, max_len);
+  const long pos = at.pos, slot = at.slot;
+  const bool live = at.live, in = at.in;
   const h16* src = qkv + (long)row * ld + (long)head * kHd;
   float y = 0.f;
   if (in) {
@@ -91,6 +105,106 @@ __global__ __launch_bounds__(kHd) void append_kernel(
     const int g = head - nh;
     kt[(((long)b * nkv + g) * kHd + d) * max_len + slot] = (h16)y;
     vc[(((long)b * nkv + g) * max_len + slot) * kHd + d] = src[(long)nkv * kHd + d];
+  }
+}
+
+// The same for 16-byte aligned rows: 32 nodes per workgroup, 8 lanes each, a lane
+// 8 elements of a head's lower half and their partners of the upper, so every
+// access of q, k and v is 16 bytes and the angles stay in registers over the
+// heads.  The rotated keys go through LDS, to be written with lanes along the
+// nodes, whose positions are consecutive.  Grid (ceil(B S / 32), ceil(nh / 4) +
+// nkv): groups of query heads, then a KV head each.
+constexpr int kAppend = 32, kHeads = 4, kKPad = kAppend + 2;
+typedef float float8v __attribute__((ext_vector_type(8)));
+
+__device__ __forceinline__ void rotate8(half8_t x, half8_t y, float8v cl, float8v ch, float8v sl,
+                                        float8v sh, half8_t& lo, half8_t& hi) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    lo[e] = (h16)((float)x[e] * cl[e] - (float)y[e] * sl[e]);
+    hi[e] = (h16)((float)y[e] * ch[e] + (float)x[e] * sh[e]);
+  }
+}
+
+__global__ __launch_bounds__(256) void append_rows_kernel(
+    const h16* __restrict__ qkv, long ld, const float* __restrict__ cos_t,
+    const float* __restrict__ sin_t, long table_rows, const int* __restrict__ depth, int trees,
+    const long* __restrict__ lens, int B, int S, int nkv, int rep, h16* __restrict__ q_out,
+    h16* __restrict__ kt, h16* __restrict__ vc, long max_len) {
+  constexpr int half = kHd / 2;
+  __shared__ h16 s_k[kHd * kKPad];
+  const int tid = threadIdx.x, tok = tid >> 3, d = 8 * (tid & 7), nh = nkv * rep;
+  const int row = blockIdx.x * kAppend + tok;
+  const bool there = row < B * S;
+  const int b = there ? row / S : 0, i = there ? row - b * S : 0;
+  const Place at = place(depth, trees, lens, b, i, S, table_rows, max_len);
+  const bool live = at.live && there, in = at.in && there;
+  float8v cl, ch, sl, sh;
+  if (in) {
+    const float* c = cos_t + at.pos * kHd + d;
+    const float* s = sin_t + at.pos * kHd + d;
+    cl = *reinterpret_cast<const float8v*>(c), ch = *reinterpret_cast<const float8v*>(c + half);
+    sl = *reinterpret_cast<const float8v*>(s), sh = *reinterpret_cast<const float8v*>(s + half);
+  }
+  const h16* src = qkv + (long)row * ld;
+  const int groups = (nh + kHeads - 1) / kHeads;
+  if ((int)blockIdx.y < groups) {
+    if (!there) return;
+    const int h0 = blockIdx.y * kHeads;
+    half8_t x[kHeads], y[kHeads];  // all loads before the first store
+    if (in)
+#pragma unroll
+      for (int k = 0; k < kHeads; ++k) {
+        const h16* p = src + (long)(h0 + k < nh ? h0 + k : nh - 1) * kHd + d;
+        x[k] = *reinterpret_cast<const half8_t*>(p);
+        y[k] = *reinterpret_cast<const half8_t*>(p + half);
+      }
+    // zero for padding, NaN past the cache or the table
+    const h16 none = live ? (h16)__builtin_nanf("") : (h16)0.f;
+#pragma unroll
+    for (int k = 0; k < kHeads; ++k) {
+      half8_t lo, hi;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) lo[e] = hi[e] = none;
+      if (in) rotate8(x[k], y[k], cl, ch, sl, sh, lo, hi);
+      if (h0 + k < nh) {
+        h16* dst = q_out + (((long)b * nh + h0 + k) * S + i) * kHd + d;
+        *reinterpret_cast<half8_t*>(dst) = lo;
+        *reinterpret_cast<half8_t*>(dst + half) = hi;
+      }
+    }
+    return;
+  }
+  const int g = blockIdx.y - groups;
+  if (in) {
+    const h16* ks = src + (long)(nh + g) * kHd + d;
+    const h16* vs = src + (long)(nh + nkv + g) * kHd + d;
+    const half8_t x = *reinterpret_cast<const half8_t*>(ks);
+    const half8_t y = *reinterpret_cast<const half8_t*>(ks + half);
+    const half8_t v0 = *reinterpret_cast<const half8_t*>(vs);
+    const half8_t v1 = *reinterpret_cast<const half8_t*>(vs + half);
+    h16* vd = vc + (((long)b * nkv + g) * max_len + at.slot) * kHd + d;
+    *reinterpret_cast<half8_t*>(vd) = v0;
+    *reinterpret_cast<half8_t*>(vd + half) = v1;
+    half8_t lo, hi;
+    rotate8(x, y, cl, ch, sl, sh, lo, hi);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      s_k[(d + e) * kKPad + tok] = lo[e];
+      s_k[(d + half + e) * kKPad + tok] = hi[e];
+    }
+  }
+  __syncthreads();
+  const int r2 = blockIdx.x * kAppend + (tid & (kAppend - 1));
+  if (r2 >= B * S) return;
+  const int b2 = r2 / S, i2 = r2 - b2 * S;
+  const Place to = place(depth, trees, lens, b2, i2, S, table_rows, max_len);
+  if (!to.in) return;
+  h16* kd = kt + ((long)b2 * nkv + g) * kHd * max_len + to.slot;
+#pragma unroll
+  for (int e = 0; e < kHd / 8; ++e) {
+    const int dd = 8 * e + (tid >> 5);
+    kd[(long)dd * max_len] = s_k[dd * kKPad + (tid & (kAppend - 1))];
   }
 }
 
@@ -976,6 +1090,19 @@ extern "C" int hn_tree_append(const void* qkv, long ld_qkv, const float* cos_t, 
   if (B == 0) return 0;
   HN_ARG_CHECK(qkv && cos_t && sin_t && depth && lens && q_out && kt && v, "%s: null operand", who);
   HN_ARG_CHECK(B * S < (1L << 31) && nkv * (rep + 1) <= 65535, "%s: too many rows or heads", who);
+  // Up to 40 nodes the launch's latency is all there is, and the kernel by elements
+  // has less of it: 1, 32, 64, 256 and 512 nodes of 32 + 2 x 8 heads take it 2.0,
+  // 2.7, 3.8, 9.2 and 15.9 us, the other 3.2, 3.1, 3.1, 3.6 and 4.4.
+  if (B * S > 40 && ld_qkv % 8 == 0 && al16(qkv) && al16(cos_t) && al16(sin_t) && al16(q_out) && al16(v)) {
+    hipLaunchKernelGGL(append_rows_kernel,
+                       dim3((unsigned)((B * S + kAppend - 1) / kAppend),
+                            (unsigned)((nkv * rep + kHeads - 1) / kHeads + nkv)),
+                       dim3(256), 0, (hipStream_t)stream, (const h16*)qkv, ld_qkv, cos_t, sin_t,
+                       table_rows, depth, (int)trees, lens, (int)B, (int)S, (int)nkv, (int)rep,
+                       (h16*)q_out, (h16*)kt, (h16*)v, max_len);
+    HN_LAUNCH_CHECK(who);
+    return 0;
+  }
   hipLaunchKernelGGL(append_kernel, dim3((unsigned)(B * S), (unsigned)(nkv * (rep + 1))), dim3(kHd),
                      0, (hipStream_t)stream, (const h16*)qkv, ld_qkv, cos_t, sin_t, table_rows, depth,
                      (int)trees, lens, (int)S, (int)nkv, (int)rep, (h16*)q_out, (h16*)kt, (h16*)v,

@@ -108,18 +108,22 @@ class KVCache:
     def wrap(cls, kt: List[torch.Tensor], v: List[torch.Tensor]) -> "KVCache":
         """A cache over given tensors, one of each kind per layer."""
         assert len(kt) == len(v) > 0 and kt[0].dim() == 4, "kt, v: a tensor per layer"
+        B, nkv, hd, n = kt[0].shape
+        assert all(t.shape == (B, nkv, hd, n) for t in kt) \
+            and all(t.shape == (B, nkv, n, hd) for t in v), \
+            "keys [B, kv_heads, hd, len], values [B, kv_heads, len, hd] in every layer"
         c = cls.__new__(cls)
         c.kt, c.v = list(kt), list(v)
         c.max_len, c.cur_len = kt[0].shape[3], 0
         return c
 
     def _layers(self):
-        """The layers' addresses for the kernels over the whole cache, the layers checked."""
-        B, nkv, hd, n = self.kt[0].shape
-        dev, want, wv = self.kt[0].device, (B, nkv, hd, n), (B, nkv, n, hd)
-        for t, w in [(t, want) for t in self.kt] + [(t, wv) for t in self.v]:
-            assert t.shape == w and t.dtype == torch.float16 and t.device == dev \
-                and t.is_contiguous(), "contiguous fp16 layers of one shape on one device"
+        """The layers' addresses, for the kernels over the whole cache."""
+        n, dev = self.kt[0].numel(), self.kt[0].get_device()
+        for t in (*self.kt, *self.v):
+            if t.numel() != n or t.dtype is not torch.float16 or t.get_device() != dev \
+                    or not t.is_contiguous():
+                raise AssertionError("contiguous fp16 layers of one shape on one device")
         arr = ctypes.c_void_p * len(self.kt)
         return arr(*[t.data_ptr() for t in self.kt]), arr(*[t.data_ptr() for t in self.v])
 

@@ -73,6 +73,29 @@ def test_append(B, nkv, rep, S, lens, n, kind, shared):
     assert torch.equal(c.v[0].double(), want[2])
 
 
+@pytest.mark.parametrize("B,nkv,rep,S,lens,n,kind,extra", [
+    (1, 1, 1, 1, [0], 8, "chain", 0), (1, 8, 4, 5, [1001], 1024, "chain", 8),
+    (5, 2, 3, 33, [0, 7, -1, 500, 480], 512, "padded", 0), (40, 1, 1, 1, list(range(40)), 45, "chain", 0),
+    (2, 1, 12, 256, [100, 1], 360, "random", 16), (3, 3, 3, 31, [50, 3, 17], 88, "roots", 0)])
+def test_append_aligned_rows(B, nkv, rep, S, lens, n, kind, extra):
+    """16-byte aligned rows: 32 nodes per workgroup, across sequences."""
+    g = torch.Generator(device=DEV).manual_seed(S)
+    rng = random.Random(S)
+    rows = [ref.random_tree(rng, S, kind) for _ in range(B)]
+    nh = nkv * rep
+    wide = torch.randn(B * S, (nh + 2 * nkv) * HD + extra, generator=g, device=DEV).half()
+    qkv = wide[:, :(nh + 2 * nkv) * HD]
+    cos, sin = _tables(n - 2)  # the cache's last positions have no table row
+    c = KVCache.wrap([torch.randn(B, nkv, HD, n, generator=g, device=DEV).half()],
+                     [torch.randn(B, nkv, n, HD, generator=g, device=DEV).half()])
+    want = ref.append(qkv, cos, sin, rows, lens, nh, c.kt[0], c.v[0])
+    q = tree_append(qkv, cos, sin, _tree(rows), torch.tensor(lens, device=DEV), c, 0, nh)
+    mag = float(qkv.abs().max()) * 2
+    _close(q, want[0], mag)
+    _close(c.kt[0], want[1], mag)
+    assert torch.equal(c.v[0].double(), want[2])
+
+
 def _attend(B, nkv, rep, S, lens, n, kind, shared=False, bound=None, spoil=True, seed=0, scale=2.0):
     g = torch.Generator(device=DEV).manual_seed(seed + S)
     rng = random.Random(seed + S)
