@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 from dataclasses import dataclass
 from typing import List, Optional
 
@@ -118,14 +119,23 @@ class KVCache:
         return c
 
     def _layers(self):
-        """The layers' addresses, for the kernels over the whole cache."""
-        n, dev = self.kt[0].numel(), self.kt[0].get_device()
-        for t in (*self.kt, *self.v):
-            if t.numel() != n or t.dtype is not torch.float16 or t.get_device() != dev \
-                    or not t.is_contiguous():
-                raise AssertionError("contiguous fp16 layers of one shape on one device")
-        arr = ctypes.c_void_p * len(self.kt)
-        return arr(*[t.data_ptr() for t in self.kt]), arr(*[t.data_ptr() for t in self.v])
+        """The layers' addresses, for the kernels over the whole cache.  The table is
+        the cache's own and is built (and the layers checked) again when a layer is
+        another tensor or has moved."""
+        ptrs = [t.data_ptr() for t in self.kt] + [t.data_ptr() for t in self.v]
+        old = getattr(self, "_table", None)
+        if old is None or old[0] != ptrs or not all(map(operator.is_, old[1], self.kt + self.v)):
+            B, nkv, hd, n = self.kt[0].shape
+            dev = self.kt[0].device
+            for ts, shape in ((self.kt, (B, nkv, hd, n)), (self.v, (B, nkv, n, hd))):
+                assert len(ts) == len(self.kt) and all(
+                    t.shape == shape and t.dtype == torch.float16 and t.device == dev
+                    and t.is_contiguous() for t in ts), \
+                    "contiguous fp16 layers of one shape on one device"
+            arr = ctypes.c_void_p * len(self.kt)
+            m = len(self.kt)
+            old = self._table = (ptrs, self.kt + self.v, arr(*ptrs[:m]), arr(*ptrs[m:]))
+        return old[2], old[3]
 
     def keep(self, lens: torch.Tensor, path: torch.Tensor, count: torch.Tensor) -> torch.Tensor:
         """After a verification (model/speculative.py), the accepted nodes' entries
@@ -363,6 +373,23 @@ class Attention(nn.Module):
         return self.o_proj(o.transpose(1, 2).reshape(B, S, nh * hd))
 
 
+    def forward_tree(self, x: torch.Tensor, rope: "RotaryEmbedding", tree, lens: torch.Tensor,
+                     cache: KVCache, layer: int, kv_bound: int) -> torch.Tensor:
+        """x [B, S, H]: the nodes of a DraftTree after lens [B] cached positions
+        each (model/speculative.py); kv_bound: a host bound of lens + S.  The
+        projections as one product, then hn_tree_append and hn_tree_attention."""
+        from .speculative import tree_append, tree_attention
+        B, S, _ = x.shape
+        if x.is_cuda:
+            qkv = self._qkv(x.reshape(B * S, -1))
+        else:
+            qkv = torch.cat([m(x) for m in (self.q_proj, self.k_proj, self.v_proj)], -1)
+            qkv = qkv.view(B * S, -1)
+        q = tree_append(qkv, rope.cos_cached.float(), rope.sin_cached.float(), tree, lens, cache,
+                        layer, self.nh)
+        return self.o_proj(tree_attention(q, tree, lens, cache, layer, kv_bound))
+
+
 def attn_softmax(scores: torch.Tensor, mask: Optional[torch.Tensor], head_dim: int) -> torch.Tensor:
     """fp16(softmax_fp32(fp16(scores / sqrt(head_dim)) + mask)) over the last
     dim (<= 1024), one launch (hn_attn_softmax): the torch formulation's
@@ -444,14 +471,18 @@ class DecoderBlock(nn.Module):
                                    layer_idx=layer_idx, slots=slots)
 
     def forward(self, x, h, rope, pos, cache: KVCache, kv_len: int, mask, top_k: int,
-                next_norm: "RMSNorm", fold: bool = True):
+                next_norm: "RMSNorm", fold: bool = True, tree=None):
         """x + attn(h), then + moe(norm(.)) (model/mixtral.py:407-427), h =
         input_layernorm(x) given by the caller.  Returns (x after both
         residual adds, next_norm of it): the next block's input and its
         normalised rows.  fold: the MoE output's residual add and next_norm
         run inside the MoE block's last launch where it allows
-        (forward_folded), else as one more launch."""
-        a = self.self_attn(h, rope, pos, cache, self.layer_idx, kv_len, mask)
+        (forward_folded), else as one more launch.  tree: the tokens are the
+        nodes of a DraftTree, pos the sequences' lengths and kv_len their bound."""
+        if tree is not None:
+            a = self.self_attn.forward_tree(h, rope, tree, pos, cache, self.layer_idx, kv_len)
+        else:
+            a = self.self_attn(h, rope, pos, cache, self.layer_idx, kv_len, mask)
         T = h.shape[0] * h.shape[1]
         gw = self.moe.router.gate.weight
         lg = None
@@ -496,17 +527,18 @@ class MixtralDecoder(nn.Module):
                        max_len, dev, self.embed_tokens.weight.dtype)
 
     def step(self, input_ids: torch.Tensor, pos: torch.Tensor, cache: KVCache, kv_len: int,
-             mask: Optional[torch.Tensor], top_k: int) -> torch.Tensor:
+             mask: Optional[torch.Tensor], top_k: int, tree=None) -> torch.Tensor:
         """One pass over every layer: tokens input_ids [B, S] at positions pos
         [S] (device int64), attention over the first kv_len cache positions.
-        Does not move cache.cur_len."""
+        Does not move cache.cur_len.  With a DraftTree, its nodes' tokens after
+        pos [B] cached positions of each sequence (forward_tree)."""
         x = self.embed_tokens(input_ids)
         x, h = add_rmsnorm(x, None, self.layers[0].input_layernorm)
         n = len(self.layers)
         for i, blk in enumerate(self.layers):
             nxt = self.layers[i + 1].input_layernorm if i + 1 < n else self.norm
             x, h = blk(x, h, self.rotary, pos, cache, kv_len, mask, top_k, nxt,
-                       fold=self.fold_moe_norm)
+                       fold=self.fold_moe_norm, tree=tree)
         return self.lm_head(h)
 
     @torch.no_grad()
@@ -547,6 +579,30 @@ class MixtralDecoder(nn.Module):
             tok = self.forward(tok, cache)[:, -1].argmax(-1, keepdim=True)
             out.append(tok)
         return torch.cat(out, dim=1)
+
+
+    @torch.no_grad()
+    def forward_tree(self, tokens: torch.Tensor, tree, lens: torch.Tensor, cache: KVCache,
+                     kv_bound: int, top_k: Optional[int] = None) -> torch.Tensor:
+        """Several drafted tokens per sequence in one pass: tokens [B, S] of a
+        DraftTree's nodes (model/speculative.py), after lens [B] (int64, on the
+        device) cached positions each -> logits [B, S, vocab] after every node.
+        kv_bound: a host bound of lens + S.  Writes cache positions lens to lens +
+        S - 1 and moves no length: KVCache.keep does, after verify_tree."""
+        assert kv_bound <= cache.max_len, f"KV cache full ({kv_bound} > {cache.max_len})"
+        return self.step(tokens, lens, cache, kv_bound, None,
+                         self.decode_top_k if top_k is None else top_k, tree)
+
+    def generate_speculative(self, input_ids: torch.Tensor, max_new_tokens: int, draft=None,
+                             temperature: float = 0.0, samples: int = 1,
+                             generator: Optional[torch.Generator] = None,
+                             max_nodes: int = 64) -> torch.Tensor:
+        """max_new_tokens after each prompt, several of them per pass where the
+        drafter (by default one that looks up repeated tokens) guessed them;
+        distributed as without it.  See model/speculative.py: generate."""
+        from .speculative import generate
+        return generate(self, input_ids, max_new_tokens, draft, temperature, samples, generator,
+                        max_nodes)
 
 
 class GraphDecoder:

@@ -21,7 +21,7 @@ definitions in torch.
 from __future__ import annotations
 
 import math
-from typing import Callable, NamedTuple, Optional, Union
+from typing import Callable, List, NamedTuple, Optional, Union
 
 import numpy as np
 import torch
@@ -316,3 +316,86 @@ def _verify_cpu(logits, tokens, tree, uniforms, draft, temps) -> Verified:
         pos = (r > 0).nonzero()
         token[b] = hit[0, 0] if len(hit) else pos[-1, 0] if len(pos) else -1
     return Verified(path, count, token)
+
+
+class Draft(NamedTuple):
+    tokens: torch.Tensor                  # [B, S - 1] int64: of nodes 1 on
+    parents: torch.Tensor                 # int32 [S] or [B, S], node 0 the last token
+    logits: Optional[torch.Tensor] = None  # [B, S, V]: the drafter's after each node
+
+
+def ngram_draft(history: List[List[int]], device, nodes: int = 8, match: int = 2) -> Draft:
+    """What followed the last earlier occurrence of each sequence's last `match`
+    tokens, as a chain of up to nodes - 1 certain proposals (the n-gram drafters of
+    the reference's inference/speculative.py); a sequence without one gets padding."""
+    rows, parents = [], []
+    for h in history:
+        tail, got = h[-match:], []
+        for at in range(len(h) - match - 1, -1, -1):
+            if h[at:at + match] == tail:
+                got = h[at + match:at + match + nodes - 1]
+                break
+        rows.append(got + [0] * (nodes - 1 - len(got)))
+        parents.append(list(range(-1, len(got))) + [PADDING] * (nodes - 1 - len(got)))
+    return Draft(torch.tensor(rows, dtype=torch.int64, device=device).view(len(rows), nodes - 1),
+                 torch.tensor(parents, dtype=torch.int32, device=device))
+
+
+@torch.no_grad()
+def generate(model, input_ids: torch.Tensor, max_new_tokens: int,
+             draft: Optional[Callable[[List[List[int]], torch.device], Draft]] = None,
+             temperature: float = 0.0, samples: int = 1,
+             generator: Optional[torch.Generator] = None, max_nodes: int = 64) -> torch.Tensor:
+    """Speculative decoding of a MixtralDecoder: prompts [B, P] (one length) ->
+    [samples * B, max_new_tokens], row s * B + b the s-th continuation of prompt b.
+    Each prompt is prefilled once and its cache forked to its samples; a pass then
+    takes the last token and the drafter's tree of each sequence, verifies, and
+    compacts the cache.  draft(history, device) -> Draft, history the tokens of
+    each sequence so far, at most max_nodes nodes.  One host synchronisation per pass."""
+    draft = draft or ngram_draft
+    B, P = input_ids.shape
+    assert samples >= 1 and max_new_tokens >= 1 and P >= 1, "samples, tokens and prompt >= 1"
+    dev, N = input_ids.device, samples * B
+    prompt = input_ids.tolist()
+    history = [list(prompt[i % B]) for i in range(N)]
+    longest = -(-(P + max_new_tokens + max_nodes) // 8) * 8  # a pass writes past what it keeps
+    cache = model.new_cache(N, longest)
+    first = type(cache).wrap([t[:B] for t in cache.kt], [t[:B] for t in cache.v])
+    logits = model.forward(input_ids, first)[:, -1:]
+    cache.fork([i % B for i in range(B, N)], list(range(B, N)), P)
+
+    def uniforms(nodes):
+        return torch.rand((N, nodes), generator=generator, device=dev)
+
+    one = DraftTree.chain(1, dev)
+    last = verify_tree(logits.repeat(samples, 1, 1), torch.zeros((N, 1), dtype=torch.int64,
+                       device=dev), one, uniforms(1), None, temperature).token
+    lens = torch.full((N,), P, dtype=torch.int64, device=dev)
+    size, out = [P] * N, [[] for _ in range(N)]
+
+    def emit(i, tokens):
+        if -1 in tokens:
+            raise RuntimeError(f"sequence {i}: no logit is finite")
+        out[i] += tokens
+        history[i] += tokens
+        return len(out[i]) >= max_new_tokens
+
+    done = [emit(i, [t]) for i, t in enumerate(last.tolist())]
+    while not all(done):
+        if any(done):  # finished sequences take no part
+            lens = torch.where(torch.tensor(done, device=dev), -1, lens)
+        d = draft(history, dev)
+        tree = DraftTree(d.parents)
+        tokens = torch.cat((last.clamp(min=0)[:, None], d.tokens), 1)
+        assert tokens.shape[1] == tree.nodes, f"{tree.nodes} nodes, {d.tokens.shape[1]} tokens"
+        bound = max(n for n, over in zip(size, done) if not over) + tree.nodes
+        logits = model.forward_tree(tokens, tree, lens, cache, bound)
+        r = verify_tree(logits, tokens, tree, uniforms(tree.nodes), d.logits, temperature)
+        lens = cache.keep(lens, r.path, r.count)
+        last = r.token
+        took = torch.gather(tokens, 1, r.path.clamp(min=0).long())
+        for i, (n, t, x) in enumerate(zip(r.count.tolist(), took.tolist(), last.tolist())):
+            if not done[i]:
+                size[i] += n
+                done[i] = emit(i, t[1:n] + [x])
+    return torch.tensor([o[:max_new_tokens] for o in out], dtype=torch.int64, device=dev)

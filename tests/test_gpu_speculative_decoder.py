@@ -1,0 +1,91 @@
+"""GPU test of speculative decoding through the decoder (MixtralDecoder.forward_tree,
+generate_speculative): the trees' logits against the same tokens fed without a
+tree, and that every token generated greedily is a largest logit of a plain
+forward pass over the finished text.
+
+Bar on fp16 logits: |got - ref| <= 3e-2 + 1e-2 |ref|, the decoder tests' bar: the
+two passes run different kernels (experts by numbers of rows, attention with and
+without fp16 scores), whose roundings compound over the layers."""
+import random
+
+import pytest
+import torch
+
+from tests import _tree_ref as ref
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda:0")
+
+
+@pytest.fixture(scope="module")
+def model():
+    from hydranet_amd.model.decoder import MixtralDecoderConfig, build_synthetic_decoder
+    cfg = MixtralDecoderConfig(num_layers=2, hidden_dim=512, intermediate_dim=1024,
+                               num_attention_heads=8, num_kv_heads=2, head_dim=128,
+                               vocab_size=512, num_experts=8, experts_per_token=2,
+                               max_position_embeddings=256)
+    return build_synthetic_decoder(cfg, DEV, decode_top_k=2, seed=3)
+
+
+def _close(got, want):
+    err = (got.float() - want.float()).abs()
+    bound = 3e-2 + 1e-2 * want.float().abs()
+    # (a router's near-tie may fall either way at a few nodes)
+    assert float((err <= bound).float().mean()) >= 0.98
+    return err
+
+
+@pytest.mark.parametrize("kind", ["chain", "random"])
+def test_tree_logits_equal_each_path_alone(model, kind):
+    from hydranet_amd.model.speculative import DraftTree
+    g = torch.Generator(device=DEV).manual_seed(5)
+    B, P, S = 2, 20, 6
+    rng = random.Random(2)
+    row = ref.random_tree(rng, S, kind)
+    ids = torch.randint(0, 512, (B, P), generator=g, device=DEV)
+    nodes = torch.randint(0, 512, (B, S), generator=g, device=DEV)
+    cache = model.new_cache(B, 64)
+    model.forward(ids, cache, top_k=2)
+    lens = torch.full((B,), P, dtype=torch.int64, device=DEV)
+    tree = DraftTree(torch.tensor(row, dtype=torch.int32, device=DEV))
+    got = model.forward_tree(nodes, tree, lens, cache, P + S)
+    for i in range(S):
+        way = ref.way_up(row, i)
+        alone = model.new_cache(B, 64)
+        want = model.forward(torch.cat((ids, nodes[:, way]), 1), alone, top_k=2)[:, -1]
+        _close(got[:, i], want)
+
+
+@pytest.mark.parametrize("samples,temperature", [(1, 0.0), (3, 0.0), (2, 0.9)])
+def test_generate(model, samples, temperature):
+    from hydranet_amd.model.speculative import Draft, ngram_draft
+    g = torch.Generator(device=DEV).manual_seed(7)
+    B, P, n = 2, 9, 21
+    ids = torch.randint(0, 512, (B, P), generator=g, device=DEV)
+    got = model.generate_speculative(ids, n, temperature=temperature, samples=samples, generator=g)
+    assert tuple(got.shape) == (samples * B, n) and int(got.min()) >= 0 and int(got.max()) < 512
+    if temperature:
+        return
+
+    def check(out):
+        text = torch.cat((ids.repeat(samples, 1), out), 1)
+        cache = model.new_cache(samples * B, 64)
+        logits = model.forward(text, cache, top_k=2)[:, P - 1:-1].float()
+        chosen = logits.gather(2, out[..., None])[..., 0]
+        top = logits.max(-1).values
+        assert float((chosen >= top - 2 * (3e-2 + 1e-2 * top.abs())).float().mean()) >= 0.95
+    check(got)
+
+    def known(history, device):
+        """A tree whose second branch is the text that the model generates."""
+        rows = []
+        for i, h in enumerate(history):
+            rest = got[i].tolist()[len(h) - P:][:3]
+            rows.append([1, 2] + rest + [0] * (3 - len(rest)))
+        return Draft(torch.tensor(rows, device=device),
+                     torch.tensor([-1, 0, 1, 0, 3, 4], dtype=torch.int32, device=device))
+    check(model.generate_speculative(ids, n, known, samples=samples))
+    text = [1, 2, 3, 4, 1, 2]
+    d = ngram_draft([text, [5, 6, 7]], DEV, nodes=4)
+    assert d.tokens.tolist() == [[3, 4, 1], [0, 0, 0]]
+    assert d.parents.tolist() == [[-1, 0, 1, 2], [-1, -2, -2, -2]]

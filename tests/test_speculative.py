@@ -218,3 +218,27 @@ def test_library_refusals_without_gpu():
             ("hn_kv_fork", (two, two, 2, 8, 4, 1, 4, i0, i1, 1, 9, None))]:
         with pytest.raises(RuntimeError, match=name):
             _lib.call(name, *args)
+
+
+def test_attention_module_chain_equals_one_token_steps():
+    """Attention.forward_tree over a chain equals its one-token steps, float64."""
+    from hydranet_amd.model.decoder import Attention, MixtralDecoderConfig, RotaryEmbedding
+    torch.manual_seed(0)
+    cfg = MixtralDecoderConfig(num_layers=1, hidden_dim=64, num_attention_heads=4,
+                               num_kv_heads=2, head_dim=16, max_position_embeddings=32)
+    att = Attention(cfg).double()
+    rope = RotaryEmbedding(16, 32, 1e6)
+    B, S = 2, 6
+    x = torch.randn(B, S, 64, dtype=torch.float64)
+    one, tree = _cache(B, 2, 16, 24), _cache(B, 2, 16, 24)
+    want = [att(x[:, t:t + 1], rope, torch.tensor([t]), one, 0, t + 1) for t in range(S)]
+    got = att.forward_tree(x, rope, DraftTree.chain(S), torch.zeros(B, dtype=torch.int64), tree, 0, S)
+    # the one-token steps' softmax is fp32
+    torch.testing.assert_close(got, torch.cat(want, 1), rtol=1e-5, atol=1e-6)
+
+
+def test_ngram_draft():
+    from hydranet_amd.model.speculative import ngram_draft
+    d = ngram_draft([[1, 2, 3, 1, 2], [4]], "cpu", nodes=4)
+    assert d.tokens.tolist() == [[3, 1, 2], [0, 0, 0]]
+    assert d.parents.tolist() == [[-1, 0, 1, 2], [-1, PADDING, PADDING, PADDING]]
