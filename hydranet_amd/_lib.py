@@ -122,12 +122,16 @@ def call(name: str, *args) -> None:
 
 
 def call_on(device: torch.device, name: str, *args) -> None:
-    """call() with `device` as the current device, where its stream launches."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        call(name, *args)
+    """call() on the current stream of `device`, added as the last argument, with it
+    as the current device."""
+    at = torch.cuda.current_device()
+    index = at if device.index is None else device.index
+    stream_ = torch._C._cuda_getCurrentRawStream(index)
+    if index == at:
+        call(name, *args, stream_)
     else:
         with torch.cuda.device(device):
-            call(name, *args)
+            call(name, *args, stream_)
 
 
 _DECODE_PATH = threading.local()

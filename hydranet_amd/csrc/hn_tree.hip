@@ -851,8 +851,7 @@ __global__ __launch_bounds__(256, 2) void share_kernel(Attend A) {
     constexpr bool EDGE = decltype(edge_stage)::value;
     const int p0 = W.first * kPos + st * SP + pg * WP;
     const uint32_t at = (uint32_t)(st % D) * kStage;
-    // operands are read one group of products ahead, no further: the scheduler
-    // would else fill the registers with them
+    // operands are read one group of products ahead
     float4v s[RT][JB];
     half8_t ka[2][4];
     auto keys = [&](int j) {
@@ -871,7 +870,6 @@ __global__ __launch_bounds__(256, 2) void share_kernel(Attend A) {
 #pragma unroll
         for (int t = 0; t < RT; ++t)
           s[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[j & 1][u], q[t][u], s[t][j], 0, 0, 0);
-      __builtin_amdgcn_sched_barrier(0);
     }
 #pragma unroll
     for (int t = 0; t < RT; ++t) {
@@ -955,7 +953,6 @@ __global__ __launch_bounds__(256, 2) void share_kernel(Attend A) {
         for (int t = 0; t < RT; ++t)
           o[t][e0 + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, p[t][x], o[t][e0 + e], 0, 0, 0);
       }
-      __builtin_amdgcn_sched_barrier(0);
     }
   };
 

@@ -21,10 +21,9 @@
 // stats_kernel reads every row once, over the whole chip: per row and chunk of
 // tokens the largest logit, its index and the sum of exponentials.  With a
 // drafter's logits, first_kernel has S(1) of the nodes whose first child is
-// rejected in the same way.  walk_kernel, one workgroup per sequence, has every
-// row's sum and every node's two probabilities from that with one round of
-// loads, walks the tree in LDS, and reads a row again only where it must: both
-// rows of a node per further rejection (S(c)), and one chunk for the draw.
+// rejected in the same way, and node_kernel what becomes of each node's children.
+// walk_kernel, one workgroup per sequence, follows that, or tests certain
+// proposals in LDS, and reads a row again only for the draw: one chunk.
 #include <float.h>
 
 #include "hn_common.h"
@@ -87,22 +86,28 @@ __device__ __forceinline__ void load8(float x[8], const T* p, int left) {
 }
 
 // x of another lane by a data-parallel-primitive move, 0 where there is none
-template <int CTL>
+template <int CTL, int ROWS = 0xf>
 __device__ __forceinline__ double moved(double x) {
   const unsigned long long w = __builtin_bit_cast(unsigned long long, x);
-  const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)w, CTL, 0xf, 0xf, false);
-  const unsigned hi = __builtin_amdgcn_update_dpp(0, (int)(w >> 32), CTL, 0xf, 0xf, false);
+  const unsigned lo = __builtin_amdgcn_update_dpp(0, (int)w, CTL, ROWS, 0xf, false);
+  const unsigned hi = __builtin_amdgcn_update_dpp(0, (int)(w >> 32), CTL, ROWS, 0xf, false);
   return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
 }
-// Sum over the wave, in lane 63: within rows of 16, then over the rows.
-__device__ __forceinline__ double sum_in_63(double x) {
+// Sums of the lanes up to each, within rows of 16, then over the rows.
+__device__ __forceinline__ double scan(double x) {
   x += moved<0x111>(x);  // row_shr:1, 2, 4, 8
   x += moved<0x112>(x);
   x += moved<0x114>(x);
   x += moved<0x118>(x);
-  x += moved<0x142>(x);  // row_bcast:15
-  x += moved<0x143>(x);  // row_bcast:31
+  x += moved<0x142, 0xa>(x);  // row_bcast:15 into rows 1 and 3
+  x += moved<0x143, 0xc>(x);  // row_bcast:31 into rows 2 and 3
   return x;
+}
+__device__ __forceinline__ double lane_of(double x, int l) {
+  const unsigned long long w = __builtin_bit_cast(unsigned long long, x);
+  const unsigned lo = __builtin_amdgcn_readlane((int)w, l);
+  const unsigned hi = __builtin_amdgcn_readlane((int)(w >> 32), l);
+  return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
 }
 
 // What a chunk of a row comes to.
@@ -123,6 +128,7 @@ __host__ __device__ inline Chunks chunks_of(long V) {
   return Chunks{(int)((blocks + per - 1) / per), (int)(per * kBlock)};
 }
 
+struct Next;
 struct Verify {
   const void *logits, *draft;
   long sb, ss, db, ds;
@@ -135,7 +141,8 @@ struct Verify {
   int* count;
   long* token;
   Part* part;     // [B][2][S][chunks]: the target's rows, the drafter's
-  double* first;  // [B][S][chunks]: S(1) of a node whose first child is rejected
+  double* first;  // [B][S][chunks]: the last S(c) of a node whose first child is rejected
+  Next* next;           // [B][S]
 };
 
 constexpr int kStat = 256;
@@ -154,6 +161,21 @@ __global__ __launch_bounds__(kStat) void stats_kernel(Verify A) {
   const int* up = A.up + (A.trees > 1 ? (long)b * A.S : 0);
   const float t = A.temps ? A.temps[b] : A.temp;
   const bool greedy = !(t > 0.f);
+  fill_table(tab);
+  const double k = greedy ? 0. : kTab / ((double)t * kLn2);
+  const T* row = (const T*)(dr ? A.draft : A.logits) +
+                 (dr ? b * A.db + node * A.ds : b * A.sb + node * A.ss);
+  const Chunks C = chunks_of(A.V);
+  const int t0 = blockIdx.x * C.size, t1 = t0 + C.size < A.V ? t0 + C.size : A.V;
+  float x[kVec][8];
+  auto load = [&](int o) {
+#pragma unroll
+    for (int j = 0; j < kVec; ++j) {
+      const int e = o + (j * kStat + tid) * 8;
+      load8(x[j], row + e, e < t1 ? t1 - e : 0);
+    }
+  };
+  if (!dr) load(t0);  // under the round trip of the checks
   if (dr && greedy) return;
   if (node && up[node] == -2) return;
   if (dr) {
@@ -161,20 +183,9 @@ __global__ __launch_bounds__(kStat) void stats_kernel(Verify A) {
     for (int i = node + 1 + tid; i < A.S; i += kStat) inner |= up[i] == node;
     if (!__syncthreads_or(inner)) return;
   }
-  fill_table(tab);
-  const double k = greedy ? 0. : kTab / ((double)t * kLn2);
-  const T* row = (const T*)(dr ? A.draft : A.logits) +
-                 (dr ? b * A.db + node * A.ds : b * A.sb + node * A.ss);
-  const Chunks C = chunks_of(A.V);
-  const int t0 = blockIdx.x * C.size, t1 = t0 + C.size < A.V ? t0 + C.size : A.V;
   Part P = {-__builtin_inff(), A.V, 0.};
   for (int o = t0; o < t1; o += kBlock) {
-    float x[kVec][8];
-#pragma unroll
-    for (int j = 0; j < kVec; ++j) {
-      const int e = o + (j * kStat + tid) * 8;
-      load8(x[j], row + e, e < t1 ? t1 - e : 0);
-    }
+    if (dr || o > t0) load(o);
     float m = -__builtin_inff();
 #pragma unroll
     for (int j = 0; j < kVec; ++j)
@@ -205,7 +216,7 @@ __global__ __launch_bounds__(kStat) void stats_kernel(Verify A) {
       for (int j = 0; j < kVec; ++j)
 #pragma unroll
         for (int i = 0; i < 8; ++i) s += exp_of(tab, x[j][i], m, k);
-      s = sum_in_63(s);
+      s = scan(s);
     }
     if ((tid & 63) == 63) s_at[wave] = at, s_s[wave] = s;
     __syncthreads();
@@ -239,12 +250,6 @@ __device__ __forceinline__ bool first_accepted(float u, double px, double qx) {
 #pragma clang fp contract(off)
   return (double)u * qx < px;
 }
-__device__ __forceinline__ double from_63(double x) {
-  const unsigned long long w = __builtin_bit_cast(unsigned long long, x);
-  const unsigned lo = __builtin_amdgcn_readlane((int)w, 63);
-  const unsigned hi = __builtin_amdgcn_readlane((int)(w >> 32), 63);
-  return __builtin_bit_cast(double, (unsigned long long)hi << 32 | lo);
-}
 __device__ __forceinline__ RowStat row_stat(const Part* p, int chunks, const double* tab, double k) {
   const int lane = threadIdx.x & 63;
   Part P = {-__builtin_inff(), 0, 0.};
@@ -252,7 +257,7 @@ __device__ __forceinline__ RowStat row_stat(const Part* p, int chunks, const dou
   float m = P.m;
   for (int off = 32; off; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
   const bool any = m > -__builtin_inff();
-  const double s = from_63(sum_in_63(any ? P.s * exp_of(tab, P.m, m, k) : 0.));
+  const double s = lane_of(scan(any ? P.s * exp_of(tab, P.m, m, k) : 0.), 63);
   return RowStat{m, s > 0. ? 1. / s : 0.};
 }
 __device__ __forceinline__ double prob_of(const double* tab, const RowStat& r, float l, double k) {
@@ -333,7 +338,7 @@ __global__ __launch_bounds__(kStat) void first_kernel(Verify A) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) s += r[i];
   }
-  s = sum_in_63(s);
+  s = scan(s);
   if ((tid & 63) == 63) s_s[tid >> 6] = s;
   __syncthreads();
   if (tid == 0) {
@@ -346,15 +351,113 @@ __global__ __launch_bounds__(kStat) void first_kernel(Verify A) {
 
 constexpr int kWalk = 1024, kWaves = kWalk / 64;
 
+// A chunk's mass, each wave's part of it into sum[ch], by a workgroup of kWalk.
+template <typename F>
+__device__ __forceinline__ void sum_chunk(F left8, const Chunks& C, int V, int ch,
+                                          double (*sum)[kWaves]) {
+  const int t0 = ch * C.size, t1 = t0 + C.size < V ? t0 + C.size : V, tid = threadIdx.x;
+  double s = 0.;
+  for (int e = t0 + tid * 8; e < t1; e += kWalk * 8) {
+    double r[8];
+    left8(r, e, t1);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += r[i];
+  }
+  s = scan(s);
+  if ((tid & 63) == 63) sum[ch][tid >> 6] = s;
+}
+
+// Where the walk goes from a node, with a drafter's logits: a workgroup per node,
+// since a node's tests start at c = 0 whatever came before, so all nodes' further
+// rejections (a pass over both rows each) run side by side.
+struct Next {
+  int node;        // the accepted child, or -1
+  double c, mass;  // else the residual's c and S(c); its chunks' masses are in first
+};
+
+template <typename T>
+__global__ __launch_bounds__(kWalk) void node_kernel(Verify A) {
+  __shared__ double tab[kTab];
+  __shared__ RowStat s_stat[2];
+  __shared__ double s_px[kMaxNodes], s_qx[kMaxNodes];
+  __shared__ float s_u[kMaxNodes];
+  __shared__ bool s_kid[kMaxNodes];  // a child whose token is in the vocabulary
+  __shared__ double s_sum[kMaxChunks][kWaves];
+  const int b = blockIdx.y, node = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const int S = A.S, V = A.V;
+  const float t = A.temps ? A.temps[b] : A.temp;
+  if (!(t > 0.f)) return;
+  const int* up = A.up + (A.trees > 1 ? (long)b * S : 0);
+  const T* p = (const T*)A.logits + b * A.sb + node * A.ss;
+  const T* q = (const T*)A.draft + b * A.db + node * A.ds;
+  float lp = 0.f, lq = 0.f;
+  bool kid = false;
+  if (tid > node && tid < S && up[tid] == node) {
+    const long x = A.tokens[(long)b * S + tid];
+    kid = x >= 0 && x < V;
+    if (kid) lp = sane((float)p[x]), lq = sane((float)q[x]), s_u[tid] = A.u[(long)b * S + tid];
+  }
+  if (tid < S) s_kid[tid] = kid;
+  fill_table(tab);
+  Next N = {-1, 0., 1.};
+  if (__syncthreads_or(kid)) {
+    const double k = kTab / ((double)t * kLn2);
+    const Chunks C = chunks_of(V);
+    if (tid < 128) {
+      const RowStat R =
+          row_stat(A.part + (((long)b * 2 + (tid >> 6)) * S + node) * C.n, C.n, tab, k);
+      if (lane == 0) s_stat[tid >> 6] = R;
+    }
+    __syncthreads();
+    if (kid) {
+      s_px[tid] = prob_of(tab, s_stat[0], lp, k);
+      s_qx[tid] = prob_of(tab, s_stat[1], lq, k);
+    }
+    __syncthreads();
+    double* first = A.first + ((long)b * S + node) * C.n;
+    bool again = false;
+    for (int i = node + 1; i < S && N.mass > kTiny; ++i) {
+      if (!s_kid[i]) continue;
+      if (N.c > 0. ? (double)s_u[i] * s_qx[i] * N.mass < s_px[i] - N.c * s_qx[i]
+                   : first_accepted(s_u[i], s_px[i], s_qx[i])) {
+        N.node = i;
+        break;
+      }
+      double s = 0.;
+      if (N.c > 0.) {
+        N.c += N.mass, again = true;
+        const Rows<T> R(p, q, s_stat[0], s_stat[1], N.c);
+        __syncthreads();  // the last sums are read
+        for (int ch = 0; ch < C.n; ++ch)
+          sum_chunk([&](double r[8], int e, int end) { R.left8(r, tab, k, e, end); }, C, V, ch,
+                    s_sum);
+        __syncthreads();
+        for (int j = lane; j < C.n * kWaves; j += 64) s += s_sum[j / kWaves][j % kWaves];
+      } else {
+        N.c = 1.;
+        if (lane < C.n) s = first[lane];
+      }
+      N.mass = lane_of(scan(s), 63);
+    }
+    if (N.node < 0 && again && tid < C.n) {
+      double s = 0.;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) s += s_sum[tid][w];
+      first[tid] = s;
+    }
+  }
+  if (tid == 0) A.next[(long)b * S + node] = N;
+}
+
+// The walk from node 0, one workgroup per sequence, and the draw.
 template <typename T>
 __global__ __launch_bounds__(kWalk) void walk_kernel(Verify A) {
   __shared__ double tab[kTab];
-  __shared__ RowStat s_stat[2][kMaxNodes];
-  __shared__ double s_px[kMaxNodes], s_qx[kMaxNodes];  // p, q (of the parent) of a node's token
-  __shared__ int s_up[kMaxNodes], s_tok[kMaxNodes], s_gone[kMaxNodes], s_top[kMaxNodes];
+  __shared__ RowStat s_stat[2];
+  __shared__ int s_up[kMaxNodes], s_tok[kMaxNodes], s_top[kMaxNodes], s_gone[kMaxNodes];
   __shared__ float s_u[kMaxNodes];
-  __shared__ double s_sum[kMaxChunks][kWaves];
-  __shared__ double s_scan[kWaves];
+  __shared__ double s_p[kMaxNodes], s_mass[kMaxNodes];  // p of a node's token; or Next's c, mass
+  __shared__ double s_sum[kMaxChunks][kWaves], s_tot[kMaxChunks], s_scan[kWaves];
   __shared__ int s_pick, s_last;
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -365,137 +468,78 @@ __global__ __launch_bounds__(kWalk) void walk_kernel(Verify A) {
   const double k = greedy ? 0. : kTab / ((double)tb * kLn2);
   const T* lg = (const T*)A.logits + b * A.sb;
   const T* dl = soft ? (const T*)A.draft + b * A.db : nullptr;
-  fill_table(tab);
+  const Part* part = A.part + (long)b * 2 * S * C.n;  // the target's rows
   if (tid < S) {
-    const int up = A.up[(A.trees > 1 ? (long)b * S : 0) + tid];
-    const long x = A.tokens[(long)b * S + tid];
-    s_up[tid] = tid ? up : -1;
-    s_tok[tid] = x >= 0 && x < V ? (int)x : -1;
+    const int up = tid ? A.up[(A.trees > 1 ? (long)b * S : 0) + tid] : -1;
+    if (soft) {
+      const Next N = A.next[(long)b * S + tid];
+      s_up[tid] = N.node, s_p[tid] = N.c, s_mass[tid] = N.mass;
+    } else {
+      const long x = A.tokens[(long)b * S + tid];
+      s_up[tid] = up;
+      s_tok[tid] = x >= 0 && x < V ? (int)x : -1;
+    }
     s_u[tid] = A.u[(long)b * S + tid];
     A.path[(long)b * S + tid] = tid ? -1 : 0;
-    // (rows that stats_kernel left out have neither a probability nor a use)
-    s_stat[0][tid] = s_stat[1][tid] = RowStat{-__builtin_inff(), 0.};
-    s_px[tid] = s_qx[tid] = 0., s_top[tid] = -1;
   }
-  __syncthreads();
-  // every row's largest logit and sum, a wave per row, a lane per chunk
-  for (int r = wave; r < (soft ? 2 : 1) * S; r += kWaves) {
-    const int dr = r >= S, node = r - (dr ? S : 0);
-    if (s_up[node] == -2) continue;
-    if (dr) {
-      bool inner = false;
-      for (int i = lane; i < S; i += 64) inner |= s_up[i] == node;
-      if (!__any(inner)) continue;
-    }
-    const Part* p = A.part + (((long)b * 2 + dr) * S + node) * C.n;
-    if (greedy) {
-      Part P = {-__builtin_inff(), V, 0.};
-      if (lane < C.n) P = p[lane];
-      float m = P.m;
-      for (int off = 32; off; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-      int at = P.m == m && m > -__builtin_inff() ? P.at : V;
-      for (int off = 32; off; off >>= 1) {
-        const int q = __shfl_xor(at, off, 64);
-        at = q < at ? q : at;
-      }
-      if (lane == 0) s_top[node] = at < V ? at : -1;
-    } else {
-      const RowStat R = row_stat(p, C.n, tab, k);
-      if (lane == 0) s_stat[dr][node] = R;
-    }
-  }
-  __syncthreads();
-  if (!greedy && tid < S && s_up[tid] >= 0 && s_tok[tid] >= 0) {
-    const int n = s_up[tid];
-    s_px[tid] = prob_of(tab, s_stat[0][n], sane((float)lg[n * A.ss + s_tok[tid]]), k);
-    if (soft) s_qx[tid] = prob_of(tab, s_stat[1][n], sane((float)dl[n * A.ds + s_tok[tid]]), k);
-  }
+  fill_table(tab);
   __syncthreads();
 
   int cur = 0, n = 1, ngone = 0;
   double c = 0., mass = 1.;
-  auto rows_of = [&]() {
-    return Rows<T>(lg + cur * A.ss, soft ? dl + cur * A.ds : nullptr, s_stat[0][cur],
-                   s_stat[1][cur], c);
+  auto accept = [&](int i) {
+    cur = i;
+    if (tid == 0) A.path[(long)b * S + n] = i;
+    ++n;
   };
-  // 8 tokens of the current node's residual, less those gone
-  auto left8 = [&](double r[8], const Rows<T>& R, int e, int end) {
-    R.left8(r, tab, k, e, end);
-    for (int j = 0; j < ngone; ++j) {
-      const int g = s_gone[j] - e;
-      if (g >= 0 && g < 8)
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (i == g) r[i] = 0.;
-    }
-  };
-  // a chunk's mass, each wave's part of it into s_sum
-  auto sum_chunk = [&](const Rows<T>& R, int ch) {
-    const int t0 = ch * C.size, t1 = t0 + C.size < V ? t0 + C.size : V;
-    double s = 0.;
-    for (int e = t0 + tid * 8; e < t1; e += kWalk * 8) {
-      double r[8];
-      left8(r, R, e, t1);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s += r[i];
-    }
-    s = sum_in_63(s);
-    if (lane == 63) s_sum[ch][wave] = s;
-  };
-  auto chunk = [&](int ch) {
-    double s = 0.;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) s += s_sum[ch][w];
-    return s;
-  };
-  // all chunks' masses, by every wave
-  auto sum_all = [&]() {
-    double s = 0.;
-    for (int j = lane; j < C.n * kWaves; j += 64) s += s_sum[j / kWaves][j % kWaves];
-    return from_63(sum_in_63(s));
-  };
-  for (int i = 1; i < S; ++i) {
-    if (s_up[i] != cur) continue;
-    const int x = s_tok[i];
-    bool take = false;
-    if (greedy) {
-      take = x >= 0 && x == s_top[cur];
-    } else if (x >= 0 && mass > kTiny) {
-      if (soft) {
-        take = c > 0. ? (double)s_u[i] * s_qx[i] * mass < s_px[i] - c * s_qx[i]
-                      : first_accepted(s_u[i], s_px[i], s_qx[i]);
-        if (!take) {
-          __syncthreads();  // the last sums are read
-          if (c > 0.) {
-            c += mass;
-            const Rows<T> R = rows_of();
-            for (int ch = 0; ch < C.n; ++ch) sum_chunk(R, ch);
-          } else {
-            c = 1.;
-            for (int j = tid; j < C.n * kWaves; j += kWalk)
-              s_sum[j / kWaves][j % kWaves] =
-                  j % kWaves ? 0. : A.first[((long)b * S + cur) * C.n + j / kWaves];
-          }
-          __syncthreads();
-          mass = sum_all();
+  if (soft) {
+    for (int i = s_up[0]; i > cur; i = s_up[cur]) accept(i);
+    c = s_p[cur], mass = s_mass[cur];
+  } else {
+    // a wave per row: its largest logit's index, or 1 / its sum and, of the row's
+    // children, their tokens' probabilities
+    for (int node = wave; node < S; node += kWaves) {
+      if (s_up[node] == -2) continue;
+      const Part* pr = part + (long)node * C.n;
+      if (greedy) {
+        Part P = {-__builtin_inff(), V, 0.};
+        if (lane < C.n) P = pr[lane];
+        float m = P.m;
+        for (int off = 32; off; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+        int at = P.m == m && m > -__builtin_inff() ? P.at : V;
+        for (int off = 32; off; off >>= 1) {
+          const int q = __shfl_xor(at, off, 64);
+          at = q < at ? q : at;
         }
+        if (lane == 0) s_top[node] = at < V ? at : -1;
       } else {
-        bool was = false;
-        for (int j = 0; j < ngone; ++j) was |= s_gone[j] == x;
-        take = !was && (double)s_u[i] * mass < s_px[i];
-        if (!take && !was) {
-          mass -= s_px[i];
-          __syncthreads();
-          if (tid == 0) s_gone[ngone] = x;
-          __syncthreads();
-          ++ngone;
-        }
+        const RowStat R = row_stat(pr, C.n, tab, k);
+        for (int i = node + 1 + lane; i < S; i += 64)
+          if (s_up[i] == node && s_tok[i] >= 0)
+            s_p[i] = prob_of(tab, R, sane((float)lg[node * A.ss + s_tok[i]]), k);
       }
     }
-    if (take) {
-      cur = i, c = 0., mass = 1., ngone = 0;
-      if (tid == 0) A.path[(long)b * S + n] = i;
-      ++n;
+    __syncthreads();
+    for (int i = 1; i < S; ++i) {
+      if (s_up[i] != cur || s_tok[i] < 0) continue;
+      const int x = s_tok[i];
+      if (greedy) {
+        if (x == s_top[cur]) accept(i);
+        continue;
+      }
+      if (!(mass > kTiny)) continue;
+      bool was = false;
+      for (int j = 0; j < ngone; ++j) was |= s_gone[j] == x;
+      if (was) continue;
+      if ((double)s_u[i] * mass < s_p[i]) {
+        accept(i), mass = 1., ngone = 0;
+      } else {
+        mass -= s_p[i];
+        __syncthreads();
+        if (tid == 0) s_gone[ngone] = x;
+        __syncthreads();
+        ++ngone;
+      }
     }
   }
   if (tid == 0) A.count[b] = n;
@@ -505,59 +549,74 @@ __global__ __launch_bounds__(kWalk) void walk_kernel(Verify A) {
   }
   if (!(mass > kTiny)) c = 0., ngone = 0;  // nothing left: the target itself
 
-  const Rows<T> R = rows_of();
   // The draw: the chunk that the target falls into, then the token.  The chunks'
   // masses are those of the last rejection, or the row's own sums, where a token
   // is gone anew.
-  if (c == 0.) {
-    __syncthreads();
-    if (tid < C.n) {
-      const Part P = A.part[((long)b * 2 * S + cur) * C.n + tid];
-      s_sum[tid][0] =
-          P.m > -__builtin_inff() ? P.s * prob_of(tab, s_stat[0][cur], P.m, k) : 0.;
-#pragma unroll
-      for (int w = 1; w < kWaves; ++w) s_sum[tid][w] = 0.;
+  if (tid < (soft ? 128 : 64)) {
+    const Part* pr = part + ((long)(tid >> 6) * S + cur) * C.n;
+    const RowStat R = row_stat(pr, C.n, tab, k);
+    if (lane == 0) s_stat[tid >> 6] = R;
+    if (c == 0. && tid < C.n) {
+      const Part P = pr[tid];
+      s_tot[tid] = P.m > -__builtin_inff() ? P.s * prob_of(tab, R, P.m, k) : 0.;
     }
-    __syncthreads();
+  } else if (c > 0. && wave == kWaves - 1 && lane < C.n) {
+    s_tot[lane] = A.first[((long)b * S + cur) * C.n + lane];
+  }
+  __syncthreads();
+  const Rows<T> R(lg + cur * A.ss, soft ? dl + cur * A.ds : nullptr, s_stat[0],
+                  soft ? s_stat[1] : RowStat{0.f, 0.}, c);
+  // 8 tokens of the residual, less those gone
+  auto left8 = [&](double r[8], int e, int end) {
+    R.left8(r, tab, k, e, end);
     for (int j = 0; j < ngone; ++j) {
-      const int ch = s_gone[j] / C.size;
-      bool done = false;
-      for (int q = 0; q < j; ++q) done |= s_gone[q] / C.size == ch;
-      if (!done) sum_chunk(R, ch);
+      const int g = s_gone[j] - e;
+      if (g >= 0 && g < 8)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i == g) r[i] = 0.;
+    }
+  };
+  for (int j = 0; j < ngone; ++j) {
+    const int ch = s_gone[j] / C.size;
+    bool done = false;
+    for (int q = 0; q < j; ++q) done |= s_gone[q] / C.size == ch;
+    if (!done) sum_chunk(left8, C, V, ch, s_sum);
+  }
+  if (tid == 0) s_pick = V, s_last = -1;
+  __syncthreads();
+  if (ngone) {
+    if (tid < ngone) {
+      double s = 0.;
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) s += s_sum[s_gone[tid] / C.size][w];
+      s_tot[s_gone[tid] / C.size] = s;  // the same value from every token of the chunk
     }
     __syncthreads();
   }
-  const double target = (double)s_u[0] * sum_all();
-  int pick = -1;
-  double before = 0., cum = 0.;
-  for (int ch = 0; ch < C.n; ++ch) {
-    const double s = chunk(ch);
-    if (s > 0.) pick = ch, before = cum;  // the last that has any, if none exceeds
-    cum += s;
-    if (s > 0. && cum > target) break;
-  }
-  if (pick < 0) {  // no logit is finite
+  // a lane per chunk
+  const double tot = lane < C.n ? s_tot[lane] : 0., cum = scan(tot);
+  const double target = (double)s_u[0] * lane_of(cum, 63);
+  const unsigned long long some = __ballot(tot > 0.), over = __ballot(tot > 0. && cum > target);
+  if (!some) {  // no logit is finite
     if (tid == 0) A.token[b] = -1;
     return;
   }
+  // the last that has any, if none exceeds the target
+  const int pick = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(some);
+  double before = lane_of(cum, pick) - lane_of(tot, pick);
   const int t0 = pick * C.size, t1 = t0 + C.size < V ? t0 + C.size : V;
-  if (tid == 0) s_pick = V, s_last = -1;
-  __syncthreads();
   for (int o = t0; o < t1; o += kBlock) {
     const int e = o + tid * 8;
     double r[8], sum = 0.;
     if (e < t1)
-      left8(r, R, e, t1);
+      left8(r, e, t1);
     else
 #pragma unroll
       for (int i = 0; i < 8; ++i) r[i] = 0.;
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum += r[i];
-    double run = sum;  // inclusive over the wave
-    for (int off = 1; off < 64; off <<= 1) {
-      const double y = __shfl_up(run, off, 64);
-      if (lane >= off) run += y;
-    }
+    double run = scan(sum);
     if (lane == 63) s_scan[wave] = run;
     __syncthreads();
     double base = before, total = before;
@@ -589,7 +648,7 @@ __global__ __launch_bounds__(kWalk) void walk_kernel(Verify A) {
 // See include/hn_int4.h.
 extern "C" long hn_verify_tree_workspace_bytes(long B, long S, long V) {
   if (B <= 0 || S <= 0 || V <= 0) return 0;
-  return B * S * chunks_of(V).n * (long)(2 * sizeof(Part) + sizeof(double));
+  return B * S * (chunks_of(V).n * (long)(2 * sizeof(Part) + sizeof(double)) + sizeof(Next));
 }
 
 // See include/hn_int4.h.
@@ -614,12 +673,14 @@ extern "C" int hn_verify_tree(const void* logits, long ld_b, long ld_s, const vo
                "%s: needs a 16-byte aligned workspace of %ld bytes (got %ld)", who, need,
                work_bytes);
   const bool soft = draft && (temps || temperature > 0.f);
+  Part* parts = (Part*)work;
+  double* first = (double*)(parts + B * 2 * S * chunks_of(V).n);
   const Verify A = {logits, draft, ld_b,  ld_s,   ld_db,  ld_ds,  tokens, up,
                     u,      temps, temperature, (int)trees, (int)S, (int)V, path, count,
-                    token,  (Part*)work,
-                    (double*)((Part*)work + B * 2 * S * chunks_of(V).n)};
+                    token,  parts, first, (Next*)(first + B * S * chunks_of(V).n)};
   const dim3 grid((unsigned)chunks_of(V).n, (unsigned)(soft ? 2 * S : S), (unsigned)B);
   const dim3 nodes((unsigned)chunks_of(V).n, (unsigned)(S - 1), (unsigned)B);
+  const dim3 per_node((unsigned)S, (unsigned)B);
   hipStream_t st = (hipStream_t)stream;
 #define HN_VERIFY(T)                                                            \
   do {                                                                          \
@@ -627,6 +688,10 @@ extern "C" int hn_verify_tree(const void* logits, long ld_b, long ld_s, const vo
     HN_LAUNCH_CHECK(who);                                                       \
     if (soft && S > 1) {                                                        \
       hipLaunchKernelGGL(first_kernel<T>, nodes, dim3(kStat), 0, st, A);        \
+      HN_LAUNCH_CHECK(who);                                                     \
+    }                                                                           \
+    if (soft) {                                                                 \
+      hipLaunchKernelGGL(node_kernel<T>, per_node, dim3(kWalk), 0, st, A);      \
       HN_LAUNCH_CHECK(who);                                                     \
     }                                                                           \
     hipLaunchKernelGGL(walk_kernel<T>, dim3((unsigned)B), dim3(kWalk), 0, st, A); \

@@ -160,7 +160,7 @@ class KVCache:
             out = torch.empty_like(lens)
             _lib.call_on(dev, "hn_kv_keep", kt, v, len(self.kt), n, B, nkv, hd, lens.data_ptr(),
                          path.data_ptr(), max(path.stride(0), S), count.data_ptr(), S,
-                         out.data_ptr(), _lib.stream(dev))
+                         out.data_ptr())
             return out
         j = torch.arange(S)
         c = count.clamp(0, S)
@@ -187,7 +187,7 @@ class KVCache:
             ints = ctypes.c_int * max(1, len(src))
             dev = self.kt[0].device
             _lib.call_on(dev, "hn_kv_fork", kt, v, len(self.kt), n, B, nkv, hd, ints(*src),
-                         ints(*dst), len(src), length, _lib.stream(dev))
+                         ints(*dst), len(src), length)
             return
         for kt, v in zip(self.kt, self.v):
             kt[dst, :, :, :length] = kt[src, :, :, :length]

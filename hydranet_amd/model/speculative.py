@@ -53,8 +53,7 @@ class DraftTree:
             self.up, self.depth = torch.empty((2, n, S), dtype=torch.int32, device=p.device)
             self.seen = torch.empty((n, S, MAX_NODES // 64), dtype=torch.int64, device=p.device)
             _lib.call_on(p.device, "hn_tree_plan", p.data_ptr(), max(p.stride(0), S), n, S,
-                         self.up.data_ptr(), self.depth.data_ptr(), self.seen.data_ptr(),
-                         _lib.stream(p.device))
+                         self.up.data_ptr(), self.depth.data_ptr(), self.seen.data_ptr())
             return
         self.up = torch.full((n, S), PADDING, dtype=torch.int32)
         self.depth = torch.full((n, S), -1, dtype=torch.int32)
@@ -121,7 +120,7 @@ def tree_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, tree: D
         _lib.call_on(dev, "hn_tree_append", qkv.data_ptr(), max(qkv.stride(0), qkv.shape[1]),
                      cos.data_ptr(), sin.data_ptr(), cos.shape[0], tree.depth.data_ptr(),
                      tree.trees, lens.data_ptr(), B, S, nkv, rep, hd, q.data_ptr(),
-                     kt.data_ptr(), v.data_ptr(), max_len, _lib.stream(dev))
+                     kt.data_ptr(), v.data_ptr(), max_len)
         return q
     depth, at = tree.depth.expand(B, S).long(), torch.arange(S)
     live = (depth >= 0) & (lens >= 0)[:, None]
@@ -176,7 +175,7 @@ def tree_attention(q: torch.Tensor, tree: DraftTree, lens: torch.Tensor, cache, 
         _lib.call_on(dev, "hn_tree_attention", q.data_ptr(), kt.data_ptr(), v.data_ptr(), max_len,
                      lens.data_ptr(), tree.seen.data_ptr(), tree.trees, B, nkv, rep, hd, S,
                      kv_bound, scale, out.data_ptr(), out.stride(1),
-                     None if work is None else work.data_ptr(), n, _lib.stream(dev))
+                     None if work is None else work.data_ptr(), n)
         return out
     at = torch.arange(kv_bound) - lens[:, None]  # node at each position, negative: cached
     node = at.clamp(0, S - 1)[:, None].expand(B, S, kv_bound)
@@ -251,8 +250,7 @@ def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, tree: DraftTree,
     _lib.call_on(dev, "hn_verify_tree", logits.data_ptr(), logits.stride(0), logits.stride(1), *d,
                  _DTYPES[logits.dtype], tokens.data_ptr(), tree.up.data_ptr(), tree.trees,
                  uniforms.data_ptr(), None if temps is None else temps.data_ptr(), temp, B, S, V,
-                 path.data_ptr(), count.data_ptr(), token.data_ptr(), work.data_ptr(), n,
-                 _lib.stream(dev))
+                 path.data_ptr(), count.data_ptr(), token.data_ptr(), work.data_ptr(), n)
     return Verified(path, count, token)
 
 
