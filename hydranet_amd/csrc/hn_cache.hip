@@ -79,46 +79,34 @@ __global__ __launch_bounds__(256) void fork_kernel(Layers L, Copies P, long max_
   }
 }
 
-// By vectors of 16 bytes: kVecs of them per thread, all loaded before the first
-// is stored, then stored to every destination.  Grid (chunks of keys, then of
-// values, sources, layers).  The last vector of a row of keys may hold positions
-// past n, which stay as they are in the destination.
-constexpr int kVecs = 8;
+// By vectors of 16 bytes, one per thread, stored to every destination past the
+// caches (non-temporal: what is written is many times what they hold).  Grid
+// (workgroups of keys, then of values; sources; layers).  The last vector of a row
+// of keys may hold positions past n, which stay as they are in the destination.
+// Bound by HBM: 2 prompts of 1901 positions to 5 sequences each, 32 layers of 8
+// heads, 603 us for 3.0 GB (5.0 TB/s, a large copy's 4.9); with 8, 4, 2 vectors
+// per thread and plain stores 673, 635, 622, with 2 and 4 non-temporal 615, 624.
 __global__ __launch_bounds__(256) void fork_vec_kernel(Layers L, Copies P, long max_len, int nkv,
-                                                       int hd, int n, int key_chunks) {
+                                                       int hd, int n, int key_groups) {
   const int layer = blockIdx.z, sg = blockIdx.y;
-  const bool keys = (int)blockIdx.x < key_chunks;
+  const bool keys = (int)blockIdx.x < key_groups;
   const int nv = keys ? (n + 7) / 8 : n * (hd / 8);  // vectors of a row
-  const int rows = keys ? nkv * hd : nkv;
-  const long pitch = keys ? max_len : max_len * hd;
+  const long idx = (long)(blockIdx.x - (keys ? 0 : key_groups)) * 256 + threadIdx.x;
+  const long row = idx / nv, col = idx - row * nv;
+  if (row >= (keys ? nkv * hd : nkv)) return;
   h16* base = keys ? L.kt[layer] : L.v[layer];
-  const long seq = (long)nkv * hd * max_len;
-  const long first = (long)(blockIdx.x - (keys ? 0 : key_chunks)) * (256 * kVecs) + threadIdx.x;
-  const long all = (long)rows * nv;
-  u32x4 x[kVecs];
-  long at[kVecs];
-#pragma unroll
-  for (int i = 0; i < kVecs; ++i) {
-    const long idx = first + i * 256;
-    const long row = idx / nv;
-    at[i] = idx < all ? row * pitch + 8 * (idx - row * nv) : -1;
-    if (at[i] >= 0) x[i] = *reinterpret_cast<const u32x4*>(base + P.src[sg] * seq + at[i]);
-  }
-  const int tail = keys && n % 8 ? n % 8 : 8;
+  const long seq = (long)nkv * hd * max_len, at = row * (keys ? max_len : max_len * hd) + 8 * col;
+  const u32x4 x = *reinterpret_cast<const u32x4*>(base + P.src[sg] * seq + at);
+  const int tail = keys && col == nv - 1 && n % 8 ? n % 8 : 8;
   for (int k = P.first[sg]; k < P.first[sg + 1]; ++k) {
-    h16* out = base + P.dst[k] * seq;
+    h16* out = base + P.dst[k] * seq + at;
+    if (tail == 8) {
+      __builtin_nontemporal_store(x, reinterpret_cast<u32x4*>(out));
+    } else {
+      const half8_t h = __builtin_bit_cast(half8_t, x);
 #pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
-      if (at[i] < 0) continue;
-      const long idx = first + i * 256;
-      if (tail == 8 || (idx + 1) % nv) {
-        *reinterpret_cast<u32x4*>(out + at[i]) = x[i];
-      } else {
-        const half8_t h = __builtin_bit_cast(half8_t, x[i]);
-#pragma unroll
-        for (int e = 0; e < 7; ++e)
-          if (e < tail) out[at[i] + e] = h[e];
-      }
+      for (int e = 0; e < 7; ++e)
+        if (e < tail) out[e] = h[e];
     }
   }
 }
@@ -170,7 +158,7 @@ extern "C" int hn_kv_fork(void* const* kt, void* const* v, long layers, long max
       HN_ARG_CHECK(dst[i] != src[j] && (i == j || dst[i] != dst[j]),
                    "%s: a destination is a source or given twice", who);
   }
-  bool vec = max_len % 8 == 0 && hd % 8 == 0 && n < (1L << 31) / hd;
+  bool vec = max_len % 8 == 0 && hd % 8 == 0 && nkv * hd * n < (1L << 35);
   for (long l = 0; l < layers; ++l) vec = vec && al16(kt[l]) && al16(v[l]);
   for (long p0 = 0; p0 < pairs; p0 += kPairs) {
     const int np = (int)(pairs - p0 < kPairs ? pairs - p0 : kPairs);
@@ -189,8 +177,8 @@ extern "C" int hn_kv_fork(void* const* kt, void* const* v, long layers, long max
       Layers L = {};
       for (int l = 0; l < m; ++l) L.kt[l] = (h16*)kt[l0 + l], L.v[l] = (h16*)v[l0 + l];
       if (vec) {
-        const long per = 256 * kVecs, kc = (nkv * hd * ((n + 7) / 8) + per - 1) / per,
-                   vc = (nkv * n * (hd / 8) + per - 1) / per;
+        const long kc = (nkv * hd * ((n + 7) / 8) + 255) / 256,
+                   vc = (nkv * n * (hd / 8) + 255) / 256;
         hipLaunchKernelGGL(fork_vec_kernel, dim3((unsigned)(kc + vc), (unsigned)ns, (unsigned)m),
                            dim3(256), 0, (hipStream_t)stream, L, P, max_len, (int)nkv, (int)hd,
                            (int)n, (int)kc);
