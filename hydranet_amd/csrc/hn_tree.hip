@@ -248,7 +248,7 @@ struct Attend {
   h16* out;
   float* part;
   long max_len, bound, ld_o;
-  int trees, B, nkv, rep, S, R, blocks, grain, wgs;
+  int trees, B, nkv, rep, S, R, blocks, shift, wgs;
   float scale;
 };
 
@@ -300,28 +300,51 @@ __device__ __forceinline__ uint32_t odd_mask(uint32_t w) {
          ((w & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u);
 }
 
-// The work is cut into grains of `grain` positions of one (sequence, KV head), in
-// order, and workgroup w of wgs (A.wgs, or T if that is less) takes grains [w T /
-// wgs, (w + 1) T / wgs) of the T there are: each the same share whatever the sequences' lengths, which
-// only the device knows.  A share is one range of positions of one head or
-// several; a head's range that is not whole leaves its sums in the workspace,
-// in entry 2 w, or 2 w + 1 if it is not w's first, for join_kernel.  The row
-// blocks of a share follow each other on one XCD, whose L2 then serves all but
-// the first.
+// The work is cut into grains of 2^shift positions of one (sequence, KV head), in
+// order, and each workgroup takes as many of them as the others (or one less),
+// whatever the sequences' lengths, which only the device knows.  Such a share is
+// one range of positions of one head or several; a head's range that is not whole
+// leaves its sums in the workspace, in entry 2 w of workgroup w, or 2 w + 1 if it
+// is not w's first, for join_kernel.  The row blocks of a share follow each other
+// on one XCD, whose L2 then serves all but the first.
 __device__ __forceinline__ int grains_of(const Attend& A, int b) {
   const long C = A.lens[b];
-  return C < 0 || C + A.S > A.bound ? 0 : (int)((C + A.S + A.grain - 1) / A.grain);
+  return C < 0 || C + A.S > A.bound ? 0 : ((int)C + A.S + (1 << A.shift) - 1) >> A.shift;
 }
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// Sums of the lanes up to each (row_shr:1, 2, 4, 8, then row_bcast:15, 31).
+__device__ __forceinline__ int lane_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+  return x;
+}
 
 // Grains of one head of the sequences below `to`, by a wave.
 __device__ __forceinline__ int grains_below(const Attend& A, int to) {
   int n = 0;
   for (int b = threadIdx.x & 63; b < to; b += 64) n += grains_of(A, b);
-  for (int off = 32; off; off >>= 1) n += __shfl_xor(n, off, 64);
-  return uniform(n);
+  return __builtin_amdgcn_readlane(lane_scan(n), 63);
 }
+
+// T grains over the workgroups: the first `more` take each + 1 of them.
+struct Split {
+  int wgs, each, more;
+  __device__ Split(int T, int most) : wgs(T < most ? T : most) {
+    each = wgs ? (int)((unsigned)T / (unsigned)wgs) : 0, more = T - each * wgs;
+  }
+  __device__ int from(int w) const { return w * each + (w < more ? w : more); }
+  __device__ int owner(int x) const {
+    const int big = more * (each + 1);
+    return x < big ? (int)((unsigned)x / (unsigned)(each + 1))
+                   : more + (int)((unsigned)(x - big) / (unsigned)each);
+  }
+};
 
 // A range of positions of one KV head: tiles [first, end).
 struct Where {
@@ -340,28 +363,23 @@ struct Share {
     const int id = blockIdx.x, grp = id / (8 * A.blocks), in = id - grp * 8 * A.blocks;
     w = 8 * grp + (in & 7), block = in >> 3;
     if (w >= A.wgs) return false;
-    const long T = (long)grains_below(A, A.B) * A.nkv;
-    const int wgs = T < A.wgs ? (int)T : A.wgs;  // each of these has a grain
+    const Split P(grains_below(A, A.B) * A.nkv, A.wgs);
     first = true, b = 0, g = 0, at = 0, n = 0, left = 0;
-    if (w >= wgs) return true;
-    const int from = (int)(w * T / wgs);
-    left = (int)((w + 1) * T / wgs) - from;
+    if (w >= P.wgs) return true;
+    const int from = P.from(w);
+    left = P.from(w + 1) - from;
     const int lane = threadIdx.x & 63;
     int base = 0;  // grains of one head of the sequences before
     for (int c = 0; c < A.B; c += 64) {
       const int t = c + lane < A.B ? grains_of(A, c + lane) : 0;
-      int sum = t;
-      for (int off = 1; off < 64; off <<= 1) {
-        const int x = __shfl_up(sum, off, 64);
-        if (lane >= off) sum += x;
-      }
+      const int sum = lane_scan(t);
       const u64 past = __ballot((base + sum) * A.nkv > from);
       if (past) {
         const int l = __builtin_ctzll(past);
         b = c + l;
         n = __builtin_amdgcn_readlane(t, l);
         const int in_b = from - (base + __builtin_amdgcn_readlane(sum, l) - n) * A.nkv;
-        g = in_b / n, at = in_b - g * n;
+        g = (int)((unsigned)in_b / (unsigned)n), at = in_b - g * n;
         break;
       }
       base += __builtin_amdgcn_readlane(sum, 63);
@@ -381,7 +399,7 @@ struct Share {
     W.b = b, W.g = g, W.bg = b * A.nkv + g, W.row0 = block * rows;
     W.tree = A.trees > 1 ? b : 0;
     W.C = uniform((int)A.lens[b]), W.L = W.C + A.S;
-    const int per = A.grain / kPos, tiles = (W.L + kPos - 1) / kPos;
+    const int per = (1 << A.shift) / kPos, tiles = (W.L + kPos - 1) / kPos;
     W.first = at * per;
     W.end = W.first + m * per < tiles ? W.first + m * per : tiles;
     W.whole = m == n;
@@ -498,19 +516,6 @@ __global__ __launch_bounds__(256, OCC) void attend_kernel(Attend A) {
   const int bg = W.bg, tree = W.tree, end = W.end, row0 = W.row0;
   const int C = W.C, L = W.L;
 
-  // queries, as each lane's operands: rows past the last are zero
-  for (int t = wave; t < RT; t += 4) {
-    const int row = row0 + 16 * t + n;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      u32x4 w = {0, 0, 0, 0};
-      if (row < A.R)
-        w = *reinterpret_cast<const u32x4*>(A.q + ((long)bg * A.R + row) * kHd + 32 * u + 8 * kg);
-      s_q[t][u][lane] = w;
-    }
-  }
-  __syncthreads();
-
   const long slab = (long)bg * kHd * A.max_len;
   const uint32_t pitch = (uint32_t)A.max_len * 2;  // bytes of a row of keys
   const __amdgpu_buffer_rsrc_t rk = rsrc(A.kt + slab, (int)(pitch * kHd));
@@ -535,12 +540,14 @@ __global__ __launch_bounds__(256, OCC) void attend_kernel(Attend A) {
   };
   // values of positions p0 + 32 kg + 8 t + j at elements 8 n on.  j has bits of
   // its own in the lane's part of the address, so it is the instruction's offset.
-  const int vlane = (kg << 13) | (n << 4);
+  // That part is made from the lane's number each time: kept over the loop it was
+  // spilled, and its reload waited for every load in flight.
   auto load_v = [&](u32x4 (&x)[8], int tile, int t) {
     const int so = tile * (kPos * kHd * 2) + t * (8 * kHd * 2);
-    int at = vlane;
-    asm volatile("" : "+v"(at));
-    at &= ~0x700;
+    int zero = 0;
+    asm volatile("" : "+s"(zero));
+    const int me = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, zero)) & 63;
+    const int at = ((me >> 4) << 13) | ((me & 15) << 4);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       x[j] = __builtin_bit_cast(
@@ -574,6 +581,19 @@ __global__ __launch_bounds__(256, OCC) void attend_kernel(Attend A) {
   int tile = W.first + wave;
 #pragma unroll
   for (int u = 0; u < D; ++u) load_k(ring[u], tile, u);
+  // queries, as each lane's operands: rows past the last are zero
+  for (int t = wave; t < RT; t += 4) {
+    const int row = row0 + 16 * t + n;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      u32x4 w = {0, 0, 0, 0};
+      if (row < A.R)
+        w = *reinterpret_cast<const u32x4*>(A.q + ((long)bg * A.R + row) * kHd + 32 * u + 8 * kg);
+      s_q[t][u][lane] = w;
+    }
+  }
+  __syncthreads();
+
   uint32_t any_odd = 0;
   // EDGE: a tile that holds nodes, or positions past the sequence
   auto walk = [&](auto edge_tile) {
@@ -1002,15 +1022,12 @@ __global__ __launch_bounds__(256) void join_kernel(Attend A, int per_head) {
   const int bg = blockIdx.x / per_head, row = 8 * (blockIdx.x - bg * per_head) + (threadIdx.x >> 5);
   const int b = bg / A.nkv, g = bg - b * A.nkv, n = grains_of(A, b);
   if (n == 0) return;
-  const long T = (long)grains_below(A, A.B) * A.nkv;
-  const long from = (long)grains_below(A, b) * A.nkv + (long)g * n;
-  // the workgroup that has grain x is the first w with (w + 1) T / wgs > x
-  const long wgs = T < A.wgs ? T : A.wgs;
-  auto owner = [&](long x) { return (int)(((x + 1) * wgs + T - 1) / T) - 1; };
-  const int w0 = owner(from), w1 = owner(from + n - 1);
+  const Split P(grains_below(A, A.B) * A.nkv, A.wgs);
+  const int from = grains_below(A, b) * A.nkv + g * n;
+  const int w0 = P.owner(from), w1 = P.owner(from + n - 1);
   if (w0 == w1 || row >= A.R) return;
   // the first range is its workgroup's second unless the head starts its share
-  const long e0 = 2L * w0 + ((long)w0 * T / wgs < from);
+  const long e0 = 2L * w0 + (P.from(w0) < from);
   const int d = 4 * (threadIdx.x & 31), k = w1 - w0 + 1;
   const float* po = A.part + (long)row * kHd + d;
   const float* pm = A.part + 2 * (long)A.wgs * A.R * kHd + (long)row * 2;
@@ -1042,15 +1059,15 @@ __global__ __launch_bounds__(256) void join_kernel(Attend A, int per_head) {
 // Which kernel, its rows per workgroup, and its workgroups: one for each that the
 // chip holds at a time (they share the work evenly), or for each grain there can be.
 struct Plan {
-  int rows, blocks, grain, wgs;
+  int rows, blocks, shift, wgs;
 };
 Plan plan_of(long B, long nkv, long rep, long S, long bound) {
   const long R = rep * S;
   Plan p;
   p.rows = R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128;
   p.blocks = (int)((R + p.rows - 1) / p.rows);
-  p.grain = p.rows <= 32 ? 4 * kPos : kPos;
-  const long most = B * nkv * ((bound + p.grain - 1) / p.grain);
+  p.shift = p.rows <= 32 ? 9 : 7;  // a tile for each of the 4 waves; one for all
+  const long most = B * nkv * (((bound - 1) >> p.shift) + 1);
   const long fill = (long)hn_device_cus() * (p.rows == 32 ? 1 : 2) / p.blocks;
   p.wgs = (int)(most < fill ? most : fill < 1 ? 1 : fill);
   return p;
@@ -1112,7 +1129,7 @@ extern "C" int hn_tree_append(const void* qkv, long ld_qkv, const float* cos_t, 
 extern "C" long hn_tree_attention_workspace_bytes(long B, long nkv, long rep, long S, long bound) {
   if (B <= 0 || nkv <= 0 || rep <= 0 || S <= 0 || bound <= 0) return 0;
   const Plan p = plan_of(B, nkv, rep, S, bound);
-  return bound <= p.grain ? 0 : 2L * p.wgs * rep * S * (kHd + 2) * 4;
+  return bound <= (1L << p.shift) ? 0 : 2L * p.wgs * rep * S * (kHd + 2) * 4;
 }
 
 // See include/hn_int4.h.
@@ -1142,7 +1159,7 @@ extern "C" int hn_tree_attention(const void* q, const void* kt, const void* v, l
                work_bytes);
   const Attend A = {(const h16*)q, (const h16*)kt, (const h16*)v, lens, seen, (h16*)out,
                     (float*)work, max_len, bound, ld_o, (int)trees, (int)B, (int)nkv, (int)rep,
-                    (int)S, (int)R, p.blocks, p.grain, p.wgs, scale};
+                    (int)S, (int)R, p.blocks, p.shift, p.wgs, scale};
   const dim3 grid((unsigned)((p.wgs + 7) / 8 * 8 * p.blocks));
   hipStream_t st = (hipStream_t)stream;
   switch (p.rows) {

@@ -16,7 +16,8 @@ reference:
 * a preallocated per-layer KV cache [B, kv_heads, max_len, head_dim] with one
   length for the whole batch (cache/kv_cache.py:26-284, SimpleKVCache);
 * top-2 routing at prefill, top-1 or top-2 at decode (TopKMode,
-  model/mixtral.py:493-531; the reference's default is top-1 at decode).
+  model/mixtral.py:493-531; the reference's default is top-1 at decode);
+* speculative decoding with one length per sequence (model/speculative.py).
 """
 from __future__ import annotations
 
