@@ -209,23 +209,24 @@ __global__ __launch_bounds__(256) void append_rows_kernel(
 }
 
 // ---------------------------------------------------------------------------
-// Attention.  One workgroup of 4 waves takes RT tiles of 16 rows of one
-// (sequence, KV head), a row being a (query head of the group, node) pair, and a
-// range of the positions; each wave walks its own tiles of 128 positions:
+// Attention.  One pass over the cache with a running maximum and sum, for the rows
+// of one (sequence, KV head), a row being a (query head of the group, node) pair:
 //   S^T = K Q^T    v_mfma_f32_16x16x32_f16, A = K, B = Q;
-//   softmax        a lane holds 32 consecutive positions of one row, 32 * (lane /
-//                  16) on, of row lane % 16;
+//   softmax        a lane holds scores of one row;
 //   O^T += V^T P   the lane's probabilities are the B operand as they are.
-// K is cached as [hd][position] and V as [position][hd], so both products
-// contract over the axis that is not dense in memory.  A lane loads 8 vectors of
-// 8 halves, an 8 x 8 block, and v_perm takes pairs of its rows apart: 32 of them
-// make the 8 operands of the block's 8 products, product j holding every lane's
-// column j.  Which positions (of K) or columns (of V) a product holds is a
-// permutation that the sums do not see, and it makes a lane's scores
-// consecutive.  So neither K nor V passes through LDS, each element is loaded
-// once per workgroup, and a wave keeps 3 to 4 blocks of 8 KB in flight: block s
-// of a tile (4 of K, then 4 of V) is replaced by block s + 4 once it is used.
-constexpr int kPos = 128;     // positions per tile
+// share_kernel walks the positions, join_kernel adds up what several workgroups
+// made of one head.
+//
+// Bounds, and time where the workgroups hold 8 KV heads of 128 and 4 query heads
+// each (a large copy moves 4.9 TB/s):
+//   32 sequences of 8000, 4 nodes     the cache's bytes: 222 us, 4.7 TB/s
+//   1 of 30000, 4 nodes               37 us, 3.3 TB/s
+//   8 of 8000, 64 nodes               120 us, 0.58 PFLOP/s: the softmax and the
+//                                     LDS reads between the products
+//   1 of 300, 1 node                  13 us: two launches, and memory's latency
+// Positions that workgroups share out as one.  Of 64 a head's ranges need not start
+// on 256 bytes of its keys: 245 us for the first of the cases above, 222 of 128.
+constexpr int kGrain = 128;
 constexpr int kOPad = kHd + 4;
 constexpr uint32_t kNone = 0xfffff000u;  // an offset past any descriptor: reads zero, no access
 constexpr float kLog2e = 1.4426950408889634f;
@@ -248,26 +249,9 @@ struct Attend {
   h16* out;
   float* part;
   long max_len, bound, ld_o;
-  int trees, B, nkv, rep, S, R, blocks, shift, wgs;
+  int trees, B, nkv, rep, S, R, blocks, wgs;
   float scale;
 };
-
-__device__ __forceinline__ uint32_t perm_lo(uint32_t a, uint32_t b) {  // (a.lo, b.lo)
-  return __builtin_amdgcn_perm(b, a, 0x05040100u);
-}
-__device__ __forceinline__ uint32_t perm_hi(uint32_t a, uint32_t b) {  // (a.hi, b.hi)
-  return __builtin_amdgcn_perm(b, a, 0x07060302u);
-}
-// column c of an 8 x 8 block
-template <int C>
-__device__ __forceinline__ half8_t column(const u32x4 r[8]) {
-  u32x4 w;
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    w[i] = C & 1 ? perm_hi(r[2 * i][C >> 1], r[2 * i + 1][C >> 1])
-                 : perm_lo(r[2 * i][C >> 1], r[2 * i + 1][C >> 1]);
-  return __builtin_bit_cast(half8_t, w);
-}
 
 // max over the four lanes, 16 apart, that hold one row.  (The swapped pair goes
 // through scalars: a bit cast of a vector's element takes element 0.)
@@ -300,7 +284,7 @@ __device__ __forceinline__ uint32_t odd_mask(uint32_t w) {
          ((w & 0x7c000000u) == 0x7c000000u ? 0xffff0000u : 0u);
 }
 
-// The work is cut into grains of 2^shift positions of one (sequence, KV head), in
+// The work is cut into grains of kGrain positions of one (sequence, KV head), in
 // order, and each workgroup takes as many of them as the others (or one less),
 // whatever the sequences' lengths, which only the device knows.  Such a share is
 // one range of positions of one head or several; a head's range that is not whole
@@ -309,7 +293,7 @@ __device__ __forceinline__ uint32_t odd_mask(uint32_t w) {
 // on one XCD, whose L2 then serves all but the first.
 __device__ __forceinline__ int grains_of(const Attend& A, int b) {
   const long C = A.lens[b];
-  return C < 0 || C + A.S > A.bound ? 0 : ((int)C + A.S + (1 << A.shift) - 1) >> A.shift;
+  return C < 0 || C + A.S > A.bound ? 0 : ((int)C + A.S + kGrain - 1) / kGrain;
 }
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -346,7 +330,7 @@ struct Split {
   }
 };
 
-// A range of positions of one KV head: tiles [first, end).
+// A range of positions of one KV head: grains [first, end).
 struct Where {
   int bg, b, g, row0, tree, first, end;
   int C, L;     // cached positions, and with the nodes
@@ -399,9 +383,7 @@ struct Share {
     W.b = b, W.g = g, W.bg = b * A.nkv + g, W.row0 = block * rows;
     W.tree = A.trees > 1 ? b : 0;
     W.C = uniform((int)A.lens[b]), W.L = W.C + A.S;
-    const int per = (1 << A.shift) / kPos, tiles = (W.L + kPos - 1) / kPos;
-    W.first = at * per;
-    W.end = W.first + m * per < tiles ? W.first + m * per : tiles;
+    W.first = at, W.end = at + m;
     W.whole = m == n;
     W.part = 2 * (long)w + !first;
     at += m, left -= m, first = false;
@@ -501,255 +483,9 @@ __device__ __forceinline__ void add_odd(const Attend& A, const Where& W, int row
   }
 }
 
-template <int RT, int D, int OCC>
-__global__ __launch_bounds__(256, OCC) void attend_kernel(Attend A) {
-  constexpr int kRows = 16 * RT;
-  __shared__ __align__(16) float s_o[4 * 16 * kOPad];
-  __shared__ float s_m[4 * kRows], s_l[4 * kRows];
-  __shared__ u32x4 s_q[RT][4][64];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n = lane & 15, kg = lane >> 4;
-  Share share;
-  if (!share.begin(A)) return;
-  for (Where W; share.next(A, kRows, W);) {
-  const int bg = W.bg, tree = W.tree, end = W.end, row0 = W.row0;
-  const int C = W.C, L = W.L;
-
-  const long slab = (long)bg * kHd * A.max_len;
-  const uint32_t pitch = (uint32_t)A.max_len * 2;  // bytes of a row of keys
-  const __amdgpu_buffer_rsrc_t rk = rsrc(A.kt + slab, (int)(pitch * kHd));
-  const __amdgpu_buffer_rsrc_t rv = rsrc(A.v + slab, (int)(pitch * kHd));
-
-  u32x4 ring[D][8];
-  // keys 32 u + 8 kg + r at positions p0 + 8 n on; a vector past the row's end
-  // (its positions are past the sequence) reads the row's last instead.  The
-  // lane's part of the address is one register, the rest a scalar that is
-  // stepped from load to load (32 of them, kept, would spill).
-  auto load_k = [&](u32x4 (&x)[8], int tile, int u) {
-    const int p0 = tile * kPos, last = (int)A.max_len - 8 - p0;
-    const uint32_t at =
-        tile < end ? (uint32_t)(8 * kg) * pitch + 2u * (uint32_t)(8 * n < last ? 8 * n : last) : kNone;
-    uint32_t step = pitch;
-    asm volatile("" : "+s"(step));
-    uint32_t so = 2u * (uint32_t)p0 + (uint32_t)(32 * u) * step;
-#pragma unroll
-    for (int r = 0; r < 8; ++r, so += step)
-      x[r] = __builtin_bit_cast(
-          u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, (int)at, (int)so, 0));
-  };
-  // values of positions p0 + 32 kg + 8 t + j at elements 8 n on.  j has bits of
-  // its own in the lane's part of the address, so it is the instruction's offset.
-  // That part is made from the lane's number each time: kept over the loop it was
-  // spilled, and its reload waited for every load in flight.
-  auto load_v = [&](u32x4 (&x)[8], int tile, int t) {
-    const int so = tile * (kPos * kHd * 2) + t * (8 * kHd * 2);
-    int zero = 0;
-    asm volatile("" : "+s"(zero));
-    const int me = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, zero)) & 63;
-    const int at = ((me >> 4) << 13) | ((me & 15) << 4);
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      x[j] = __builtin_bit_cast(
-          u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, at | (j << 8), so, 0));
-  };
-  // the same of a sequence's last tiles: past its end, zero (their probabilities
-  // are, and what a longer sequence left there may be anything)
-  auto load_v_end = [&](u32x4 (&x)[8], int tile, int t) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int p = tile * kPos + 32 * kg + 8 * t + j;
-      const uint32_t at = p < L ? (uint32_t)p * (kHd * 2) + 16 * n : kNone;
-      x[j] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rv, (int)at, 0, 0));
-    }
-  };
-
-  float4v o[RT][8], l[RT];
-  float mx[RT];
-#pragma unroll
-  for (int t = 0; t < RT; ++t) {
-    mx[t] = -__builtin_inff();
-    l[t] = (float4v)(0.f);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) o[t][e] = (float4v)(0.f);
-  }
-  const float scale = A.scale * kLog2e;
-  half8_t ones;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) ones[i] = (h16)1.f;
-
-  int tile = W.first + wave;
-#pragma unroll
-  for (int u = 0; u < D; ++u) load_k(ring[u], tile, u);
-  // queries, as each lane's operands: rows past the last are zero
-  for (int t = wave; t < RT; t += 4) {
-    const int row = row0 + 16 * t + n;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      u32x4 w = {0, 0, 0, 0};
-      if (row < A.R)
-        w = *reinterpret_cast<const u32x4*>(A.q + ((long)bg * A.R + row) * kHd + 32 * u + 8 * kg);
-      s_q[t][u][lane] = w;
-    }
-  }
-  __syncthreads();
-
-  uint32_t any_odd = 0;
-  // EDGE: a tile that holds nodes, or positions past the sequence
-  auto walk = [&](auto edge_tile) {
-    constexpr bool EDGE = decltype(edge_tile)::value;
-    // block c of the tile is used: block c + D, of the next tile's keys past 8
-    auto next = [&](int c) {
-      const int a = c + D;
-      if (a < 4)
-        load_k(ring[c % D], tile, a);
-      else if (a >= 8)
-        load_k(ring[c % D], tile + 4, a - 8);
-      else if constexpr (EDGE)
-        load_v_end(ring[c % D], tile, a - 4);
-      else
-        load_v(ring[c % D], tile, a - 4);
-    };
-    float4v s[RT][8];
-#pragma unroll
-    for (int t = 0; t < RT; ++t)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) s[t][j] = (float4v)(0.f);
-#define HN_QK(J)                                                                                 \
-  {                                                                                              \
-    const half8_t a = column<J>(ring[u % D]);                                                        \
-    _Pragma("unroll") for (int t = 0; t < RT; ++t) s[t][J] =                                     \
-        __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q[t], s[t][J], 0, 0, 0);                       \
-  }
-    int ql = lane;
-    asm volatile("" : "+v"(ql));  // queries are read again for each tile, not kept in registers
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      half8_t q[RT];
-#pragma unroll
-      for (int t = 0; t < RT; ++t) q[t] = __builtin_bit_cast(half8_t, s_q[t][u][ql]);
-      HN_QK(0) HN_QK(1)
-      __builtin_amdgcn_sched_barrier(0);
-      HN_QK(2) HN_QK(3)
-      __builtin_amdgcn_sched_barrier(0);
-      HN_QK(4) HN_QK(5)
-      __builtin_amdgcn_sched_barrier(0);
-      HN_QK(6) HN_QK(7)
-      __builtin_amdgcn_sched_barrier(0);
-      next(u);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-#undef HN_QK
-    const int p0 = tile * kPos;
-    half8_t p[RT][4];
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-      if constexpr (EDGE) {
-        const int row = row0 + 16 * t + n;
-        const int node = row < A.R ? row % A.S : 0;
-        const uint32_t w = window(A.seen + ((long)tree * A.S + node) * kWords, p0 + 32 * kg - C);
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (!((w >> (8 * r + j)) & 1u)) s[t][j][r] = -__builtin_inff();
-      }
-      float tm = s[t][0][0];
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) tm = fmaxf(tm, s[t][j][r]);
-      tm = row_max(tm) * scale;
-      if (__any(tm > mx[t] + kLag)) {
-        const float nm = fmaxf(mx[t], tm);
-        const float al = nm == mx[t] ? 1.f : __builtin_amdgcn_exp2f(mx[t] - nm);
-        l[t] *= al;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) o[t][e] *= al;
-        mx[t] = nm;
-      }
-      // a row that has seen nothing yet: every score is -inf
-      const float ref = mx[t] == -__builtin_inff() ? 0.f : mx[t] - kUp;
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          p[t][r][j] = (h16)__builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j][r], scale, -ref));
-      __builtin_amdgcn_sched_barrier(0);
-    }
-#define HN_PV(E)                                                                                 \
-  {                                                                                              \
-    const half8_t a = column<E>(ring[u % D]);                                                        \
-    _Pragma("unroll") for (int t = 0; t < RT; ++t) o[t][E] =                                     \
-        __builtin_amdgcn_mfma_f32_16x16x32_f16(a, p[t][u], o[t][E], 0, 0, 0);                    \
-  }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if constexpr (EDGE) {
-        // a node's value that is no number must not reach, as 0 times it, the
-        // rows that do not see it: taken out here, added to the others at the end
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const bool node = p0 + 32 * kg + 8 * u + j >= C;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t w = ring[u % D][j][i], m = node ? odd_mask(w) : 0u;
-            any_odd |= m;
-            ring[u % D][j][i] = w & ~m;
-          }
-          asm volatile("" : "+v"(any_odd));  // now, not from kept masks at the end
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < RT; ++t)
-        l[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, p[t][u], l[t], 0, 0, 0);
-      HN_PV(0) HN_PV(1)
-      __builtin_amdgcn_sched_barrier(0);
-      HN_PV(2) HN_PV(3)
-      __builtin_amdgcn_sched_barrier(0);
-      HN_PV(4) HN_PV(5)
-      __builtin_amdgcn_sched_barrier(0);
-      HN_PV(6) HN_PV(7)
-      __builtin_amdgcn_sched_barrier(0);
-      next(4 + u);
-      __builtin_amdgcn_sched_barrier(0);
-    }
-#undef HN_PV
-  };
-  const int inner = C / kPos < end ? C / kPos : end;  // tiles all rows see whole
-  for (; tile < inner; tile += 4) walk(Bool<false>{});
-  for (; tile < end; tile += 4) walk(Bool<true>{});
-  if (__any(any_odd != 0))  // rare
-    add_odd<RT>(A, W, row0, n, o, [&](int e, int r) { return 32 * kg + 8 * r + e; },
-                [&](int p) {
-                  const int at = p / kPos;
-                  return at >= W.first && at < end && ((at - W.first) & 3) == wave;
-                });
-
-  if (kg == 0)
-#pragma unroll
-    for (int t = 0; t < RT; ++t)
-      s_m[wave * kRows + 16 * t + n] = mx[t], s_l[wave * kRows + 16 * t + n] = l[t][0];
-#pragma unroll
-  for (int t = 0; t < RT; ++t) {
-    if (t) __syncthreads();
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        *reinterpret_cast<float4v*>(s_o + (wave * 16 + n) * kOPad + 32 * kg + 8 * r + 4 * h) =
-            float4v{o[t][4 * h][r], o[t][4 * h + 1][r], o[t][4 * h + 2][r], o[t][4 * h + 3][r]};
-    __syncthreads();
-    finish<1, 4>(A, W, s_o, s_m, s_l, t, kRows);
-  }
-  __syncthreads();  // the next range's waves write what the rows are read from
-  }
-  share.rest(A, kRows);
-}
-
-// ---------------------------------------------------------------------------
-// Many rows per KV head: the tiles of K and V shared through LDS.  4 waves, RG
-// groups of 32 rows by PG parts of a stage of SP = 64 positions.  A stage of keys
+// The walk.  4 waves, RG groups of 32 rows by PG parts of a stage of SP = 64
+// positions.  K is cached as [hd][position] and V as [position][hd], so both
+// products contract over the axis that is not dense in memory.  A stage of keys
 // [128 hd][SP] and values [SP][128 hd] goes from memory to LDS as it lies
 // (buffer_load ... lds), one stage ahead, and ds_read_b64_tr_b16 turns it on the
 // way to the registers: 16 lanes read 4 rows of 16 halves, and lane i gets column
@@ -757,10 +493,14 @@ __global__ __launch_bounds__(256, OCC) void attend_kernel(Attend A) {
 // + 4 kg + r of its part, of row lane % 16, and with the values' rows taken as {4
 // kg + r, 16 + 4 kg + r} they are the second product's operand as they are.
 // Two workgroups per CU: one's loads and barriers under the other's arithmetic.
+// (Waves on positions of their own that turn 8 x 8 blocks in registers with v_perm,
+// without LDS: with 16 / 32 rows per wave 16.4 / 17.4 us for 16 nodes of one
+// sequence of 1500 that takes 14.4 here, 241 / 227 for the first of the cases above
+// and 38 / 33 for the second.)
 //
 // Both transposing reads take 32 bytes of each of 16 rows; a row's 16-byte chunks
 // are stored at chunk ^ (2 * key(row)), so that the 8 rows that half a wave reads
-// cover the 64 banks once.
+// cover the 64 banks once: the counter of bank conflicts stays at 0.
 constexpr int kSP = 64;
 __device__ __forceinline__ int key_of_k(int hd) { return ((hd >> 1) & 1) | ((hd >> 2) & 2); }
 
@@ -791,6 +531,7 @@ __global__ __launch_bounds__(256, 2) void share_kernel(Attend A) {
   if (!share.begin(A)) return;
   for (Where W; share.next(A, 32 * RG, W);) {
   const int row0 = W.row0 + 32 * rg;  // this wave's rows
+  const bool busy = row0 < A.R;
 
   half8_t q[RT][4];
 #pragma unroll
@@ -818,11 +559,11 @@ __global__ __launch_bounds__(256, 2) void share_kernel(Attend A) {
   const int kc = (lane % kChunks) ^ (2 * key_of_k(kRowK * wave + kr));
   const uint32_t kat = (uint32_t)kr * pitch + 16 * kc;
   const uint32_t vat = vr * (kHd * 2) + 16 * ((lane & 15) ^ (2 * ((4 * wave + vr) & 7)));
-  const int stages = kPos / SP * (W.end - W.first);
+  const int stages = kGrain / SP * (W.end - W.first);
   // positions past the sequence read as zero: their probabilities are, and what a
   // longer sequence left there may be anything
   auto issue = [&](int st) {
-    const int p0 = W.first * kPos + st * SP;
+    const int p0 = W.first * kGrain + st * SP;
     const uint32_t at = lds0 + (uint32_t)(st % D) * kStage + wave * 1024;
     const uint32_t ka = st < stages && p0 + 8 * kc < W.L ? kat : kNone;
 #pragma unroll
@@ -869,7 +610,7 @@ __global__ __launch_bounds__(256, 2) void share_kernel(Attend A) {
   // scores and probabilities of a stage
   auto scores = [&](auto edge_stage, int st) __attribute__((always_inline)) {
     constexpr bool EDGE = decltype(edge_stage)::value;
-    const int p0 = W.first * kPos + st * SP + pg * WP;
+    const int p0 = W.first * kGrain + st * SP + pg * WP;
     const uint32_t at = (uint32_t)(st % D) * kStage;
     // operands are read one group of products ahead
     float4v s[RT][JB];
@@ -933,7 +674,7 @@ __global__ __launch_bounds__(256, 2) void share_kernel(Attend A) {
   // its values, by those probabilities
   auto values = [&](auto edge_stage, int st) __attribute__((always_inline)) {
     constexpr bool EDGE = decltype(edge_stage)::value;
-    const int p0 = W.first * kPos + st * SP + pg * WP;
+    const int p0 = W.first * kGrain + st * SP + pg * WP;
     const uint32_t at = (uint32_t)(st % D) * kStage;
     constexpr int EB = 4;  // operands per group
     half8_t va[2][EB];
@@ -982,10 +723,11 @@ __global__ __launch_bounds__(256, 2) void share_kernel(Attend A) {
     wait_vmcnt<0>();  // this wave's part of the stage has landed
     stage_barrier();  // everyone's, and the stage before is used
     issue(st + 1);
+    if (!busy) return;
     scores(edge_stage, st);
     values(edge_stage, st);
   };
-  const int seen_whole = W.C / SP - W.first * (kPos / SP);  // stages before the nodes
+  const int seen_whole = W.C / SP - W.first * (kGrain / SP);  // stages before the nodes
   const int inner = seen_whole < stages ? seen_whole : stages;
   for (; st < inner; ++st) stage(Bool<false>{});
   for (; st < stages; ++st) stage(Bool<true>{});
@@ -994,7 +736,7 @@ __global__ __launch_bounds__(256, 2) void share_kernel(Attend A) {
   if (__any(any_odd != 0))
     add_odd<RT>(A, W, row0, n, o, [&](int e, int r) { return 16 * e + 4 * kg + r; },
                 [&](int p) {
-                  const int at = p / kPos;
+                  const int at = p / kGrain;
                   return at >= W.first && at < W.end && p / WP % PG == pg;
                 });
   float* s_o = reinterpret_cast<float*>(s_buf);
@@ -1016,34 +758,56 @@ __global__ __launch_bounds__(256, 2) void share_kernel(Attend A) {
   share.rest(A, 32 * RG);
 }
 
-// The ranges' sums joined: 32 threads per row, 4 elements each, of a head that
-// several workgroups share; a workgroup takes 8 rows of one head.
+// The ranges' sums joined, of heads that several workgroups share: 32 threads per
+// row, 4 elements each, G such groups taking every G-th range of it; a workgroup
+// has 8 / G rows of one head.  Where there are few rows their ranges are many, and
+// each costs the wait for a load.
+template <int G>
 __global__ __launch_bounds__(256) void join_kernel(Attend A, int per_head) {
-  const int bg = blockIdx.x / per_head, row = 8 * (blockIdx.x - bg * per_head) + (threadIdx.x >> 5);
+  constexpr int kRows = 8 / G;
+  __shared__ float4v s_x[G][kRows][32];
+  __shared__ float s_m[G][kRows], s_s[G][kRows];
+  const int bg = blockIdx.x / per_head, t = threadIdx.x >> 5, grp = t / kRows, rr = t - grp * kRows;
+  const int row = kRows * (blockIdx.x - bg * per_head) + rr;
   const int b = bg / A.nkv, g = bg - b * A.nkv, n = grains_of(A, b);
   if (n == 0) return;
   const Split P(grains_below(A, A.B) * A.nkv, A.wgs);
   const int from = grains_below(A, b) * A.nkv + g * n;
-  const int w0 = P.owner(from), w1 = P.owner(from + n - 1);
-  if (w0 == w1 || row >= A.R) return;
+  const int w0 = P.owner(from), k = P.owner(from + n - 1) - w0 + 1;
+  if (k == 1) return;
   // the first range is its workgroup's second unless the head starts its share
   const long e0 = 2L * w0 + (P.from(w0) < from);
-  const int d = 4 * (threadIdx.x & 31), k = w1 - w0 + 1;
-  const float* po = A.part + (long)row * kHd + d;
-  const float* pm = A.part + 2 * (long)A.wgs * A.R * kHd + (long)row * 2;
+  const int d = 4 * (threadIdx.x & 31);
+  const float* po = A.part + (long)(row < A.R ? row : 0) * kHd + d;
+  const float* pm = A.part + 2 * (long)A.wgs * A.R * kHd + (long)(row < A.R ? row : 0) * 2;
   auto entry = [&](int i) { return (i == 0 ? e0 : 2L * (w0 + i)) * A.R; };
   float m = -__builtin_inff();
 #pragma unroll 4
-  for (int i = 0; i < k; ++i) m = fmaxf(m, pm[entry(i) * 2]);
+  for (int i = grp; i < k; i += G) m = fmaxf(m, pm[entry(i) * 2]);
+  if (G > 1) {
+    if (d == 0) s_m[grp][rr] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < G; ++i) m = fmaxf(m, s_m[i][rr]);
+  }
   const float ref = m == -__builtin_inff() ? 0.f : m;
   float sum = 0.f;
   float4v x = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
-  for (int i = 0; i < k; ++i) {
+  for (int i = grp; i < k; i += G) {
     const float al = __builtin_amdgcn_exp2f(pm[entry(i) * 2] - ref);
     sum += al * pm[entry(i) * 2 + 1];
     x += al * *reinterpret_cast<const float4v*>(po + entry(i) * kHd);
   }
+  if (G > 1) {
+    s_x[grp][rr][threadIdx.x & 31] = x;
+    if (d == 0) s_s[grp][rr] = sum;
+    __syncthreads();
+    if (grp) return;
+#pragma unroll
+    for (int i = 1; i < G; ++i) x += s_x[i][rr][threadIdx.x & 31], sum += s_s[i][rr];
+  }
+  if (row >= A.R) return;
   const int head = row / A.S, node = row - head * A.S;
   const u64* see = A.seen + ((A.trees > 1 ? (long)b * A.S : 0) + node) * kWords;
   const bool live = (see[node >> 6] >> (node & 63)) & 1;
@@ -1056,19 +820,22 @@ __global__ __launch_bounds__(256) void join_kernel(Attend A, int per_head) {
                              (long)(g * A.rep + head) * kHd + d) = y;
 }
 
-// Which kernel, its rows per workgroup, and its workgroups: one for each that the
-// chip holds at a time (they share the work evenly), or for each grain there can be.
+// Rows per workgroup, and workgroups: as many as the chip holds at a time, two per
+// CU (they share the work evenly), or one for each grain that there can be.  One
+// per CU took 157 us for 8 sequences of 8000 with 64 nodes, two take 120.
+// 64 or 128 rows, the other half of the waves on the other half of a stage or on
+// rows of their own: of 32 sequences of 8000, 16 rows 222 / 258 us and 64 rows
+// 239 / 252, and 68 rows, which take two workgroups of 64, 290 / 248.
 struct Plan {
-  int rows, blocks, shift, wgs;
+  int rows, blocks, wgs;
 };
 Plan plan_of(long B, long nkv, long rep, long S, long bound) {
   const long R = rep * S;
   Plan p;
-  p.rows = R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128;
+  p.rows = R <= 64 ? 64 : 128;
   p.blocks = (int)((R + p.rows - 1) / p.rows);
-  p.shift = p.rows <= 32 ? 9 : 7;  // a tile for each of the 4 waves; one for all
-  const long most = B * nkv * (((bound - 1) >> p.shift) + 1);
-  const long fill = (long)hn_device_cus() * (p.rows == 32 ? 1 : 2) / p.blocks;
+  const long most = B * nkv * ((bound - 1) / kGrain + 1);
+  const long fill = 2L * hn_device_cus() / p.blocks;
   p.wgs = (int)(most < fill ? most : fill < 1 ? 1 : fill);
   return p;
 }
@@ -1129,7 +896,7 @@ extern "C" int hn_tree_append(const void* qkv, long ld_qkv, const float* cos_t, 
 extern "C" long hn_tree_attention_workspace_bytes(long B, long nkv, long rep, long S, long bound) {
   if (B <= 0 || nkv <= 0 || rep <= 0 || S <= 0 || bound <= 0) return 0;
   const Plan p = plan_of(B, nkv, rep, S, bound);
-  return bound <= (1L << p.shift) ? 0 : 2L * p.wgs * rep * S * (kHd + 2) * 4;
+  return bound <= kGrain ? 0 : 2L * p.wgs * rep * S * (kHd + 2) * 4;
 }
 
 // See include/hn_int4.h.
@@ -1149,9 +916,9 @@ extern "C" int hn_tree_attention(const void* q, const void* kt, const void* v, l
                    ld_o >= nkv * rep * hd && lens && seen,
                "%s: operands must be 16-byte aligned, ld_o >= heads * %d", who, kHd);
   const Plan p = plan_of(B, nkv, rep, S, bound);
-  const long R = rep * S, per_head = (R + 7) / 8;
-  HN_ARG_CHECK(B * nkv * ((bound + kPos - 1) / kPos) < (1L << 31) &&
-                   B * nkv * per_head < (1L << 31) && (p.wgs + 7L) / 8 * 8 * p.blocks < (1L << 31),
+  const long R = rep * S;
+  HN_ARG_CHECK(B * nkv * ((bound + kGrain - 1) / kGrain) < (1L << 31) &&
+                   B * nkv * R < (1L << 31) && (p.wgs + 7L) / 8 * 8 * p.blocks < (1L << 31),
                "%s: too many rows", who);
   const long need = hn_tree_attention_workspace_bytes(B, nkv, rep, S, bound);
   HN_ARG_CHECK(need == 0 || (work && al16(work) && work_bytes >= need),
@@ -1159,18 +926,19 @@ extern "C" int hn_tree_attention(const void* q, const void* kt, const void* v, l
                work_bytes);
   const Attend A = {(const h16*)q, (const h16*)kt, (const h16*)v, lens, seen, (h16*)out,
                     (float*)work, max_len, bound, ld_o, (int)trees, (int)B, (int)nkv, (int)rep,
-                    (int)S, (int)R, p.blocks, p.shift, p.wgs, scale};
+                    (int)S, (int)R, p.blocks, p.wgs, scale};
   const dim3 grid((unsigned)((p.wgs + 7) / 8 * 8 * p.blocks));
   hipStream_t st = (hipStream_t)stream;
-  switch (p.rows) {
-    case 16: hipLaunchKernelGGL((attend_kernel<1, 4, 2>), grid, dim3(256), 0, st, A); break;
-    case 32: hipLaunchKernelGGL((attend_kernel<2, 4, 1>), grid, dim3(256), 0, st, A); break;
-    case 64: hipLaunchKernelGGL((share_kernel<2, 2>), grid, dim3(256), 0, st, A); break;
-    default: hipLaunchKernelGGL((share_kernel<4, 1>), grid, dim3(256), 0, st, A);
-  }
+  const auto kern = p.rows == 64 ? share_kernel<2, 2> : share_kernel<4, 1>;
+  hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, A);
   HN_LAUNCH_CHECK(who);
   if (need) {  // a head of several grains may be shared
-    hipLaunchKernelGGL(join_kernel, dim3((unsigned)(B * nkv * per_head)), dim3(256), 0, st, A,
+    // whole calls: 512 rows 15.1 / 14.4 us (G = 1 / 8) over 1500 positions, 1024 rows
+    // 63 / 52 over 30000, 2048 rows of 8 sequences 24 / 26, 8192 rows 37 / 44
+    const bool few = B * nkv * R <= 1024;
+    const auto join = few ? join_kernel<8> : join_kernel<1>;
+    const long per_head = few ? R : (R + 7) / 8;
+    hipLaunchKernelGGL(join, dim3((unsigned)(B * nkv * per_head)), dim3(256), 0, st, A,
                        (int)per_head);
     HN_LAUNCH_CHECK(who);
   }
