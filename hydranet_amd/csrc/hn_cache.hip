@@ -41,14 +41,14 @@ __global__ __launch_bounds__(256) void keep_kernel(Layers L, long max_len, int n
 #pragma unroll
       for (int j = 0; j < kStep; ++j) {
         at[j] = j0 + j < n ? p[j0 + j] : 0;
-        if (at[j] > j0 + j && C + at[j] < max_len) {
+        if (at[j] > j0 + j && at[j] < max_len - C) {
           kr[j] = kt[(long)d * max_len + at[j]];
           vr[j] = v[(long)at[j] * hd + d];
         }
       }
 #pragma unroll
       for (int j = 0; j < kStep; ++j)
-        if (at[j] > j0 + j && C + at[j] < max_len) {
+        if (at[j] > j0 + j && at[j] < max_len - C) {
           kt[(long)d * max_len + j0 + j] = kr[j];
           v[(long)(j0 + j) * hd + d] = vr[j];
         }
@@ -158,7 +158,7 @@ extern "C" int hn_kv_fork(void* const* kt, void* const* v, long layers, long max
       HN_ARG_CHECK(dst[i] != src[j] && (i == j || dst[i] != dst[j]),
                    "%s: a destination is a source or given twice", who);
   }
-  bool vec = max_len % 8 == 0 && hd % 8 == 0 && nkv * hd * n < (1L << 35);
+  bool vec = max_len % 8 == 0 && hd % 8 == 0 && nkv * hd * n < (1L << 34);
   for (long l = 0; l < layers; ++l) vec = vec && al16(kt[l]) && al16(v[l]);
   for (long p0 = 0; p0 < pairs; p0 += kPairs) {
     const int np = (int)(pairs - p0 < kPairs ? pairs - p0 : kPairs);

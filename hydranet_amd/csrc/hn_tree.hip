@@ -74,8 +74,9 @@ __device__ __forceinline__ Place place(const int* depth, int trees, const long* 
                                        int S, long table_rows, long max_len) {
   const int dep = depth[(trees > 1 ? (long)b * S : 0) + i];
   const long C = lens[b];
-  Place p = {C + dep, C + i, C >= 0 && dep >= 0, false};
-  p.in = p.live && p.pos < table_rows && p.slot < max_len;
+  Place p = {0, 0, C >= 0 && dep >= 0, false};
+  p.in = p.live && C < table_rows - dep && C < max_len - i;
+  if (p.in) p.pos = C + dep, p.slot = C + i;
   return p;
 }
 
@@ -293,7 +294,7 @@ __device__ __forceinline__ uint32_t odd_mask(uint32_t w) {
 // on one XCD, whose L2 then serves all but the first.
 __device__ __forceinline__ int grains_of(const Attend& A, int b) {
   const long C = A.lens[b];
-  return C < 0 || C + A.S > A.bound ? 0 : ((int)C + A.S + kGrain - 1) / kGrain;
+  return C < 0 || C > A.bound - A.S ? 0 : ((int)C + A.S + kGrain - 1) / kGrain;
 }
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }

@@ -141,7 +141,7 @@ struct Verify {
   int* count;
   long* token;
   Part* part;     // [B][2][S][chunks]: the target's rows, the drafter's
-  double* first;  // [B][S][chunks]: the last S(c) of a node whose first child is rejected
+  double* first;  // [B][S][chunks]: the last S(c) of a node whose first child is rejected, or -1
   Next* next;           // [B][S]
 };
 
@@ -244,12 +244,6 @@ struct RowStat {
   float m;
   double z;
 };
-// Whether a first child is accepted: u q(x) < p(x).  (first_kernel and the walk
-// decide alike.)
-__device__ __forceinline__ bool first_accepted(float u, double px, double qx) {
-#pragma clang fp contract(off)
-  return (double)u * qx < px;
-}
 __device__ __forceinline__ RowStat row_stat(const Part* p, int chunks, const double* tab, double k) {
   const int lane = threadIdx.x & 63;
   Part P = {-__builtin_inff(), 0, 0.};
@@ -294,7 +288,7 @@ struct Rows {
 // The mass that a node's first rejection leaves, S(1), by chunks over the whole
 // chip: the walk needs it at each node whose first child is rejected, and most
 // trees need little more.  (A node that the walk does not come to is summed for
-// nothing.)  Grid (chunks, S, B).
+// nothing.)  -1 where that child is accepted.  Grid (chunks, S - 1, B).
 template <typename T>
 __global__ __launch_bounds__(kStat) void first_kernel(Verify A) {
   __shared__ double tab[kTab], s_s[kStat / 64];
@@ -325,7 +319,8 @@ __global__ __launch_bounds__(kStat) void first_kernel(Verify A) {
   if (tid == 0) {
     const double px = prob_of(tab, P, sane((float)p[tok[child]]), k);
     const double qx = prob_of(tab, Q, sane((float)q[tok[child]]), k);
-    s_need = !first_accepted(A.u[(long)b * A.S + child], px, qx);
+    s_need = !((double)A.u[(long)b * A.S + child] * qx < px);
+    if (!s_need) A.first[((long)b * A.S + node) * C.n + blockIdx.x] = -1.;
   }
   __syncthreads();
   if (!s_need) return;
@@ -415,11 +410,12 @@ __global__ __launch_bounds__(kWalk) void node_kernel(Verify A) {
     }
     __syncthreads();
     double* first = A.first + ((long)b * S + node) * C.n;
+    const double left = lane < C.n ? first[lane] : 0.;  // by the first child's rejection
     bool again = false;
     for (int i = node + 1; i < S && N.mass > kTiny; ++i) {
       if (!s_kid[i]) continue;
       if (N.c > 0. ? (double)s_u[i] * s_qx[i] * N.mass < s_px[i] - N.c * s_qx[i]
-                   : first_accepted(s_u[i], s_px[i], s_qx[i])) {
+                   : lane_of(left, 0) < 0.) {
         N.node = i;
         break;
       }
@@ -434,8 +430,7 @@ __global__ __launch_bounds__(kWalk) void node_kernel(Verify A) {
         __syncthreads();
         for (int j = lane; j < C.n * kWaves; j += 64) s += s_sum[j / kWaves][j % kWaves];
       } else {
-        N.c = 1.;
-        if (lane < C.n) s = first[lane];
+        N.c = 1., s = left;
       }
       N.mass = lane_of(scan(s), 63);
     }

@@ -271,7 +271,7 @@ def _verify_cpu(logits, tokens, tree, uniforms, draft, temps) -> Verified:
         x = torch.where(x.isnan(), -math.inf, x.double()).clamp(max=torch.finfo(torch.float32).max)
         if x.max() == -math.inf:
             return torch.zeros(V, dtype=torch.float64)
-        if t <= 0:
+        if not t > 0:
             return torch.nn.functional.one_hot((x == x.max()).nonzero()[0, 0], V).double()
         return torch.softmax(x / t, 0)
 
@@ -286,7 +286,7 @@ def _verify_cpu(logits, tokens, tree, uniforms, draft, temps) -> Verified:
             x = int(tokens[b, i])
             if up[i] != cur or not 0 <= x < V or mass <= tiny:
                 continue
-            if t <= 0:
+            if not t > 0:
                 q, take = None, bool(p[x] > 0)
             elif draft is None:
                 q, take = None, u[i] * mass < float(r[x])

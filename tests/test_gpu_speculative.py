@@ -408,6 +408,97 @@ def test_a_step_together_on_a_stream_and_replayed():
             assert torch.equal(a, b)
 
 
+@pytest.mark.parametrize("B,nkv,rep,S,most,kind", [
+    (150, 2, 4, 3, 700, "padded"), (70, 1, 1, 1, 2500, "chain"), (67, 1, 2, 40, 300, "random"),
+    (130, 8, 4, 1, 200, "chain")])
+def test_attention_many_sequences(B, nkv, rep, S, most, kind):
+    """More sequences than a wave has lanes, of any lengths, some without a part."""
+    rng = random.Random(B)
+    lens = [rng.choice((0, -1, most, rng.randint(0, most), rng.randint(0, 130))) for _ in range(B)]
+    lens[64:66] = [-1, -1]
+    n = -(-(most + S) // 8) * 8
+    got, q, c, rows, _ = _attend(B, nkv, rep, S, lens, n, kind)
+    _attention_close(got, q, c, rows, lens)
+
+
+@pytest.mark.parametrize("B,nkv,rep,S,lens", [(1, 1, 4, 256, [900]), (2, 2, 4, 200, [0, 1111]),
+                                              (1, 1, 16, 100, [5000])])
+def test_attention_many_row_blocks(B, nkv, rep, S, lens):
+    got, q, c, rows, _ = _attend(B, nkv, rep, S, lens, -(-(max(lens) + S) // 8) * 8, "random")
+    _attention_close(got, q, c, rows, lens)
+
+
+def test_lengths_past_everything():
+    """A length near the largest int64 counts as past the cache; the others are as ever."""
+    top = 2 ** 63 - 1
+    S, n, nh, nkv = 9, 128, 8, 2
+    rng = random.Random(0)
+    rows = [ref.random_tree(rng, S, "random") for _ in range(4)]
+    tree = _tree(rows)
+    lens = torch.tensor([top, 40, top - 4, 2 ** 32 + 5], device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(0)
+    cos, sin = _tables(n)
+    for width in (0, 6):  # rows of both kinds
+        qkv = torch.randn(4 * S, (nh + 2 * nkv) * HD + width, generator=g, device=DEV).half()
+        qkv = qkv[:, :(nh + 2 * nkv) * HD]
+        c, _ = _caches(1, 4, nkv, HD, n)
+        before = c.kt[0].clone(), c.v[0].clone()
+        q = tree_append(qkv, cos, sin, tree, lens, c, 0, nh)
+        o = tree_attention(q, tree, lens, c, 0, n).view(4, S, nh, HD)
+        for b in (0, 2, 3):
+            assert bool(q[b].isnan().all()) and bool(o[b].isnan().all())
+            assert torch.equal(c.kt[0][b], before[0][b]) and torch.equal(c.v[0][b], before[1][b])
+        assert not bool(q[1].isnan().any()) and not bool(o[1].isnan().any())
+    path = torch.arange(S, dtype=torch.int32, device=DEV).repeat(4, 1)
+    path[:, 1] = 3
+    before = c.kt[0].clone(), c.v[0].clone()
+    c.keep(lens, path, torch.full((4,), 2, dtype=torch.int32, device=DEV))
+    for b in (0, 2, 3):
+        assert torch.equal(c.kt[0][b], before[0][b]) and torch.equal(c.v[0][b], before[1][b])
+    assert torch.equal(c.v[0][1, :, 41], before[1][1, :, 43])
+
+
+@pytest.mark.parametrize("B,S,V,soft,kind", [(2, 4, 600001, True, "star"), (1, 3, 1100000, False, "star"),
+                                             (1, 9, 530000, True, "star")])
+@pytest.mark.parametrize("temp", [0.0, 0.9])
+def test_verify_vocabularies_of_several_blocks_per_chunk(B, S, V, soft, kind, temp):
+    rows, logits, draft, tokens, u = _verify_inputs(B, S, V, torch.float16, soft, kind, V)
+    u[:, 1:] = 1.0 - u[:, 1:] / 64  # rejections
+    got = verify_tree(logits, tokens, _tree(rows), u, draft, temp)
+    _verify_check(got, rows, logits, draft, tokens, u, [temp] * B)
+
+
+def test_two_streams_at_once():
+    """Attention and verification of different inputs on two streams, interleaved: each what it
+    is alone."""
+    jobs = []
+    for seed, (B, S, C) in enumerate(((3, 40, 3000), (2, 7, 6000))):
+        lens = [C - 100 * b for b in range(B)]
+        got, q, c, rows, tree = _attend(B, 2, 4, S, lens, -(-(C + S) // 8) * 8, "random", seed=seed)
+        vin = _verify_inputs(B, S, 33000, torch.float16, True, "star", seed)
+        jobs.append((q, tree, torch.tensor(lens, device=DEV), c, C + S, vin, _tree(vin[0])))
+
+    def run(j):
+        q, tree, ln, c, bound, (_, lg, d, t, u), vt = j
+        return [tree_attention(q, tree, ln, c, 0, bound), *verify_tree(lg, t, vt, u, d, 0.8)]
+
+    want = [run(j) for j in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(device=DEV) for _ in jobs]
+    out = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        for i, j in enumerate(jobs):
+            with torch.cuda.stream(streams[i]):
+                out[i].append(run(j))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for o in out[i]:
+            for a, b in zip(o, want[i]):
+                assert torch.equal(a, b)
+
+
 def test_refusals_on_the_gpu():
     c = KVCache.wrap([torch.zeros(2, 1, HD, 16, device=DEV).half()],
                      [torch.zeros(2, 1, 16, HD, device=DEV).half()])
