@@ -24,6 +24,15 @@
 // rejected in the same way, and node_kernel what becomes of each node's children.
 // walk_kernel, one workgroup per sequence, follows that, or tests certain
 // proposals in LDS, and reads a row again only for the draw: one chunk.
+//
+// Times: 5 nodes over 32000 tokens, greedy, one sequence: stats 4.2 us, walk 3.4
+// (latency of two launches).  8 trees of 61 nodes, 4 children each, over 32000,
+// fp16: stats 22 us, first 16, node 45, walk 13.  32 chains of 6 over 128000, fp32:
+// 48 (4.4 TB/s), 24, 5, 14.  Of the 22 us half are the 26 million exponentials at
+// 18 vector instructions each, the rest their rows' arrival; the 45 are three passes
+// by one workgroup, one after the other since each needs the mass that the last one
+// left.  Without gain there: leaving out nodes that the walk cannot reach, the next
+// block's loads under the arithmetic, four exponentials interleaved (44 us in all).
 #include <float.h>
 
 #include "hn_common.h"
