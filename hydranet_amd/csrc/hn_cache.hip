@@ -14,48 +14,65 @@ struct Layers {
   h16* v[kLayers];
 };
 
-// Grid (B * nkv, layers), a thread per element of a position.  Positions go in
-// ascending order, kStep at a time: the sources of a step are read before its
-// destinations are written, and path[j] >= j, so a later source (at or past its
-// own j) is never an earlier destination.
-// Bound by the keys' cache lines: a position's 128 elements lie in as many rows of
-// K^T, 2 bytes of each.  32 sequences, 32 layers of 8 heads, paths of 61 nodes'
-// trees: 94 us, 135 MB fetched and 53 MB written for 33 MB moved.  Threads that read
-// and write whole lines of a row, 64 or 128 bytes, took 139 and 266 us.
+// Grid (B * nkv, layers, 2): keys, values.  Positions go in ascending order, kStep at
+// a time: the sources of a step are read before its destinations are written, and
+// path[j] >= j, so a later source (at or past its own j) is never an earlier
+// destination.  Of the keys, which lie 2 bytes to a row, 8 lanes take a row's step,
+// whose destinations are next to each other: a thread per row, 8 moves in flight,
+// asked the caches for 8 times the lines (94 us for the 74 below).
+// Bound by the keys' lines: a position's 128 elements lie in as many rows of K^T, 2
+// bytes of each.  32 sequences, 32 layers of 8 heads, 128 moved positions: 74 us,
+// 88 MB fetched and 53 MB written for 34 MB of moves.  Threads that read and wrote
+// whole lines of a row, 64 or 128 bytes, took 139 and 266 us; 256 threads for 128
+// rows 77, 8 rows in flight per lane 73, two layers per workgroup 66 (but the same as
+// before on a cache that was not just read, 87 us a call).
 constexpr int kStep = 8;
 __global__ __launch_bounds__(256) void keep_kernel(Layers L, long max_len, int nkv, int hd,
                                                    const long* __restrict__ lens,
                                                    const int* __restrict__ path, long ld_p,
                                                    const int* __restrict__ count, int S,
                                                    long* __restrict__ lens_out) {
-  const int bg = blockIdx.x, b = bg / nkv, layer = blockIdx.y;
+  constexpr int kRows = 4;  // rows of keys in flight per lane
+  const int bg = blockIdx.x, b = bg / nkv, layer = blockIdx.y, tid = threadIdx.x;
   const long C = lens[b];
   int n = count[b];
   n = n < 0 ? 0 : n > S ? S : n;
-  if (lens_out && layer == 0 && bg == b * nkv && threadIdx.x == 0)
+  if (lens_out && layer == 0 && bg == b * nkv && blockIdx.z == 0 && tid == 0)
     lens_out[b] = C < 0 ? C : C + n;
   if (C < 0) return;
-  h16* kt = L.kt[layer] + (long)bg * hd * max_len + C;
-  h16* v = L.v[layer] + ((long)bg * max_len + C) * hd;
+  const long left = max_len - C;
   const int* p = path + (long)b * ld_p;
-  for (int d = threadIdx.x; d < hd; d += blockDim.x)
+  if (blockIdx.z == 0) {
+    h16* kt = L.kt[layer] + (long)bg * hd * max_len + C;
+    const int j = tid & (kStep - 1), r = tid / kStep, rows = blockDim.x / kStep;
     for (int j0 = 0; j0 < n; j0 += kStep) {
-      h16 kr[kStep], vr[kStep];
+      const int to = j0 + j, at = to < n ? p[to] : 0;
+      const bool moves = at > to && at < left;
+      for (int d0 = r; d0 < hd; d0 += kRows * rows) {
+        h16 x[kRows];
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+          if (moves && d0 + i * rows < hd) x[i] = kt[(long)(d0 + i * rows) * max_len + at];
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+          if (moves && d0 + i * rows < hd) kt[(long)(d0 + i * rows) * max_len + to] = x[i];
+      }
+    }
+    return;
+  }
+  h16* v = L.v[layer] + ((long)bg * max_len + C) * hd;
+  for (int d = tid; d < hd; d += blockDim.x)
+    for (int j0 = 0; j0 < n; j0 += kStep) {
+      h16 x[kStep];
       int at[kStep];
 #pragma unroll
       for (int j = 0; j < kStep; ++j) {
         at[j] = j0 + j < n ? p[j0 + j] : 0;
-        if (at[j] > j0 + j && at[j] < max_len - C) {
-          kr[j] = kt[(long)d * max_len + at[j]];
-          vr[j] = v[(long)at[j] * hd + d];
-        }
+        if (at[j] > j0 + j && at[j] < left) x[j] = v[(long)at[j] * hd + d];
       }
 #pragma unroll
       for (int j = 0; j < kStep; ++j)
-        if (at[j] > j0 + j && at[j] < max_len - C) {
-          kt[(long)d * max_len + j0 + j] = kr[j];
-          v[(long)(j0 + j) * hd + d] = vr[j];
-        }
+        if (at[j] > j0 + j && at[j] < left) v[(long)(j0 + j) * hd + d] = x[j];
     }
 }
 
@@ -135,7 +152,7 @@ extern "C" int hn_kv_keep(void* const* kt, void* const* v, long layers, long max
     const int m = (int)(layers - l0 < kLayers ? layers - l0 : kLayers);
     Layers L = {};
     for (int l = 0; l < m; ++l) L.kt[l] = (h16*)kt[l0 + l], L.v[l] = (h16*)v[l0 + l];
-    hipLaunchKernelGGL(keep_kernel, dim3((unsigned)(B * nkv), (unsigned)m),
+    hipLaunchKernelGGL(keep_kernel, dim3((unsigned)(B * nkv), (unsigned)m, 2),
                        dim3(hd <= 128 ? 128 : 256), 0, (hipStream_t)stream, L, max_len, (int)nkv,
                        (int)hd, lens, path, ld_path, count, (int)S, l0 ? nullptr : lens_out);
     HN_LAUNCH_CHECK(who);
