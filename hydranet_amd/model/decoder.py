@@ -138,6 +138,9 @@ class KVCache:
             old = self._table = (ptrs, self.kt + self.v, arr(*ptrs[:m]), arr(*ptrs[m:]))
         return old[2], old[3]
 
+    def __getstate__(self):  # (a copy's layers are elsewhere)
+        return {k: v for k, v in self.__dict__.items() if k != "_table"}
+
     def keep(self, lens: torch.Tensor, path: torch.Tensor, count: torch.Tensor) -> torch.Tensor:
         """After a verification (model/speculative.py), the accepted nodes' entries
         in every layer go from positions lens + path[:, j] to lens + j, j < count,

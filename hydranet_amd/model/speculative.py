@@ -317,8 +317,9 @@ def _verify_cpu(logits, tokens, tree, uniforms, draft, temps) -> Verified:
 
 
 class Draft(NamedTuple):
-    tokens: torch.Tensor                  # [B, S - 1] int64: of nodes 1 on
-    parents: torch.Tensor                 # int32 [S] or [B, S], node 0 the last token
+    tokens: torch.Tensor                  # [B, S - 1] int64: of nodes 1 on (outside the
+    #                                       vocabulary: never accepted)
+    parents: torch.Tensor                 # int32 [S] or [B, S], node 0 (-1) the last token
     logits: Optional[torch.Tensor] = None  # [B, S, V]: the drafter's after each node
 
 
@@ -359,14 +360,14 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int,
     longest = -(-(P + max_new_tokens + max_nodes) // 8) * 8  # a pass writes past what it keeps
     cache = model.new_cache(N, longest)
     first = type(cache).wrap([t[:B] for t in cache.kt], [t[:B] for t in cache.v])
-    logits = model.forward(input_ids, first)[:, -1:]
+    first_logits = model.forward(input_ids, first)[:, -1:]
     cache.fork([i % B for i in range(B, N)], list(range(B, N)), P)
 
     def uniforms(nodes):
         return torch.rand((N, nodes), generator=generator, device=dev)
 
     one = DraftTree.chain(1, dev)
-    last = verify_tree(logits.repeat(samples, 1, 1), torch.zeros((N, 1), dtype=torch.int64,
+    last = verify_tree(first_logits.repeat(samples, 1, 1), torch.zeros((N, 1), dtype=torch.int64,
                        device=dev), one, uniforms(1), None, temperature).token
     lens = torch.full((N,), P, dtype=torch.int64, device=dev)
     size, out = [P] * N, [[] for _ in range(N)]
@@ -387,7 +388,8 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int,
         tokens = torch.cat((last.clamp(min=0)[:, None], d.tokens), 1)
         assert tokens.shape[1] == tree.nodes, f"{tree.nodes} nodes, {d.tokens.shape[1]} tokens"
         bound = max(n for n, over in zip(size, done) if not over) + tree.nodes
-        logits = model.forward_tree(tokens, tree, lens, cache, bound)
+        inside = tokens.clamp(0, first_logits.shape[-1] - 1)
+        logits = model.forward_tree(inside, tree, lens, cache, bound)
         r = verify_tree(logits, tokens, tree, uniforms(tree.nodes), d.logits, temperature)
         lens = cache.keep(lens, r.path, r.count)
         last = r.token

@@ -242,3 +242,69 @@ def test_ngram_draft():
     d = ngram_draft([[1, 2, 3, 1, 2], [4]], "cpu", nodes=4)
     assert d.tokens.tolist() == [[3, 1, 2], [0, 0, 0]]
     assert d.parents.tolist() == [[-1, 0, 1, 2], [-1, PADDING, PADDING, PADDING]]
+
+
+class _Counting:
+    """A model whose next token is the last plus one; its cache holds the tokens."""
+
+    def __init__(self, vocab):
+        self.vocab, self.passes = vocab, 0
+
+    def new_cache(self, batch, max_len):
+        z = torch.zeros(batch, 1, 2, max_len, dtype=torch.float16)
+        return KVCache.wrap([z], [z.transpose(2, 3).contiguous()])
+
+    def _logits(self, ids):
+        assert int(ids.min()) >= 0 and int(ids.max()) < self.vocab
+        return 9.0 * torch.nn.functional.one_hot((ids + 1) % self.vocab, self.vocab).float()
+
+    def forward(self, ids, cache):
+        cache.kt[0][:, 0, :, :ids.shape[1]] = ids[:, None].half()
+        return self._logits(ids)
+
+    def forward_tree(self, tokens, tree, lens, cache, bound):
+        self.passes += 1
+        for b in range(tokens.shape[0]):
+            C = int(lens[b])
+            if C >= 0:
+                assert C + tokens.shape[1] <= bound <= cache.max_len
+                # what was kept is the text so far: consecutive numbers
+                text = cache.kt[0][b, 0, 0, :C].long()
+                assert torch.equal(text, (text[0] + torch.arange(C)) % self.vocab)
+                assert int(tokens[b, 0]) == (int(text[-1]) + 1) % self.vocab
+                cache.kt[0][b, 0, :, C:C + tokens.shape[1]] = tokens[b].half()
+        return self._logits(tokens)
+
+
+def test_generate_with_right_wrong_and_impossible_drafts():
+    from hydranet_amd.model.speculative import Draft, generate
+    V, n = 50, 23
+
+    def draft(history, device):
+        rows = []
+        for i, h in enumerate(history):
+            t = h[-1]
+            right = [(t + 1) % V, (t + 2) % V, (t + 3) % V]
+            rows.append([-7, V + 3] + (right if i % 2 == 0 else [right[0], V, -1]))
+        return Draft(torch.tensor(rows), torch.tensor([-1, 0, 0, 0, 3, 4], dtype=torch.int32))
+
+    prompt = torch.tensor([[3, 4, 5], [48, 49, 0]])
+    for samples in (1, 2):
+        model = _Counting(V)
+        out = generate(model, prompt, n, draft, samples=samples, max_nodes=6)
+        for i in range(2 * samples):
+            want = (prompt[i % 2, -1] + 1 + torch.arange(n)) % V
+            assert torch.equal(out[i], want)
+        assert model.passes == 11  # two tokens a pass at the least, after the first
+    assert torch.equal(generate(_Counting(V), prompt, n), out[:2])
+
+
+def test_a_cache_is_copied_after_its_layers_were_passed_to_a_kernel():
+    import copy
+    c = KVCache.wrap([torch.zeros(1, 1, 4, 8).half()], [torch.zeros(1, 1, 8, 4).half()])
+    a = c._layers()
+    d = copy.deepcopy(c)
+    b = d._layers()
+    assert a[0][0] == c.kt[0].data_ptr() and b[0][0] == d.kt[0].data_ptr() != a[0][0]
+    c.v[0] = torch.ones(1, 1, 8, 4).half()
+    assert c._layers()[1][0] == c.v[0].data_ptr()
