@@ -27,12 +27,13 @@
 //
 // Times: 5 nodes over 32000 tokens, greedy, one sequence: stats 4.2 us, walk 3.4
 // (latency of two launches).  8 trees of 61 nodes, 4 children each, over 32000,
-// fp16: stats 22 us, first 16, node 45, walk 13.  32 chains of 6 over 128000, fp32:
-// 48 (4.4 TB/s), 24, 5, 14.  Of the 22 us half are the 26 million exponentials at
-// 18 vector instructions each, the rest their rows' arrival; the 45 are three passes
+// fp16: stats 22 us, first 16, node 41, walk 13.  32 chains of 6 over 128000, fp32:
+// 48 (4.4 TB/s), 25, 6, 14.  Of the 22 us half are the 26 million exponentials at
+// 18 vector instructions each, the rest their rows' arrival; the 41 are three passes
 // by one workgroup, one after the other since each needs the mass that the last one
-// left.  Without gain there: leaving out nodes that the walk cannot reach, the next
-// block's loads under the arithmetic, four exponentials interleaved (44 us in all).
+// left.  With little gain there (47 to 44 us together, without the shorter passes):
+// leaving out nodes that the walk cannot reach, the next block's loads under the
+// arithmetic, four exponentials interleaved.
 #include <float.h>
 
 #include "hn_common.h"
@@ -277,6 +278,10 @@ struct Rows {
   __device__ Rows(const T* p_, const T* q_, RowStat P, RowStat Q, double c)
       : p(p_), q(q_), pm(P.z > 0. ? P.m : 0.), pz(P.z), qm(Q.z > 0. ? Q.m : 0.), qz(c * Q.z),
         both(c > 0.) {}  // without a finite logit: exponents of -inf, sums of 0
+  __device__ __forceinline__ double left(float x, float y, const double* tab, double k) const {
+    const double d = exp_of(tab, x, pm, k) * pz - exp_of(tab, y, qm, k) * qz;
+    return d > 0. ? d : 0.;
+  }
   __device__ __forceinline__ void left8(double r[8], const double* tab, double k, int e,
                                         int end) const {
     float x[8], y[8];
@@ -379,6 +384,20 @@ struct Next {
   double c, mass;  // else the residual's c and S(c); its chunks' masses are in first
 };
 
+// The tokens that a pass leaves mass, as c only grows the only ones that the next can:
+// the logits of those that a wave came by, in its order, and where its chunks end.  A
+// third of 32000 tokens or less in trees of 4 children each, whose nodes took 47 us
+// with each pass over whole rows and 41 with the passes after the first over these.
+// Where they do not fit, the next pass reads the rows again.
+template <typename T>
+struct Kept {
+  static constexpr int kMost = 2048 / sizeof(T);  // 64 KB: two workgroups per CU
+  struct Two {
+    T p, q;
+  } of[kWaves][kMost];
+  unsigned short end[kMaxChunks][kWaves];
+};
+
 template <typename T>
 __global__ __launch_bounds__(kWalk) void node_kernel(Verify A) {
   __shared__ double tab[kTab];
@@ -387,8 +406,10 @@ __global__ __launch_bounds__(kWalk) void node_kernel(Verify A) {
   __shared__ float s_u[kMaxNodes];
   __shared__ bool s_kid[kMaxNodes];  // a child whose token is in the vocabulary
   __shared__ double s_sum[kMaxChunks][kWaves];
+  __shared__ Kept<T> s_kept;
+  __shared__ int s_last;
   const int b = blockIdx.y, node = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
-  const int S = A.S, V = A.V;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), S = A.S, V = A.V;
   const float t = A.temps ? A.temps[b] : A.temp;
   if (!(t > 0.f)) return;
   const int* up = A.up + (A.trees > 1 ? (long)b * S : 0);
@@ -402,9 +423,11 @@ __global__ __launch_bounds__(kWalk) void node_kernel(Verify A) {
     if (kid) lp = sane((float)p[x]), lq = sane((float)q[x]), s_u[tid] = A.u[(long)b * S + tid];
   }
   if (tid < S) s_kid[tid] = kid;
+  if (tid == 0) s_last = 0;
   fill_table(tab);
   Next N = {-1, 0., 1.};
   if (__syncthreads_or(kid)) {
+    if (kid) atomicMax(&s_last, tid);
     const double k = kTab / ((double)t * kLn2);
     const Chunks C = chunks_of(V);
     if (tid < 128) {
@@ -420,7 +443,7 @@ __global__ __launch_bounds__(kWalk) void node_kernel(Verify A) {
     __syncthreads();
     double* first = A.first + ((long)b * S + node) * C.n;
     const double left = lane < C.n ? first[lane] : 0.;  // by the first child's rejection
-    bool again = false;
+    bool again = false, kept = false;
     for (int i = node + 1; i < S && N.mass > kTiny; ++i) {
       if (!s_kid[i]) continue;
       if (N.c > 0. ? (double)s_u[i] * s_qx[i] * N.mass < s_px[i] - N.c * s_qx[i]
@@ -433,10 +456,53 @@ __global__ __launch_bounds__(kWalk) void node_kernel(Verify A) {
         N.c += N.mass, again = true;
         const Rows<T> R(p, q, s_stat[0], s_stat[1], N.c);
         __syncthreads();  // the last sums are read
-        for (int ch = 0; ch < C.n; ++ch)
-          sum_chunk([&](double r[8], int e, int end) { R.left8(r, tab, k, e, end); }, C, V, ch,
-                    s_sum);
-        __syncthreads();
+        if (kept) {
+          for (int ch = 0, j = 0; ch < C.n; ++ch) {
+            const int end = s_kept.end[ch][wave];
+            double part = 0.;
+            for (int e = j + lane; e < end; e += 64) {
+              const auto w = s_kept.of[wave][e];
+              part += R.left(sane((float)w.p), sane((float)w.q), tab, k);
+            }
+            part = scan(part);
+            if (lane == 63) s_sum[ch][wave] = part;
+            j = end;
+          }
+          __syncthreads();
+        } else if (i < s_last) {  // there may be another pass
+          int len = 0;
+          for (int ch = 0; ch < C.n; ++ch) {
+            const int t0 = ch * C.size, t1 = t0 + C.size < V ? t0 + C.size : V;
+            double part = 0.;
+            for (int o = t0; o < t1; o += kBlock) {
+              float x[8], y[8];
+              const int at = o + tid * 8;
+              load8(x, p + at, t1 - at);
+              load8(y, q + at, t1 - at);
+              double r[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) r[e] = R.left(x[e], y[e], tab, k);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                part += r[e];
+                const unsigned long long some = __ballot(r[e] > 0.);
+                const int to = len + __builtin_amdgcn_mbcnt_hi(
+                                         some >> 32, __builtin_amdgcn_mbcnt_lo((unsigned)some, 0));
+                if (r[e] > 0. && to < Kept<T>::kMost) s_kept.of[wave][to] = {(T)x[e], (T)y[e]};
+                len += __popcll(some);
+              }
+            }
+            part = scan(part);
+            if (lane == 63) s_sum[ch][wave] = part;
+            if (lane == 0) s_kept.end[ch][wave] = len < Kept<T>::kMost ? len : Kept<T>::kMost;
+          }
+          kept = !__syncthreads_or(len > Kept<T>::kMost);
+        } else {
+          for (int ch = 0; ch < C.n; ++ch)
+            sum_chunk([&](double r[8], int e, int end) { R.left8(r, tab, k, e, end); }, C, V, ch,
+                      s_sum);
+          __syncthreads();
+        }
         for (int j = lane; j < C.n * kWaves; j += 64) s += s_sum[j / kWaves][j % kWaves];
       } else {
         N.c = 1., s = left;

@@ -468,6 +468,27 @@ def test_verify_vocabularies_of_several_blocks_per_chunk(B, S, V, soft, kind, te
     _verify_check(got, rows, logits, draft, tokens, u, [temp] * B)
 
 
+@pytest.mark.parametrize("V", [90, 7000, 20001, 100003])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("near", [0.02, 1.5])
+def test_verify_many_rejections_of_one_node(V, dtype, near):
+    """Up to 30 children of one node, few accepted: residuals of many tokens (a drafter near the
+    target) and of few, whose tokens fit on the chip or do not."""
+    B, S = 6, 31
+    g = torch.Generator(device=DEV).manual_seed(V)
+    logits = torch.randn(B, S, V, generator=g, device=DEV)
+    draft = (logits + near * torch.randn(B, S, V, generator=g, device=DEV)).to(dtype)
+    logits = logits.to(dtype)
+    q = torch.softmax(draft[:, 0].float(), -1)
+    tokens = torch.cat((torch.zeros(B, 1, dtype=torch.int64, device=DEV),
+                        torch.multinomial(q, S - 1, replacement=True, generator=g)), 1)
+    u = torch.rand(B, S, generator=g, device=DEV)
+    u[:, 1:] = 1.0 - u[:, 1:] / 1024
+    rows = [[-1] + [0] * (S - 1)] * B
+    got = verify_tree(logits, tokens, _tree(rows), u, draft, 1.0)
+    _verify_check(got, rows, logits, draft, tokens, u, [1.0] * B)
+
+
 def test_two_streams_at_once():
     """Attention and verification of different inputs on two streams, interleaved: each what it
     is alone."""
