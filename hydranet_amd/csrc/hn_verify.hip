@@ -29,7 +29,7 @@
 // (latency of two launches).  8 trees of 61 nodes, 4 children each, over 32000,
 // fp16: stats 22 us, first 16, node 41, walk 13.  32 chains of 6 over 128000, fp32:
 // 48 (4.4 TB/s), 25, 6, 14.  Of the 22 us half are the 26 million exponentials at
-// 18 vector instructions each, the rest their rows' arrival; the 41 are three passes
+// 19 vector instructions each, the rest their rows' arrival; the 41 are three passes
 // by one workgroup, one after the other since each needs the mass that the last one
 // left.  With little gain there (47 to 44 us together, without the shorter passes):
 // leaving out nodes that the walk cannot reach, the next block's loads under the
