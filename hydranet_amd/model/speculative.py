@@ -180,16 +180,23 @@ def tree_attention(q: torch.Tensor, tree: DraftTree, lens: torch.Tensor, cache, 
     at = torch.arange(kv_bound) - lens[:, None]  # node at each position, negative: cached
     node = at.clamp(0, S - 1)[:, None].expand(B, S, kv_bound)
     see = torch.gather(tree.visible().expand(B, S, S), 2, node) & (at < S)[:, None]
-    see = (see | (at < 0)[:, None]) & (tree.depth.expand(B, S) >= 0)[..., None]
-    see = (see & (lens >= 0)[:, None, None])[:, None, None]
+    live = (tree.depth.expand(B, S) >= 0) & (lens >= 0)[:, None]
+    see = ((see | (at < 0)[:, None]) & live[..., None])[:, None, None]
     wide = torch.float64 if q.dtype == torch.float64 else torch.float32
     s = torch.matmul(q.to(wide), kt[..., :kv_bound].to(wide)) / math.sqrt(hd)
     s = s.view(B, nkv, rep, S, kv_bound).masked_fill(~see, -math.inf)
-    p = torch.where(see, torch.softmax(s, -1), 0.0).nan_to_num(0.0)
+    p = torch.where(see, torch.softmax(s, -1), 0.0)
     vv = v[:, :, :kv_bound].to(wide)
     vv = torch.where((at < S)[:, None, :, None], vv, 0.0)  # positions no node sees
-    o = torch.matmul(p.view(B, nkv, rep * S, kv_bound), vv).view(B, nkv * rep, S, hd)
-    o = torch.where((lens + S > kv_bound)[:, None, None, None] & see.any(-1).view(B, 1, S, 1),
+    # a node's value that is no number reaches the rows that see it, not the product,
+    # where 0 times it would reach every row
+    odd = ~vv.isfinite() & (at >= 0)[:, None, :, None]
+    o = torch.matmul(p.view(B, nkv, rep * S, kv_bound), torch.where(odd, 0.0, vv))
+    o = o.view(B, nkv, rep, S, hd)
+    for b, n in odd.any(3).any(1).nonzero().tolist():
+        o[b, :, :, see[b, 0, 0, :, n]] += torch.where(odd, vv, 0.0)[b, :, n][:, None, None]
+    o = torch.where(live[:, None, None, :, None], o, 0.0).view(B, nkv * rep, S, hd)
+    o = torch.where((lens + S > kv_bound)[:, None, None, None] & live[:, None, :, None],
                     math.nan, o)
     return o.transpose(1, 2).reshape(B, S, nkv * rep * hd).to(q.dtype)
 

@@ -308,3 +308,76 @@ def test_a_cache_is_copied_after_its_layers_were_passed_to_a_kernel():
     assert a[0][0] == c.kt[0].data_ptr() and b[0][0] == d.kt[0].data_ptr() != a[0][0]
     c.v[0] = torch.ones(1, 1, 8, 4).half()
     assert c._layers()[1][0] == c.v[0].data_ptr()
+
+
+def _random_attention(rows, C, n, nkv=2, rep=2, hd=8, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    B, S = len(rows), len(rows[0])
+    c = KVCache.wrap([torch.randn(B, nkv, hd, n, generator=g, dtype=torch.float64)],
+                     [torch.randn(B, nkv, n, hd, generator=g, dtype=torch.float64)])
+    q = torch.randn(B, nkv, rep * S, hd, generator=g, dtype=torch.float64)
+    return q, c, torch.full((B,), C, dtype=torch.int64)
+
+
+def test_attention_hidden_nodes_hold_nan_and_infinities():
+    """A branch whose keys or values overflowed changes no row outside it, and reaches the rows
+    that see it."""
+    S, C, hd = 8, 5, 8
+    rows = [[-1, 0, 0, 0, 0, 0, 3, -2]]
+    q, clean, lens = _random_attention(rows, C, 16)
+    c = KVCache.wrap([clean.kt[0].clone()], [clean.v[0].clone()])
+    c.kt[0][:, :, 5, C + 2] = float("nan")
+    c.v[0][:, :, C + 3, 7] = float("inf")
+    c.v[0][:, 1, C + 4, 6] = float("nan")
+    c.v[0][:, :, C + 5] = -float("inf")
+    c.v[0][:, :, C + 7] = float("nan")  # padding's
+    a = tree_attention(q, _tree(rows), lens, clean, 0, 16).view(S, 2, 2, hd)
+    b = tree_attention(q, _tree(rows), lens, c, 0, 16).view(S, 2, 2, hd)
+    # sums of 13 terms below 4, perhaps in another order: 16 roundings of 2^-53 times 4, twice
+    close = dict(rtol=0, atol=2.0 ** -45)
+    torch.testing.assert_close(a[[0, 1]], b[[0, 1]], **close)
+    assert bool(b[2].isnan().all())
+    for i in (3, 6):  # the node and its child
+        torch.testing.assert_close(a[i, ..., :7], b[i, ..., :7], **close)
+        assert bool(b[i, ..., 7].isposinf().all())
+    torch.testing.assert_close(a[4, 0], b[4, 0], **close)
+    torch.testing.assert_close(a[4, 1, :, [0, 1, 2, 3, 4, 5, 7]],
+                               b[4, 1, :, [0, 1, 2, 3, 4, 5, 7]], **close)
+    assert bool(b[4, 1, :, 6].isnan().all()) and bool(b[5].isneginf().all())
+    assert bool((b[7] == 0).all())
+
+
+def test_attention_nan_that_a_row_sees():
+    """A cached key, a query: the rows that hold them are NaN; padding and inactive sequences stay
+    zero whatever the cache holds."""
+    rows = [[-1, 0, -2], [-1, 0, 1], [-1, 0, 1]]
+    q, c, lens = _random_attention(rows, 6, 12)
+    lens[2] = -1
+    c.kt[0][0, 0, 3, 2] = float("nan")
+    c.v[0][0, 1, 4] = float("inf")
+    c.v[0][2] = float("nan")
+    q.view(3, 2, 2, 3, 8)[1, 1, 0, 2, 5] = float("nan")
+    o = tree_attention(q, _tree(rows), lens, c, 0, 12).view(3, 3, 2, 2, 8)
+    assert bool(o[0, :2, 0].isnan().all()) and bool(o[0, :2, 1].isposinf().all())
+    assert bool((o[0, 2] == 0).all()) and bool((o[2] == 0).all())
+    bad = o[1].isnan()
+    assert bool(bad[2, 1, 0].all()) and int(bad.sum()) == 8
+
+
+def test_attention_of_a_node_past_the_table_is_nan():
+    B, nkv, rep, hd, n, S = 1, 1, 2, 8, 16, 3
+    c = KVCache.wrap([torch.randn(B, nkv, hd, n)], [torch.randn(B, nkv, n, hd)])
+    tab, tree, lens = torch.rand(10, hd), DraftTree.chain(S), torch.tensor([8])
+    q = tree_append(torch.randn(S, 4 * hd), tab, tab, tree, lens, c, 0, rep)
+    o = tree_attention(q, tree, lens, c, 0, n)
+    assert bool(o[0, 2].isnan().all()) and not bool(o[0, :2].isnan().any())
+
+
+def test_attention_with_a_head_of_infinite_scores():
+    """Every visible score at -inf, or one at +inf: no probabilities."""
+    rows = [[-1, 0]]
+    q, c, lens = _random_attention(rows, 3, 8, rep=1)
+    q.fill_(1.0)
+    c.kt[0][:, 0] = -float("inf")
+    c.kt[0][:, 1, 0, 1] = float("inf")
+    assert bool(tree_attention(q, _tree(rows), lens, c, 0, 8).isnan().all())
