@@ -168,7 +168,7 @@ class KVCache:
             return out
         j = torch.arange(S)
         c = count.clamp(0, S)
-        src = lens[:, None] + path
+        src = lens.clamp(max=2 ** 62)[:, None] + path  # (no sum wraps)
         ok = (j < c[:, None]) & (path >= j) & (lens >= 0)[:, None] & (src < n)
         b, j = ok.nonzero(as_tuple=True)
         for kt, v in zip(self.kt, self.v):

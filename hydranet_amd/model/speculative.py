@@ -124,7 +124,8 @@ def tree_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, tree: D
         return q
     depth, at = tree.depth.expand(B, S).long(), torch.arange(S)
     live = (depth >= 0) & (lens >= 0)[:, None]
-    pos, slot = lens[:, None] + depth, lens[:, None] + at
+    start = lens.clamp(max=2 ** 62)[:, None]  # (no sum wraps)
+    pos, slot = start + depth, start + at
     ok = live & (pos < cos.shape[0]) & (slot < max_len)
     x = qkv.view(B, S, num_heads + 2 * nkv, hd)
     x32 = x if x.dtype == torch.float64 else x.float()
@@ -196,7 +197,7 @@ def tree_attention(q: torch.Tensor, tree: DraftTree, lens: torch.Tensor, cache, 
     for b, n in odd.any(3).any(1).nonzero().tolist():
         o[b, :, :, see[b, 0, 0, :, n]] += torch.where(odd, vv, 0.0)[b, :, n][:, None, None]
     o = torch.where(live[:, None, None, :, None], o, 0.0).view(B, nkv * rep, S, hd)
-    o = torch.where((lens + S > kv_bound)[:, None, None, None] & live[:, None, :, None],
+    o = torch.where((lens > kv_bound - S)[:, None, None, None] & live[:, None, :, None],
                     math.nan, o)
     return o.transpose(1, 2).reshape(B, S, nkv * rep * hd).to(q.dtype)
 

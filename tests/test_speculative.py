@@ -381,3 +381,24 @@ def test_attention_with_a_head_of_infinite_scores():
     c.kt[0][:, 0] = -float("inf")
     c.kt[0][:, 1, 0, 1] = float("inf")
     assert bool(tree_attention(q, _tree(rows), lens, c, 0, 8).isnan().all())
+
+
+def test_lengths_past_everything():
+    """A length near the largest int64 counts as past the cache; the others are as ever."""
+    top, S, n, hd = 2 ** 63 - 1, 4, 16, 8
+    lens = torch.tensor([top, 5, top - 2, 2 ** 32 + 5])
+    tree, tab = DraftTree.chain(S), torch.rand(n, hd)
+    c = _cache(4, 1, hd, n)
+    kt, v = c.kt[0].clone(), c.v[0].clone()
+    q = tree_append(torch.randn(4 * S, 4 * hd, dtype=torch.float64), tab, tab, tree, lens, c, 0, 2)
+    o = tree_attention(q, tree, lens, c, 0, n)
+    for b in (0, 2, 3):
+        assert bool(q[b].isnan().all()) and bool(o[b].isnan().all())
+        assert torch.equal(c.kt[0][b], kt[b]) and torch.equal(c.v[0][b], v[b])
+    assert not bool(q[1].isnan().any()) and not bool(o[1].isnan().any())
+    kt, v = c.kt[0].clone(), c.v[0].clone()
+    path = torch.tensor([[0, 2, 3, -1]] * 4, dtype=torch.int32)
+    c.keep(lens, path, torch.full((4,), 3, dtype=torch.int32))
+    for b in (0, 2, 3):
+        assert torch.equal(c.kt[0][b], kt[b]) and torch.equal(c.v[0][b], v[b])
+    assert torch.equal(c.v[0][1, :, 6], v[1, :, 7]) and torch.equal(c.kt[0][1, ..., 7], kt[1, ..., 8])
