@@ -6,6 +6,8 @@
 // it, is padding.  Node i of a sequence with C = lens[b] cached positions sits
 // at cache position C + i, its rotary position is C + depth(i), and it sees
 // positions [0, C) and those of itself and its ancestors.
+#include <float.h>
+
 #include "hn_common.h"
 #include "hn_lds_dma.h"
 
@@ -913,6 +915,9 @@ extern "C" int hn_tree_attention(const void* q, const void* kt, const void* v, l
   HN_ARG_CHECK(bound >= S && bound <= max_len && max_len % 8 == 0 && max_len < (1L << 23),
                "%s: need nodes <= bound <= max_len, max_len %% 8 == 0, below 2^23", who);
   if (B == 0) return 0;
+  // (the kernel masks scores and takes their maximum before it scales them)
+  HN_ARG_CHECK(scale > 0.f && scale <= FLT_MAX / kLog2e, "%s: scale must be finite and above 0",
+               who);
   HN_ARG_CHECK(al16(q) && al16(kt) && al16(v) && al16(out) && ld_o % 8 == 0 &&
                    ld_o >= nkv * rep * hd && lens && seen,
                "%s: operands must be 16-byte aligned, ld_o >= heads * %d", who, kHd);

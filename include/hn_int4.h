@@ -476,8 +476,9 @@ int hn_tree_append(const void* qkv, long ld_qkv, const float* cos_t, const float
  *   hn_tree_plan.  bound: at least C_b + S of every sequence (it sizes the
  *   launch; a sequence past it gives NaN).  Rows of padding nodes and of
  *   sequences with a negative length are zero.  A position that a row does not
- *   see has no effect on it, whatever it holds.  hd 128, max_len a multiple of 8
- *   below 2^23, 16-byte aligned operands, ld_o a multiple of 8.  work:
+ *   see has no effect on it, whatever it holds.  scale above 0 and finite, also
+ *   times log2(e).  hd 128, max_len a multiple of 8 below 2^23, 16-byte aligned
+ *   operands, ld_o a multiple of 8.  work:
  *   hn_tree_attention_workspace_bytes(...) bytes, any contents. */
 long hn_tree_attention_workspace_bytes(long B, long nkv, long rep, long S, long bound);
 int hn_tree_attention(const void* q, const void* kt, const void* v, long max_len, const long* lens,

@@ -402,3 +402,15 @@ def test_lengths_past_everything():
     for b in (0, 2, 3):
         assert torch.equal(c.kt[0][b], kt[b]) and torch.equal(c.v[0][b], v[b])
     assert torch.equal(c.v[0][1, :, 6], v[1, :, 7]) and torch.equal(c.kt[0][1, ..., 7], kt[1, ..., 8])
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.0, -1.0, float("inf"), -float("inf"), float("nan"), 3e38])
+def test_library_refuses_scales_without_gpu(scale):
+    """Scores are masked before they are scaled: a scale that is not above zero, or not finite
+    (also as a power of two), is refused before any HIP call."""
+    import ctypes
+    from hydranet_amd import _lib
+    P = ctypes.c_void_p(16)
+    with pytest.raises(RuntimeError, match="hn_tree_attention: scale"):
+        _lib.call("hn_tree_attention", P, P, P, 16, P, P, 1, 1, 1, 1, 128, 1, 9, scale, P, 128, P,
+                  1 << 30, None)
