@@ -915,11 +915,12 @@ extern "C" int hn_tree_attention(const void* q, const void* kt, const void* v, l
   HN_ARG_CHECK(bound >= S && bound <= max_len && max_len % 8 == 0 && max_len < (1L << 23),
                "%s: need nodes <= bound <= max_len, max_len %% 8 == 0, below 2^23", who);
   if (B == 0) return 0;
+  HN_ARG_CHECK(q && kt && v && lens && seen && out, "%s: null operand", who);
   // (the kernel masks scores and takes their maximum before it scales them)
   HN_ARG_CHECK(scale > 0.f && scale <= FLT_MAX / kLog2e, "%s: scale must be finite and above 0",
                who);
   HN_ARG_CHECK(al16(q) && al16(kt) && al16(v) && al16(out) && ld_o % 8 == 0 &&
-                   ld_o >= nkv * rep * hd && lens && seen,
+                   ld_o >= nkv * rep * hd,
                "%s: operands must be 16-byte aligned, ld_o >= heads * %d", who, kHd);
   const Plan p = plan_of(B, nkv, rep, S, bound);
   const long R = rep * S;

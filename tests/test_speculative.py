@@ -414,3 +414,14 @@ def test_library_refuses_scales_without_gpu(scale):
     with pytest.raises(RuntimeError, match="hn_tree_attention: scale"):
         _lib.call("hn_tree_attention", P, P, P, 16, P, P, 1, 1, 1, 1, 128, 1, 9, scale, P, 128, P,
                   1 << 30, None)
+
+
+@pytest.mark.parametrize("which", [0, 1, 2, 4, 5, 14])
+def test_library_refuses_null_operands_without_gpu(which):
+    import ctypes
+    from hydranet_amd import _lib
+    P = ctypes.c_void_p(16)
+    args = [P, P, P, 16, P, P, 1, 1, 1, 1, 128, 1, 9, 1.0, P, 128, P, 1 << 30, None]
+    args[which] = None
+    with pytest.raises(RuntimeError, match="hn_tree_attention: null operand"):
+        _lib.call("hn_tree_attention", *args)
