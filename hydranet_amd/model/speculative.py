@@ -381,6 +381,8 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int,
     size, out = [P] * N, [[] for _ in range(N)]
 
     def emit(i, tokens):
+        # (a draft may reach past the last position of the model: no logits there)
+        tokens = tokens[:max_new_tokens - len(out[i])]
         if -1 in tokens:
             raise RuntimeError(f"sequence {i}: no logit is finite")
         out[i] += tokens
@@ -406,4 +408,4 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int,
             if not done[i]:
                 size[i] += n
                 done[i] = emit(i, t[1:n] + [x])
-    return torch.tensor([o[:max_new_tokens] for o in out], dtype=torch.int64, device=dev)
+    return torch.tensor(out, dtype=torch.int64, device=dev)

@@ -425,3 +425,42 @@ def test_library_refuses_null_operands_without_gpu(which):
     args[which] = None
     with pytest.raises(RuntimeError, match="hn_tree_attention: null operand"):
         _lib.call("hn_tree_attention", *args)
+
+
+class _Short(_Counting):
+    """No position from `rows` on: the nodes there have no logits."""
+
+    def __init__(self, vocab, rows):
+        super().__init__(vocab)
+        self.rows = rows
+
+    def forward_tree(self, tokens, tree, lens, cache, bound):
+        logits = super().forward_tree(tokens, tree, lens, cache, bound)
+        past = lens[:, None] + tree.depth >= self.rows
+        return torch.where(past[..., None], float("nan"), logits)
+
+
+@pytest.mark.parametrize("wide", [1, 2, 3, 5, 9])
+@pytest.mark.parametrize("over", [0, 1])
+def test_generate_up_to_the_models_last_position(wide, over):
+    """A draft may reach past the last position; what is asked for does not."""
+    from hydranet_amd.model.speculative import Draft, generate
+    V, n, seen = 50, 11, []
+
+    def draft(history, device):
+        seen.append([list(h) for h in history])
+        rows = [[(h[-1] + 1 + j) % V for j in range(wide)] for h in history]
+        return Draft(torch.tensor(rows), torch.arange(-1, wide, dtype=torch.int32))
+
+    prompt = torch.tensor([[3, 4, 5], [48, 49, 0]])
+    # (the last token asked for is never fed: the text may be one longer than the table)
+    out = generate(_Short(V, 3 + n - over), prompt, n, draft)
+    want = (prompt[:, -1:] + 1 + torch.arange(n)) % V
+    assert torch.equal(out, want)
+    assert all(len(h) <= 3 + n and min(h) >= 0 for hs in seen for h in hs)
+
+
+def test_generate_without_a_finite_logit():
+    from hydranet_amd.model.speculative import generate
+    with pytest.raises(RuntimeError, match="no logit is finite"):
+        generate(_Short(50, 7), torch.tensor([[3, 4, 5]]), 9)
