@@ -307,9 +307,13 @@ class Attention(nn.Module):
         rep = nh // nkv
         if x.is_cuda:
             from .. import _lib
-            # positions are < cache.max_len (checked by the callers), so the
-            # RoPE table rows read are in range
-            assert cache.max_len <= rope.cos_cached.shape[0], "RoPE table shorter than the cache"
+            # positions are < kv_len (checked by the callers), so the RoPE table rows
+            # read are in range; the kernels leave out a position past the cache, and
+            # with a longer cache than the table one past the table likewise
+            rows = rope.cos_cached.shape[0]
+            assert kv_len <= rows, "RoPE table shorter than the positions"
+            if cache.max_len > rows:
+                pos = pos.masked_fill(pos >= rows, cache.max_len)
             assert x.dtype == torch.float16 and pos.dtype == torch.int64
             # the kernel reads fp32 tables (a module-wide .half() would have cast them)
             cos_t = rope.cos_cached.float().contiguous()
@@ -605,6 +609,9 @@ class MixtralDecoder(nn.Module):
         drafter (by default one that looks up repeated tokens) guessed them;
         distributed as without it.  See model/speculative.py: generate."""
         from .speculative import generate
+        rows, P = self.rotary.cos_cached.shape[0], input_ids.shape[1]
+        assert P + max_new_tokens - 1 <= rows, \
+            f"{max_new_tokens} tokens after {P}: the model has {rows} positions"
         return generate(self, input_ids, max_new_tokens, draft, temperature, samples, generator,
                         max_nodes)
 
@@ -627,6 +634,8 @@ class GraphDecoder:
         dev = tok.device
         if cache.cur_len >= cache.max_len:
             raise RuntimeError(f"KV cache full ({cache.max_len} positions)")
+        rows = model.rotary.cos_cached.shape[0]
+        assert cache.max_len <= rows, f"RoPE table shorter than the cache ({rows} positions)"
         self.bucket = bucket
         self.tok = tok.clone()
         self.pos = torch.full((1,), cache.cur_len, dtype=torch.int64, device=dev)

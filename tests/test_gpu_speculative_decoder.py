@@ -89,3 +89,62 @@ def test_generate(model, samples, temperature):
     d = ngram_draft([text, [5, 6, 7]], DEV, nodes=4)
     assert d.tokens.tolist() == [[3, 4, 1], [0, 0, 0]]
     assert d.parents.tolist() == [[-1, 0, 1, 2], [-1, -2, -2, -2]]
+
+
+def _near_largest(model, text, P, out):
+    """Whether each token of out is a largest logit of a plain pass over the text, within the
+    bar on both logits."""
+    B, n = out.shape
+    logits = model.forward(text, model.new_cache(B, text.shape[1]), top_k=2)[:, P - 1:P - 1 + n]
+    logits = logits.float()
+    chosen, top = logits.gather(2, out[..., None])[..., 0], logits.max(-1).values
+    return chosen >= top - 2 * (3e-2 + 1e-2 * top.abs())
+
+
+@pytest.mark.parametrize("P,n", [(200, 56), (250, 6), (255, 1), (256, 1), (249, 8)])
+def test_generate_up_to_the_models_last_position(model, P, n):
+    """256 positions: the last token fed is at most the 256th, so the text is at most 257."""
+    from hydranet_amd.model.speculative import Draft
+    g = torch.Generator(device=DEV).manual_seed(P)
+    ids = torch.randint(0, 512, (2, P), generator=g, device=DEV)
+
+    def wide(history, device):
+        """Three nodes that reach past the end, and repeat whatever came last."""
+        return Draft(torch.tensor([[h[-1]] * 3 for h in history], device=device),
+                     torch.arange(-1, 3, dtype=torch.int32, device=device))
+    for draft in (None, wide):
+        out = model.generate_speculative(ids, n, draft)
+        text = torch.cat((ids, out), 1)
+        assert tuple(text.shape) == (2, P + n) and int(out.min()) >= 0
+        # (0.95 as above: a router's near-tie may fall either way)
+        assert float(_near_largest(model, text[:, :256], P, out).float().mean()) >= 0.95
+
+
+def test_texts_past_the_last_position_are_refused(model):
+    from hydranet_amd.model.decoder import GraphDecoder
+    ids = torch.zeros((1, 250), dtype=torch.int64, device=DEV)
+    with pytest.raises(AssertionError, match="positions"):
+        model.generate_speculative(ids, 8)
+    cache = model.new_cache(1, 264)  # longer than the table
+    tok = model.forward(ids, cache)[:, -1].argmax(-1, keepdim=True)
+    with pytest.raises(AssertionError, match="RoPE table"):
+        GraphDecoder(model, cache, tok)
+    for _ in range(6):
+        tok = model.forward(tok, cache)[:, -1].argmax(-1, keepdim=True)
+    with pytest.raises(AssertionError, match="RoPE table"):
+        model.forward(tok, cache)
+
+
+def test_positions_past_the_table_are_outside_a_longer_cache(model):
+    """Prefill and a one-token step at positions that the table lacks write nothing there."""
+    cache = model.new_cache(1, 264)
+    ids = torch.zeros((1, 70), dtype=torch.int64, device=DEV)
+    pos = torch.arange(256, 326, device=DEV)
+    model.step(ids[:, :1], pos[:1], cache, 256, None, 2)
+    assert not any(bool(t.any()) for t in cache.kt + cache.v)
+    pos[0] = 3
+    model.step(ids, pos, cache, 256, None, 2)
+    for kt, v in zip(cache.kt, cache.v):
+        assert bool((v[0, :, 3] != 0).any()) and bool((kt[0, ..., 3] != 0).any())
+        for t in (v[0].transpose(1, 2), kt[0]):
+            assert not bool(t[..., :3].any()) and not bool(t[..., 4:].any())
