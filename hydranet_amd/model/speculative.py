@@ -397,6 +397,7 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int,
         tree = DraftTree(d.parents)
         tokens = torch.cat((last.clamp(min=0)[:, None], d.tokens), 1)
         assert tokens.shape[1] == tree.nodes, f"{tree.nodes} nodes, {d.tokens.shape[1]} tokens"
+        assert tree.nodes <= max_nodes, f"at most {max_nodes} nodes, the draft has {tree.nodes}"
         bound = max(n for n, over in zip(size, done) if not over) + tree.nodes
         inside = tokens.clamp(0, first_logits.shape[-1] - 1)
         logits = model.forward_tree(inside, tree, lens, cache, bound)

@@ -464,3 +464,17 @@ def test_generate_without_a_finite_logit():
     from hydranet_amd.model.speculative import generate
     with pytest.raises(RuntimeError, match="no logit is finite"):
         generate(_Short(50, 7), torch.tensor([[3, 4, 5]]), 9)
+
+
+def test_generate_refuses_a_draft_wider_than_said():
+    """At once, not where the cache happens to end."""
+    from hydranet_amd.model.speculative import Draft, generate
+    model = _Counting(50)
+
+    def draft(history, device):
+        return Draft(torch.zeros(len(history), 5, dtype=torch.int64),
+                     torch.arange(-1, 5, dtype=torch.int32))
+    with pytest.raises(AssertionError, match="at most 5 nodes"):
+        generate(model, torch.tensor([[3, 4, 5]]), 30, draft, max_nodes=5)
+    assert model.passes == 0
+    assert generate(model, torch.tensor([[3, 4, 5]]), 30, draft, max_nodes=6).shape == (1, 30)
