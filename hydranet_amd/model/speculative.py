@@ -358,7 +358,8 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int,
     Each prompt is prefilled once and its cache forked to its samples; a pass then
     takes the last token and the drafter's tree of each sequence, verifies, and
     compacts the cache.  draft(history, device) -> Draft, history the tokens of
-    each sequence so far, at most max_nodes nodes.  One host synchronisation per pass."""
+    each sequence so far, at most max_nodes nodes.  A pass reads the device back once
+    (beside what the drafter does)."""
     draft = draft or ngram_draft
     B, P = input_ids.shape
     assert samples >= 1 and max_new_tokens >= 1 and P >= 1, "samples, tokens and prompt >= 1"
@@ -389,9 +390,10 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int,
         history[i] += tokens
         return len(out[i]) >= max_new_tokens
 
-    done = [emit(i, [t]) for i, t in enumerate(last.tolist())]
+    done, out_of = [emit(i, [t]) for i, t in enumerate(last.tolist())], 0
     while not all(done):
-        if any(done):  # finished sequences take no part
+        if sum(done) > out_of:  # finished sequences take no part
+            out_of = sum(done)
             lens = torch.where(torch.tensor(done, device=dev), -1, lens)
         d = draft(history, dev)
         tree = DraftTree(d.parents)
@@ -405,7 +407,8 @@ def generate(model, input_ids: torch.Tensor, max_new_tokens: int,
         lens = cache.keep(lens, r.path, r.count)
         last = r.token
         took = torch.gather(tokens, 1, r.path.clamp(min=0).long())
-        for i, (n, t, x) in enumerate(zip(r.count.tolist(), took.tolist(), last.tolist())):
+        back = torch.cat((r.count[:, None].long(), last[:, None], took), 1)
+        for i, (n, x, *t) in enumerate(back.tolist()):
             if not done[i]:
                 size[i] += n
                 done[i] = emit(i, t[1:n] + [x])

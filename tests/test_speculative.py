@@ -478,3 +478,32 @@ def test_generate_refuses_a_draft_wider_than_said():
         generate(model, torch.tensor([[3, 4, 5]]), 30, draft, max_nodes=5)
     assert model.passes == 0
     assert generate(model, torch.tensor([[3, 4, 5]]), 30, draft, max_nodes=6).shape == (1, 30)
+
+
+def test_generate_reads_the_device_back_once_a_pass(monkeypatch):
+    from hydranet_amd.model import speculative
+    from hydranet_amd.model.speculative import Draft, generate
+    V, n, reads, inside = 50, 12, [0], [0]
+
+    def draft(history, device):  # the second sequence's is wrong, so that the first ends before
+        return Draft(torch.tensor([[(h[-1] + 1 + j) % V if h[0] == 3 else 0 for j in range(2)]
+                                   for h in history]),
+                     torch.tensor([-1, 0, 1], dtype=torch.int32))
+
+    def tolist(self, _old=torch.Tensor.tolist):
+        reads[0] += not inside[0]
+        return _old(self)
+    monkeypatch.setattr(torch.Tensor, "tolist", tolist)
+    for owner, name in ((speculative, "verify_tree"), (DraftTree, "__init__")):  # GPU: kernels
+        def kernel(*args, _old=getattr(owner, name)):
+            inside[0] += 1
+            try:
+                return _old(*args)
+            finally:
+                inside[0] -= 1
+        monkeypatch.setattr(owner, name, kernel)
+    model = _Counting(V)
+    out = generate(model, torch.tensor([[3, 4, 5], [13, 14, 15]]), n, draft)
+    assert out.flatten().numpy().tolist() == [*range(6, 6 + n), *range(16, 16 + n)]
+    assert model.passes == n - 1
+    assert reads[0] == model.passes + 2  # and the prompt and the first tokens
