@@ -148,3 +148,54 @@ def test_positions_past_the_table_are_outside_a_longer_cache(model):
         assert bool((v[0, :, 3] != 0).any()) and bool((kt[0, ..., 3] != 0).any())
         for t in (v[0].transpose(1, 2), kt[0]):
             assert not bool(t[..., :3].any()) and not bool(t[..., 4:].any())
+
+
+@pytest.mark.parametrize("samples", [1, 2])
+def test_generate_accepts_what_the_model_would_say(model, samples):
+    """A drafter that knows the text: few passes, kept nodes that were not next to each other,
+    and the text again (where the two part, both tokens are largest logits within the bar)."""
+    from hydranet_amd.model.speculative import Draft
+    g = torch.Generator(device=DEV).manual_seed(11)
+    B, P, n = 2, 9, 25
+    ids = torch.randint(0, 512, (B, P), generator=g, device=DEV)
+    want = model.generate_speculative(ids, n, samples=samples)
+
+    def known(history, device):  # nodes 1 and 2 are wrong, 3 to 5 the text
+        rows = []
+        for i, h in enumerate(history):
+            rest = want[i].tolist()[len(h) - P:][:3]
+            rows.append([511 - h[-1], 0] + rest + [0] * (3 - len(rest)))
+        return Draft(torch.tensor(rows, device=device),
+                     torch.tensor([-1, 0, 1, 0, 3, 4], dtype=torch.int32, device=device))
+    passes, plain = [0], model.forward_tree
+
+    def counted(*args):
+        passes[0] += 1
+        return plain(*args)
+    model.forward_tree = counted
+    try:
+        got = model.generate_speculative(ids, n, known, samples=samples)
+    finally:
+        del model.forward_tree
+    text = torch.cat((ids.repeat(samples, 1), got), 1)
+    same = (got == want).cumprod(1).bool()  # up to where they part
+    at = same.sum(1)
+    for i in range(samples * B):
+        if at[i] < n:
+            two = torch.cat((text[i:i + 1, :P + at[i]], want[i:i + 1, at[i]:at[i] + 1]), 1)
+            for t in (text[i:i + 1, :P + at[i] + 1], two):
+                assert bool(_near_largest(model, t, t.shape[1] - 1, t[:, -1:]).all())
+    # four tokens a pass, after the first, where the text is the same to its end
+    if bool((at == n).all()):
+        assert passes[0] == (n - 1) // 4
+    assert passes[0] <= (n - 1) // 2
+
+
+def test_generate_at_a_low_temperature_is_greedy(model):
+    """At 1e-4 a logit that is 3e-3 lower has e^-30 of the largest's probability."""
+    g = torch.Generator(device=DEV).manual_seed(12)
+    P, n = 9, 17
+    ids = torch.randint(0, 512, (2, P), generator=g, device=DEV)
+    out = model.generate_speculative(ids, n, temperature=1e-4, samples=2, generator=g)
+    text = torch.cat((ids.repeat(2, 1), out), 1)
+    assert float(_near_largest(model, text, P, out).float().mean()) >= 0.95

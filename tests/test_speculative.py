@@ -507,3 +507,47 @@ def test_generate_reads_the_device_back_once_a_pass(monkeypatch):
     assert out.flatten().numpy().tolist() == [*range(6, 6 + n), *range(16, 16 + n)]
     assert model.passes == n - 1
     assert reads[0] == model.passes + 2  # and the prompt and the first tokens
+
+
+class _Markov:
+    """A model whose next token hangs on the last one alone."""
+
+    def __init__(self, table):
+        self.table = table
+
+    def new_cache(self, batch, max_len):
+        return KVCache.wrap([torch.zeros(batch, 1, 1, max_len)], [torch.zeros(batch, 1, max_len, 1)])
+
+    def forward(self, ids, cache):
+        return self.table[ids]
+
+    def forward_tree(self, tokens, tree, lens, cache, bound):
+        return self.table[tokens]
+
+
+@pytest.mark.parametrize("soft", [True, False])
+def test_generate_keeps_the_models_distribution(soft):
+    """The first three tokens after a prompt, jointly, with trees of two branches drawn from
+    another model (or certain).  N draws: a frequency's deviation is sqrt(p (1 - p) / N); 5 of
+    it."""
+    from hydranet_amd.model.speculative import Draft, generate
+    g = torch.Generator().manual_seed(4)
+    V, N, T = 3, 6000, 0.7
+    table, other = torch.randn(V, V, generator=g), torch.randn(V, V, generator=g)
+    q = torch.softmax(other / T, -1)
+    parents = torch.tensor([-1, 0, 0, 1, 2], dtype=torch.int32)
+
+    def draft(history, device):
+        last = torch.tensor([h[-1] for h in history])
+        if not soft:
+            return Draft(torch.stack((last, (last + 1) % V, last, last), 1), parents)
+        a = torch.multinomial(q[last], 2, replacement=True, generator=g)
+        b = torch.multinomial(q[a.flatten()], 1, generator=g).view(N, 2)
+        nodes = torch.cat((last[:, None], a, b), 1)
+        return Draft(nodes[:, 1:], parents, other[nodes])
+
+    out = generate(_Markov(table), torch.tensor([[1]]), 3, draft, T, samples=N, generator=g)
+    p = torch.softmax(table.double() / T, -1)
+    want = p[1][:, None, None] * p[:, :, None] * p[None]
+    got = torch.bincount((out * torch.tensor([V * V, V, 1])).sum(1), minlength=V ** 3).double() / N
+    assert bool(((got.view(V, V, V) - want).abs() < 5 * (want * (1 - want) / N).sqrt()).all())
