@@ -199,3 +199,98 @@ def test_generate_at_a_low_temperature_is_greedy(model):
     out = model.generate_speculative(ids, n, temperature=1e-4, samples=2, generator=g)
     text = torch.cat((ids.repeat(2, 1), out), 1)
     assert float(_near_largest(model, text, P, out).float().mean()) >= 0.95
+
+
+@pytest.mark.parametrize("S", [6, 61])
+def test_a_decoder_pass_captured_and_replayed(model, S):
+    """forward_tree, verification and compaction of a step in one graph, replayed with other
+    inputs: the eager pass each time.  (12 and 122 tokens: the MoE layers' decode and prefill
+    kernels.)"""
+    from hydranet_amd.model.decoder import KVCache
+    from hydranet_amd.model.speculative import DraftTree, verify_tree
+    B, rng = 2, random.Random(S)
+    tree = DraftTree(torch.tensor([ref.random_tree(rng, S, "padded") for _ in range(B)],
+                                  dtype=torch.int32, device=DEV))
+    g = torch.Generator(device=DEV).manual_seed(S)
+    cache = model.new_cache(B, 256)
+    start = [[torch.randn(t.shape, generator=g, device=DEV).half() for t in ts]
+             for ts in (cache.kt, cache.v)]
+
+    def inputs():
+        return [torch.randint(0, 512, (B, S), generator=g, device=DEV),
+                torch.randint(0, 190, (B,), generator=g, device=DEV),
+                torch.rand(B, S, generator=g, device=DEV)]
+
+    def step(c, x):
+        logits = model.forward_tree(x[0], tree, x[1], c, 256)
+        r = verify_tree(logits, x[0], tree, x[2], None, 0.1)
+        return [logits, *r, c.keep(x[1], r.path, r.count)]
+
+    st = inputs()
+    side = torch.cuda.Stream(device=DEV)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(cache, st)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(cache, st)
+    for _ in range(4):
+        for a, b in zip(st, inputs()):
+            a.copy_(b)
+        for ts, olds in zip((cache.kt, cache.v), start):
+            for t, old in zip(ts, olds):
+                t.copy_(old)
+        other = KVCache.wrap(*[[t.clone() for t in ts] for ts in start])
+        want = step(other, st)
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got + cache.kt + cache.v, want + other.kt + other.v):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("S", [4, 61])
+def test_a_sequence_past_the_positions_changes_no_other(model, S):
+    """Rows without numbers reach no expert; the other sequence's rows are what they are beside a
+    sequence that takes no part."""
+    from hydranet_amd.model.speculative import DraftTree
+    g = torch.Generator(device=DEV).manual_seed(S)
+    tokens = torch.randint(0, 512, (2, S), generator=g, device=DEV)
+    tree, out = DraftTree.chain(S, DEV), []
+    kv = None
+    for second in (320, 255, -1):  # past the cache, its first node in the table, none
+        cache = model.new_cache(2, 320)
+        kv = kv or [torch.randn(t.shape, generator=g, device=DEV).half() for t in cache.kt + cache.v]
+        for t, x in zip(cache.kt + cache.v, kv):
+            t.copy_(x)
+        lens = torch.tensor([100, second], device=DEV)
+        out.append(model.forward_tree(tokens, tree, lens, cache, 255 + S))
+    _close(out[0][0], out[2][0])
+    _close(out[1][0], out[2][0])
+    assert bool(out[0][1].isnan().all()) and bool(out[1][1, 1:].isnan().all())
+    assert not bool(out[1][1, 0].isnan().any()) and not bool(out[2].isnan().any())
+
+
+def test_int4_attention_tree_logits_equal_each_path_alone():
+    from hydranet_amd.model.decoder import (MixtralDecoderConfig, build_synthetic_decoder,
+                                            convert_dense_to_int4)
+    from hydranet_amd.model.speculative import DraftTree
+    cfg = MixtralDecoderConfig(num_layers=2, hidden_dim=512, intermediate_dim=1024,
+                               num_attention_heads=8, num_kv_heads=2, head_dim=128,
+                               vocab_size=512, num_experts=8, experts_per_token=2,
+                               max_position_embeddings=256)
+    m = convert_dense_to_int4(build_synthetic_decoder(cfg, DEV, decode_top_k=2, seed=3))
+    g = torch.Generator(device=DEV).manual_seed(5)
+    row = [-1, 0, 0, 1, 2, 2]
+    ids = torch.randint(0, 512, (2, 20), generator=g, device=DEV)
+    nodes = torch.randint(0, 512, (2, 6), generator=g, device=DEV)
+    cache = m.new_cache(2, 64)
+    m.forward(ids, cache, top_k=2)
+    lens = torch.full((2,), 20, dtype=torch.int64, device=DEV)
+    got = m.forward_tree(nodes, DraftTree(torch.tensor(row, dtype=torch.int32, device=DEV)), lens,
+                         cache, 26)
+    for i in range(6):
+        text = torch.cat((ids, nodes[:, ref.way_up(row, i)]), 1)
+        _close(got[:, i], m.forward(text, m.new_cache(2, 64), top_k=2)[:, -1])
+    out = m.generate_speculative(ids, 9)
+    assert tuple(out.shape) == (2, 9)
