@@ -20,9 +20,11 @@ struct Layers {
 // destination.  Of the keys, which lie 2 bytes to a row, 8 lanes take a row's step,
 // whose destinations are next to each other: a thread per row, 8 moves in flight,
 // asked the caches for 8 times the lines (94 us for the 74 below).
-// Bound by the keys' lines: a position's 128 elements lie in as many rows of K^T, 2
-// bytes of each.  32 sequences, 32 layers of 8 heads, 128 moved positions: 74 us,
-// 88 MB fetched and 53 MB written for 34 MB of moves.  Threads that read and wrote
+// Bound by memory's requests, not its bytes: a position's 128 elements lie in as many
+// rows of K^T, 2 bytes of each.  32 sequences, 32 layers of 8 heads, 128 moved
+// positions: 73 us, in which 88 MB are fetched and 53 MB written for 34 MB of moves,
+// 29 us at a copy's rate.  Of the 1.13 million writes that reach memory 0.97 million
+// are parts of a 64-byte line, and the waves wait during 84 % of their cycles.  Threads that read and wrote
 // whole lines of a row, 64 or 128 bytes, took 139 and 266 us; 256 threads for 128
 // rows 77, 8 rows in flight per lane 73, two layers per workgroup 66 (but the same as
 // before on a cache that was not just read, 87 us a call).
@@ -105,8 +107,9 @@ __global__ __launch_bounds__(256) void fork_kernel(Layers L, Copies P, long max_
 // (workgroups of keys, then of values; sources; layers).  The last vector of a row
 // of keys may hold positions past n, which stay as they are in the destination.
 // Bound by HBM: 2 prompts of 1901 positions to 5 sequences each, 32 layers of 8
-// heads, 603 us for 3.0 GB (5.0 TB/s, a large copy's 4.9); with 8, 4, 2 vectors
-// per thread and plain stores 673, 635, 622, with 2 and 4 non-temporal 615, 624.
+// heads, 588 us for 3.0 GB (5.1 TB/s, a large copy's 4.9).  Whole calls, timed on
+// one day: 603 us; with 8, 4, 2 vectors per thread and plain stores 673, 635, 622,
+// with 2 and 4 non-temporal 615, 624.
 __global__ __launch_bounds__(256) void fork_vec_kernel(Layers L, Copies P, long max_len, int nkv,
                                                        int hd, int n, int key_groups) {
   const int layer = blockIdx.z, sg = blockIdx.y;

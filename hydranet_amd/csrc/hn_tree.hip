@@ -235,7 +235,12 @@ constexpr uint32_t kNone = 0xfffff000u;  // an offset past any descriptor: reads
 constexpr float kLog2e = 1.4426950408889634f;
 // Probabilities are 2^8 times the softmax's, relative to a maximum that follows
 // the true one only when it lags by 2^6: below 2^14, so fp16 holds them, and
-// those down to 2^-22 of the largest are normal numbers.
+// those down to 2^-22 of the largest are normal numbers.  They are rounded to fp16
+// because that is what the matrix instruction multiplies with fp16 values (in two
+// parts, high and low, the second product would take twice as many); a row's sum is
+// of the rounded ones, so that their weights still add up to 1.  The rows' relative
+// error against 64 bits is 2.3e-4 to 2.7e-4 in the cases above, of which rounding
+// the result to fp16 alone is 2.1e-4.
 constexpr float kUp = 8.f, kLag = 6.f;
 
 typedef float float4v __attribute__((ext_vector_type(4)));
@@ -876,7 +881,11 @@ extern "C" int hn_tree_append(const void* qkv, long ld_qkv, const float* cos_t, 
   HN_ARG_CHECK(B * S < (1L << 31) && nkv * (rep + 1) <= 65535, "%s: too many rows or heads", who);
   // Up to 40 nodes the launch's latency is all there is, and the kernel by elements
   // has less of it: 1, 32, 64, 256 and 512 nodes of 32 + 2 x 8 heads take it 2.0,
-  // 2.7, 3.8, 9.2 and 15.9 us, the other 3.2, 3.1, 3.1, 3.6 and 4.4.
+  // 2.9, 3.6, 8.0 and 16.1 us, the other 3.2, 3.1, 3.4, 3.7 and 4.4.  The crossing is
+  // near 50 nodes there; with fewer heads it comes later, with more a little sooner,
+  // and the rule is off by less than a microsecond: 64 and 256 nodes of 1 + 2 heads
+  // 2.4 and 2.5 us by elements, 3.0 and 3.1 by rows; of 8 + 2 x 2 heads 2.4 and 3.6, 3.3
+  // and 3.4; 32 nodes of 96 + 2 x 8 heads 3.8 by elements, where 64 take 3.5 by rows.
   if (B * S > 40 && ld_qkv % 8 == 0 && al16(qkv) && al16(cos_t) && al16(sin_t) && al16(q_out) && al16(v)) {
     hipLaunchKernelGGL(append_rows_kernel,
                        dim3((unsigned)((B * S + kAppend - 1) / kAppend),

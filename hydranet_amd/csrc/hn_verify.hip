@@ -28,7 +28,8 @@
 // Times: 5 nodes over 32000 tokens, greedy, one sequence: stats 4.2 us, walk 3.4
 // (latency of two launches).  8 trees of 61 nodes, 4 children each, over 32000,
 // fp16: stats 22 us, first 16, node 41, walk 13.  32 chains of 6 over 128000, fp32:
-// 48 (4.4 TB/s), 25, 6, 14.  Of the 22 us half are the 26 million exponentials at
+// 48 (4.4 TB/s), 25, 6, 14.  Certain proposals, whole calls: the 8 trees 46 us, the 32
+// chains 44 (their rows 20 at a copy's rate), 5 nodes of one sequence 23.  Of the 22 us half are the 26 million exponentials at
 // 19 vector instructions each, the rest their rows' arrival; the 41 are three passes
 // by one workgroup, one after the other since each needs the mass that the last one
 // left.  With little gain there (47 to 44 us together, without the shorter passes):

@@ -16,7 +16,8 @@ A sequence's length is an entry of a device tensor lens [B] (int64; negative: it
 takes no part), so sequences advance by their own accepted counts without a host
 synchronisation, and every step can be captured into a graph.  On the GPU each
 function is one library call (include/hn_int4.h); on the CPU, the same
-definitions in torch.
+definitions in torch, also of what is no number: a position that a row does not
+see has no effect on it, whatever it holds.
 """
 from __future__ import annotations
 
@@ -220,7 +221,7 @@ def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, tree: DraftTree,
     logits: the drafter's after each node, from whose softmax (at the same
     temperature) its children were drawn; None: every drafted token is a certain
     proposal.  temperature: a number, or fp32 [B]; 0 takes the largest logit (the
-    lowest index of equals).  Children are tested in order of index: accepted
+    lowest index of equals; numbers are rounded to fp32).  Children are tested in order of index: accepted
     with probability min(1, r(x) / q(x)), r = p at first and norm(max(r - q, 0))
     after a rejection (a certain proposal's: r without its token)."""
     assert logits.dim() == 3 and logits.dtype in _DTYPES, "logits: fp16, bf16 or fp32 [B, S, V]"
