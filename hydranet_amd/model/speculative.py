@@ -220,10 +220,11 @@ def verify_tree(logits: torch.Tensor, tokens: torch.Tensor, tree: DraftTree,
     node i, entry 0 draws the token after the accepted nodes.  draft_logits, like
     logits: the drafter's after each node, from whose softmax (at the same
     temperature) its children were drawn; None: every drafted token is a certain
-    proposal.  temperature: a number, or fp32 [B]; 0 takes the largest logit (the
-    lowest index of equals; numbers are rounded to fp32).  Children are tested in order of index: accepted
-    with probability min(1, r(x) / q(x)), r = p at first and norm(max(r - q, 0))
-    after a rejection (a certain proposal's: r without its token)."""
+    proposal.  temperature: a number (rounded to fp32), or fp32 [B]; 0 takes the
+    largest logit (the lowest index of equals).  Children are tested in order of
+    index: accepted with probability min(1, r(x) / q(x)), r = p at first and
+    norm(max(r - q, 0)) after a rejection (a certain proposal's: r without its
+    token)."""
     assert logits.dim() == 3 and logits.dtype in _DTYPES, "logits: fp16, bf16 or fp32 [B, S, V]"
     B, S, V = logits.shape
     dev = logits.device
