@@ -57,6 +57,13 @@ SIGNATURES: dict[str, list] = {
     "hn_verify_tree": [P, L, L, P, L, L, I, P, P, L, P, P, F, L, L, L, P, P, P, P, L, P],
     "hn_kv_keep": [P, P, L, L, L, L, L, P, P, L, P, L, P, P],
     "hn_kv_fork": [P, P, L, L, L, L, L, P, P, L, L, P],
+    "hn_paged_append": [P, L, I, P, P, L, L, I, P, L, L, L, P, P, L, L, L, L, L, L, P, P, P, P],
+    "hn_paged_attention_workspace_bytes": [L, L, L, L, L, L, L],
+    "hn_paged_attention": [P, L, I, P, P, P, L, L, L, P, P, L, L, L, L, L, L, L, L, F, P, L, P, L,
+                           P],
+    "hn_page_copy": [P, P, L, L, L, P, P, L, P],
+    "hn_adjust_logits": [P, L, I, P, L, L, P, P, P, P, P, F, F, F, P, L, P, L, L, P, L, L, L, P,
+                         L, P],
     "hn_grouped_expert_mlp_int4": [P, P, P, P, P, L, L, L, L, L, L, P, P, P, L, P],
     "hn_set_decode_path": [I],
     "hn_gemm_workspace_bytes": [],
@@ -85,7 +92,8 @@ ROUTE_MAX_ASSIGN = 1024   # T * k
 RESTYPES = {"hn_skinny_workspace_bytes": ctypes.c_long,
             "hn_attn_prefill_workspace_bytes": ctypes.c_long,
             "hn_tree_attention_workspace_bytes": ctypes.c_long,
-            "hn_verify_tree_workspace_bytes": ctypes.c_long, "hn_gemm_workspace_bytes": ctypes.c_long,
+            "hn_verify_tree_workspace_bytes": ctypes.c_long,
+            "hn_paged_attention_workspace_bytes": ctypes.c_long, "hn_gemm_workspace_bytes": ctypes.c_long,
             "hn_moe_decode_layer_partials": ctypes.c_long}
 
 # Tokens per weight matrix up to which the decode (skinny / streaming) kernels run

@@ -17,7 +17,8 @@ reference:
   length for the whole batch (cache/kv_cache.py:26-284, SimpleKVCache);
 * top-2 routing at prefill, top-1 or top-2 at decode (TopKMode,
   model/mixtral.py:493-531; the reference's default is top-1 at decode);
-* speculative decoding with one length per sequence (model/speculative.py).
+* speculative decoding with one length per sequence (model/speculative.py);
+* sequences of any lengths over a paged cache (model/paged.py).
 """
 from __future__ import annotations
 
@@ -397,6 +398,19 @@ class Attention(nn.Module):
                         layer, self.nh)
         return self.o_proj(tree_attention(q, tree, lens, cache, layer, kv_bound))
 
+    def forward_paged(self, x: torch.Tensor, rope, batch, cache, layer: int) -> torch.Tensor:
+        """x [1, rows, H]: a PagedBatch's rows over a PagedKVCache (model/paged.py),
+        rope a RotaryTable.  The projections as one product, then hn_paged_append and
+        hn_paged_attention."""
+        from .paged import paged_append, paged_attention
+        x2 = x.reshape(batch.rows, -1)
+        if x.is_cuda:
+            qkv = self._qkv(x2)
+        else:
+            qkv = torch.cat([m(x2) for m in (self.q_proj, self.k_proj, self.v_proj)], -1)
+        q = paged_append(qkv, rope, batch, cache, layer, self.nh)
+        return self.o_proj(paged_attention(q, batch, cache, layer)).view(x.shape)
+
 
 def attn_softmax(scores: torch.Tensor, mask: Optional[torch.Tensor], head_dim: int) -> torch.Tensor:
     """fp16(softmax_fp32(fp16(scores / sqrt(head_dim)) + mask)) over the last
@@ -479,15 +493,18 @@ class DecoderBlock(nn.Module):
                                    layer_idx=layer_idx, slots=slots)
 
     def forward(self, x, h, rope, pos, cache: KVCache, kv_len: int, mask, top_k: int,
-                next_norm: "RMSNorm", fold: bool = True, tree=None):
+                next_norm: "RMSNorm", fold: bool = True, tree=None, batch=None):
         """x + attn(h), then + moe(norm(.)) (model/mixtral.py:407-427), h =
         input_layernorm(x) given by the caller.  Returns (x after both
         residual adds, next_norm of it): the next block's input and its
         normalised rows.  fold: the MoE output's residual add and next_norm
         run inside the MoE block's last launch where it allows
         (forward_folded), else as one more launch.  tree: the tokens are the
-        nodes of a DraftTree, pos the sequences' lengths and kv_len their bound."""
-        if tree is not None:
+        nodes of a DraftTree, pos the sequences' lengths and kv_len their bound.
+        batch: they are the rows of a PagedBatch, rope a RotaryTable."""
+        if batch is not None:
+            a = self.self_attn.forward_paged(h, rope, batch, cache, self.layer_idx)
+        elif tree is not None:
             a = self.self_attn.forward_tree(h, rope, tree, pos, cache, self.layer_idx, kv_len)
         else:
             a = self.self_attn(h, rope, pos, cache, self.layer_idx, kv_len, mask)
@@ -535,19 +552,22 @@ class MixtralDecoder(nn.Module):
                        max_len, dev, self.embed_tokens.weight.dtype)
 
     def step(self, input_ids: torch.Tensor, pos: torch.Tensor, cache: KVCache, kv_len: int,
-             mask: Optional[torch.Tensor], top_k: int, tree=None) -> torch.Tensor:
+             mask: Optional[torch.Tensor], top_k: int, tree=None, batch=None,
+             last: Optional[torch.Tensor] = None) -> torch.Tensor:
         """One pass over every layer: tokens input_ids [B, S] at positions pos
         [S] (device int64), attention over the first kv_len cache positions.
         Does not move cache.cur_len.  With a DraftTree, its nodes' tokens after
-        pos [B] cached positions of each sequence (forward_tree)."""
+        pos [B] cached positions of each sequence (forward_tree).  With a PagedBatch,
+        its rows [1, rows] (forward_paged), the logits of the rows `last` alone."""
+        rope = self.rotary if batch is None else self._rope_table()
         x = self.embed_tokens(input_ids)
         x, h = add_rmsnorm(x, None, self.layers[0].input_layernorm)
         n = len(self.layers)
         for i, blk in enumerate(self.layers):
             nxt = self.layers[i + 1].input_layernorm if i + 1 < n else self.norm
-            x, h = blk(x, h, self.rotary, pos, cache, kv_len, mask, top_k, nxt,
-                       fold=self.fold_moe_norm, tree=tree)
-        return self.lm_head(h)
+            x, h = blk(x, h, rope, pos, cache, kv_len, mask, top_k, nxt,
+                       fold=self.fold_moe_norm, tree=tree, batch=batch)
+        return self.lm_head(h if last is None else h[:, last])
 
     @torch.no_grad()
     def forward(self, input_ids: torch.Tensor, cache: KVCache,
@@ -600,6 +620,36 @@ class MixtralDecoder(nn.Module):
         assert kv_bound <= cache.max_len, f"KV cache full ({kv_bound} > {cache.max_len})"
         return self.step(tokens, lens, cache, kv_bound, None,
                          self.decode_top_k if top_k is None else top_k, tree)
+
+    def _rope_table(self):
+        """The decoder's angles as a RotaryTable, made again when the module's are others."""
+        from .paged import RotaryTable
+        cos, sin = self.rotary.cos_cached, self.rotary.sin_cached
+        old = getattr(self, "_rope", None)
+        if old is None or old[0] is not cos or old[1] is not sin \
+                or old[2] != (cos._version, sin._version):
+            half = cos.shape[1] // 2
+            table = RotaryTable.wrap(cos[:, :half].float(), sin[:, :half].float())
+            old = self._rope = (cos, sin, (cos._version, sin._version), table)
+        return old[3]
+
+    @torch.no_grad()
+    def forward_paged(self, tokens: torch.Tensor, batch, cache, top_k: Optional[int] = None,
+                      last: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """One pass of a PagedBatch's rows (tokens [rows]) over a PagedKVCache (both
+        model/paged.py) -> logits [rows, vocab], or [len(last), vocab] of the rows that
+        last (int64) names.  Appends the rows to the pages; the lengths are the
+        caller's to move."""
+        assert tuple(tokens.shape) == (batch.rows,), f"{tuple(tokens.shape)} tokens for " \
+                                                     f"{batch.rows} rows"
+        return self.step(tokens[None], None, cache, batch.kv_bound, None,
+                         self.decode_top_k if top_k is None else top_k, batch=batch, last=last)[0]
+
+    def generate_paged(self, prompts, max_new_tokens: int, **options) -> List[List[int]]:
+        """max_new_tokens after each of the prompts, of any lengths, from a paged cache,
+        sampled with penalties, biases and grammars: see model/paged.py: generate."""
+        from .paged import generate
+        return generate(self, prompts, max_new_tokens, **options)
 
     def generate_speculative(self, input_ids: torch.Tensor, max_new_tokens: int, draft=None,
                              temperature: float = 0.0, samples: int = 1,

@@ -528,6 +528,75 @@ int hn_kv_keep(void* const* kt, void* const* v, long layers, long max_len, long 
 int hn_kv_fork(void* const* kt, void* const* v, long layers, long max_len, long B, long nkv,
                long hd, const int* src, const int* dst, long pairs, long n, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * A paged KV cache (in place of the reference's unwired paged design,
+ * cache/kv_cache.py:293-760).  A page holds `page` positions (a power of two, 16
+ * to 1024) of every KV head: keys k [num_pages][nkv][page][hd], values v
+ * [num_pages][nkv][page / 8][hd][8] (eight consecutive positions of a dimension
+ * side by side), fp16 (dtype 0) or bf16 (1), hd 64, 128 or 256, 16-byte aligned.
+ * table [B][ld_table] int32 (device): row b names the pages of sequence b, `cols`
+ * of them; a sequence's positions i * page on lie in page table[b][i].  lens [B]
+ * int64 (device): cached positions C_b before the step, negative for a sequence
+ * that takes no part.  Rows starts[b] to starts[b + 1] - 1 of the step's T (starts
+ * [B + 1] int32 on the device, not decreasing, from 0; NULL: T = B, row b) are
+ * sequence b's tokens at positions C_b on.  Rows of no sequence are left as they
+ * are in every output.  Sequences may share pages that neither writes.
+ *
+ * hn_paged_append: qkv [T][ld_qkv] (nh query heads, nkv keys, nkv values of hd);
+ *   the first `rotary` dimensions of queries and keys are rotated with cos_t /
+ *   sin_t [table_rows][rotary / 2] fp32, in pairs (i, i + rotary / 2), or (2 i, 2 i
+ *   + 1) with interleaved; fp32 products, rounded once.  Queries go to q_out
+ *   [T][nh * hd], keys and values to their pages.  Rows of a sequence with a
+ *   negative length write no page and zero queries; a row whose position is past
+ *   cos_t, or whose page the table does not name (past its columns, or an id
+ *   outside [0, num_pages)), writes no page and NaN queries. */
+int hn_paged_append(const void* qkv, long ld_qkv, int dtype, const float* cos_t,
+                    const float* sin_t, long table_rows, long rotary, int interleaved,
+                    const int* table, long ld_table, long cols, long num_pages, const long* lens,
+                    const int* starts, long B, long T, long nh, long nkv, long hd, long page,
+                    void* q_out, void* k, void* v, void* stream);
+
+/* hn_paged_attention: out[t * ld_o + h * hd + d] = softmax(scale * q k) v over the
+ *   positions up to row t's own (its key and value in the pages already), query
+ *   head h over KV head h / (nh / nkv); fp32 scores, statistics and sums.  q
+ *   [T][ld_q].  Rows of a sequence with a negative length are zero; those of a
+ *   sequence of which the table does not name every page are NaN.  A position
+ *   that a row does not see has no effect on it, whatever it holds.  max_new and
+ *   bound: about the most rows and positions (C_b + rows) of a sequence; they
+ *   choose the launch, not the result.  scale above 0 and finite, also times
+ *   log2(e); 16-byte aligned operands, ld_q and ld_o multiples of 8.  work:
+ *   hn_paged_attention_workspace_bytes(...) bytes, 16-byte aligned, any contents. */
+long hn_paged_attention_workspace_bytes(long B, long T, long nh, long nkv, long hd, long max_new,
+                                        long bound);
+int hn_paged_attention(const void* q, long ld_q, int dtype, const void* k, const void* v,
+                       const int* table, long ld_table, long cols, long num_pages,
+                       const long* lens, const int* starts, long B, long T, long nh, long nkv,
+                       long hd, long page, long max_new, long bound, float scale, void* out,
+                       long ld_o, void* work, long work_bytes, void* stream);
+
+/* hn_page_copy: page src[i] copied to page dst[i], i < pairs, in every layer.  k, v
+ *   (the layers' device pointers, 16-byte aligned), src and dst are HOST arrays;
+ *   page_bytes: of the keys (or values) of one page, a multiple of 16.  A page may
+ *   be a source several times, a destination once, and none both. */
+int hn_page_copy(void* const* k, void* const* v, long layers, long page_bytes, long num_pages,
+                 const int* src, const int* dst, long pairs, void* stream);
+
+/* hn_adjust_logits: out[b][v] = logits[b][v] (rows of V at ld; dtype 0 fp16, 1
+ *   bf16, 2 fp32) adjusted, in fp32, rounded once; out may be logits itself.  In
+ *   order, with text[b][0 .. n), n = min(lens[b], width) (lens NULL: width):
+ *   a token anywhere in it: x = x > 0 ? x / repetition : x * repetition; a token
+ *   c > 0 times in text[b][first[b] .. n) (first NULL: 0): x -= frequency * c +
+ *   presence; x += bias[b][i] of the last i < biases with bias_ids[b][i] = v; v's
+ *   bit of allowed[b] (32 to an int32, the lowest first; NULL: all) zero: x = -inf.
+ *   Ids outside [0, V) count for nothing.  repetition, presence, frequency: [B]
+ *   fp32 on the device, or NULL for repetition1, presence1, frequency1. */
+int hn_adjust_logits(const void* logits, long ld, int dtype, const long* text, long ld_text,
+                     long width, const long* lens, const long* first, const float* repetition,
+                     const float* presence, const float* frequency, float repetition1,
+                     float presence1, float frequency1, const long* bias_ids, long ld_ids,
+                     const float* bias, long ld_bias, long biases, const int* allowed,
+                     long ld_allowed, long B, long V, void* out, long ld_out, void* stream);
+
 /* Decode kernel family for hn_int4_linear, hn_int4_gate_up_silu,
  * hn_expert_mlp_int4 and hn_grouped_expert_mlp_int4, for the calling thread
  * only (each thread starts at 0; a switch never affects another thread):
