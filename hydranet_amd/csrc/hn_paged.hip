@@ -44,56 +44,511 @@ __global__ __launch_bounds__(256) void append_kernel(Step P, const T* __restrict
   else if (in) k[((pg * P.nkv + head - nh) * P.page + slot) * hd + d] = (T)y;
 }
 
-// One wave per (row, query head).
+// ---------------------------------------------------------------------------
+// Attention.  One pass over a sequence's pages with a running maximum and sum, for the
+// rows of one (sequence, KV head), a row being a (new token, query head of the group)
+// pair.  A wave takes 32 positions at a time:
+//   S^T = K Q^T    v_mfma_f32_16x16x32, A = K, B = Q, two blocks of 16 positions;
+//   softmax        a lane holds 8 scores of one row;
+//   O^T += V^T P   the lane's probabilities are the B operand as they are.
+// Both products read their operands from memory to registers as they lie: a key's
+// dimensions are consecutive, and so are 8 positions of a value's dimension.  Block t's
+// row 4 c + i is position 8 c + 4 t + i, so that a lane's scores of both blocks are the 8
+// consecutive positions that its lane of the value operand holds.
+constexpr int kTile = 32;
+constexpr float kLog2e = 1.4426950408889634f;
+// Probabilities are 2^8 times the softmax's, relative to a maximum that follows the true
+// one only when it lags by 2^6: below 2^14, so fp16 holds them, and those down to 2^-22
+// of the largest are normal numbers.  They are rounded to the cache's type because that
+// is what the matrix instruction multiplies with the values; a row's sum is of the
+// rounded ones, so that their weights still add up to 1.
+constexpr float kUp = 8.f, kLag = 6.f;
+// Positions that workgroups share out as one.
+constexpr int kGrain = 128;
+
+typedef float float4v __attribute__((ext_vector_type(4)));
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+
+template <class T>
+struct Vec;
+template <>
+struct Vec<h16> {
+  typedef half8_t t;
+  static constexpr uint32_t inf = 0x7c00u;
+  static __device__ __forceinline__ float4v mfma(t a, t b, float4v c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Vec<b16> {
+  typedef bf8 t;
+  static constexpr uint32_t inf = 0x7f80u;
+  static __device__ __forceinline__ float4v mfma(t a, t b, float4v c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+};
+
+template <class T>
+struct Attend {
+  Step P;
+  const T *q, *k, *v;
+  T* out;
+  float* part;  // entries of R rows of HD sums, then of R (maximum, sum)
+  long ld_q, ld_o;
+  int rep, max_new, R, wgs;
+  float scale;
+};
+
+// max over the four lanes, 16 apart, that hold one row
+__device__ __forceinline__ float row_max(float x) {
+  const uint32_t w = __builtin_bit_cast(uint32_t, x);
+  const auto a = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+  const uint32_t a0 = a[0], a1 = a[1];
+  x = fmaxf(__builtin_bit_cast(float, a0), __builtin_bit_cast(float, a1));
+  const uint32_t v = __builtin_bit_cast(uint32_t, x);
+  const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  const uint32_t b0 = b[0], b1 = b[1];
+  return fmaxf(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
+}
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// A sequence's rows [row, row + n) of the step, its cached positions C and the end L of
+// those that are read.  Positions past the table's are all one to a row that sees them,
+// so neither C nor L exceeds the first of them by more than 1.  n < 0: rows that are
+// zero (no part), or NaN (more than max_new).
+struct Run {
+  int row, n, C, L;
+  bool none, nan;
+};
+template <class T>
+__device__ __forceinline__ Run run_of(const Attend<T>& A, int b) {
+  const Step& P = A.P;
+  Run r = {b, 1, 0, 0, false, false};
+  if (P.starts) {
+    r.row = min(max(P.starts[b], 0), P.T);
+    r.n = max(min(P.starts[b + 1], P.T) - r.row, 0);
+  }
+  const long C = P.lens[b];
+  const int cap = (int)(P.cols * P.page);
+  r.none = C < 0, r.nan = !r.none && r.n > A.max_new;
+  if (r.n == 0 || r.none || r.nan) return r;
+  r.C = C > cap ? cap + 1 : (int)C;
+  r.L = min(r.C + r.n, cap + 1);
+  return r;
+}
+
+// The rows of a run that none attends for, of KV head g.
 template <class T, int HD>
-__global__ __launch_bounds__(64) void attend_kernel(Step P, const T* __restrict__ q, long ld_q,
-                                                    const T* __restrict__ k,
-                                                    const T* __restrict__ v, int rep, float scale,
-                                                    T* __restrict__ out, long ld_o) {
-  __shared__ float s_q[HD], s_p[64];
-  __shared__ long s_pg[64];
-  const int t = blockIdx.x, head = blockIdx.y, lane = threadIdx.x, g = head / rep;
-  const Row r = row_of(P, t);
-  if (r.b < 0) return;
-  for (int d = lane; d < HD; d += 64) s_q[d] = (float)q[(long)t * ld_q + (long)head * HD + d];
-  float m = -__builtin_inff(), sum = 0.f, o[HD / 64] = {};
-  // the sequence's positions with its last row: all on pages that are named, or none is read
-  const long L = r.pos < 0 ? 0 : r.pos + (P.starts ? min(P.starts[r.b + 1], P.T) - t : 1);
-  bool bad = L > P.cols * P.page;
-  for (long p0 = lane * (long)P.page; !bad && p0 < L; p0 += 64 * P.page)
-    bad = page_of(P, r.b, p0) < 0;
-  bad = __any(bad);
-  for (long p0 = 0; !bad && p0 <= r.pos; p0 += 64) {
-    const long p = p0 + lane;
-    float s = -__builtin_inff();
-    long pg = 0;
-    if (p <= r.pos) {
-      pg = page_of(P, r.b, p);
-      const T* kp = k + ((pg * P.nkv + g) * P.page + (p & (P.page - 1))) * HD;
-      s = 0.f;
-      for (int d = 0; d < HD; ++d) s += s_q[d] * (float)kp[d];
-      s *= scale;
+__device__ __forceinline__ void fill(const Attend<T>& A, const Run& r, int g, int part, int parts) {
+  const T x = (T)(r.nan ? __builtin_nanf("") : 0.f);
+  typename Vec<T>::t y;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = x;
+  const int cols = A.rep * (HD / 8);
+  for (long i = (long)part * blockDim.x + threadIdx.x; i < (long)r.n * cols;
+       i += (long)parts * blockDim.x) {
+    const int t = (int)(i / cols), c = (int)(i - (long)t * cols);
+    *reinterpret_cast<typename Vec<T>::t*>(A.out + (long)(r.row + t) * A.ld_o +
+                                           (long)g * A.rep * HD + 8 * c) = y;
+  }
+}
+
+// Sums of the lanes up to each (row_shr:1, 2, 4, 8, then row_bcast:15, 31).
+__device__ __forceinline__ int lane_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+  return x;
+}
+
+template <class T>
+__device__ __forceinline__ int grains_of(const Attend<T>& A, int b) {
+  return (run_of(A, b).L + kGrain - 1) / kGrain;
+}
+
+// The grains of all (sequence, KV head) pairs in order, dealt evenly: the first `more` of
+// wgs workgroups take each + 1 of them.
+struct Deal {
+  int wgs, each, more;
+  __device__ Deal(int total, int most) : wgs(min(total, most)) {
+    each = wgs ? total / wgs : 0, more = total - each * wgs;
+  }
+  __device__ int from(int w) const { return w * each + min(w, more); }
+  __device__ int owner(int x) const {
+    const int big = more * (each + 1);
+    return x < big ? x / (each + 1) : more + (x - big) / each;
+  }
+};
+
+// Grains of one head of the sequences below `to`, by a wave.
+template <class T>
+__device__ __forceinline__ int grains_below(const Attend<T>& A, int to) {
+  int n = 0;
+  for (int b = threadIdx.x & 63; b < to; b += 64) n += grains_of(A, b);
+  return __builtin_amdgcn_readlane(lane_scan(n), 63);
+}
+
+// The sums of NT x 16 rows over a wave's positions.
+template <class T, int HD, int NT>
+struct Sums {
+  float4v o[NT][HD / 16], l[NT];
+  float mx[NT];
+};
+
+// A wave's tiles `wave`, `wave` + NW, .. of [first, end) of a run, for rows row0 on of KV
+// head g.  All rows see the positions up to lo, none sees past hi.  The next tile's keys
+// are asked for when this one's scores are there, its values after this one's product:
+// about a tile is in flight throughout, in the registers of one.
+template <class T, int HD, int NT, int NW>
+__device__ __forceinline__ void walk(const Attend<T>& A, Sums<T, HD, NT>& W, const Run& r, int b,
+                                     int g, int row0, int first, int end, int lo, int hi, int wave,
+                                     int lane) {
+  typedef typename Vec<T>::t V8;
+  const Step& P = A.P;
+  const int shift = __builtin_ctz(P.page), mask = P.page - 1, n = lane & 15, kg = lane >> 4;
+  V8 q[NT][HD / 32];
+  int lim[NT];  // the last position that this lane's row sees
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int row = row0 + 16 * t + n, tok = row / A.rep, head = row - tok * A.rep;
+    const bool in = row < A.rep * r.n;
+    const T* src = A.q + (long)(r.row + tok) * A.ld_q + (long)(g * A.rep + head) * HD + 8 * kg;
+#pragma unroll
+    for (int u = 0; u < HD / 32; ++u) {
+      u32x4 w = {0, 0, 0, 0};
+      if (in) w = *reinterpret_cast<const u32x4*>(src + 32 * u);
+      q[t][u] = __builtin_bit_cast(V8, w);
     }
-    float top = s;
-    for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
-    const float nm = fmaxf(m, top), al = __expf(m - nm);
-    const float e = p <= r.pos ? __expf(s - nm) : 0.f;
-    m = nm;
+    lim[t] = in ? r.C + tok : lo;
+    W.mx[t] = -__builtin_inff();
+    W.l[t] = (float4v)(0.f);
+#pragma unroll
+    for (int e = 0; e < HD / 16; ++e) W.o[t][e] = (float4v)(0.f);
+  }
+  const int tiles = (min(end, hi + 1) - first + kTile - 1) / kTile;
+  const int mine = (tiles - wave + NW - 1) / NW;
+  if (mine <= 0) return;
+  auto start = [&](int i) { return first + kTile * (wave + NW * min(i, mine - 1)); };
+  // The pages of a tile's halves of 16 positions as this lane has them: of its key rows
+  // and of its values.
+  const int* table = P.table + (long)b * P.ld;
+  struct Ids {
+    int k, v;
+  };
+  auto ids = [&](int i) {
+    const int p0 = start(i);
+    const int ck = (p0 + 8 * (n >> 2)) >> shift, cv = (p0 + 8 * kg) >> shift;
+    return Ids{ck < P.cols ? table[ck] : -1, cv < P.cols ? table[cv] : -1};
+  };
+  auto named = [&](int id) { return id >= 0 && id < P.pages; };
+  auto base = [&](const T* x, int id) {
+    return x + ((long)(named(id) ? id : 0) * P.nkv + g) * P.page * HD;
+  };
+  V8 k[2][HD / 32], v[HD / 16];
+  auto keys = [&](int i, int id) {
+    const T* x = base(A.k, id) + ((start(i) + 8 * (n >> 2) + (n & 3)) & mask) * HD + 8 * kg;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int u = 0; u < HD / 32; ++u)
+        k[j][u] = *reinterpret_cast<const V8*>(x + 4 * j * HD + 32 * u);
+  };
+  auto values = [&](int i, int id) {
+    const T* x = base(A.v, id) + ((start(i) + 8 * kg) & mask) * HD + 8 * n;
+#pragma unroll
+    for (int e = 0; e < HD / 16; ++e) v[e] = *reinterpret_cast<const V8*>(x + 128 * e);
+  };
+  const float scale = A.scale * kLog2e;
+  V8 ones;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ones[i] = (T)1.f;
+
+  Ids id = ids(0), next = ids(1);
+  keys(0, id.k);
+  values(0, id.v);
+  for (int i = 0; i < mine; ++i) {
+    const Ids after = ids(i + 2);
+    const int p0 = start(i), at = p0 + 8 * kg;  // this lane's 8 positions
+    const bool bad = !named(id.v);              // they lie on no page
+    const bool edge = p0 + kTile - 1 > lo || __any(bad);
+    float4v s[NT][2];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        s[t][j] = (float4v)(0.f);
+#pragma unroll
+        for (int u = 0; u < HD / 32; ++u) s[t][j] = Vec<T>::mfma(k[j][u], q[t][u], s[t][j]);
+      }
+    keys(i + 1, next.k);
+    V8 p[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      if (edge)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            if (bad) s[t][j][c] = __builtin_nanf("");
+            if (at + 4 * j + c > lim[t]) s[t][j][c] = -__builtin_inff();
+          }
+      float tm = s[t][0][0];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tm = fmaxf(tm, s[t][j][c]);
+      tm = row_max(tm) * scale;
+      if (__any(tm > W.mx[t] + kLag)) {
+        const float nm = fmaxf(W.mx[t], tm);
+        const float al = nm == W.mx[t] ? 1.f : __builtin_amdgcn_exp2f(W.mx[t] - nm);
+        W.l[t] *= al;
+#pragma unroll
+        for (int e = 0; e < HD / 16; ++e) W.o[t][e] *= al;
+        W.mx[t] = nm;
+      }
+      const float ref = W.mx[t] == -__builtin_inff() ? 0.f : W.mx[t] - kUp;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          p[t][4 * j + c] = (T)__builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j][c], scale, -ref));
+      W.l[t] = Vec<T>::mfma(ones, p[t], W.l[t]);
+    }
+    bool odd = false;
+    if (edge) {
+      // values at positions that no row sees have probabilities of zero, but may be
+      // anything; those that only some rows see must not reach the others as 0 times
+      // a NaN or infinity
+#pragma unroll
+      for (int e = 0; e < HD / 16; ++e) {
+        u32x4 w = __builtin_bit_cast(u32x4, v[e]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const uint32_t m =
+              (at + 2 * c <= hi ? 0xffffu : 0u) | (at + 2 * c + 1 <= hi ? 0xffff0000u : 0u);
+          w[c] = bad ? 0u : w[c] & m;
+          odd |= (w[c] & Vec<T>::inf) == Vec<T>::inf ||
+                 (w[c] >> 16 & Vec<T>::inf) == Vec<T>::inf;
+        }
+        v[e] = __builtin_bit_cast(V8, w);
+      }
+      odd = lo < hi && __any(odd);
+    }
+    if (odd) {
+      // left out of the product; that a row sees one is counted, of each kind, by products
+      // of ones
+#pragma unroll
+      for (int e = 0; e < HD / 16; ++e) {
+        V8 up, down, nan;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const float f = (float)v[e][c];
+          up[c] = (T)(f == __builtin_inff() ? 1.f : 0.f);
+          down[c] = (T)(f == -__builtin_inff() ? 1.f : 0.f);
+          nan[c] = (T)(f != f ? 1.f : 0.f);
+          if (!(__builtin_fabsf(f) < __builtin_inff())) v[e][c] = (T)0.f;
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          V8 see;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) see[c] = (T)(at + c > lim[t] ? 0.f : 1.f);
+          const float4v z = (float4v)(0.f);
+          const float4v cu = Vec<T>::mfma(up, see, z), cd = Vec<T>::mfma(down, see, z);
+          const float4v cn = Vec<T>::mfma(nan, see, z);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            float y = cu[c] > 0.f ? __builtin_inff() : 0.f;
+            if (cd[c] > 0.f) y -= __builtin_inff();
+            if (cn[c] > 0.f) y = __builtin_nanf("");
+            W.o[t][e][c] += y;
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < HD / 16; ++e)
+#pragma unroll
+      for (int t = 0; t < NT; ++t) W.o[t][e] = Vec<T>::mfma(v[e], p[t], W.o[t][e]);
+    values(i + 1, next.v);
+    id = next, next = after;
+  }
+}
+
+// The waves' sums of 16 rows joined, then the rows themselves, or the range's entry of
+// the workspace.
+template <class T, int HD, int NT, int NW>
+__device__ __forceinline__ void finish(const Attend<T>& A, const Sums<T, HD, NT>& W, const Run& r,
+                                       int g, int row0, long entry, float* s_o, float* s_m,
+                                       int wave, int lane) {
+  constexpr int kPad = HD + 4;
+  const int n = lane & 15, kg = lane >> 4, rows = A.rep * r.n;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    __syncthreads();  // (the last use of the buffers)
+    if (row0 + 16 * t + n < rows) {
+      if (kg == 0) s_m[(wave * 16 + n) * 2] = W.mx[t], s_m[(wave * 16 + n) * 2 + 1] = W.l[t][0];
+#pragma unroll
+      for (int e = 0; e < HD / 16; ++e)
+        *reinterpret_cast<float4v*>(s_o + (wave * 16 + n) * kPad + 16 * e + 4 * kg) = W.o[t][e];
+    }
     __syncthreads();
-    s_p[lane] = e, s_pg[lane] = pg;
-    __syncthreads();
-    sum *= al;
-    for (int i = 0; i < HD / 64; ++i) o[i] *= al;
-    for (int j = 0; j < 64 && p0 + j <= r.pos; ++j) {
-      const int slot = (int)((p0 + j) & (P.page - 1));
-      const T* vp = v + ((s_pg[j] * P.nkv + g) * P.page + (slot & ~7)) * HD + (slot & 7);
-      sum += s_p[j];
-      for (int i = 0; i < HD / 64; ++i) o[i] += s_p[j] * (float)vp[(lane + 64 * i) * 8];
+    for (int i = threadIdx.x; i < 16 * (HD / 8); i += 64 * NW) {
+      const int rr = i / (HD / 8), d = 8 * (i % (HD / 8)), row = row0 + 16 * t + rr;
+      if (row >= rows) continue;
+      float m = -__builtin_inff();
+#pragma unroll
+      for (int w = 0; w < NW; ++w) m = fmaxf(m, s_m[(w * 16 + rr) * 2]);
+      const float ref = m == -__builtin_inff() ? 0.f : m;
+      float sum = 0.f, x[8] = {};
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        // a wave without tiles has sums of zero and weight exp2(-inf) = 0
+        const float al = __builtin_amdgcn_exp2f(s_m[(w * 16 + rr) * 2] - ref);
+        sum += al * s_m[(w * 16 + rr) * 2 + 1];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] += al * s_o[(w * 16 + rr) * kPad + d + j];
+      }
+      if (entry < 0) {
+        const int tok = row / A.rep, head = row - tok * A.rep;
+        const float is = 1.f / sum;
+        typename Vec<T>::t y;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[j] = (T)(x[j] * is);
+        *reinterpret_cast<typename Vec<T>::t*>(A.out + (long)(r.row + tok) * A.ld_o +
+                                               (long)(g * A.rep + head) * HD + d) = y;
+      } else {
+        const long at = entry * A.R + row;
+#pragma unroll
+        for (int j = 0; j < 8; j += 4)
+          *reinterpret_cast<float4v*>(A.part + at * HD + d + j) =
+              float4v{x[j], x[j + 1], x[j + 2], x[j + 3]};
+        float* pm = A.part + 2 * (long)A.wgs * A.R * HD + at * 2;
+        if (d == 0) pm[0] = m, pm[1] = sum;
+      }
     }
   }
-  for (int i = 0; i < HD / 64; ++i)
-    out[(long)t * ld_o + (long)head * HD + lane + 64 * i] =
-        (T)(r.pos < 0 ? 0.f : bad ? __builtin_nanf("") : o[i] / sum);
+}
+
+// A workgroup per (KV head, block of 16 NT rows, sequence), over all of its positions.
+template <class T, int HD, int NT, int NW>
+__global__ __launch_bounds__(64 * NW) void whole_kernel(Attend<T> A) {
+  __shared__ __align__(16) float s_o[NW * 16 * (HD + 4)];
+  __shared__ float s_m[NW * 16 * 2];
+  const int g = blockIdx.x, b = blockIdx.z, row0 = (gridDim.y - 1 - blockIdx.y) * 16 * NT;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const Run r = run_of(A, b);
+  if (r.none || r.nan) return fill<T, HD>(A, r, g, blockIdx.y, gridDim.y);
+  if (row0 >= A.rep * r.n) return;
+  Sums<T, HD, NT> W;
+  const int last = min((row0 + 16 * NT - 1) / A.rep, r.n - 1);
+  const int lo = r.C + row0 / A.rep, hi = min(r.C + last, r.L - 1);
+  walk<T, HD, NT, NW>(A, W, r, b, g, row0, 0, r.L, lo, hi, wave, lane);
+  finish<T, HD, NT, NW>(A, W, r, g, row0, -1, s_o, s_m, wave, lane);
+}
+
+// The grains of all (sequence, KV head) pairs in order, an even share of them for each
+// workgroup, wherever the sequences' borders are: one range of positions of one head, or
+// several.  A head's range that is not whole leaves its sums in the workspace, in entry
+// 2 w of workgroup w, or 2 w + 1 if it is not w's first, for join_kernel.
+template <class T, int HD, int NT, int NW>
+__global__ __launch_bounds__(64 * NW) void share_kernel(Attend<T> A) {
+  __shared__ __align__(16) float s_o[NW * 16 * (HD + 4)];
+  __shared__ float s_m[NW * 16 * 2];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), w = blockIdx.x;
+  const int nkv = A.P.nkv;
+  const Deal D(uniform(grains_below(A, A.P.B)) * nkv, A.wgs);
+  for (int e = w; e < A.P.B; e += A.wgs) {
+    const Run r = run_of(A, e);
+    if (r.none || r.nan)
+      for (int g = 0; g < nkv; ++g) fill<T, HD>(A, r, g, 0, 1);
+  }
+  if (w >= D.wgs) return;
+  const int from = D.from(w);
+  int left = D.from(w + 1) - from, b = 0, g = 0, at = 0, n = 0;
+  int base = 0;  // grains of one head of the sequences before
+  for (int c = 0; c < A.P.B; c += 64) {
+    const int t = c + lane < A.P.B ? grains_of(A, c + lane) : 0;
+    const int sum = lane_scan(t);
+    const unsigned long long past = __ballot((base + sum) * nkv > from);
+    if (past) {
+      const int i = __builtin_ctzll(past);
+      b = c + i;
+      n = __builtin_amdgcn_readlane(t, i);
+      const int in = from - (base + __builtin_amdgcn_readlane(sum, i) - n) * nkv;
+      g = in / n, at = in - g * n;
+      break;
+    }
+    base += __builtin_amdgcn_readlane(sum, 63);
+  }
+  for (bool start = true; left > 0; start = false) {
+    while (at >= n) {  // the next head that has grains
+      at = 0;
+      if (n > 0 && ++g < nkv) break;
+      g = 0;
+      if (++b >= A.P.B) return;  // (cannot be: the grains left are of some head)
+      n = uniform(grains_of(A, b));
+    }
+    const int m = min(n - at, left);
+    const Run r = run_of(A, b);
+    Sums<T, HD, NT> W;
+    walk<T, HD, NT, NW>(A, W, r, b, g, 0, at * kGrain, (at + m) * kGrain, r.C, r.L - 1, wave,
+                        lane);
+    finish<T, HD, NT, NW>(A, W, r, g, 0, m == n ? -1 : 2 * (long)w + !start, s_o, s_m, wave,
+                          lane);
+    at += m, left -= m;
+  }
+}
+
+// The entries of a head whose positions several workgroups had, joined: a workgroup per
+// row, HD / 4 lanes across and 256 / (HD / 4) entries at a time.
+template <class T, int HD>
+__global__ __launch_bounds__(256) void join_kernel(Attend<T> A) {
+  constexpr int kAcross = HD / 4, kAt = 256 / kAcross;
+  __shared__ float4v s_o[kAt][kAcross];
+  __shared__ float s_m[kAt], s_l[kAt];
+  const int b = blockIdx.z, g = blockIdx.y, row = blockIdx.x, nkv = A.P.nkv;
+  const Run r = run_of(A, b);
+  if (r.L == 0 || row >= A.rep * r.n) return;
+  const int n = grains_of(A, b), below = uniform(grains_below(A, b));
+  const Deal D(uniform(grains_below(A, A.P.B)) * nkv, A.wgs);
+  const int x0 = below * nkv + g * n;  // this head's first grain
+  const int w0 = D.owner(x0), w1 = D.owner(x0 + n - 1);
+  if (w0 == w1) return;
+  const int c = threadIdx.x % kAcross, at = threadIdx.x / kAcross;
+  float m = -__builtin_inff(), sum = 0.f;
+  float4v o = (float4v)(0.f);
+  const float* ms = A.part + 2 * (long)A.wgs * A.R * HD;
+  for (int w = w0 + at; w <= w1; w += kAt) {
+    const long e = (2 * (long)w + (D.from(w) < x0)) * A.R + row;
+    const float em = ms[2 * e], el = ms[2 * e + 1];
+    const float4v eo = *reinterpret_cast<const float4v*>(A.part + e * HD + 4 * c);
+    const float nm = fmaxf(m, em), ref = nm == -__builtin_inff() ? 0.f : nm;
+    const float a = __builtin_amdgcn_exp2f(m - ref), z = __builtin_amdgcn_exp2f(em - ref);
+    o = o * a + eo * z, sum = sum * a + el * z, m = nm;
+  }
+  s_o[at][c] = o;
+  if (c == 0) s_m[at] = m, s_l[at] = sum;
+  __syncthreads();
+  if (at) return;
+#pragma unroll
+  for (int i = 0; i < kAt; ++i) m = fmaxf(m, s_m[i]);
+  const float ref = m == -__builtin_inff() ? 0.f : m;
+  o = (float4v)(0.f), sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kAt; ++i) {
+    const float a = __builtin_amdgcn_exp2f(s_m[i] - ref);
+    o += s_o[i][c] * a, sum += s_l[i] * a;
+  }
+  const int tok = row / A.rep, head = row - tok * A.rep;
+  T* dst = A.out + (long)(r.row + tok) * A.ld_o + (long)(g * A.rep + head) * HD + 4 * c;
+  const float is = 1.f / sum;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) dst[i] = (T)(o[i] * is);
 }
 
 // Pages src[i] to dst[i] of every layer; the addresses and pairs go in the arguments.
@@ -126,7 +581,7 @@ int check_step(const char* who, const Step& P, const void* qkv, const void* k, c
                "%s: %d sequences, %ld rows, %ld pages, a table of %ld columns (row %ld)", who, P.B,
                T, P.pages, P.cols, P.ld);
   if (P.B == 0 || T == 0) return 0;
-  HN_ARG_CHECK(qkv && k && v && P.table && P.lens, "%s: null operand", who);
+  HN_ARG_CHECK(qkv && k && v && (P.cols == 0 || P.table) && P.lens, "%s: null operand", who);
   HN_ARG_CHECK((uintptr_t)k % 16 == 0 && (uintptr_t)v % 16 == 0, "%s: pages not 16-byte aligned",
                who);
   return 0;
@@ -147,20 +602,49 @@ int append(const Step& P, const void* qkv, long ld, const float* cos_t, const fl
   return 0;
 }
 
-template <class T>
-int attend(const Step& P, const void* q, long ld_q, const void* k, const void* v, int nh, int hd,
-           float scale, void* out, long ld_o, hipStream_t stream) {
-  const dim3 grid(P.T, nh);
-  const int rep = nh / P.nkv;
-#define HN_ATTEND(HD)                                                                     \
-  attend_kernel<T, HD><<<grid, 64, 0, stream>>>(P, (const T*)q, ld_q, (const T*)k,        \
-                                                (const T*)v, rep, scale, (T*)out, ld_o)
-  if (hd == 64) HN_ATTEND(64);
-  else if (hd == 128) HN_ATTEND(128);
-  else HN_ATTEND(256);
-#undef HN_ATTEND
+// Rows of one (sequence, KV head) up to which a workgroup's positions are shared out.
+constexpr int kShareRows = 32;
+// Positions up to which one workgroup takes all of a head's.
+constexpr long kWhole = 2048;
+
+// The workgroups that share the positions, 0: a workgroup per head.
+int share_wgs(long rows, long hd, long bound) {
+  return rows > (hd == 256 ? 16 : kShareRows) || bound <= kWhole ? 0 : 2 * hn_device_cus();
+}
+
+long part_bytes(long wgs, long rows, long hd) { return 2 * wgs * rows * (hd + 2) * 4; }
+
+template <class T, int HD, int NT>
+int attend_rows(const Attend<T>& A, int B, int nkv, hipStream_t stream) {
+  if (A.wgs) {
+    share_kernel<T, HD, NT, 4><<<A.wgs, 256, 0, stream>>>(A);
+    HN_LAUNCH_CHECK("hn_paged_attention");
+    join_kernel<T, HD><<<dim3(A.R, nkv, B), 256, 0, stream>>>(A);
+  } else {
+    constexpr int NW = NT == 1 && HD < 256 ? 8 : 4;
+    whole_kernel<T, HD, NT, NW>
+        <<<dim3(nkv, hn_cdiv(A.R, 16 * NT), B), 64 * NW, 0, stream>>>(A);
+  }
   HN_LAUNCH_CHECK("hn_paged_attention");
   return 0;
+}
+
+template <class T, int HD>
+int attend_hd(const Attend<T>& A, int B, int nkv, hipStream_t stream) {
+  if (A.R <= 16) return attend_rows<T, HD, 1>(A, B, nkv, stream);
+  return attend_rows<T, HD, HD == 256 ? 1 : 2>(A, B, nkv, stream);
+}
+
+template <class T>
+int attend(const Step& P, const void* q, long ld_q, const void* k, const void* v, int nh, int hd,
+           int max_new, int wgs, float scale, void* out, long ld_o, void* work,
+           hipStream_t stream) {
+  const int rep = nh / P.nkv;
+  const Attend<T> A = {P, (const T*)q, (const T*)k, (const T*)v, (T*)out, (float*)work, ld_q, ld_o,
+                       rep, max_new, rep * max_new, wgs, scale};
+  if (hd == 64) return attend_hd<T, 64>(A, P.B, P.nkv, stream);
+  if (hd == 128) return attend_hd<T, 128>(A, P.B, P.nkv, stream);
+  return attend_hd<T, 256>(A, P.B, P.nkv, stream);
 }
 
 }  // namespace
@@ -187,7 +671,9 @@ extern "C" int hn_paged_append(const void* qkv, long ld_qkv, int dtype, const fl
 
 extern "C" long hn_paged_attention_workspace_bytes(long B, long T, long nh, long nkv, long hd,
                                                    long max_new, long bound) {
-  return 0;
+  if (B <= 0 || T <= 0 || nkv <= 0 || nh < nkv || hd <= 0 || max_new <= 0) return 0;
+  const long rows = nh / nkv * max_new;
+  return part_bytes(share_wgs(rows, hd, bound), rows, hd);
 }
 
 extern "C" int hn_paged_attention(const void* q, long ld_q, int dtype, const void* k,
@@ -198,17 +684,29 @@ extern "C" int hn_paged_attention(const void* q, long ld_q, int dtype, const voi
                                   long work_bytes, void* stream) {
   const Step P = step_of(table, ld_table, cols, num_pages, lens, starts, B, T, nkv, page);
   if (int rc = check_step("hn_paged_attention", P, q, k, v, nh, hd, T, dtype)) return rc;
-  HN_ARG_CHECK(max_new >= 1 && bound >= 1, "hn_paged_attention: max_new %ld, bound %ld", max_new,
-               bound);
+  HN_ARG_CHECK(max_new >= 1 && bound >= 1 && max_new <= (1l << 24) / nh,
+               "hn_paged_attention: max_new %ld, bound %ld", max_new, bound);
+  HN_ARG_CHECK(B < 65536 && nkv < 65536 &&
+                   (cols < 1l << 26 && cols * page < 1l << 30) &&
+                   (double)B * nkv * (cols * page / kGrain + 1) < 2147483648.0,
+               "hn_paged_attention: %ld sequences of %ld pages", B, cols);
   HN_ARG_CHECK(scale > 0.f && scale * 1.4426950408889634f < __builtin_inff(),
                "hn_paged_attention: scale %g", (double)scale);
   if (B == 0 || T == 0) return 0;
+  HN_ARG_CHECK(num_pages >= 1, "hn_paged_attention: no pages");
   HN_ARG_CHECK(out && ld_q >= nh * hd && ld_o >= nh * hd && ld_q % 8 == 0 && ld_o % 8 == 0 &&
                    (uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0,
                "hn_paged_attention: rows of %ld, strides of %ld and %ld: 16-byte aligned rows",
                nh * hd, ld_q, ld_o);
-  return (dtype == 0 ? attend<h16> : attend<b16>)(P, q, ld_q, k, v, (int)nh, (int)hd, scale, out,
-                                                  ld_o, (hipStream_t)stream);
+  const long rows = nh / nkv * max_new;
+  const int wgs = share_wgs(rows, hd, bound);
+  HN_ARG_CHECK(wgs == 0 || (work && (uintptr_t)work % 16 == 0 &&
+                            work_bytes >= part_bytes(wgs, rows, hd)),
+               "hn_paged_attention: a workspace of %ld bytes, %ld given",
+               part_bytes(wgs, rows, hd), work ? work_bytes : 0);
+  return (dtype == 0 ? attend<h16> : attend<b16>)(P, q, ld_q, k, v, (int)nh, (int)hd,
+                                                  (int)max_new, wgs, scale, out, ld_o, work,
+                                                  (hipStream_t)stream);
 }
 
 extern "C" int hn_page_copy(void* const* k, void* const* v, long layers, long page_bytes,

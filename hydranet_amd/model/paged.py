@@ -216,9 +216,9 @@ class PagedBatch:
     names the pages of sequence b in order (PagedKVCache.table); lens int64 [B]: its
     cached positions before the step, negative: it takes no part.  starts int32 [B + 1]
     (not decreasing, from 0): sequence b's new tokens are rows starts[b] to starts[b +
-    1] - 1 of the step's `rows`; None: one row each.  kv_bound and max_new: about the
-    most positions (with the new ones) and new rows of a sequence, for the launches'
-    sizes; the results do not go by them.  The tensors are read when the kernels run,
+    1] - 1 of the step's `rows`, at most max_new each; None: one row each.  kv_bound: about
+    the most positions of a sequence (with the new ones), for the launches' sizes; the
+    results do not go by it.  The tensors are read when the kernels run,
     so a captured step may be replayed after they were changed in place."""
 
     def __init__(self, table: torch.Tensor, lens: torch.Tensor, kv_bound: int,
@@ -347,8 +347,8 @@ def paged_attention(q: torch.Tensor, batch: PagedBatch, cache: PagedKVCache, lay
     """Attention of a step's rows (paged_append's queries [rows, heads * hd], their keys
     and values in the pages) over the positions up to their own -> [rows, heads * hd].
     scale: of the scores, 1 / sqrt(hd) by default.  Rows of a sequence that takes no
-    part and of no sequence are zero; rows of one of which not every page is named are
-    NaN."""
+    part and of no sequence are zero; a row that sees a position whose page is not named
+    is NaN, and so are the rows of a run of more than the batch's max_new."""
     nkv, hd = cache.kv_heads, cache.head_dim
     assert q.dim() == 2 and hd > 0 and q.shape[1] % hd == 0, f"q [rows, heads * {hd}]"
     nh = q.shape[1] // hd
@@ -374,11 +374,14 @@ def paged_attention(q: torch.Tensor, batch: PagedBatch, cache: PagedKVCache, lay
     for b, first, m, C in batch._runs():
         if C < 0:
             continue
-        L = min(C, 2 ** 62) + m
         pages = batch._pages(cache, b)
-        if cache.pages_for(L) > len(pages):
-            out[first:first + m] = math.nan
+        out[first:first + m] = math.nan
+        if m > batch.max_new:
             continue
+        m = min(m, len(pages) * cache.page_size - C)  # rows all of whose pages are named
+        if m <= 0:
+            continue
+        L = C + m
         at = torch.tensor(pages[:cache.pages_for(L)])
         kk = k[at].transpose(0, 1).reshape(nkv, -1, hd)[:, :L].to(wide)
         vv = v[at].permute(1, 0, 2, 4, 3).reshape(nkv, -1, hd)[:, :L].to(wide)

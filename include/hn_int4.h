@@ -559,12 +559,13 @@ int hn_paged_append(const void* qkv, long ld_qkv, int dtype, const float* cos_t,
 /* hn_paged_attention: out[t * ld_o + h * hd + d] = softmax(scale * q k) v over the
  *   positions up to row t's own (its key and value in the pages already), query
  *   head h over KV head h / (nh / nkv); fp32 scores, statistics and sums.  q
- *   [T][ld_q].  Rows of a sequence with a negative length are zero; those of a
- *   sequence of which the table does not name every page are NaN.  A position
- *   that a row does not see has no effect on it, whatever it holds.  max_new and
- *   bound: about the most rows and positions (C_b + rows) of a sequence; they
- *   choose the launch, not the result.  scale above 0 and finite, also times
- *   log2(e); 16-byte aligned operands, ld_q and ld_o multiples of 8.  work:
+ *   [T][ld_q].  Rows of a sequence with a negative length are zero; a row that
+ *   sees a position whose page the table does not name is NaN, and so are the rows
+ *   of a sequence with more than max_new of them.  A position that a row does not
+ *   see has no effect on it, whatever it holds.  bound: about the most positions
+ *   (C_b + rows) of a sequence; it chooses the launch, not the result.  scale above
+ *   0 and finite, also times log2(e); 16-byte aligned operands, ld_q and ld_o
+ *   multiples of 8; cols * page < 2^30.  work:
  *   hn_paged_attention_workspace_bytes(...) bytes, 16-byte aligned, any contents. */
 long hn_paged_attention_workspace_bytes(long B, long T, long nh, long nkv, long hd, long max_new,
                                         long bound);

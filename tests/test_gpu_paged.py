@@ -78,29 +78,42 @@ def test_attention_large_scores(counts):
     assert ((got.double().cpu() - want).abs() <= bound).all()
 
 
-@pytest.mark.parametrize("counts", [None, [30, 1, 100]])
-def test_pages_that_are_not_named(counts):
-    """A sequence with a missing page, an id past the pages, a table too short: NaN rows of
-    its own, and the others' as they are."""
+@pytest.mark.parametrize("hint", [None, 5000])
+@pytest.mark.parametrize("counts", [None, [1, 5, 2], [30, 40, 100]])
+def test_pages_that_are_not_named(counts, hint):
+    """A missing page, an id past the pages, a table too short: NaN in the rows that see the
+    place, and all others as they are."""
     from hydranet_amd.model.paged import paged_attention
-    s = ref.make(4, [100, 200, 90], counts, 2, 128, 16, torch.float16, DEV)
+    s = ref.make(4, [100, 180, 90], counts, 2, 128, 16, torch.float16, DEV, poison=True)
     q = torch.randn(s["rows"], 8 * 128, generator=s["gen"]).half().to(DEV)
-    want = paged_attention(q, ref.batch(s, counts is None), _cache(s), 0)
-    a, b = int(s["starts"][1]), int(s["starts"][2])
-    for value, col in ((-1, 0), (s["k"].shape[0], 3), (-2 ** 31, 12), (2 ** 31 - 1, 7)):
-        bad = dict(s, table=s["table"].clone())
-        bad["table"][1, col] = value
-        got = paged_attention(q, ref.batch(bad, counts is None), _cache(s), 0)
-        assert got[a:b].isnan().all()
-        assert torch.equal(got[:a], want[:a]) and torch.equal(got[b:], want[b:])
-    short = dict(s, table=s["table"][:, :12].contiguous())  # 192 positions
-    got = paged_attention(q, ref.batch(short, counts is None), _cache(s), 0)
-    assert got[a:b].isnan().all() and torch.equal(got[:a], want[:a])
-    far = dict(s, lens=s["lens"].clone())
-    far["lens"][1] = 2 ** 63 - 1
-    got = paged_attention(q, ref.batch(far, counts is None, 300), _cache(s), 0)
-    assert got[a:b].isnan().all() and torch.equal(got[:a], want[:a])
-    assert torch.equal(got[b:], want[b:])
+    want = paged_attention(q, ref.batch(s, counts is None, hint), _cache(s), 0)
+    starts = s["starts"].tolist()
+    assert want.isfinite().all()
+
+    def check(bad, first):
+        """NaN from position `first` of sequence 1 on."""
+        got = paged_attention(q, ref.batch(bad, counts is None, hint or 300), _cache(s), 0)
+        for row, b, pos in ref.tokens({n: s[n].cpu() for n in ("starts", "lens")}):
+            if b == 1 and pos >= first:
+                assert got[row].isnan().all()
+            else:
+                assert torch.equal(got[row], want[row])
+    for value, col in ((-1, 0), (s["k"].shape[0], 3), (-2 ** 31, 11), (2 ** 31 - 1, 12)):
+        if counts is None and col == 12:
+            continue  # (positions 192 on: none of a single token's)
+        if col < s["table"].shape[1]:
+            bad = dict(s, table=s["table"].clone())
+            bad["table"][1, col] = value
+            check(bad, 16 * col)
+    check(dict(s, table=s["table"][:, :12].contiguous()), 192)
+    check(dict(s, table=torch.cat((s["table"][:, :12], s["table"]), 1)[:, :12]), 192)
+    for C in (2 ** 63 - 1, 2 ** 31, 10 ** 6):
+        far = dict(s, lens=s["lens"].clone())
+        far["lens"][1] = C
+        check(far, 0)
+    none = dict(s, table=s["table"][:, :0])
+    got = paged_attention(q, ref.batch(none, counts is None, hint), _cache(s), 0)
+    assert got.isnan().all() and starts[-1] == s["rows"]
 
 
 @pytest.mark.parametrize("rep,hd", [(4, 128), (1, 64), (20, 64), (2, 256)])
@@ -200,14 +213,14 @@ def test_append_outside(counts):
 
 def test_rows_of_no_sequence():
     """Rows behind the last sequence (and before the first) come back zero and write
-    nothing; a run longer than max_new is whole."""
+    nothing; a run longer than max_new has NaN rows."""
     from hydranet_amd.model.paged import PagedBatch, RotaryTable, paged_append, paged_attention
     s = ref.make(9, [30, 5], [100, 7], 2, 128, 16, torch.float16, DEV)
     rows = s["rows"] + 13
     cos, sin = ref.tables(128, 200)
     rope = RotaryTable.wrap(cos.to(DEV), sin.to(DEV))
     qkv = torch.randn(rows, 8 * 128, generator=s["gen"]).half().to(DEV)
-    one = PagedBatch(s["table"], s["lens"], 50, s["starts"], rows, 2)
+    one = PagedBatch(s["table"], s["lens"], 50, s["starts"], rows, 100)
     q = paged_append(qkv, rope, one, _cache(s), 0, 4)
     out = paged_attention(q, one, _cache(s), 0)
     for x in (q, out):
@@ -218,6 +231,11 @@ def test_rows_of_no_sequence():
     q2 = torch.cat((q[:4], q[:rows - 4]))
     out2 = paged_attention(q2, late, _cache(s), 0)
     assert not out2[:4].any() and torch.equal(out2[4:4 + s["rows"]], out[:s["rows"]])
+    for hint in (50, 5000):
+        few = PagedBatch(s["table"], s["lens"], hint, s["starts"], rows, 7)
+        out3 = paged_attention(q, few, _cache(s), 0)
+        assert out3[:100].isnan().all() and not out3[s["rows"]:].any()
+        assert ((out3[100:s["rows"]].double().cpu() - want[100:]).abs() <= bound[100:]).all()
 
 
 def test_page_copy():

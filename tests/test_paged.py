@@ -45,14 +45,18 @@ def test_attention_values_that_are_no_numbers():
 
 
 def test_attention_pages_that_are_not_named():
-    s = ref.make(4, [20, 40], [2, 3], 2, 8, 16, torch.float32)
+    s = ref.make(4, [20, 30], [2, 3], 2, 8, 16, torch.float32)
     q = torch.randn(5, 32, generator=s["gen"])
     want = paged_attention(q, ref.batch(s, False), _cache(s), 0)
-    for value, col in ((-1, 0), (s["k"].shape[0], 2), (-2 ** 31, 1)):
+    for value, col in ((-1, 0), (s["k"].shape[0], 1), (-2 ** 31, 2)):
         bad = dict(s, table=s["table"].clone())
         bad["table"][1, col] = value
         got = paged_attention(q, ref.batch(bad, False), _cache(s), 0)
-        assert got[2:].isnan().all() and torch.equal(got[:2], want[:2])
+        first = 2 + max(0, 16 * col - 30)  # the row at the page's first position
+        assert got[first:].isnan().all() and torch.equal(got[:first], want[:first])
+    few = PagedBatch(s["table"], s["lens"], 50, s["starts"], 5, 2)
+    got = paged_attention(q, few, _cache(s), 0)
+    assert got[2:].isnan().all() and torch.equal(got[:2], want[:2])
     s["lens"][1] = 2 ** 63 - 1
     assert paged_attention(q, ref.batch(s, False, 50), _cache(s), 0)[2:].isnan().all()
 
