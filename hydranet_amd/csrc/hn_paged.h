@@ -12,23 +12,33 @@ struct Step {
   int B, T, nkv, page;
 };
 
-// Row t's sequence (-1: no sequence's) and position (-1: its sequence takes no part).
-// By a whole wave: the sequences that end at or before t are counted by ballots.
+// A row's sequence (-1: no sequence's) and position (-1: its sequence takes no part).
 struct Row {
   int b;
   long pos;
 };
-__device__ __forceinline__ Row row_of(const Step& P, int t) {
-  int b = t, first = t;
-  if (P.starts) {
-    b = 0;
-    for (int c = threadIdx.x & 63; c - (int)(threadIdx.x & 63) < P.B; c += 64)
-      b += __popcll(__ballot(c < P.B && P.starts[c < P.B ? c + 1 : P.B] <= t));
-    if (b >= P.B || (first = P.starts[b]) > t) return {-1, -1};
-  }
+__device__ __forceinline__ Row row_in(const Step& P, int b, int n) {
   const long C = P.lens[b];
   if (C < 0) return {b, -1};
-  return {b, (C < 1l << 62 ? C : 1l << 62) + (t - first)};  // (no sum wraps)
+  return {b, (C < 1l << 62 ? C : 1l << 62) + n};  // (no sum wraps)
+}
+// Row t, of sequence b or a later one.
+__device__ __forceinline__ Row row_from(const Step& P, int t, int b) {
+  while (b < P.B && P.starts[b + 1] <= t) ++b;
+  if (b >= P.B || P.starts[b] > t) return {-1, -1};
+  return row_in(P, b, t - P.starts[b]);
+}
+// Row t, by a whole wave whose first lane's row is none behind the others': the sequences
+// that end at or before that row are counted by ballots, a lane goes on from there.
+__device__ __forceinline__ Row row_near(const Step& P, int t) {
+  if (!P.starts) return row_in(P, t, 0);
+  const int lane = threadIdx.x & 63, t0 = __builtin_amdgcn_readfirstlane(t);
+  int b = 0;
+  for (int c = 0; c < P.B; c += 64) {
+    const int at = c + lane;
+    b += __popcll(__ballot(at < P.B && P.starts[at < P.B ? at + 1 : P.B] <= t0));
+  }
+  return row_from(P, t, b);
 }
 
 // The page of a position, -1 where the table names none.

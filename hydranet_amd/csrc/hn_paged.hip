@@ -10,7 +10,31 @@
 
 namespace {
 
-// One thread per element, grid (T, nh + 2 nkv).
+typedef float float4v __attribute__((ext_vector_type(4)));
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+
+template <class T>
+struct Vec;
+template <>
+struct Vec<h16> {
+  typedef half8_t t;
+  static constexpr uint32_t inf = 0x7c00u;
+  static __device__ __forceinline__ float4v mfma(t a, t b, float4v c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Vec<b16> {
+  typedef bf8 t;
+  static constexpr uint32_t inf = 0x7f80u;
+  static __device__ __forceinline__ float4v mfma(t a, t b, float4v c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  }
+};
+
+// ---------------------------------------------------------------------------
+// The append.  One thread per element, grid (T, nh + 2 nkv): rows and rotated parts of any
+// alignment.
 template <class T>
 __global__ __launch_bounds__(256) void append_kernel(Step P, const T* __restrict__ qkv, long ld,
                                                      const float* __restrict__ cos_t,
@@ -19,8 +43,11 @@ __global__ __launch_bounds__(256) void append_kernel(Step P, const T* __restrict
                                                      T* __restrict__ q_out, T* __restrict__ k,
                                                      T* __restrict__ v) {
   const int t = blockIdx.x, head = blockIdx.y, d = threadIdx.x;
-  const Row r = row_of(P, t);
-  if (r.b < 0 || d >= hd) return;
+  const Row r = row_near(P, t);
+  if (r.b < 0) {
+    if (head < nh) q_out[((long)t * nh + head) * hd + d] = (T)0.f;
+    return;
+  }
   long pg = -1;
   const bool in = r.pos >= 0 && r.pos < rows && (pg = page_of(P, r.b, r.pos)) >= 0;
   const int slot = (int)(r.pos & (P.page - 1));
@@ -44,6 +71,135 @@ __global__ __launch_bounds__(256) void append_kernel(Step P, const T* __restrict
   else if (in) k[((pg * P.nkv + head - nh) * P.page + slot) * hd + d] = (T)y;
 }
 
+// The same by 16-byte vectors.  Queries and keys: a thread has 16 elements of a head at a
+// time, the two vectors of 8 pairs (or of 16 dimensions that stay), so their 8 angles stay
+// in registers over its NI heads; HD / 16 threads a head, `across` heads of a token side by
+// side.  Values: a thread has 8 dimensions of the new rows among 8 slots of a page, which
+// are 128 consecutive bytes; it writes them whole where all 8 are new, else its rows' 2
+// bytes each.
+template <class T, int HD, int NI>
+__global__ __launch_bounds__(256) void append_rows_kernel(
+    Step P, const T* __restrict__ qkv, long ld, const float* __restrict__ cos_t,
+    const float* __restrict__ sin_t, long rows, int rd, int pairs, int nh, int across, int qx,
+    int qk, T* __restrict__ q_out, T* __restrict__ kc, T* __restrict__ vc) {
+  typedef typename Vec<T>::t V8;
+  constexpr int kUnits = HD / 16;
+  const int tid = threadIdx.x;
+  if ((int)blockIdx.x < qk) {
+    const int u = tid % kUnits, slot = tid / kUnits;
+    const int t = (blockIdx.x % qx) * (256 / kUnits / across) + slot / across;
+    const int h0 = (blockIdx.x / qx) * across * NI + slot % across;
+    const bool there = t < P.T;
+    // where the 16 elements lie, and the first of their angles
+    const bool turn = 16 * u < rd;
+    const int lo = !turn || pairs ? 16 * u : 8 * u;
+    const int hi = !turn || pairs ? lo + 8 : lo + rd / 2;
+    const T* src = qkv + (long)(there ? t : 0) * ld;
+    V8 x[NI], y[NI];
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int h = min(h0 + i * across, nh + P.nkv - 1);
+      x[i] = *reinterpret_cast<const V8*>(src + (long)h * HD + lo);
+      y[i] = *reinterpret_cast<const V8*>(src + (long)h * HD + hi);
+    }
+    const Row r = row_near(P, there ? t : P.T - 1);
+    if (!there) return;
+    const long pg = r.b >= 0 && r.pos >= 0 && r.pos < rows ? page_of(P, r.b, r.pos) : -1;
+    if (pg >= 0 && turn) {
+      float4v c[2], s[2];
+      const long at = r.pos * (rd / 2) + 8 * u;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        c[j] = *reinterpret_cast<const float4v*>(cos_t + at + 4 * j);
+        s[j] = *reinterpret_cast<const float4v*>(sin_t + at + 4 * j);
+      }
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const V8 a = x[i], b = y[i];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          // pair j: elements 2 j and 2 j + 1 of both vectors, or j of each
+          const float f = (float)(pairs ? (j < 4 ? a[2 * j] : b[(2 * j) & 7]) : a[j]);
+          const float z = (float)(pairs ? (j < 4 ? a[(2 * j + 1) & 7] : b[(2 * j + 1) & 7]) : b[j]);
+          const float cj = c[j >> 2][j & 3], sj = s[j >> 2][j & 3];
+          const T f2 = (T)(f * cj - z * sj), z2 = (T)(z * cj + f * sj);
+          if (!pairs) x[i][j] = f2, y[i][j] = z2;
+          else if (j < 4) x[i][(2 * j) & 7] = f2, x[i][(2 * j + 1) & 7] = z2;
+          else y[i][(2 * j) & 7] = f2, y[i][(2 * j + 1) & 7] = z2;
+        }
+      }
+    }
+    const T none = (T)(r.pos < 0 ? 0.f : __builtin_nanf(""));
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int h = h0 + i * across;
+      if (h >= nh + P.nkv || (h >= nh && pg < 0)) continue;
+      if (pg < 0)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[i][j] = y[i][j] = none;
+      T* dst = h < nh ? q_out + ((long)t * nh + h) * HD
+                      : kc + ((pg * P.nkv + h - nh) * P.page + (r.pos & (P.page - 1))) * HD;
+      *reinterpret_cast<V8*>(dst + lo) = x[i];
+      *reinterpret_cast<V8*>(dst + hi) = y[i];
+    }
+    return;
+  }
+  // The rows that share 8 slots are the first one's (of the run, or at the first slot); a
+  // thread looks for those among `step` rows.
+  const int cols = P.nkv * (HD / 8), step = P.starts ? 8 : 1;
+  const long id = (long)(blockIdx.x - qk) * 256 + tid;
+  const int g = (int)(id / cols), c = (int)(id - (long)g * cols) * 8;
+  const long t0 = (long)g * step;
+  Row r = row_near(P, (int)min(t0, (long)P.T - 1));
+  int t = (int)t0;
+  if (t0 >= P.T) return;
+  const int end = min(t + step, P.T);
+  const T* src = qkv + (long)(nh + P.nkv) * HD + c;
+  while (t < end) {
+    // (rows before the first sequence: r.b -1; behind the last: nothing follows)
+    if (r.b < 0) {
+      if (t >= P.starts[0]) return;
+      t = P.starts[0];
+      if (t >= end) return;
+      r = row_from(P, t, 0);
+      continue;
+    }
+    const int first = P.starts ? P.starts[r.b] : t, stop = P.starts ? min(P.starts[r.b + 1], P.T) : t + 1;
+    int n = stop - t;  // rows to go on by
+    if (r.pos >= 0) {
+      const int in = (int)(r.pos & 7);
+      n = min(n, 8 - in);
+      const long pg = r.pos < rows && (in == 0 || t == first) ? page_of(P, r.b, r.pos) : -1;
+      if (pg >= 0) {
+        const int m = (int)min((long)n, rows - r.pos);
+        const int slot = (int)(r.pos & (P.page - 1));
+        T* dst = vc + ((pg * P.nkv + c / HD) * P.page + (slot & ~7)) * HD + (c % HD) * 8;
+        V8 x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          x[j] = *reinterpret_cast<const V8*>(src + (long)(t + min(j, m - 1)) * ld);
+        if (m == 8) {
+#pragma unroll
+          for (int d = 0; d < 8; ++d) {
+            V8 y;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) y[j] = x[j][d];
+            *reinterpret_cast<V8*>(dst + 8 * d) = y;
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (j < m)
+#pragma unroll
+              for (int d = 0; d < 8; ++d) dst[8 * d + in + j] = x[j][d];
+        }
+      }
+    }
+    t += n;
+    if (t < end) r = row_from(P, t, r.b);
+  }
+}
+
 // ---------------------------------------------------------------------------
 // Attention.  One pass over a sequence's pages with a running maximum and sum, for the
 // rows of one (sequence, KV head), a row being a (new token, query head of the group)
@@ -65,28 +221,6 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kUp = 8.f, kLag = 6.f;
 // Positions that workgroups share out as one.
 constexpr int kGrain = 128;
-
-typedef float float4v __attribute__((ext_vector_type(4)));
-typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
-
-template <class T>
-struct Vec;
-template <>
-struct Vec<h16> {
-  typedef half8_t t;
-  static constexpr uint32_t inf = 0x7c00u;
-  static __device__ __forceinline__ float4v mfma(t a, t b, float4v c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-  }
-};
-template <>
-struct Vec<b16> {
-  typedef bf8 t;
-  static constexpr uint32_t inf = 0x7f80u;
-  static __device__ __forceinline__ float4v mfma(t a, t b, float4v c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
-  }
-};
 
 template <class T>
 struct Attend {
@@ -138,7 +272,7 @@ __device__ __forceinline__ Run run_of(const Attend<T>& A, int b) {
   return r;
 }
 
-// The rows of a run that none attends for, of KV head g.
+// The rows of a run that none attends for, of KV head g; and of no run.
 template <class T, int HD>
 __device__ __forceinline__ void fill(const Attend<T>& A, const Run& r, int g, int part, int parts) {
   const T x = (T)(r.nan ? __builtin_nanf("") : 0.f);
@@ -152,6 +286,14 @@ __device__ __forceinline__ void fill(const Attend<T>& A, const Run& r, int g, in
     *reinterpret_cast<typename Vec<T>::t*>(A.out + (long)(r.row + t) * A.ld_o +
                                            (long)g * A.rep * HD + 8 * c) = y;
   }
+}
+
+template <class T, int HD>
+__device__ __forceinline__ void fill_rest(const Attend<T>& A, int g, int part, int parts) {
+  if (!A.P.starts) return;
+  const int first = min(max(A.P.starts[0], 0), A.P.T), end = min(max(A.P.starts[A.P.B], first), A.P.T);
+  fill<T, HD>(A, Run{0, first, 0, 0, true, false}, g, part, parts);
+  fill<T, HD>(A, Run{end, A.P.T - end, 0, 0, true, false}, g, part, parts);
 }
 
 // Sums of the lanes up to each (row_shr:1, 2, 4, 8, then row_bcast:15, 31).
@@ -442,6 +584,7 @@ __global__ __launch_bounds__(64 * NW) void whole_kernel(Attend<T> A) {
   const int g = blockIdx.x, b = blockIdx.z, row0 = (gridDim.y - 1 - blockIdx.y) * 16 * NT;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const Run r = run_of(A, b);
+  if (b == 0) fill_rest<T, HD>(A, g, blockIdx.y, gridDim.y);
   if (r.none || r.nan) return fill<T, HD>(A, r, g, blockIdx.y, gridDim.y);
   if (row0 >= A.rep * r.n) return;
   Sums<T, HD, NT> W;
@@ -467,6 +610,7 @@ __global__ __launch_bounds__(64 * NW) void share_kernel(Attend<T> A) {
     if (r.none || r.nan)
       for (int g = 0; g < nkv; ++g) fill<T, HD>(A, r, g, 0, 1);
   }
+  for (int g = 0; g < nkv; ++g) fill_rest<T, HD>(A, g, w, A.wgs);
   if (w >= D.wgs) return;
   const int from = D.from(w);
   int left = D.from(w + 1) - from, b = 0, g = 0, at = 0, n = 0;
@@ -592,12 +736,40 @@ Step step_of(const int* table, long ld_table, long cols, long num_pages, const l
   return Step{table, ld_table, cols, num_pages, lens, starts, (int)B, (int)T, (int)nkv, (int)page};
 }
 
+// Rows from which a thread takes four heads of a token, so that it reads the angles once.
+constexpr int kManyRows = 1024;
+
+template <class T, int HD>
+void append_rows(const Step& P, const T* qkv, long ld, const float* cos_t, const float* sin_t,
+                 long rows, int rd, int pairs, int nh, T* q_out, T* k, T* v, hipStream_t stream) {
+  constexpr int kSlots = 256 / (HD / 16);
+  const bool many = P.T >= kManyRows;
+  const int across = many ? 1 : kSlots, heads = many ? 4 : kSlots;
+  const int qx = hn_cdiv(P.T, kSlots / across), qk = qx * hn_cdiv(nh + P.nkv, heads);
+  const long groups = P.starts ? hn_cdiv(P.T, 8) : P.T;
+  const int grid = qk + hn_cdiv(groups * P.nkv * (HD / 8), 256);
+  if (many)
+    append_rows_kernel<T, HD, 4><<<grid, 256, 0, stream>>>(
+        P, qkv, ld, cos_t, sin_t, rows, rd, pairs, nh, across, qx, qk, q_out, k, v);
+  else
+    append_rows_kernel<T, HD, 1><<<grid, 256, 0, stream>>>(
+        P, qkv, ld, cos_t, sin_t, rows, rd, pairs, nh, across, qx, qk, q_out, k, v);
+}
+
 template <class T>
-int append(const Step& P, const void* qkv, long ld, const float* cos_t, const float* sin_t,
-           long rows, int rd, int pairs, int nh, int hd, void* q_out, void* k, void* v,
+int append(const Step& P, const void* qkv_, long ld, const float* cos_t, const float* sin_t,
+           long rows, int rd, int pairs, int nh, int hd, void* q_, void* k_, void* v_,
            hipStream_t stream) {
-  append_kernel<T><<<dim3(P.T, nh + 2 * P.nkv), hd, 0, stream>>>(
-      P, (const T*)qkv, ld, cos_t, sin_t, rows, rd, pairs, nh, hd, (T*)q_out, (T*)k, (T*)v);
+  const T* qkv = (const T*)qkv_;
+  T *q = (T*)q_, *k = (T*)k_, *v = (T*)v_;
+  const bool vectors = ((uintptr_t)qkv | (uintptr_t)q | (uintptr_t)cos_t | (uintptr_t)sin_t) % 16 == 0 &&
+                       ld % 8 == 0 && rd % 16 == 0;
+  if (!vectors)
+    append_kernel<T><<<dim3(P.T, nh + 2 * P.nkv), hd, 0, stream>>>(P, qkv, ld, cos_t, sin_t, rows,
+                                                                  rd, pairs, nh, hd, q, k, v);
+  else if (hd == 64) append_rows<T, 64>(P, qkv, ld, cos_t, sin_t, rows, rd, pairs, nh, q, k, v, stream);
+  else if (hd == 128) append_rows<T, 128>(P, qkv, ld, cos_t, sin_t, rows, rd, pairs, nh, q, k, v, stream);
+  else append_rows<T, 256>(P, qkv, ld, cos_t, sin_t, rows, rd, pairs, nh, q, k, v, stream);
   HN_LAUNCH_CHECK("hn_paged_append");
   return 0;
 }
@@ -660,6 +832,8 @@ extern "C" int hn_paged_append(const void* qkv, long ld_qkv, int dtype, const fl
   HN_ARG_CHECK(rotary >= 0 && rotary <= hd && rotary % 2 == 0 && table_rows >= 0,
                "hn_paged_append: %ld rotated dimensions of %ld, %ld positions", rotary, hd,
                table_rows);
+  HN_ARG_CHECK(nh + 2 * nkv < 65536 && T * (nh + 2 * nkv) < 1l << 31,
+               "hn_paged_append: %ld rows of %ld heads", T, nh + 2 * nkv);
   if (B == 0 || T == 0) return 0;
   HN_ARG_CHECK(q_out && (rotary == 0 || (cos_t && sin_t)), "hn_paged_append: null operand");
   HN_ARG_CHECK(ld_qkv >= (nh + 2 * nkv) * hd, "hn_paged_append: rows of %ld, a stride of %ld",

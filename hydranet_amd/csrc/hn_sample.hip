@@ -18,61 +18,129 @@ struct Adjust {
   long V;
 };
 
-constexpr int kThreads = 256, kChunk = 2048;
+constexpr int kThreads = 1024;
 constexpr uint32_t kSeen = 1u << 31;
 
-// A workgroup takes kChunk tokens of a row.  Their counts are gathered in LDS from the
-// whole text (integers, so any order gives the same), and of several biases for a
-// token the last one's index.
-template <class T>
+// N elements at any alignment of the element's own.
+template <class T, int N>
+struct Some {
+  T x[N];
+};
+template <class T, int N>
+__device__ __forceinline__ Some<T, N> read(const T* p) {
+  Some<T, N> s;
+  __builtin_memcpy(&s, p, sizeof s);
+  return s;
+}
+
+// A workgroup takes kThreads * N tokens of a row, N neighbours a thread.  How often each
+// is in the text is gathered in LDS from the whole text (integers, so any order gives the
+// same), and of several biases for a token the last one's index.  The logits are on their
+// way meanwhile.
+template <class T, int N>
 __global__ __launch_bounds__(kThreads) void adjust_kernel(Adjust A, const T* logits, long ld,
                                                           T* out, long ld_o) {
-  __shared__ uint32_t s_count[kChunk];
-  __shared__ int s_bias[kChunk];
+  extern __shared__ uint32_t s_count[];
+  constexpr int kChunk = kThreads * N;
+  int* s_bias = reinterpret_cast<int*>(s_count + kChunk);
   const int b = blockIdx.y, tid = threadIdx.x;
-  const long v0 = (long)blockIdx.x * kChunk;
-  for (int i = tid; i < kChunk; i += kThreads) s_count[i] = 0, s_bias[i] = -1;
-  __syncthreads();
-  if (A.text) {
-    long n = A.lens ? A.lens[b] : A.width;
-    n = n < A.width ? n : A.width;
-    const long first = A.first ? A.first[b] : 0;
-    const long* text = A.text + b * A.ld_text;
-    for (long i = tid; i < n; i += kThreads) {
-      const unsigned long at = (unsigned long)(text[i] - v0);
-      if (at >= kChunk) continue;
-      if (i < first) atomicOr(&s_count[at], kSeen);
-      else atomicAdd(&s_count[at], 1u);
-    }
+  const long v0 = (long)blockIdx.x * kChunk, v = v0 + tid * N;
+  const T* src = logits + b * ld + v;
+  T x[N];
+  const bool whole = v + N <= A.V;
+  if (whole) {
+    const Some<T, N> s = read<T, N>(src);
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = s.x[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = v + i < A.V ? src[i] : (T)0.f;
   }
-  for (long i = tid; i < A.n; i += kThreads) {
-    const unsigned long at = (unsigned long)(A.ids[b * A.ld_ids + i] - v0);
-    if (at < kChunk) atomicMax(&s_bias[at], (int)i);
-  }
-  __syncthreads();
+  // (N neighbours' bits lie in one word: v is a multiple of N)
+  const uint32_t word = A.allowed && v < A.V ? A.allowed[b * A.ld_allowed + (v >> 5)] : ~0u;
   const float r = A.rep ? A.rep[b] : A.rep1, pres = A.pres ? A.pres[b] : A.pres1;
   const float freq = A.freq ? A.freq[b] : A.freq1;
-  for (int i = tid; i < kChunk && v0 + i < A.V; i += kThreads) {
-    const long v = v0 + i;
-    float x = (float)logits[b * ld + v];
-    const uint32_t c = s_count[i];
-    if (c) {
-      x = x > 0.f ? x / r : x * r;
-      const uint32_t n = c & ~kSeen;
-      if (n) x = x - freq * (float)n - pres;
+  const bool counts = A.text != nullptr, biases = A.n > 0;
+  if (counts || biases) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      s_count[tid + i * kThreads] = 0;
+      if (biases) s_bias[tid + i * kThreads] = -1;
     }
-    if (s_bias[i] >= 0) x += A.bias[b * A.ld_bias + s_bias[i]];
-    if (A.allowed && !((A.allowed[b * A.ld_allowed + (v >> 5)] >> (v & 31)) & 1))
-      x = -__builtin_inff();
-    out[b * ld_o + v] = (T)x;
+    __syncthreads();
+    if (counts) {
+      long n = A.lens ? A.lens[b] : A.width;
+      n = n < A.width ? n : A.width;
+      const long first = A.first ? A.first[b] : 0;
+      const long* text = A.text + b * A.ld_text;
+      auto count = [&](long token, long i) {
+        const unsigned long at = (unsigned long)(token - v0);
+        if (at >= kChunk) return;
+        if (i < first) atomicOr(&s_count[at], kSeen);
+        else atomicAdd(&s_count[at], 1u);
+      };
+      long i = 2 * tid;
+      for (; i + 6 * kThreads + 1 < n; i += 8 * kThreads) {
+        Some<long, 2> t[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) t[j] = read<long, 2>(text + i + 2 * j * kThreads);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          count(t[j].x[0], i + 2 * j * kThreads);
+          count(t[j].x[1], i + 2 * j * kThreads + 1);
+        }
+      }
+      for (; i < n; i += 2 * kThreads) {
+        count(text[i], i);
+        if (i + 1 < n) count(text[i + 1], i + 1);
+      }
+    }
+    for (long i = tid; i < A.n; i += kThreads) {
+      const unsigned long at = (unsigned long)(A.ids[b * A.ld_ids + i] - v0);
+      if (at < kChunk) atomicMax(&s_bias[at], (int)i);
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float y = (float)x[i];
+    const uint32_t c = counts ? s_count[tid * N + i] : 0u;
+    if (c) {
+      y = y > 0.f ? y / r : y * r;
+      const uint32_t n = c & ~kSeen;
+      if (n) y = y - freq * (float)n - pres;
+    }
+    const int at = biases ? s_bias[tid * N + i] : -1;
+    if (at >= 0) y += A.bias[b * A.ld_bias + at];
+    if (!((word >> ((v + i) & 31)) & 1u)) y = -__builtin_inff();
+    x[i] = (T)y;
+  }
+  T* dst = out + b * ld_o + v;
+  if (whole) {
+    Some<T, N> s;
+#pragma unroll
+    for (int i = 0; i < N; ++i) s.x[i] = x[i];
+    __builtin_memcpy(dst, &s, sizeof s);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (v + i < A.V) dst[i] = x[i];
   }
 }
 
+// As few tokens a thread as give about two workgroups per CU, 8 at most: every workgroup
+// reads the whole text.
 template <class T>
 int adjust(const Adjust& A, const void* logits, long ld, void* out, long ld_o, long B,
            hipStream_t stream) {
-  adjust_kernel<T><<<dim3(hn_cdiv(A.V, kChunk), B), kThreads, 0, stream>>>(
-      A, (const T*)logits, ld, (T*)out, ld_o);
+  const long wgs = B * hn_cdiv(A.V, kThreads), most = 2 * hn_device_cus();
+  auto launch = [&](auto kernel, int n) {
+    kernel<<<dim3(hn_cdiv(A.V, kThreads * n), B), kThreads, kThreads * n * (A.n ? 8 : 4), stream>>>(
+        A, (const T*)logits, ld, (T*)out, ld_o);
+  };
+  if (wgs <= most) launch(adjust_kernel<T, 1>, 1);
+  else if (wgs <= 4 * most) launch(adjust_kernel<T, 4>, 4);
+  else launch(adjust_kernel<T, 8>, 8);
   HN_LAUNCH_CHECK("hn_adjust_logits");
   return 0;
 }

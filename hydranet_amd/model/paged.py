@@ -304,9 +304,7 @@ def paged_append(qkv: torch.Tensor, rope: RotaryTable, batch: PagedBatch, cache:
     if qkv.is_cuda:
         if qkv.stride(1) != 1 or T > 1 and qkv.stride(0) < qkv.shape[1]:
             qkv = qkv.contiguous()
-        # (rows of no sequence are left as they are)
-        make = torch.empty if batch.starts is None else torch.zeros
-        q = make((T, num_heads * hd), dtype=qkv.dtype, device=dev)
+        q = torch.empty((T, num_heads * hd), dtype=qkv.dtype, device=dev)
         _lib.call_on(dev, "hn_paged_append", qkv.data_ptr(), max(qkv.stride(0), qkv.shape[1]),
                      _DTYPES[qkv.dtype], rope.cos.data_ptr(), rope.sin.data_ptr(),
                      rope.cos.shape[0], rope.dim, rope.layout == "interleaved",
@@ -359,8 +357,7 @@ def paged_attention(q: torch.Tensor, batch: PagedBatch, cache: PagedKVCache, lay
     k, v = cache.k[layer], cache.v[layer]
     if q.is_cuda:
         q = _lib.aligned_rows(q)
-        make = torch.empty if batch.starts is None else torch.zeros
-        out = make((T, nh * hd), dtype=q.dtype, device=dev)
+        out = torch.empty((T, nh * hd), dtype=q.dtype, device=dev)
         n = _lib.lib().hn_paged_attention_workspace_bytes(batch.size, T, nh, nkv, hd,
                                                           batch.max_new, batch.kv_bound)
         work = torch.empty(n, dtype=torch.uint8, device=dev) if n else None

@@ -539,8 +539,8 @@ int hn_kv_fork(void* const* kt, void* const* v, long layers, long max_len, long 
  * int64 (device): cached positions C_b before the step, negative for a sequence
  * that takes no part.  Rows starts[b] to starts[b + 1] - 1 of the step's T (starts
  * [B + 1] int32 on the device, not decreasing, from 0; NULL: T = B, row b) are
- * sequence b's tokens at positions C_b on.  Rows of no sequence are left as they
- * are in every output.  Sequences may share pages that neither writes.
+ * sequence b's tokens at positions C_b on.  Rows of no sequence write no page and
+ * are zero in the outputs.  Sequences may share pages that neither writes.
  *
  * hn_paged_append: qkv [T][ld_qkv] (nh query heads, nkv keys, nkv values of hd);
  *   the first `rotary` dimensions of queries and keys are rotated with cos_t /
