@@ -6,6 +6,7 @@
 // sequence b in order.  A sequence with C = lens[b] >= 0 cached positions adds rows
 // starts[b] to starts[b + 1] of the step (one row, b, without starts) at positions C on;
 // a row sees the positions up to its own.
+#include "hn_lds_dma.h"
 #include "hn_paged.h"
 
 namespace {
@@ -334,6 +335,52 @@ __device__ __forceinline__ int grains_below(const Attend<T>& A, int to) {
   return __builtin_amdgcn_readlane(lane_scan(n), 63);
 }
 
+// Of 8 positions from `at` on, the values that must not reach a product: at positions past
+// hi, which no row sees (their probabilities are zero, but what lies there may be
+// anything), and, at those past lo, which only some rows see, NaN and infinities, as 0
+// times them would reach the others.  Returns whether there was such a one.
+template <class T, int E>
+__device__ __forceinline__ uint32_t clean(typename Vec<T>::t (&v)[E], int at, int lo, int hi) {
+  uint32_t odd = 0;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    u32x4 w = __builtin_bit_cast(u32x4, v[e]);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int p = at + 2 * c;
+      w[c] &= (p <= hi ? 0xffffu : 0u) | (p + 1 <= hi ? 0xffff0000u : 0u);
+      const uint32_t m = (p > lo && (w[c] & Vec<T>::inf) == Vec<T>::inf ? 0xffffu : 0u) |
+                         (p + 1 > lo && (w[c] >> 16 & Vec<T>::inf) == Vec<T>::inf ? 0xffff0000u : 0u);
+      odd |= m, w[c] &= ~m;
+    }
+    v[e] = __builtin_bit_cast(typename Vec<T>::t, w);
+  }
+  return odd;
+}
+
+// Those values, added to the rows that see them.  mine(p): whether this wave had position p.
+template <class T, int HD, int NT, class F>
+__device__ __forceinline__ void add_odd(const Attend<T>& A, float4v (&o)[NT][HD / 16],
+                                        const int (&lim)[NT], int b, int g, int lo, int hi, int kg,
+                                        F mine) {
+  const Step& P = A.P;
+  for (int p = lo + 1; p <= hi; ++p) {
+    const long id = mine(p) ? page_of(P, b, p) : -1;
+    if (id < 0) continue;
+    const int slot = p & (P.page - 1);
+    const T* v = A.v + ((id * P.nkv + g) * P.page + (slot & ~7)) * HD + (slot & 7);
+#pragma unroll
+    for (int e = 0; e < HD / 16; ++e)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float x = (float)v[8 * (16 * e + 4 * kg + c)];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+          if (p <= lim[t] && !(__builtin_fabsf(x) < __builtin_inff())) o[t][e][c] += x;
+      }
+  }
+}
+
 // The sums of NT x 16 rows over a wave's positions.
 template <class T, int HD, int NT>
 struct Sums {
@@ -409,6 +456,7 @@ __device__ __forceinline__ void walk(const Attend<T>& A, Sums<T, HD, NT>& W, con
 #pragma unroll
   for (int i = 0; i < 8; ++i) ones[i] = (T)1.f;
 
+  uint32_t odd = 0;
   Ids id = ids(0), next = ids(1);
   keys(0, id.k);
   values(0, id.v);
@@ -443,9 +491,8 @@ __device__ __forceinline__ void walk(const Attend<T>& A, Sums<T, HD, NT>& W, con
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int c = 0; c < 4; ++c) tm = fmaxf(tm, s[t][j][c]);
-      tm = row_max(tm) * scale;
-      if (__any(tm > W.mx[t] + kLag)) {
-        const float nm = fmaxf(W.mx[t], tm);
+      if (__any(tm * scale > W.mx[t] + kLag)) {
+        const float nm = fmaxf(W.mx[t], row_max(tm) * scale);
         const float al = nm == W.mx[t] ? 1.f : __builtin_amdgcn_exp2f(W.mx[t] - nm);
         W.l[t] *= al;
 #pragma unroll
@@ -460,58 +507,8 @@ __device__ __forceinline__ void walk(const Attend<T>& A, Sums<T, HD, NT>& W, con
           p[t][4 * j + c] = (T)__builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j][c], scale, -ref));
       W.l[t] = Vec<T>::mfma(ones, p[t], W.l[t]);
     }
-    bool odd = false;
-    if (edge) {
-      // values at positions that no row sees have probabilities of zero, but may be
-      // anything; those that only some rows see must not reach the others as 0 times
-      // a NaN or infinity
-#pragma unroll
-      for (int e = 0; e < HD / 16; ++e) {
-        u32x4 w = __builtin_bit_cast(u32x4, v[e]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const uint32_t m =
-              (at + 2 * c <= hi ? 0xffffu : 0u) | (at + 2 * c + 1 <= hi ? 0xffff0000u : 0u);
-          w[c] = bad ? 0u : w[c] & m;
-          odd |= (w[c] & Vec<T>::inf) == Vec<T>::inf ||
-                 (w[c] >> 16 & Vec<T>::inf) == Vec<T>::inf;
-        }
-        v[e] = __builtin_bit_cast(V8, w);
-      }
-      odd = lo < hi && __any(odd);
-    }
-    if (odd) {
-      // left out of the product; that a row sees one is counted, of each kind, by products
-      // of ones
-#pragma unroll
-      for (int e = 0; e < HD / 16; ++e) {
-        V8 up, down, nan;
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const float f = (float)v[e][c];
-          up[c] = (T)(f == __builtin_inff() ? 1.f : 0.f);
-          down[c] = (T)(f == -__builtin_inff() ? 1.f : 0.f);
-          nan[c] = (T)(f != f ? 1.f : 0.f);
-          if (!(__builtin_fabsf(f) < __builtin_inff())) v[e][c] = (T)0.f;
-        }
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          V8 see;
-#pragma unroll
-          for (int c = 0; c < 8; ++c) see[c] = (T)(at + c > lim[t] ? 0.f : 1.f);
-          const float4v z = (float4v)(0.f);
-          const float4v cu = Vec<T>::mfma(up, see, z), cd = Vec<T>::mfma(down, see, z);
-          const float4v cn = Vec<T>::mfma(nan, see, z);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            float y = cu[c] > 0.f ? __builtin_inff() : 0.f;
-            if (cd[c] > 0.f) y -= __builtin_inff();
-            if (cn[c] > 0.f) y = __builtin_nanf("");
-            W.o[t][e][c] += y;
-          }
-        }
-      }
-    }
+    // (values on no page were read from another one: no row gets a number that it sees)
+    if (edge) odd |= clean<T>(v, bad ? hi + 1 : at, lo, hi);
 #pragma unroll
     for (int e = 0; e < HD / 16; ++e)
 #pragma unroll
@@ -519,6 +516,10 @@ __device__ __forceinline__ void walk(const Attend<T>& A, Sums<T, HD, NT>& W, con
     values(i + 1, next.v);
     id = next, next = after;
   }
+  if (lo < hi && __any(odd))
+    add_odd<T, HD, NT>(A, W.o, lim, b, g, lo, hi, kg, [&](int p) {
+      return p >= first && p < first + kTile * tiles && (p - first) / kTile % NW == wave;
+    });
 }
 
 // The waves' sums of 16 rows joined, then the rows themselves, or the range's entry of
@@ -572,6 +573,226 @@ __device__ __forceinline__ void finish(const Attend<T>& A, const Sums<T, HD, NT>
         float* pm = A.part + 2 * (long)A.wgs * A.R * HD + at * 2;
         if (d == 0) pm[0] = m, pm[1] = sum;
       }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Runs of many rows.  A workgroup of 4 waves takes 128 rows of one (sequence, KV head), 32
+// a wave, and walks the positions in stages of 64 that all four read from LDS; the next
+// stage goes from memory to LDS (buffer_load ... lds) meanwhile.  A stage lies there as
+// in the pages, but that a key's 16-byte chunks are at chunk ^ key(position), so that the
+// 16 positions that a read takes cover the banks once.  Two workgroups per CU: one's
+// loads and softmax under the other's products.
+constexpr int kStage = 64, kBlock = 128;
+
+template <class T, int HD>
+__global__ __launch_bounds__(256, 2) void block_kernel(Attend<T> A) {
+  typedef typename Vec<T>::t V8;
+  constexpr int NT = 2, kChunks = HD / 8;            // 16-byte chunks of a key
+  constexpr int kBytes = kStage * HD * 2;            // of a stage's keys, and of its values
+  constexpr int kPos = 64 / kChunks;                 // keys per DMA instruction
+  constexpr int kDma = kBytes / 1024 / 4;            // instructions per wave and operand
+  __shared__ __align__(1024) unsigned char s_buf[4 * kBytes];
+  const Step& P = A.P;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+  const int n = lane & 15, kg = lane >> 4;
+  const int g = blockIdx.x, b = blockIdx.z, part = gridDim.y - 1 - blockIdx.y;
+  const Run r = run_of(A, b);
+  if (b == 0) fill_rest<T, HD>(A, g, part, gridDim.y);
+  if (r.none || r.nan) return fill<T, HD>(A, r, g, part, gridDim.y);
+  const int rows = A.rep * r.n;
+  if (part * kBlock >= rows) return;
+  const int row0 = part * kBlock + 32 * wave;
+  const bool busy = row0 < rows;
+
+  V8 q[NT][HD / 32];
+  int lim[NT];
+  // positions that all of this wave's rows see, none sees, and none of the workgroup's
+  const int lo = r.C + row0 / A.rep;
+  const int hi = min(r.C + min((row0 + 31) / A.rep, r.n - 1), r.L - 1);
+  const int top = min(r.C + min((part * kBlock + kBlock - 1) / A.rep, r.n - 1), r.L - 1);
+  float4v o[NT][HD / 16], l[NT];
+  float mx[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int row = row0 + 16 * t + n, tok = row / A.rep, head = row - tok * A.rep;
+    const bool in = row < rows;
+    const T* src = A.q + (long)(r.row + tok) * A.ld_q + (long)(g * A.rep + head) * HD + 8 * kg;
+#pragma unroll
+    for (int u = 0; u < HD / 32; ++u) {
+      u32x4 w = {0, 0, 0, 0};
+      if (in) w = *reinterpret_cast<const u32x4*>(src + 32 * u);
+      q[t][u] = __builtin_bit_cast(V8, w);
+    }
+    lim[t] = in ? r.C + tok : lo;
+    mx[t] = -__builtin_inff();
+    l[t] = (float4v)(0.f);
+#pragma unroll
+    for (int e = 0; e < HD / 16; ++e) o[t][e] = (float4v)(0.f);
+  }
+
+  const int shift = __builtin_ctz(P.page), stages = top / kStage + 1;
+  // The pages of a stage's positions by sixteens (-1: none): scalars, read ahead through
+  // the scalar cache, so that no wait for them is one for the stage on its way.
+  typedef const __attribute__((address_space(4))) int* Table;
+  const Table table = (Table)(uintptr_t)(P.table + (long)b * P.ld);
+  struct Ids {
+    int id[kStage / 16];
+  };
+  auto pages = [&](int st) {
+    Ids x;
+#pragma unroll
+    for (int i = 0; i < kStage / 16; ++i) {
+      const int col = (st * kStage + 16 * i) >> shift;
+      const int id = col < P.cols ? table[col] : -1;
+      x.id[i] = id >= 0 && id < P.pages ? id : -1;
+    }
+    return x;
+  };
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)s_buf;
+  // DMA: instruction i of wave w moves KB w + 4 i of a stage's keys and of its values.  A
+  // page that is not there reads as zero (a descriptor of no bytes).
+  const int head_bytes = P.page * HD * 2;
+  auto issue = [&](int st, const Ids& x) {
+    auto page = [&](int i) { return i == 0 ? x.id[0] : i == 1 ? x.id[1] : i == 2 ? x.id[2] : x.id[3]; };
+    const uint32_t at = lds0 + (uint32_t)(st & 1) * 2 * kBytes + wave * 1024;
+    const int p0 = st * kStage;
+    auto where = [&](const T* x, int id) {
+      return rsrc(x + ((long)max(id, 0) * P.nkv + g) * P.page * HD, id < 0 ? 0 : head_bytes);
+    };
+#pragma unroll
+    for (int i = 0; i < kDma; ++i) {
+      const int kp = kPos * (wave + 4 * i), pos = kp + lane / kChunks;  // within the stage
+      const int m = ((pos >> 3) & 3) * 4 + (pos & 3), key = kChunks == 16 ? m : m >> 1;
+      const int id = page(kp >> 4);
+      dma_b128(where(A.k, id), (lane / kChunks) * HD * 2 + 16 * ((lane % kChunks) ^ key),
+               (uint32_t)((p0 + kp) & (P.page - 1)) * HD * 2, at + i * 4096);
+    }
+#pragma unroll
+    for (int i = 0; i < kDma; ++i) {
+      // KB j of the values: 512 / HD positions' worth, in slots of 8
+      const int j = wave + 4 * i, vp = j * 512 / HD & ~7;
+      const int id = page(vp >> 4);
+      dma_b128(where(A.v, id), 16 * lane,
+               (uint32_t)((p0 + vp) & (P.page - 1)) * HD * 2 + (j * 1024) % (16 * HD),
+               at + kBytes + i * 4096);
+    }
+  };
+
+  // this lane's part of the reads
+  uint32_t k_at[HD / 32];
+  const int mine = kChunks == 16 ? n : n >> 1;
+#pragma unroll
+  for (int u = 0; u < HD / 32; ++u)
+    k_at[u] = lds0 + (8 * (n >> 2) + (n & 3)) * HD * 2 + 16 * ((4 * u + kg) ^ mine);
+  const uint32_t v_at = lds0 + kBytes + kg * HD * 16 + n * 16;
+  const float scale = A.scale * kLog2e;
+  V8 ones;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) ones[i] = (T)1.f;
+
+  uint32_t odd = 0;
+  auto compute = [&](bool edge, int st, uint32_t bad) __attribute__((always_inline)) {
+    const uint32_t at = (uint32_t)(st & 1) * 2 * kBytes;
+    const int p0 = st * kStage;
+    V8 p[NT][2];
+    float4v s[NT][4];  // block 2 h + j of half h
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      V8 k[HD / 32];
+#pragma unroll
+      for (int u = 0; u < HD / 32; ++u)
+        k[u] = lds_read<V8>(k_at[u] + at + (32 * (x >> 1) + 4 * (x & 1)) * HD * 2);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        s[t][x] = (float4v)(0.f);
+#pragma unroll
+        for (int u = 0; u < HD / 32; ++u) s[t][x] = Vec<T>::mfma(k[u], q[t][u], s[t][x]);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      if (edge) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const bool none = bad >> (2 * (x >> 1) + (kg >> 1)) & 1;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            if (none) s[t][x][c] = __builtin_nanf("");
+            if (p0 + 32 * (x >> 1) + 8 * kg + 4 * (x & 1) + c > lim[t])
+              s[t][x][c] = -__builtin_inff();
+          }
+        }
+      }
+      float tm = s[t][0][0];
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tm = fmaxf(tm, s[t][x][c]);
+      if (__any(tm * scale > mx[t] + kLag)) {
+        const float nm = fmaxf(mx[t], row_max(tm) * scale);
+        const float al = nm == mx[t] ? 1.f : __builtin_amdgcn_exp2f(mx[t] - nm);
+        l[t] *= al;
+#pragma unroll
+        for (int e = 0; e < HD / 16; ++e) o[t][e] *= al;
+        mx[t] = nm;
+      }
+      const float ref = mx[t] == -__builtin_inff() ? 0.f : mx[t] - kUp;
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          p[t][x >> 1][4 * (x & 1) + c] =
+              (T)__builtin_amdgcn_exp2f(__builtin_fmaf(s[t][x][c], scale, -ref));
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) l[t] = Vec<T>::mfma(ones, p[t][h], l[t]);
+#pragma unroll
+      for (int e0 = 0; e0 < HD / 16; e0 += 4) {
+        V8 v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = lds_read<V8>(v_at + at + h * HD * 64 + (e0 + e) * 256);
+        if (edge) odd |= clean<T>(v, p0 + 32 * h + 8 * kg, lo, hi);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+#pragma unroll
+          for (int t = 0; t < NT; ++t) o[t][e0 + e] = Vec<T>::mfma(v[e], p[t][h], o[t][e0 + e]);
+      }
+    }
+  };
+
+  Ids id = pages(0), next = pages(1);
+  issue(0, id);
+  for (int st = 0; st < stages; ++st) {
+    wait_vmcnt<0>();  // this wave's part of the stage has landed
+    stage_barrier();  // everyone's, and the stage before is used
+    if (st + 1 < stages) issue(st + 1, next);
+    uint32_t bad = 0;
+#pragma unroll
+    for (int i = 0; i < kStage / 16; ++i) bad |= id.id[i] < 0 ? 1u << i : 0u;
+    id = next, next = pages(st + 2);
+    if (!busy || st * kStage > hi) continue;
+    compute(st * kStage + kStage - 1 > lo || bad, st, bad);
+  }
+  if (!busy) return;
+  if (__any(odd))
+    add_odd<T, HD, NT>(A, o, lim, b, g, lo, hi, kg, [](int) { return true; });
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int row = row0 + 16 * t + n, tok = row / A.rep, head = row - tok * A.rep;
+    if (row >= rows) continue;
+    const float is = 1.f / l[t][0];
+    T* dst = A.out + (long)(r.row + tok) * A.ld_o + (long)(g * A.rep + head) * HD + 4 * kg;
+#pragma unroll
+    for (int e = 0; e < HD / 16; ++e) {
+      typedef T V4 __attribute__((ext_vector_type(4)));
+      V4 y;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) y[c] = (T)(o[t][e][c] * is);
+      *reinterpret_cast<V4*>(dst + 16 * e) = y;
     }
   }
 }
@@ -803,6 +1024,12 @@ int attend_rows(const Attend<T>& A, int B, int nkv, hipStream_t stream) {
 
 template <class T, int HD>
 int attend_hd(const Attend<T>& A, int B, int nkv, hipStream_t stream) {
+  if constexpr (HD != 256)
+    if (A.R > kShareRows) {
+      block_kernel<T, HD><<<dim3(nkv, hn_cdiv(A.R, kBlock), B), 256, 0, stream>>>(A);
+      HN_LAUNCH_CHECK("hn_paged_attention");
+      return 0;
+    }
   if (A.R <= 16) return attend_rows<T, HD, 1>(A, B, nkv, stream);
   return attend_rows<T, HD, HD == 256 ? 1 : 2>(A, B, nkv, stream);
 }
