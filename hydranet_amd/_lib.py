@@ -57,10 +57,9 @@ SIGNATURES: dict[str, list] = {
     "hn_verify_tree": [P, L, L, P, L, L, I, P, P, L, P, P, F, L, L, L, P, P, P, P, L, P],
     "hn_kv_keep": [P, P, L, L, L, L, L, P, P, L, P, L, P, P],
     "hn_kv_fork": [P, P, L, L, L, L, L, P, P, L, L, P],
-    "hn_paged_append": [P, L, I, P, P, L, L, I, P, L, L, L, P, P, L, L, L, L, L, L, P, P, P, P],
-    "hn_paged_attention_workspace_bytes": [L, L, L, L, L, L, L],
-    "hn_paged_attention": [P, L, I, P, P, P, L, L, L, P, P, L, L, L, L, L, L, L, L, F, P, L, P, L,
-                           P],
+    "hn_paged_append": [P, P, L, I, P, P, L, L, I, P, P, P, P],
+    "hn_paged_attention_workspace_bytes": [P],
+    "hn_paged_attention": [P, P, L, I, P, P, F, P, L, P, L, P],
     "hn_page_copy": [P, P, L, L, L, P, P, L, P],
     "hn_adjust_logits": [P, L, I, P, L, L, P, P, P, P, P, F, F, F, P, L, P, L, L, P, L, L, L, P,
                          L, P],
@@ -83,6 +82,13 @@ SIGNATURES: dict[str, list] = {
     "hn_moe_route_experts_decode": [P, P, L, L, L, I, F, F, P, L, P, L, L, L, P, P, P, P, P, P,
                                     P, P, P, P, P, P, L, P, L, P, L, P],
 }
+
+class PagedStep(ctypes.Structure):
+    """hn_paged_step of include/hn_int4.h."""
+    _fields_ = [("table", P), ("ld_table", L), ("cols", L), ("num_pages", L), ("lens", P),
+                ("starts", P)] + [(n, L) for n in ("B", "T", "nh", "nkv", "hd", "page", "max_new",
+                                                   "bound")]
+
 
 # Sizes up to which hn_moe_route (one launch: logits, top-k, permutation,
 # gather) applies; larger batches use the separate kernels.

@@ -6,6 +6,7 @@
 // sequence b in order.  A sequence with C = lens[b] >= 0 cached positions adds rows
 // starts[b] to starts[b + 1] of the step (one row, b, without starts) at positions C on;
 // a row sees the positions up to its own.
+#include "../../include/hn_int4.h"
 #include "hn_lds_dma.h"
 #include "hn_paged.h"
 
@@ -934,27 +935,25 @@ bool fits(long hd, long page) {
          (page & (page - 1)) == 0;
 }
 
-int check_step(const char* who, const Step& P, const void* qkv, const void* k, const void* v,
-               long nh, long hd, long T, int dtype) {
+// Checks a step, and fills what the kernels take of it.
+int check_step(const char* who, const hn_paged_step* s, const void* x, const void* k,
+               const void* v, int dtype, Step& P) {
+  HN_ARG_CHECK(s, "%s: null step", who);
   HN_ARG_CHECK(dtype == 0 || dtype == 1, "%s: dtype %d (0 fp16, 1 bf16)", who, dtype);
-  HN_ARG_CHECK(P.nkv > 0 && nh > 0 && nh % P.nkv == 0 && nh < 1 << 16,
-               "%s: %ld heads over %d KV heads", who, nh, P.nkv);
-  HN_ARG_CHECK(fits(hd, P.page), "%s: heads of 64, 128 or 256 (got %ld), pages of 16 to 1024 "
-               "positions, a power of two (got %d)", who, hd, P.page);
-  HN_ARG_CHECK(P.B >= 0 && T >= 0 && T < 1 << 30 && P.pages >= 0 && P.cols >= 0 &&
-                   P.ld >= P.cols && (P.starts || T == P.B),
-               "%s: %d sequences, %ld rows, %ld pages, a table of %ld columns (row %ld)", who, P.B,
-               T, P.pages, P.cols, P.ld);
-  if (P.B == 0 || T == 0) return 0;
-  HN_ARG_CHECK(qkv && k && v && (P.cols == 0 || P.table) && P.lens, "%s: null operand", who);
-  HN_ARG_CHECK((uintptr_t)k % 16 == 0 && (uintptr_t)v % 16 == 0, "%s: pages not 16-byte aligned",
-               who);
+  HN_ARG_CHECK(s->nkv > 0 && s->nh > 0 && s->nh % s->nkv == 0 && s->nh < 1 << 16,
+               "%s: %ld heads over %ld KV heads", who, s->nh, s->nkv);
+  HN_ARG_CHECK(fits(s->hd, s->page), "%s: heads of 64, 128 or 256 (got %ld), pages of 16 to 1024 "
+               "positions, a power of two (got %ld)", who, s->hd, s->page);
+  HN_ARG_CHECK(s->B >= 0 && s->B < 65536 && s->T >= 0 && s->T < 1 << 30 && s->num_pages >= 0 &&
+                   s->cols >= 0 && s->ld_table >= s->cols && (s->starts || s->T == s->B),
+               "%s: %ld sequences, %ld rows, %ld pages, a table of %ld columns (row %ld)", who,
+               s->B, s->T, s->num_pages, s->cols, s->ld_table);
+  P = Step{s->table, s->ld_table, s->cols, s->num_pages, s->lens, s->starts, (int)s->B, (int)s->T,
+           (int)s->nkv, (int)s->page};
+  if (s->B == 0 || s->T == 0) return 0;
+  HN_ARG_CHECK(x && k && v && (s->cols == 0 || s->table) && s->lens, "%s: null operand", who);
+  HN_ARG_CHECK(((uintptr_t)k | (uintptr_t)v) % 16 == 0, "%s: pages not 16-byte aligned", who);
   return 0;
-}
-
-Step step_of(const int* table, long ld_table, long cols, long num_pages, const long* lens,
-             const int* starts, long B, long T, long nkv, long page) {
-  return Step{table, ld_table, cols, num_pages, lens, starts, (int)B, (int)T, (int)nkv, (int)page};
 }
 
 // Rows from which a thread takes four heads of a token, so that it reads the angles once.
@@ -1048,59 +1047,56 @@ int attend(const Step& P, const void* q, long ld_q, const void* k, const void* v
 
 }  // namespace
 
-extern "C" int hn_paged_append(const void* qkv, long ld_qkv, int dtype, const float* cos_t,
-                               const float* sin_t, long table_rows, long rotary, int interleaved,
-                               const int* table, long ld_table, long cols, long num_pages,
-                               const long* lens, const int* starts, long B, long T, long nh,
-                               long nkv, long hd, long page, void* q_out, void* k, void* v,
+extern "C" int hn_paged_append(const hn_paged_step* step, const void* qkv, long ld_qkv, int dtype,
+                               const float* cos_t, const float* sin_t, long table_rows,
+                               long rotary, int interleaved, void* q_out, void* k, void* v,
                                void* stream) {
-  const Step P = step_of(table, ld_table, cols, num_pages, lens, starts, B, T, nkv, page);
-  if (int rc = check_step("hn_paged_append", P, qkv, k, v, nh, hd, T, dtype)) return rc;
+  Step P;
+  if (int rc = check_step("hn_paged_append", step, qkv, k, v, dtype, P)) return rc;
+  const long nh = step->nh, hd = step->hd, heads = nh + 2 * step->nkv;
   HN_ARG_CHECK(rotary >= 0 && rotary <= hd && rotary % 2 == 0 && table_rows >= 0,
                "hn_paged_append: %ld rotated dimensions of %ld, %ld positions", rotary, hd,
                table_rows);
-  HN_ARG_CHECK(nh + 2 * nkv < 65536 && T * (nh + 2 * nkv) < 1l << 31,
-               "hn_paged_append: %ld rows of %ld heads", T, nh + 2 * nkv);
-  if (B == 0 || T == 0) return 0;
+  HN_ARG_CHECK(heads < 65536 && P.T * heads < 1l << 31, "hn_paged_append: %d rows of %ld heads",
+               P.T, heads);
+  if (P.B == 0 || P.T == 0) return 0;
   HN_ARG_CHECK(q_out && (rotary == 0 || (cos_t && sin_t)), "hn_paged_append: null operand");
-  HN_ARG_CHECK(ld_qkv >= (nh + 2 * nkv) * hd, "hn_paged_append: rows of %ld, a stride of %ld",
-               (nh + 2 * nkv) * hd, ld_qkv);
+  HN_ARG_CHECK(ld_qkv >= heads * hd, "hn_paged_append: rows of %ld, a stride of %ld", heads * hd,
+               ld_qkv);
   return (dtype == 0 ? append<h16> : append<b16>)(P, qkv, ld_qkv, cos_t, sin_t, table_rows,
                                                   (int)rotary, interleaved, (int)nh, (int)hd,
                                                   q_out, k, v, (hipStream_t)stream);
 }
 
-extern "C" long hn_paged_attention_workspace_bytes(long B, long T, long nh, long nkv, long hd,
-                                                   long max_new, long bound) {
-  if (B <= 0 || T <= 0 || nkv <= 0 || nh < nkv || hd <= 0 || max_new <= 0) return 0;
-  const long rows = nh / nkv * max_new;
-  return part_bytes(share_wgs(rows, hd, bound), rows, hd);
+extern "C" long hn_paged_attention_workspace_bytes(const hn_paged_step* s) {
+  if (!s || s->B <= 0 || s->T <= 0 || s->nkv <= 0 || s->nh < s->nkv || s->hd <= 0 ||
+      s->max_new <= 0)
+    return 0;
+  const long rows = s->nh / s->nkv * s->max_new;
+  return part_bytes(share_wgs(rows, s->hd, s->bound), rows, s->hd);
 }
 
-extern "C" int hn_paged_attention(const void* q, long ld_q, int dtype, const void* k,
-                                  const void* v, const int* table, long ld_table, long cols,
-                                  long num_pages, const long* lens, const int* starts, long B,
-                                  long T, long nh, long nkv, long hd, long page, long max_new,
-                                  long bound, float scale, void* out, long ld_o, void* work,
-                                  long work_bytes, void* stream) {
-  const Step P = step_of(table, ld_table, cols, num_pages, lens, starts, B, T, nkv, page);
-  if (int rc = check_step("hn_paged_attention", P, q, k, v, nh, hd, T, dtype)) return rc;
-  HN_ARG_CHECK(max_new >= 1 && bound >= 1 && max_new <= (1l << 24) / nh,
-               "hn_paged_attention: max_new %ld, bound %ld", max_new, bound);
-  HN_ARG_CHECK(B < 65536 && nkv < 65536 &&
-                   (cols < 1l << 26 && cols * page < 1l << 30) &&
-                   (double)B * nkv * (cols * page / kGrain + 1) < 2147483648.0,
-               "hn_paged_attention: %ld sequences of %ld pages", B, cols);
+extern "C" int hn_paged_attention(const hn_paged_step* step, const void* q, long ld_q, int dtype,
+                                  const void* k, const void* v, float scale, void* out, long ld_o,
+                                  void* work, long work_bytes, void* stream) {
+  Step P;
+  if (int rc = check_step("hn_paged_attention", step, q, k, v, dtype, P)) return rc;
+  const long nh = step->nh, nkv = step->nkv, hd = step->hd, max_new = step->max_new;
+  HN_ARG_CHECK(max_new >= 1 && step->bound >= 1 && max_new <= (1l << 24) / nh,
+               "hn_paged_attention: max_new %ld, bound %ld", max_new, step->bound);
+  HN_ARG_CHECK(P.cols < 1l << 26 && P.cols * P.page < 1l << 30 &&
+                   (double)P.B * nkv * (P.cols * P.page / kGrain + 1) < 2147483648.0,
+               "hn_paged_attention: %d sequences of %ld pages", P.B, P.cols);
   HN_ARG_CHECK(scale > 0.f && scale * 1.4426950408889634f < __builtin_inff(),
                "hn_paged_attention: scale %g", (double)scale);
-  if (B == 0 || T == 0) return 0;
-  HN_ARG_CHECK(num_pages >= 1, "hn_paged_attention: no pages");
+  if (P.B == 0 || P.T == 0) return 0;
+  HN_ARG_CHECK(P.pages >= 1, "hn_paged_attention: no pages");
   HN_ARG_CHECK(out && ld_q >= nh * hd && ld_o >= nh * hd && ld_q % 8 == 0 && ld_o % 8 == 0 &&
-                   (uintptr_t)q % 16 == 0 && (uintptr_t)out % 16 == 0,
+                   ((uintptr_t)q | (uintptr_t)out) % 16 == 0,
                "hn_paged_attention: rows of %ld, strides of %ld and %ld: 16-byte aligned rows",
                nh * hd, ld_q, ld_o);
   const long rows = nh / nkv * max_new;
-  const int wgs = share_wgs(rows, hd, bound);
+  const int wgs = share_wgs(rows, hd, step->bound);
   HN_ARG_CHECK(wgs == 0 || (work && (uintptr_t)work % 16 == 0 &&
                             work_bytes >= part_bytes(wgs, rows, hd)),
                "hn_paged_attention: a workspace of %ld bytes, %ld given",

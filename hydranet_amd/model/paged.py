@@ -22,7 +22,6 @@ import ctypes
 import math
 from typing import Dict, List, Optional, Sequence
 
-import numpy as np
 import torch
 
 from .. import _lib
@@ -208,7 +207,13 @@ class RotaryTable:
         assert cos.dim() == 2 and cos.shape == sin.shape and cos.device == sin.device \
             and cos.dtype == sin.dtype == torch.float32, "cos, sin: fp32 [positions, dim / 2]"
         self.cos, self.sin, self.layout = cos.contiguous(), sin.contiguous(), layout
-        self.dim = 2 * cos.shape[1]
+        self.dim, self.device = 2 * cos.shape[1], cos.device
+
+    @property
+    def args(self):
+        """The angles' arguments of a library call."""
+        return (self.cos.data_ptr(), self.sin.data_ptr(), self.cos.shape[0], self.dim,
+                self.layout == "interleaved")
 
 
 class PagedBatch:
@@ -245,13 +250,32 @@ class PagedBatch:
         self.table, self.lens, self.starts = table, lens, starts
         self.size, self.rows, self.max_new, self.kv_bound = B, rows, max_new, kv_bound
         self.device = dev
+        self._made = None
 
-    def _args(self, cache: PagedKVCache):
-        """The batch's arguments of a library call."""
+    def _step(self, cache: PagedKVCache, num_heads: int):
+        """(the C struct of this step over a cache, its address, the attention's workspace),
+        made once for all layers."""
+        old = self._made
+        if old is not None and old[0] is cache and old[1] == num_heads:
+            return old[2]
+        nkv, hd = cache.kv_heads, cache.head_dim
+        assert num_heads > 0 and num_heads % nkv == 0, f"{num_heads} heads over {nkv} KV heads"
+        assert hd in (64, 128, 256), f"heads of 64, 128 or 256 (got {hd})"
+        assert self.device == cache.k[0].device, \
+            f"the batch on {self.device}, the cache on {cache.k[0].device}"
         t = self.table
-        return (t.data_ptr(), max(t.stride(0), t.shape[1]), t.shape[1], cache.num_pages,
-                self.lens.data_ptr(), None if self.starts is None else self.starts.data_ptr(),
-                self.size, self.rows)
+        s = _lib.PagedStep(t.data_ptr(), max(t.stride(0), t.shape[1]), t.shape[1],
+                           cache.num_pages, self.lens.data_ptr(),
+                           None if self.starts is None else self.starts.data_ptr(), self.size,
+                           self.rows, num_heads, nkv, hd, cache.page_size, self.max_new,
+                           self.kv_bound)
+        at = ctypes.addressof(s)
+        made = (s, at, _lib.lib().hn_paged_attention_workspace_bytes(at))
+        self._made = (cache, num_heads, made)
+        return made
+
+    def __getstate__(self):  # (a copy's tensors are elsewhere)
+        return dict(self.__dict__, _made=None)
 
     def _runs(self):
         """On the CPU: (sequence, first row, rows, cached positions) of each run."""
@@ -271,19 +295,17 @@ class PagedBatch:
         return ids
 
 
-def _check(batch: PagedBatch, cache: PagedKVCache, layer: int, x: torch.Tensor, num_heads: int,
-           columns: int, name: str) -> None:
+def _check(batch: PagedBatch, cache: PagedKVCache, layer: int, x: torch.Tensor,
+           columns: int, name: str) -> torch.Tensor:
+    """The layer's keys, if the call's tensors fit."""
     assert 0 <= layer < len(cache.k), f"layer {layer} of {len(cache.k)}"
-    nkv, hd = cache.kv_heads, cache.head_dim
-    assert num_heads > 0 and num_heads % nkv == 0, f"{num_heads} heads over {nkv} KV heads"
-    assert tuple(x.shape) == (batch.rows, columns), \
+    k = cache.k[layer]
+    assert x.shape == (batch.rows, columns), \
         f"{name} {tuple(x.shape)} vs {batch.rows} rows of {columns}"
-    assert x.device == batch.device == cache.k[layer].device, \
-        f"{name} on {x.device}, the batch on {batch.device}, the cache on {cache.k[layer].device}"
-    assert x.dtype == cache.k[layer].dtype, f"{name} {x.dtype}, the cache {cache.k[layer].dtype}"
-    if x.is_cuda:
-        assert x.dtype in _DTYPES and hd in (64, 128, 256), \
-            f"fp16 or bf16 heads of 64, 128 or 256 (got {x.dtype}, {hd})"
+    assert x.device == batch.device == k.device, \
+        f"{name} on {x.device}, the batch on {batch.device}, the cache on {k.device}"
+    assert x.dtype == k.dtype, f"{name} {x.dtype}, the cache {k.dtype}"
+    return k
 
 
 def paged_append(qkv: torch.Tensor, rope: RotaryTable, batch: PagedBatch, cache: PagedKVCache,
@@ -295,20 +317,20 @@ def paged_append(qkv: torch.Tensor, rope: RotaryTable, batch: PagedBatch, cache:
     hd].  fp32 products, rounded once.  Rows of a sequence that takes no part write no
     page and have zero queries, rows of no sequence too; a row past the table of angles,
     or whose page is not named, writes no page and has NaN queries."""
-    nkv, hd = cache.kv_heads, cache.head_dim
-    _check(batch, cache, layer, qkv, num_heads, (num_heads + 2 * nkv) * hd, "qkv")
-    assert rope.cos.device == qkv.device and rope.dim <= hd, \
-        f"{rope.dim} rotated dimensions of {hd}, the angles on {rope.cos.device}"
-    T, dev = batch.rows, qkv.device
-    k, v = cache.k[layer], cache.v[layer]
+    nkv, hd, T = cache.kv_heads, cache.head_dim, batch.rows
+    assert num_heads > 0 and num_heads % nkv == 0, f"{num_heads} heads over {nkv} KV heads"
+    columns = (num_heads + 2 * nkv) * hd
+    k, v = _check(batch, cache, layer, qkv, columns, "qkv"), cache.v[layer]
+    assert rope.device == qkv.device and rope.dim <= hd, \
+        f"{rope.dim} rotated dimensions of {hd}, the angles on {rope.device}"
     if qkv.is_cuda:
-        if qkv.stride(1) != 1 or T > 1 and qkv.stride(0) < qkv.shape[1]:
-            qkv = qkv.contiguous()
-        q = torch.empty((T, num_heads * hd), dtype=qkv.dtype, device=dev)
-        _lib.call_on(dev, "hn_paged_append", qkv.data_ptr(), max(qkv.stride(0), qkv.shape[1]),
-                     _DTYPES[qkv.dtype], rope.cos.data_ptr(), rope.sin.data_ptr(),
-                     rope.cos.shape[0], rope.dim, rope.layout == "interleaved",
-                     *batch._args(cache), num_heads, nkv, hd, cache.page_size, q.data_ptr(),
+        assert qkv.dtype in _DTYPES, f"fp16 or bf16 rows (got {qkv.dtype})"
+        ld, last = qkv.stride()
+        if last != 1 or ld < columns:
+            qkv, ld = qkv.contiguous(), columns
+        q = qkv.new_empty((T, num_heads * hd))
+        _lib.call_on(qkv.device, "hn_paged_append", batch._step(cache, num_heads)[1],
+                     qkv.data_ptr(), ld, _DTYPES[qkv.dtype], *rope.args, q.data_ptr(),
                      k.data_ptr(), v.data_ptr())
         return q
     wide = torch.float64 if qkv.dtype == torch.float64 else torch.float32
@@ -347,24 +369,25 @@ def paged_attention(q: torch.Tensor, batch: PagedBatch, cache: PagedKVCache, lay
     scale: of the scores, 1 / sqrt(hd) by default.  Rows of a sequence that takes no
     part and of no sequence are zero; a row that sees a position whose page is not named
     is NaN, and so are the rows of a run of more than the batch's max_new."""
-    nkv, hd = cache.kv_heads, cache.head_dim
-    assert q.dim() == 2 and hd > 0 and q.shape[1] % hd == 0, f"q [rows, heads * {hd}]"
-    nh = q.shape[1] // hd
-    _check(batch, cache, layer, q, nh, nh * hd, "q")
-    scale = float(np.float32(1.0) / np.float32(math.sqrt(hd))) if scale is None else float(scale)
+    nkv, hd, T = cache.kv_heads, cache.head_dim, batch.rows
+    assert q.dim() == 2 and q.shape[1] % hd == 0, f"q [rows, heads * {hd}]"
+    columns = q.shape[1]
+    nh = columns // hd
+    assert nh > 0 and nh % nkv == 0, f"{nh} heads over {nkv} KV heads"
+    k, v = _check(batch, cache, layer, q, columns, "q"), cache.v[layer]
+    scale = 1.0 / math.sqrt(hd) if scale is None else float(scale)
     assert 0.0 < scale < 2e38, f"scale {scale}"
-    T, dev = batch.rows, q.device
-    k, v = cache.k[layer], cache.v[layer]
     if q.is_cuda:
-        q = _lib.aligned_rows(q)
-        out = torch.empty((T, nh * hd), dtype=q.dtype, device=dev)
-        n = _lib.lib().hn_paged_attention_workspace_bytes(batch.size, T, nh, nkv, hd,
-                                                          batch.max_new, batch.kv_bound)
-        work = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-        _lib.call_on(dev, "hn_paged_attention", q.data_ptr(), max(q.stride(0), nh * hd),
-                     _DTYPES[q.dtype], k.data_ptr(), v.data_ptr(), *batch._args(cache), nh, nkv,
-                     hd, cache.page_size, batch.max_new, batch.kv_bound, scale, out.data_ptr(),
-                     nh * hd, None if work is None else work.data_ptr(), n)
+        assert q.dtype in _DTYPES, f"fp16 or bf16 rows (got {q.dtype})"
+        ld, last = q.stride()
+        if last != 1 or ld % 8 or ld < columns or q.data_ptr() % 16:
+            q, ld = _lib.aligned_rows(q.contiguous()), columns
+        out = q.new_empty((T, columns))
+        _, step, n = batch._step(cache, nh)
+        work = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+        _lib.call_on(q.device, "hn_paged_attention", step, q.data_ptr(), ld, _DTYPES[q.dtype],
+                     k.data_ptr(), v.data_ptr(), scale, out.data_ptr(), columns,
+                     None if work is None else work.data_ptr(), n)
         return out
     wide = torch.float64 if q.dtype == torch.float64 else torch.float32
     out = torch.zeros((T, nkv, nh // nkv, hd), dtype=q.dtype)

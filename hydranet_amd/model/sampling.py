@@ -15,14 +15,13 @@ from .. import _lib
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 
 
-def _rows(x: torch.Tensor) -> torch.Tensor:
-    """x with its last axis dense and rows that do not overlap."""
-    return x if x.stride(1) == 1 and (x.shape[0] == 1 or x.stride(0) >= x.shape[1]) \
-        else x.contiguous()
-
-
-def _ld(x: torch.Tensor) -> int:
-    return max(x.stride(0), x.shape[1])
+def _rows(x: torch.Tensor):
+    """x with its last axis dense and rows that do not overlap, and their stride."""
+    ld, last = x.stride()
+    if last != 1 or ld < x.shape[1]:
+        x = x.contiguous()
+        ld = x.shape[1]
+    return x, ld
 
 
 def adjust_logits(logits: torch.Tensor, text: Optional[torch.Tensor] = None,
@@ -45,64 +44,80 @@ def adjust_logits(logits: torch.Tensor, text: Optional[torch.Tensor] = None,
     word, the lowest bit first) is zero become -inf.  repetition (above 0), presence and
     frequency: numbers, or fp32 [B].  out: logits itself, or another tensor of its
     shape, type and device that does not overlap it; None: a new one."""
-    assert logits.dim() == 2 and logits.dtype in _DTYPES, "logits: fp16, bf16 or fp32 [B, V]"
+    dt, dev = logits.dtype, logits.device
+    assert logits.dim() == 2 and dt in _DTYPES and logits.shape[1] > 0, \
+        "logits: fp16, bf16 or fp32 [B, V], V > 0"
     B, V = logits.shape
-    dev = logits.device
-    assert V > 0, "logits: fp16, bf16 or fp32 [B, V], V > 0"
     assert text is not None or (lens is None and prompt is None), "lens and prompt are of a text"
     if text is not None:
         assert text.dtype == torch.int64 and text.dim() == 2 and text.shape[0] == B \
             and text.device == dev, f"text: int64 [{B}, width] on {dev}"
-    for name, x in (("lens", lens), ("prompt", prompt)):
-        assert x is None or (x.dtype == torch.int64 and tuple(x.shape) == (B,)
-                             and x.device == dev), f"{name}: int64 [{B}] on {dev}"
-    amounts = []
-    for name, x, low in (("repetition", repetition, 0.0), ("presence", presence, None),
-                         ("frequency", frequency, None)):
-        if isinstance(x, torch.Tensor):
-            assert x.dtype == torch.float32 and tuple(x.shape) == (B,) and x.device == dev, \
-                f"{name}: a number or fp32 [{B}] on {dev}"
-            amounts.append((x.contiguous(), 0.0))
-        else:
-            x = float(x)
-            assert math.isfinite(x) and (low is None or x > low), f"{name} {x}"
-            amounts.append((None, x))
-    ids = values = None
+        lens, prompt = _each(lens, "lens", B, dev), _each(prompt, "prompt", B, dev)
+    rep, rep1 = _amount(repetition, "repetition", B, dev)
+    assert rep is not None or rep1 > 0.0, f"repetition {rep1}"
+    pres, pres1 = _amount(presence, "presence", B, dev)
+    freq, freq1 = _amount(frequency, "frequency", B, dev)
+    ids, values = (None, None) if bias is None else bias
     if bias is not None:
-        ids, values = bias
         assert ids.dtype == torch.int64 and ids.dim() == 2 and ids.shape[0] == B \
             and values.dtype == torch.float32 and values.shape == ids.shape \
             and ids.device == values.device == dev, \
             f"bias: (int64 [{B}, n], fp32 [{B}, n]) on {dev}"
-    assert allowed is None or (allowed.dtype == torch.int32 and allowed.dim() == 2
-                               and allowed.shape[0] == B and allowed.shape[1] >= -(-V // 32)
-                               and allowed.device == dev), \
-        f"allowed: int32 [{B}, {-(-V // 32)}] on {dev}"
+    if allowed is not None:
+        assert allowed.dtype == torch.int32 and allowed.dim() == 2 and allowed.shape[0] == B \
+            and allowed.shape[1] >= -(-V // 32) and allowed.device == dev, \
+            f"allowed: int32 [{B}, {-(-V // 32)}] on {dev}"
     if out is not None:
-        assert out.shape == logits.shape and out.dtype == logits.dtype and out.device == dev \
-            and out.stride(1) == 1 and (B == 1 or out.stride(0) >= V), \
+        assert out.shape == logits.shape and out.dtype == dt and out.device == dev \
+            and out.stride(1) == 1 and (B <= 1 or out.stride(0) >= V), \
             "out: shape, type and device of logits, dense rows"
     if not logits.is_cuda:
         y = _adjust_cpu(logits, text, lens, prompt, [
-            torch.full((B,), n) if x is None else x for x, n in amounts], ids, values, allowed)
+            torch.full((B,), n) if x is None else x
+            for x, n in ((rep, rep1), (pres, pres1), (freq, freq1))], ids, values, allowed)
         return y if out is None else out.copy_(y)
-    src = logits if out is logits else _rows(logits)
-    out = torch.empty((B, V), dtype=logits.dtype, device=dev) if out is None else out
-    t, i, v, a = (None if x is None else _rows(x) for x in (text, ids, values, allowed))
-    lens, prompt = (None if x is None else x.contiguous() for x in (lens, prompt))
-
-    def at(x):
-        return None if x is None else x.data_ptr()
-
-    def ld(x):
-        return 0 if x is None else _ld(x)
-
-    _lib.call_on(dev, "hn_adjust_logits", src.data_ptr(), _ld(src), _DTYPES[logits.dtype], at(t),
-                 ld(t), 0 if t is None else t.shape[1], at(lens), at(prompt),
-                 *(at(x) for x, _ in amounts), *(n for _, n in amounts), at(i), ld(i), at(v),
-                 ld(v), 0 if i is None else i.shape[1], at(a), ld(a), B, V, out.data_ptr(),
-                 _ld(out))
+    src, ld = (logits, max(out.stride(0), V)) if out is logits else _rows(logits)
+    if out is None:
+        out = src.new_empty((B, V))
+    at = ld_t = width = at_lens = at_prompt = at_ids = ld_i = at_v = ld_v = n = at_a = ld_a = 0
+    if text is not None:
+        text, ld_t = _rows(text)
+        at, width = text.data_ptr(), text.shape[1]
+        at_lens = 0 if lens is None else lens.data_ptr()
+        at_prompt = 0 if prompt is None else prompt.data_ptr()
+    if ids is not None:
+        ids, ld_i = _rows(ids)
+        values, ld_v = _rows(values)
+        at_ids, at_v, n = ids.data_ptr(), values.data_ptr(), ids.shape[1]
+    if allowed is not None:
+        allowed, ld_a = _rows(allowed)
+        at_a = allowed.data_ptr()
+    _lib.call_on(dev, "hn_adjust_logits", src.data_ptr(), ld, _DTYPES[dt], at, ld_t, width,
+                 at_lens, at_prompt, 0 if rep is None else rep.data_ptr(),
+                 0 if pres is None else pres.data_ptr(), 0 if freq is None else freq.data_ptr(),
+                 rep1, pres1, freq1, at_ids, ld_i, at_v, ld_v, n, at_a, ld_a, B, V,
+                 out.data_ptr(), max(out.stride(0), V))
     return out
+
+
+def _each(x, name, B, dev):
+    """An int64 [B] or None."""
+    if x is None:
+        return None
+    assert x.dtype == torch.int64 and x.shape == (B,) and x.device == dev, \
+        f"{name}: int64 [{B}] on {dev}"
+    return x if x.stride(0) == 1 else x.contiguous()
+
+
+def _amount(x, name, B, dev):
+    """(fp32 [B] or None, else the number)."""
+    if isinstance(x, torch.Tensor):
+        assert x.dtype == torch.float32 and x.shape == (B,) and x.device == dev, \
+            f"{name}: a number or fp32 [{B}] on {dev}"
+        return (x if x.stride(0) == 1 else x.contiguous()), 0.0
+    x = float(x)
+    assert math.isfinite(x), f"{name} {x}"
+    return None, x
 
 
 def _adjust_cpu(logits, text, lens, prompt, amounts, ids, values, allowed) -> torch.Tensor:

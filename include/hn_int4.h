@@ -534,15 +534,26 @@ int hn_kv_fork(void* const* kt, void* const* v, long layers, long max_len, long 
  * to 1024) of every KV head: keys k [num_pages][nkv][page][hd], values v
  * [num_pages][nkv][page / 8][hd][8] (eight consecutive positions of a dimension
  * side by side), fp16 (dtype 0) or bf16 (1), hd 64, 128 or 256, 16-byte aligned.
- * table [B][ld_table] int32 (device): row b names the pages of sequence b, `cols`
- * of them; a sequence's positions i * page on lie in page table[b][i].  lens [B]
- * int64 (device): cached positions C_b before the step, negative for a sequence
- * that takes no part.  Rows starts[b] to starts[b + 1] - 1 of the step's T (starts
- * [B + 1] int32 on the device, not decreasing, from 0; NULL: T = B, row b) are
- * sequence b's tokens at positions C_b on.  Rows of no sequence write no page and
- * are zero in the outputs.  Sequences may share pages that neither writes.
  *
- * hn_paged_append: qkv [T][ld_qkv] (nh query heads, nkv keys, nkv values of hd);
+ * A step, a HOST struct that a call reads before it returns: table [B][ld_table]
+ * int32 (device): row b names the pages of sequence b, `cols` of them; a sequence's
+ * positions i * page on lie in page table[b][i].  lens [B] int64 (device): cached
+ * positions C_b before the step, negative for a sequence that takes no part.  Rows
+ * starts[b] to starts[b + 1] - 1 of the step's T (starts [B + 1] int32 on the
+ * device, not decreasing; NULL: T = B, row b) are sequence b's tokens at positions
+ * C_b on.  Rows of no sequence write no page and are zero in the outputs.
+ * Sequences may share pages that neither writes.  nh query heads over nkv KV heads.
+ * max_new: the most rows of a sequence; bound: about the most positions (C_b +
+ * rows), which chooses the launch, not the result. */
+typedef struct hn_paged_step {
+  const int* table;
+  long ld_table, cols, num_pages;
+  const long* lens;
+  const int* starts;
+  long B, T, nh, nkv, hd, page, max_new, bound;
+} hn_paged_step;
+
+/* hn_paged_append: qkv [T][ld_qkv] (nh query heads, nkv keys, nkv values of hd);
  *   the first `rotary` dimensions of queries and keys are rotated with cos_t /
  *   sin_t [table_rows][rotary / 2] fp32, in pairs (i, i + rotary / 2), or (2 i, 2 i
  *   + 1) with interleaved; fp32 products, rounded once.  Queries go to q_out
@@ -550,11 +561,9 @@ int hn_kv_fork(void* const* kt, void* const* v, long layers, long max_len, long 
  *   negative length write no page and zero queries; a row whose position is past
  *   cos_t, or whose page the table does not name (past its columns, or an id
  *   outside [0, num_pages)), writes no page and NaN queries. */
-int hn_paged_append(const void* qkv, long ld_qkv, int dtype, const float* cos_t,
-                    const float* sin_t, long table_rows, long rotary, int interleaved,
-                    const int* table, long ld_table, long cols, long num_pages, const long* lens,
-                    const int* starts, long B, long T, long nh, long nkv, long hd, long page,
-                    void* q_out, void* k, void* v, void* stream);
+int hn_paged_append(const hn_paged_step* step, const void* qkv, long ld_qkv, int dtype,
+                    const float* cos_t, const float* sin_t, long table_rows, long rotary,
+                    int interleaved, void* q_out, void* k, void* v, void* stream);
 
 /* hn_paged_attention: out[t * ld_o + h * hd + d] = softmax(scale * q k) v over the
  *   positions up to row t's own (its key and value in the pages already), query
@@ -562,18 +571,14 @@ int hn_paged_append(const void* qkv, long ld_qkv, int dtype, const float* cos_t,
  *   [T][ld_q].  Rows of a sequence with a negative length are zero; a row that
  *   sees a position whose page the table does not name is NaN, and so are the rows
  *   of a sequence with more than max_new of them.  A position that a row does not
- *   see has no effect on it, whatever it holds.  bound: about the most positions
- *   (C_b + rows) of a sequence; it chooses the launch, not the result.  scale above
- *   0 and finite, also times log2(e); 16-byte aligned operands, ld_q and ld_o
- *   multiples of 8; cols * page < 2^30.  work:
- *   hn_paged_attention_workspace_bytes(...) bytes, 16-byte aligned, any contents. */
-long hn_paged_attention_workspace_bytes(long B, long T, long nh, long nkv, long hd, long max_new,
-                                        long bound);
-int hn_paged_attention(const void* q, long ld_q, int dtype, const void* k, const void* v,
-                       const int* table, long ld_table, long cols, long num_pages,
-                       const long* lens, const int* starts, long B, long T, long nh, long nkv,
-                       long hd, long page, long max_new, long bound, float scale, void* out,
-                       long ld_o, void* work, long work_bytes, void* stream);
+ *   see has no effect on it, whatever it holds.  scale above 0 and finite, also
+ *   times log2(e); 16-byte aligned operands, ld_q and ld_o multiples of 8; cols *
+ *   page < 2^30.  work: hn_paged_attention_workspace_bytes(step) bytes, 16-byte
+ *   aligned, any contents. */
+long hn_paged_attention_workspace_bytes(const hn_paged_step* step);
+int hn_paged_attention(const hn_paged_step* step, const void* q, long ld_q, int dtype,
+                       const void* k, const void* v, float scale, void* out, long ld_o,
+                       void* work, long work_bytes, void* stream);
 
 /* hn_page_copy: page src[i] copied to page dst[i], i < pairs, in every layer.  k, v
  *   (the layers' device pointers, 16-byte aligned), src and dst are HOST arrays;

@@ -284,26 +284,40 @@ def test_library_refusals():
     """The C entries refuse before any GPU work; calls over nothing succeed."""
     from hydranet_amd import _lib
 
-    def append(dtype=0, rotary=128, B=1, T=1, nh=4, nkv=1, hd=128, page=16, ld=768, cols=1,
-               starts=None, p=16, cos=16, ldt=1, n=1):
-        _lib.call("hn_paged_append", p, ld, dtype, cos, cos, 8, rotary, 0, p, ldt, cols, n, p,
-                  starts, B, T, nh, nkv, hd, page, p, p, p, None)
+    import ctypes
 
-    def attend(dtype=0, B=1, T=1, nh=4, nkv=1, hd=128, page=16, ld=512, p=16, scale=0.1, new=1,
-               bound=1, out=16, work=None, bytes_=0, starts=None):
-        _lib.call("hn_paged_attention", p, ld, dtype, p, p, p, 1, 1, 1, p, starts, B, T, nh, nkv,
-                  hd, page, new, bound, scale, out, 512, work, bytes_, None)
+    def step(B=1, T=1, nh=4, nkv=1, hd=128, page=16, cols=1, ldt=1, n=1, starts=None, p=16, new=1,
+             bound=1, table=16):
+        s = _lib.PagedStep(p and table, ldt, cols, n, p, starts, B, T, nh, nkv, hd, page, new,
+                           bound)
+        step.last = s
+        return ctypes.addressof(s)
+
+    def append(dtype=0, rotary=128, ld=768, p=16, cos=16, no=False, **kw):
+        at = None if no else step(p=p, **kw)
+        _lib.call("hn_paged_append", at, p, ld, dtype, cos, cos, 8, rotary, 0, p, p, p, None)
+
+    def attend(dtype=0, ld=512, p=16, scale=0.1, out=16, work=None, bytes_=0, no=False, **kw):
+        at = None if no else step(p=p, **kw)
+        _lib.call("hn_paged_attention", at, p, ld, dtype, p, p, scale, out, 512, work, bytes_,
+                  None)
     append(B=0, T=0, p=None), append(B=2, T=0, starts=16, p=None), attend(B=0, T=0, p=None)
-    for kw in (dict(dtype=2), dict(rotary=130), dict(rotary=3), dict(rotary=-2), dict(T=2),
-               dict(B=-1, T=-1), dict(nh=3, nkv=2), dict(nkv=0), dict(hd=96), dict(page=24),
-               dict(page=8), dict(page=2048), dict(ld=767), dict(cols=2), dict(p=None),
-               dict(p=8), dict(cos=None), dict(n=-1)):
+    sizes = (dict(dtype=2), dict(T=2), dict(B=-1, T=-1), dict(nh=3, nkv=2), dict(nkv=0),
+             dict(hd=96), dict(page=24), dict(page=8), dict(page=2048), dict(cols=2),
+             dict(p=None), dict(p=8), dict(n=-1), dict(table=None), dict(no=True),
+             dict(B=70000, T=70000))
+    for kw in sizes + (dict(rotary=130), dict(rotary=3), dict(rotary=-2), dict(ld=767),
+                       dict(cos=None), dict(T=1 << 29, starts=16)):
         with pytest.raises(RuntimeError, match="hn_paged_append"):
             append(**kw)
-    for kw in (dict(dtype=2), dict(T=2), dict(nh=5, nkv=2), dict(hd=80), dict(page=17),
-               dict(ld=504), dict(ld=514), dict(p=None), dict(p=8), dict(out=None), dict(out=8),
-               dict(scale=0.0), dict(scale=math.nan), dict(scale=3e38), dict(new=0),
-               dict(bound=0)):
+    long = dict(cols=129, ldt=129, bound=3000)
+    need = _lib.lib().hn_paged_attention_workspace_bytes(step(**long))
+    assert need > 0 and _lib.lib().hn_paged_attention_workspace_bytes(step(bound=100)) == 0
+    for kw in sizes + (dict(ld=504), dict(ld=514), dict(out=None), dict(out=8), dict(scale=0.0),
+                       dict(scale=math.nan), dict(scale=3e38), dict(new=0), dict(bound=0),
+                       dict(n=0), dict(cols=1 << 26, ldt=1 << 26), long,
+                       dict(long, work=16, bytes_=need - 1), dict(long, work=8, bytes_=need),
+                       dict(new=1 << 23)):
         with pytest.raises(RuntimeError, match="hn_paged_attention"):
             attend(**kw)
 
@@ -316,7 +330,6 @@ def test_library_refusals():
                dict(B=70000)):
         with pytest.raises(RuntimeError, match="hn_adjust_logits"):
             adjust(**kw)
-    import ctypes
     one, ptr = (ctypes.c_int * 1)(0), (ctypes.c_void_p * 1)(16)
     two = (ctypes.c_int * 1)(5)
     for a in ((ptr, ptr, 1, 24, 4, one, one, 1), (ptr, ptr, 1, 32, 4, one, two, 1),
