@@ -214,6 +214,7 @@ __global__ __launch_bounds__(256) void append_rows_kernel(
 // row 4 c + i is position 8 c + 4 t + i, so that a lane's scores of both blocks are the 8
 // consecutive positions that its lane of the value operand holds.
 constexpr int kTile = 32;
+constexpr int NW = 4;  // waves of a workgroup
 constexpr float kLog2e = 1.4426950408889634f;
 // Probabilities are 2^8 times the softmax's, relative to a maximum that follows the true
 // one only when it lags by 2^6: below 2^14, so fp16 holds them, and those down to 2^-22
@@ -393,7 +394,7 @@ struct Sums {
 // head g.  All rows see the positions up to lo, none sees past hi.  The next tile's keys
 // are asked for when this one's scores are there, its values after this one's product:
 // about a tile is in flight throughout, in the registers of one.
-template <class T, int HD, int NT, int NW>
+template <class T, int HD, int NT>
 __device__ __forceinline__ void walk(const Attend<T>& A, Sums<T, HD, NT>& W, const Run& r, int b,
                                      int g, int row0, int first, int end, int lo, int hi, int wave,
                                      int lane) {
@@ -525,7 +526,7 @@ __device__ __forceinline__ void walk(const Attend<T>& A, Sums<T, HD, NT>& W, con
 
 // The waves' sums of 16 rows joined, then the rows themselves, or the range's entry of
 // the workspace.
-template <class T, int HD, int NT, int NW>
+template <class T, int HD, int NT>
 __device__ __forceinline__ void finish(const Attend<T>& A, const Sums<T, HD, NT>& W, const Run& r,
                                        int g, int row0, long entry, float* s_o, float* s_m,
                                        int wave, int lane) {
@@ -799,7 +800,7 @@ __global__ __launch_bounds__(256, 2) void block_kernel(Attend<T> A) {
 }
 
 // A workgroup per (KV head, block of 16 NT rows, sequence), over all of its positions.
-template <class T, int HD, int NT, int NW>
+template <class T, int HD, int NT>
 __global__ __launch_bounds__(64 * NW) void whole_kernel(Attend<T> A) {
   __shared__ __align__(16) float s_o[NW * 16 * (HD + 4)];
   __shared__ float s_m[NW * 16 * 2];
@@ -812,32 +813,25 @@ __global__ __launch_bounds__(64 * NW) void whole_kernel(Attend<T> A) {
   Sums<T, HD, NT> W;
   const int last = min((row0 + 16 * NT - 1) / A.rep, r.n - 1);
   const int lo = r.C + row0 / A.rep, hi = min(r.C + last, r.L - 1);
-  walk<T, HD, NT, NW>(A, W, r, b, g, row0, 0, r.L, lo, hi, wave, lane);
-  finish<T, HD, NT, NW>(A, W, r, g, row0, -1, s_o, s_m, wave, lane);
+  walk<T, HD, NT>(A, W, r, b, g, row0, 0, r.L, lo, hi, wave, lane);
+  finish<T, HD, NT>(A, W, r, g, row0, -1, s_o, s_m, wave, lane);
 }
 
 // The grains of all (sequence, KV head) pairs in order, an even share of them for each
 // workgroup, wherever the sequences' borders are: one range of positions of one head, or
 // several.  A head's range that is not whole leaves its sums in the workspace, in entry
 // 2 w of workgroup w, or 2 w + 1 if it is not w's first, for join_kernel.
-template <class T, int HD, int NT, int NW>
+template <class T, int HD, int NT>
 __global__ __launch_bounds__(64 * NW) void share_kernel(Attend<T> A) {
   __shared__ __align__(16) float s_o[NW * 16 * (HD + 4)];
   __shared__ float s_m[NW * 16 * 2];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), w = blockIdx.x;
   const int nkv = A.P.nkv;
   const Deal D(uniform(grains_below(A, A.P.B)) * nkv, A.wgs);
-  for (int e = w; e < A.P.B; e += A.wgs) {
-    const Run r = run_of(A, e);
-    if (r.none || r.nan)
-      for (int g = 0; g < nkv; ++g) fill<T, HD>(A, r, g, 0, 1);
-  }
-  for (int g = 0; g < nkv; ++g) fill_rest<T, HD>(A, g, w, A.wgs);
-  if (w >= D.wgs) return;
   const int from = D.from(w);
-  int left = D.from(w + 1) - from, b = 0, g = 0, at = 0, n = 0;
+  int left = w < D.wgs ? D.from(w + 1) - from : 0, b = 0, g = 0, at = 0, n = 0;
   int base = 0;  // grains of one head of the sequences before
-  for (int c = 0; c < A.P.B; c += 64) {
+  for (int c = 0; c < A.P.B && left; c += 64) {
     const int t = c + lane < A.P.B ? grains_of(A, c + lane) : 0;
     const int sum = lane_scan(t);
     const unsigned long long past = __ballot((base + sum) * nkv > from);
@@ -862,12 +856,18 @@ __global__ __launch_bounds__(64 * NW) void share_kernel(Attend<T> A) {
     const int m = min(n - at, left);
     const Run r = run_of(A, b);
     Sums<T, HD, NT> W;
-    walk<T, HD, NT, NW>(A, W, r, b, g, 0, at * kGrain, (at + m) * kGrain, r.C, r.L - 1, wave,
+    walk<T, HD, NT>(A, W, r, b, g, 0, at * kGrain, (at + m) * kGrain, r.C, r.L - 1, wave,
                         lane);
-    finish<T, HD, NT, NW>(A, W, r, g, 0, m == n ? -1 : 2 * (long)w + !start, s_o, s_m, wave,
+    finish<T, HD, NT>(A, W, r, g, 0, m == n ? -1 : 2 * (long)w + !start, s_o, s_m, wave,
                           lane);
     at += m, left -= m;
   }
+  for (int e = w; e < A.P.B; e += A.wgs) {
+    const Run r = run_of(A, e);
+    if (r.none || r.nan)
+      for (int g = 0; g < nkv; ++g) fill<T, HD>(A, r, g, 0, 1);
+  }
+  for (int g = 0; g < nkv; ++g) fill_rest<T, HD>(A, g, w, A.wgs);
 }
 
 // The entries of a head whose positions several workgroups had, joined: a workgroup per
@@ -880,8 +880,15 @@ __global__ __launch_bounds__(256) void join_kernel(Attend<T> A) {
   const int b = blockIdx.z, g = blockIdx.y, row = blockIdx.x, nkv = A.P.nkv;
   const Run r = run_of(A, b);
   if (r.L == 0 || row >= A.rep * r.n) return;
-  const int n = grains_of(A, b), below = uniform(grains_below(A, b));
-  const Deal D(uniform(grains_below(A, A.P.B)) * nkv, A.wgs);
+  int below = 0, total = 0;  // grains of one head
+  for (int e = threadIdx.x & 63; e < A.P.B; e += 64) {
+    const int t = grains_of(A, e);
+    total += t, below += e < b ? t : 0;
+  }
+  below = __builtin_amdgcn_readlane(lane_scan(below), 63);
+  total = __builtin_amdgcn_readlane(lane_scan(total), 63);
+  const int n = (r.L + kGrain - 1) / kGrain;
+  const Deal D(total * nkv, A.wgs);
   const int x0 = below * nkv + g * n;  // this head's first grain
   const int w0 = D.owner(x0), w1 = D.owner(x0 + n - 1);
   if (w0 == w1) return;
@@ -889,13 +896,28 @@ __global__ __launch_bounds__(256) void join_kernel(Attend<T> A) {
   float m = -__builtin_inff(), sum = 0.f;
   float4v o = (float4v)(0.f);
   const float* ms = A.part + 2 * (long)A.wgs * A.R * HD;
-  for (int w = w0 + at; w <= w1; w += kAt) {
-    const long e = (2 * (long)w + (D.from(w) < x0)) * A.R + row;
-    const float em = ms[2 * e], el = ms[2 * e + 1];
-    const float4v eo = *reinterpret_cast<const float4v*>(A.part + e * HD + 4 * c);
-    const float nm = fmaxf(m, em), ref = nm == -__builtin_inff() ? 0.f : nm;
-    const float a = __builtin_amdgcn_exp2f(m - ref), z = __builtin_amdgcn_exp2f(em - ref);
-    o = o * a + eo * z, sum = sum * a + el * z, m = nm;
+  for (int w = w0 + at; w <= w1; w += 4 * kAt) {
+    float em[4], el[4];
+    float4v eo[4];  // four entries asked for together
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int x = min(w + i * kAt, w1);
+      const long e = (2 * (long)x + (D.from(x) < x0)) * A.R + row;
+      em[i] = ms[2 * e], el[i] = ms[2 * e + 1];
+      eo[i] = *reinterpret_cast<const float4v*>(A.part + e * HD + 4 * c);
+    }
+    float nm = m;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) nm = fmaxf(nm, em[i]);
+    const float ref = nm == -__builtin_inff() ? 0.f : nm;
+    const float a = __builtin_amdgcn_exp2f(m - ref);
+    o *= a, sum *= a, m = nm;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (w + i * kAt > w1) continue;
+      const float z = __builtin_amdgcn_exp2f(em[i] - ref);
+      o += eo[i] * z, sum += el[i] * z;
+    }
   }
   s_o[at][c] = o;
   if (c == 0) s_m[at] = m, s_l[at] = sum;
@@ -996,12 +1018,16 @@ int append(const Step& P, const void* qkv_, long ld, const float* cos_t, const f
 
 // Rows of one (sequence, KV head) up to which a workgroup's positions are shared out.
 constexpr int kShareRows = 32;
-// Positions up to which one workgroup takes all of a head's.
-constexpr long kWhole = 2048;
 
-// The workgroups that share the positions, 0: a workgroup per head.
-int share_wgs(long rows, long hd, long bound) {
-  return rows > (hd == 256 ? 16 : kShareRows) || bound <= kWhole ? 0 : 2 * hn_device_cus();
+// The workgroups that share the positions, or 0: a workgroup per head.  That one needs no
+// join, but its longest head is the last to end, and few heads leave the chip idle.  (One
+// token, 8 KV heads of 128, shared / per head, us: 1 sequence of 100 8.5 / 5.8, of 300 9.2 /
+// 11.9, of 700 9.9 / 17; 64 of 250 22.9 / 18.4, of 1000 54 / 49, of 150 to 8000 200 / 241; 256
+// of 1 to 1000 138 / 107.)
+int share_wgs(long heads, long rows, long hd, long bound) {
+  const long wgs = 2 * hn_device_cus();
+  if (rows > (hd == 256 ? 16 : kShareRows) || bound <= kGrain) return 0;
+  return heads >= wgs && bound <= 2048 * (heads / wgs) ? 0 : (int)wgs;
 }
 
 long part_bytes(long wgs, long rows, long hd) { return 2 * wgs * rows * (hd + 2) * 4; }
@@ -1009,12 +1035,11 @@ long part_bytes(long wgs, long rows, long hd) { return 2 * wgs * rows * (hd + 2)
 template <class T, int HD, int NT>
 int attend_rows(const Attend<T>& A, int B, int nkv, hipStream_t stream) {
   if (A.wgs) {
-    share_kernel<T, HD, NT, 4><<<A.wgs, 256, 0, stream>>>(A);
+    share_kernel<T, HD, NT><<<A.wgs, 256, 0, stream>>>(A);
     HN_LAUNCH_CHECK("hn_paged_attention");
     join_kernel<T, HD><<<dim3(A.R, nkv, B), 256, 0, stream>>>(A);
   } else {
-    constexpr int NW = NT == 1 && HD < 256 ? 8 : 4;
-    whole_kernel<T, HD, NT, NW>
+    whole_kernel<T, HD, NT>
         <<<dim3(nkv, hn_cdiv(A.R, 16 * NT), B), 64 * NW, 0, stream>>>(A);
   }
   HN_LAUNCH_CHECK("hn_paged_attention");
@@ -1073,7 +1098,7 @@ extern "C" long hn_paged_attention_workspace_bytes(const hn_paged_step* s) {
       s->max_new <= 0)
     return 0;
   const long rows = s->nh / s->nkv * s->max_new;
-  return part_bytes(share_wgs(rows, s->hd, s->bound), rows, s->hd);
+  return part_bytes(share_wgs(s->B * s->nkv, rows, s->hd, s->bound), rows, s->hd);
 }
 
 extern "C" int hn_paged_attention(const hn_paged_step* step, const void* q, long ld_q, int dtype,
@@ -1096,7 +1121,7 @@ extern "C" int hn_paged_attention(const hn_paged_step* step, const void* q, long
                "hn_paged_attention: rows of %ld, strides of %ld and %ld: 16-byte aligned rows",
                nh * hd, ld_q, ld_o);
   const long rows = nh / nkv * max_new;
-  const int wgs = share_wgs(rows, hd, step->bound);
+  const int wgs = share_wgs(P.B * nkv, rows, hd, step->bound);
   HN_ARG_CHECK(wgs == 0 || (work && (uintptr_t)work % 16 == 0 &&
                             work_bytes >= part_bytes(wgs, rows, hd)),
                "hn_paged_attention: a workspace of %ld bytes, %ld given",
