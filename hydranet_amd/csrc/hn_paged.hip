@@ -215,6 +215,9 @@ __global__ __launch_bounds__(256) void append_rows_kernel(
 // consecutive positions that its lane of the value operand holds.
 constexpr int kTile = 32;
 constexpr int NW = 4;  // waves of a workgroup
+// Workgroups that a CU's registers hold at once.  (Three of 128 dimensions spill: one text of
+// 31777 43 us, two 33.)
+constexpr int resident(long hd) { return hd == 256 ? 1 : 2; }
 constexpr float kLog2e = 1.4426950408889634f;
 // Probabilities are 2^8 times the softmax's, relative to a maximum that follows the true
 // one only when it lags by 2^6: below 2^14, so fp16 holds them, and those down to 2^-22
@@ -801,7 +804,7 @@ __global__ __launch_bounds__(256, 2) void block_kernel(Attend<T> A) {
 
 // A workgroup per (KV head, block of 16 NT rows, sequence), over all of its positions.
 template <class T, int HD, int NT>
-__global__ __launch_bounds__(64 * NW) void whole_kernel(Attend<T> A) {
+__global__ __launch_bounds__(64 * NW, resident(HD)) void whole_kernel(Attend<T> A) {
   __shared__ __align__(16) float s_o[NW * 16 * (HD + 4)];
   __shared__ float s_m[NW * 16 * 2];
   const int g = blockIdx.x, b = blockIdx.z, row0 = (gridDim.y - 1 - blockIdx.y) * 16 * NT;
@@ -822,7 +825,7 @@ __global__ __launch_bounds__(64 * NW) void whole_kernel(Attend<T> A) {
 // several.  A head's range that is not whole leaves its sums in the workspace, in entry
 // 2 w of workgroup w, or 2 w + 1 if it is not w's first, for join_kernel.
 template <class T, int HD, int NT>
-__global__ __launch_bounds__(64 * NW) void share_kernel(Attend<T> A) {
+__global__ __launch_bounds__(64 * NW, resident(HD)) void share_kernel(Attend<T> A) {
   __shared__ __align__(16) float s_o[NW * 16 * (HD + 4)];
   __shared__ float s_m[NW * 16 * 2];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), w = blockIdx.x;
@@ -1025,9 +1028,9 @@ constexpr int kShareRows = 32;
 // 11.9, of 700 9.9 / 17; 64 of 250 22.9 / 18.4, of 1000 54 / 49, of 150 to 8000 200 / 241; 256
 // of 1 to 1000 138 / 107.)
 int share_wgs(long heads, long rows, long hd, long bound) {
-  const long wgs = 2 * hn_device_cus();
+  const int cus = hn_device_cus();
   if (rows > (hd == 256 ? 16 : kShareRows) || bound <= kGrain) return 0;
-  return heads >= wgs && bound <= 2048 * (heads / wgs) ? 0 : (int)wgs;
+  return heads >= 2 * cus && bound <= 1024 * (heads / cus) ? 0 : cus * resident(hd);
 }
 
 long part_bytes(long wgs, long rows, long hd) { return 2 * wgs * rows * (hd + 2) * 4; }
