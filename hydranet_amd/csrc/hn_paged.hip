@@ -227,6 +227,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kUp = 8.f, kLag = 6.f;
 // Positions that workgroups share out as one.
 constexpr int kGrain = 128;
+// Positions that a share of a block's has at least.
+constexpr long kShare = 256;
 
 template <class T>
 struct Attend {
@@ -236,6 +238,8 @@ struct Attend {
   float* part;  // entries of R rows of HD sums, then of R (maximum, sum)
   long ld_q, ld_o;
   int rep, max_new, R, wgs;
+  int shares, each;  // of a block's positions, and the stages of one
+  long entries;
   float scale;
 };
 
@@ -347,6 +351,7 @@ __device__ __forceinline__ int grains_below(const Attend<T>& A, int to) {
 template <class T, int E>
 __device__ __forceinline__ uint32_t clean(typename Vec<T>::t (&v)[E], int at, int lo, int hi) {
   uint32_t odd = 0;
+  asm volatile("" : "+v"(at));  // (nothing of this stays in registers where it is not used)
 #pragma unroll
   for (int e = 0; e < E; ++e) {
     u32x4 w = __builtin_bit_cast(u32x4, v[e]);
@@ -584,39 +589,46 @@ __device__ __forceinline__ void finish(const Attend<T>& A, const Sums<T, HD, NT>
 
 // ---------------------------------------------------------------------------
 // Runs of many rows.  A workgroup of 4 waves takes 128 rows of one (sequence, KV head), 32
-// a wave, and walks the positions in stages of 64 that all four read from LDS; the next
-// stage goes from memory to LDS (buffer_load ... lds) meanwhile.  A stage lies there as
-// in the pages, but that a key's 16-byte chunks are at chunk ^ key(position), so that the
-// 16 positions that a read takes cover the banks once.  Two workgroups per CU: one's
-// loads and softmax under the other's products.
-constexpr int kStage = 64, kBlock = 128;
+// a wave, and walks the positions in stages that all four read from LDS; the next stage
+// goes from memory to LDS (buffer_load ... lds) meanwhile.  A stage lies there as in the
+// pages, but that a key's 16-byte chunks are at chunk ^ key(position), so that the 16
+// positions that a read takes cover the banks once.  Two workgroups per CU: one's loads
+// and softmax under the other's products.
+constexpr int kBlock = 128;
+constexpr int stage_of(int hd) { return hd == 256 ? 32 : 64; }
 
+// The blocks of a run, and the stages of one: up to the last position that its rows see.
+template <class T>
+__device__ __forceinline__ int blocks_of(const Attend<T>& A, const Run& r) {
+  return r.L ? (A.rep * r.n + kBlock - 1) / kBlock : 0;
+}
 template <class T, int HD>
-__global__ __launch_bounds__(256, 2) void block_kernel(Attend<T> A) {
+__device__ __forceinline__ int stages_of(const Attend<T>& A, const Run& r, int block) {
+  const int top = r.C + min((block * kBlock + kBlock - 1) / A.rep, r.n - 1);
+  return min(top, r.L - 1) / stage_of(HD) + 1;
+}
+
+// Stages [from, to) of a block: its rows, or, with entry >= 0, their sums to the workspace.
+template <class T, int HD>
+__device__ __forceinline__ void block_range(const Attend<T>& A, const Run& r, int b, int g,
+                                            int block, int from, int to, long entry,
+                                            unsigned char* s_buf) {
   typedef typename Vec<T>::t V8;
-  constexpr int NT = 2, kChunks = HD / 8;            // 16-byte chunks of a key
-  constexpr int kBytes = kStage * HD * 2;            // of a stage's keys, and of its values
-  constexpr int kPos = 64 / kChunks;                 // keys per DMA instruction
-  constexpr int kDma = kBytes / 1024 / 4;            // instructions per wave and operand
-  __shared__ __align__(1024) unsigned char s_buf[4 * kBytes];
+  constexpr int SP = stage_of(HD), NT = 2, kChunks = HD / 8;  // 16-byte chunks of a key
+  constexpr int kBytes = SP * HD * 2;      // of a stage's keys, and of its values
+  constexpr int kPos = 64 / kChunks;       // keys per DMA instruction
+  constexpr int kDma = kBytes / 1024 / 4;  // instructions per wave and operand
   const Step& P = A.P;
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
   const int n = lane & 15, kg = lane >> 4;
-  const int g = blockIdx.x, b = blockIdx.z, part = gridDim.y - 1 - blockIdx.y;
-  const Run r = run_of(A, b);
-  if (b == 0) fill_rest<T, HD>(A, g, part, gridDim.y);
-  if (r.none || r.nan) return fill<T, HD>(A, r, g, part, gridDim.y);
-  const int rows = A.rep * r.n;
-  if (part * kBlock >= rows) return;
-  const int row0 = part * kBlock + 32 * wave;
+  const int rows = A.rep * r.n, row0 = block * kBlock + 32 * wave;
   const bool busy = row0 < rows;
 
   V8 q[NT][HD / 32];
   int lim[NT];
-  // positions that all of this wave's rows see, none sees, and none of the workgroup's
+  // positions that all of this wave's rows see, and past which none sees any
   const int lo = r.C + row0 / A.rep;
   const int hi = min(r.C + min((row0 + 31) / A.rep, r.n - 1), r.L - 1);
-  const int top = min(r.C + min((part * kBlock + kBlock - 1) / A.rep, r.n - 1), r.L - 1);
   float4v o[NT][HD / 16], l[NT];
   float mx[NT];
 #pragma unroll
@@ -637,57 +649,58 @@ __global__ __launch_bounds__(256, 2) void block_kernel(Attend<T> A) {
     for (int e = 0; e < HD / 16; ++e) o[t][e] = (float4v)(0.f);
   }
 
-  const int shift = __builtin_ctz(P.page), stages = top / kStage + 1;
+  const int shift = __builtin_ctz(P.page);
   // The pages of a stage's positions by sixteens (-1: none): scalars, read ahead through
   // the scalar cache, so that no wait for them is one for the stage on its way.
   typedef const __attribute__((address_space(4))) int* Table;
   const Table table = (Table)(uintptr_t)(P.table + (long)b * P.ld);
   struct Ids {
-    int id[kStage / 16];
+    int id[SP / 16];
   };
+  const bool one = P.page >= SP;  // a stage lies on one page
   auto pages = [&](int st) {
     Ids x;
-#pragma unroll
-    for (int i = 0; i < kStage / 16; ++i) {
-      const int col = (st * kStage + 16 * i) >> shift;
+    auto at = [&](int i) {
+      const int col = (st * SP + 16 * i) >> shift;
       const int id = col < P.cols ? table[col] : -1;
-      x.id[i] = id >= 0 && id < P.pages ? id : -1;
-    }
+      return id >= 0 && id < P.pages ? id : -1;
+    };
+    x.id[0] = at(0);
+#pragma unroll
+    for (int i = 1; i < SP / 16; ++i) x.id[i] = one ? x.id[0] : at(i);
     return x;
   };
   const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)s_buf;
   // DMA: instruction i of wave w moves KB w + 4 i of a stage's keys and of its values.  A
   // page that is not there reads as zero (a descriptor of no bytes).
   const int head_bytes = P.page * HD * 2;
+  const long page_elems = (long)P.nkv * P.page * HD, head = (long)g * P.page * HD;
+  const T *keys0 = A.k + head, *values0 = A.v + head;
   auto issue = [&](int st, const Ids& x) {
-    auto page = [&](int i) { return i == 0 ? x.id[0] : i == 1 ? x.id[1] : i == 2 ? x.id[2] : x.id[3]; };
     const uint32_t at = lds0 + (uint32_t)(st & 1) * 2 * kBytes + wave * 1024;
-    const int p0 = st * kStage;
-    auto where = [&](const T* x, int id) {
-      return rsrc(x + ((long)max(id, 0) * P.nkv + g) * P.page * HD, id < 0 ? 0 : head_bytes);
-    };
 #pragma unroll
     for (int i = 0; i < kDma; ++i) {
+      // the page of instruction i's positions, kPos * (wave + 4 i) on (or the 8 around them)
+      const int j = kPos * 4 * i / 16;
+      const int id = kPos == 8 && wave >> 1 ? x.id[j + (kPos == 8)] : x.id[j];
+      const long page = max(id, 0) * page_elems;
+      const int bytes = id < 0 ? 0 : head_bytes;
       const int kp = kPos * (wave + 4 * i), pos = kp + lane / kChunks;  // within the stage
-      const int m = ((pos >> 3) & 3) * 4 + (pos & 3), key = kChunks == 16 ? m : m >> 1;
-      const int id = page(kp >> 4);
-      dma_b128(where(A.k, id), (lane / kChunks) * HD * 2 + 16 * ((lane % kChunks) ^ key),
-               (uint32_t)((p0 + kp) & (P.page - 1)) * HD * 2, at + i * 4096);
-    }
-#pragma unroll
-    for (int i = 0; i < kDma; ++i) {
-      // KB j of the values: 512 / HD positions' worth, in slots of 8
-      const int j = wave + 4 * i, vp = j * 512 / HD & ~7;
-      const int id = page(vp >> 4);
-      dma_b128(where(A.v, id), 16 * lane,
-               (uint32_t)((p0 + vp) & (P.page - 1)) * HD * 2 + (j * 1024) % (16 * HD),
+      const int m = ((pos >> 3) & 3) * 4 + (pos & 3), key = kChunks == 8 ? m >> 1 : m;
+      dma_b128(rsrc(keys0 + page, bytes),
+               (lane / kChunks) * HD * 2 + 16 * ((lane % kChunks) ^ key),
+               (uint32_t)((st * SP + kp) & (P.page - 1)) * HD * 2, at + i * 4096);
+      // KB kb of the values: 512 / HD positions' worth, in slots of 8
+      const int kb = wave + 4 * i, vp = kb * 512 / HD & ~7;
+      dma_b128(rsrc(values0 + page, bytes), 16 * lane,
+               (uint32_t)((st * SP + vp) & (P.page - 1)) * HD * 2 + (kb * 1024) % (16 * HD),
                at + kBytes + i * 4096);
     }
   };
 
   // this lane's part of the reads
   uint32_t k_at[HD / 32];
-  const int mine = kChunks == 16 ? n : n >> 1;
+  const int mine = kChunks == 8 ? n >> 1 : n;
 #pragma unroll
   for (int u = 0; u < HD / 32; ++u)
     k_at[u] = lds0 + (8 * (n >> 2) + (n & 3)) * HD * 2 + 16 * ((4 * u + kg) ^ mine);
@@ -698,41 +711,53 @@ __global__ __launch_bounds__(256, 2) void block_kernel(Attend<T> A) {
   for (int i = 0; i < 8; ++i) ones[i] = (T)1.f;
 
   uint32_t odd = 0;
-  auto compute = [&](bool edge, int st, uint32_t bad) __attribute__((always_inline)) {
-    const uint32_t at = (uint32_t)(st & 1) * 2 * kBytes;
-    const int p0 = st * kStage;
-    V8 p[NT][2];
-    float4v s[NT][4];  // block 2 h + j of half h
+  Ids id = pages(from), next = pages(from + 1);
+  issue(from, id);
+  for (int st = from; st < to; ++st) {
+    wait_vmcnt<0>();  // this wave's part of the stage has landed
+    stage_barrier();  // everyone's, and the stage before is used
+    if (st + 1 < to) issue(st + 1, next);
+    uint32_t bad = 0;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
+    for (int i = 0; i < SP / 16; ++i) bad |= id.id[i] < 0 ? 1u << i : 0u;
+    id = next, next = pages(st + 2);
+    const uint32_t here = (uint32_t)(st & 1) * 2 * kBytes;
+    // (Waves without rows, or past the last position that theirs see, go along.)
+    const bool edge = st * SP + SP - 1 > lo || bad;
+    const int p0 = st * SP;
+    float4v s[NT][SP / 16];  // block 2 h + j of half h
+#pragma unroll
+    for (int x = 0; x < SP / 16; ++x) {
       V8 k[HD / 32];
 #pragma unroll
       for (int u = 0; u < HD / 32; ++u)
-        k[u] = lds_read<V8>(k_at[u] + at + (32 * (x >> 1) + 4 * (x & 1)) * HD * 2);
+        k[u] = lds_read<V8>(k_at[u] + here + (32 * (x >> 1) + 4 * (x & 1)) * HD * 2);
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        s[t][x] = (float4v)(0.f);
+      for (int t = 0; t < NT; ++t) s[t][x] = (float4v)(0.f);
 #pragma unroll
-        for (int u = 0; u < HD / 32; ++u) s[t][x] = Vec<T>::mfma(k[u], q[t][u], s[t][x]);
-      }
+      for (int u = 0; u < HD / 32; ++u)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) s[t][x] = Vec<T>::mfma(k[u], q[t][u], s[t][x]);
     }
+    V8 p[NT][SP / 32];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
       if (edge) {
+        int see = lim[t] - p0 - 8 * kg;
+        asm volatile("" : "+v"(see));  // (else as many differences from it stay in registers)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
+        for (int x = 0; x < SP / 16; ++x) {
           const bool none = bad >> (2 * (x >> 1) + (kg >> 1)) & 1;
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             if (none) s[t][x][c] = __builtin_nanf("");
-            if (p0 + 32 * (x >> 1) + 8 * kg + 4 * (x & 1) + c > lim[t])
-              s[t][x][c] = -__builtin_inff();
+            if (32 * (x >> 1) + 4 * (x & 1) + c > see) s[t][x][c] = -__builtin_inff();
           }
         }
       }
       float tm = s[t][0][0];
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
+      for (int x = 0; x < SP / 16; ++x)
 #pragma unroll
         for (int c = 0; c < 4; ++c) tm = fmaxf(tm, s[t][x][c]);
       if (__any(tm * scale > mx[t] + kLag)) {
@@ -745,21 +770,22 @@ __global__ __launch_bounds__(256, 2) void block_kernel(Attend<T> A) {
       }
       const float ref = mx[t] == -__builtin_inff() ? 0.f : mx[t] - kUp;
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
+      for (int x = 0; x < SP / 16; ++x)
 #pragma unroll
         for (int c = 0; c < 4; ++c)
           p[t][x >> 1][4 * (x & 1) + c] =
               (T)__builtin_amdgcn_exp2f(__builtin_fmaf(s[t][x][c], scale, -ref));
     }
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < SP / 32; ++h) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) l[t] = Vec<T>::mfma(ones, p[t][h], l[t]);
 #pragma unroll
       for (int e0 = 0; e0 < HD / 16; e0 += 4) {
         V8 v[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] = lds_read<V8>(v_at + at + h * HD * 64 + (e0 + e) * 256);
+        for (int e = 0; e < 4; ++e)
+          v[e] = lds_read<V8>(v_at + here + h * HD * 64 + (e0 + e) * 256);
         if (edge) odd |= clean<T>(v, p0 + 32 * h + 8 * kg, lo, hi);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
@@ -767,28 +793,24 @@ __global__ __launch_bounds__(256, 2) void block_kernel(Attend<T> A) {
           for (int t = 0; t < NT; ++t) o[t][e0 + e] = Vec<T>::mfma(v[e], p[t][h], o[t][e0 + e]);
       }
     }
-  };
-
-  Ids id = pages(0), next = pages(1);
-  issue(0, id);
-  for (int st = 0; st < stages; ++st) {
-    wait_vmcnt<0>();  // this wave's part of the stage has landed
-    stage_barrier();  // everyone's, and the stage before is used
-    if (st + 1 < stages) issue(st + 1, next);
-    uint32_t bad = 0;
-#pragma unroll
-    for (int i = 0; i < kStage / 16; ++i) bad |= id.id[i] < 0 ? 1u << i : 0u;
-    id = next, next = pages(st + 2);
-    if (!busy || st * kStage > hi) continue;
-    compute(st * kStage + kStage - 1 > lo || bad, st, bad);
   }
   if (!busy) return;
   if (__any(odd))
-    add_odd<T, HD, NT>(A, o, lim, b, g, lo, hi, kg, [](int) { return true; });
+    add_odd<T, HD, NT>(A, o, lim, b, g, lo, hi, kg,
+                       [&](int p) { return p / SP >= from && p / SP < to; });
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int row = row0 + 16 * t + n, tok = row / A.rep, head = row - tok * A.rep;
     if (row >= rows) continue;
+    if (entry >= 0) {
+      const long at = entry * kBlock + (row - block * kBlock);
+      float* dst = A.part + at * HD + 4 * kg;
+#pragma unroll
+      for (int e = 0; e < HD / 16; ++e) *reinterpret_cast<float4v*>(dst + 16 * e) = o[t][e];
+      float* pm = A.part + A.entries * kBlock * HD + at * 2;
+      if (kg == 0) pm[0] = mx[t], pm[1] = l[t][0];
+      continue;
+    }
     const float is = 1.f / l[t][0];
     T* dst = A.out + (long)(r.row + tok) * A.ld_o + (long)(g * A.rep + head) * HD + 4 * kg;
 #pragma unroll
@@ -800,6 +822,74 @@ __global__ __launch_bounds__(256, 2) void block_kernel(Attend<T> A) {
       *reinterpret_cast<V4*>(dst + 16 * e) = y;
     }
   }
+}
+
+// A workgroup per (KV head, block and share of its positions, sequence), the longest blocks
+// of a run first.  A block's A.each stages a share (the rest in the last); its entry of the
+// workspace goes by the block and the share.
+template <class T, int HD>
+__global__ __launch_bounds__(256, resident(HD)) void block_kernel(Attend<T> A) {
+  __shared__ __align__(1024) unsigned char s_buf[8 * stage_of(HD) * HD];
+  const int g = blockIdx.x, b = blockIdx.z, part = gridDim.y - 1 - blockIdx.y;
+  const int block = part / A.shares, share = part - block * A.shares;
+  const Run r = run_of(A, b);
+  if (b == 0) fill_rest<T, HD>(A, g, part, gridDim.y);
+  if (r.none || r.nan) return fill<T, HD>(A, r, g, part, gridDim.y);
+  if (block >= blocks_of(A, r)) return;
+  const int stages = stages_of<T, HD>(A, r, block), from = share * A.each;
+  if (from >= stages) return;
+  const int to = share == A.shares - 1 ? stages : min(from + A.each, stages);
+  const long entry = (((long)b * A.P.nkv + g) * gridDim.y) + part;
+  block_range<T, HD>(A, r, b, g, block, from, to, to - from == stages ? -1 : entry, s_buf);
+}
+
+// The entries of a block's shares joined, 1024 / HD rows at a time.  Grid (nkv, blocks *
+// HD / 8, B).
+template <class T, int HD>
+__global__ __launch_bounds__(256) void join_blocks_kernel(Attend<T> A) {
+  constexpr int kAcross = HD / 4, kRows = 256 / kAcross;
+  const int g = blockIdx.x, b = blockIdx.z, block = blockIdx.y / (HD / 8);
+  const Run r = run_of(A, b);
+  if (block >= blocks_of(A, r)) return;
+  const int stages = stages_of<T, HD>(A, r, block);
+  const int n = min((stages + A.each - 1) / A.each, A.shares);
+  const int c = threadIdx.x % kAcross;
+  const int in = blockIdx.y % (HD / 8) * kRows + threadIdx.x / kAcross, row = block * kBlock + in;
+  if (n < 2 || row >= A.rep * r.n) return;
+  const long blocks = gridDim.y / (HD / 8), first = (((long)b * A.P.nkv + g) * blocks + block) * A.shares;
+  const float* ms = A.part + A.entries * kBlock * HD;
+  float m = -__builtin_inff(), sum = 0.f;
+  float4v o = (float4v)(0.f);
+  for (int i = 0; i < n; i += 4) {
+    float em[4], el[4];
+    float4v eo[4];  // four entries asked for together
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const long e = (first + min(i + j, n - 1)) * kBlock + in;
+      em[j] = ms[2 * e], el[j] = ms[2 * e + 1];
+      eo[j] = *reinterpret_cast<const float4v*>(A.part + e * HD + 4 * c);
+    }
+    float nm = m;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) nm = fmaxf(nm, em[j]);
+    const float ref = nm == -__builtin_inff() ? 0.f : nm;
+    const float a = __builtin_amdgcn_exp2f(m - ref);
+    o *= a, sum *= a, m = nm;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (i + j >= n) continue;
+      const float z = __builtin_amdgcn_exp2f(em[j] - ref);
+      o += eo[j] * z, sum += el[j] * z;
+    }
+  }
+  const int tok = row / A.rep, head = row - tok * A.rep;
+  const float is = 1.f / sum;
+  typedef T V4 __attribute__((ext_vector_type(4)));
+  V4 y;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) y[j] = (T)(o[j] * is);
+  *reinterpret_cast<V4*>(A.out + (long)(r.row + tok) * A.ld_o + (long)(g * A.rep + head) * HD +
+                         4 * c) = y;
 }
 
 // A workgroup per (KV head, block of 16 NT rows, sequence), over all of its positions.
@@ -1019,21 +1109,41 @@ int append(const Step& P, const void* qkv_, long ld, const float* cos_t, const f
   return 0;
 }
 
-// Rows of one (sequence, KV head) up to which a workgroup's positions are shared out.
-constexpr int kShareRows = 32;
+// Rows of one (sequence, KV head) up to which a workgroup takes all of them for a share of
+// the positions; more go by blocks.
+constexpr int share_rows(long hd) { return hd == 256 ? 16 : 32; }
 
-// The workgroups that share the positions, or 0: a workgroup per head.  That one needs no
-// join, but its longest head is the last to end, and few heads leave the chip idle.  (One
-// token, 8 KV heads of 128, shared / per head, us: 1 sequence of 100 8.5 / 5.8, of 300 9.2 /
-// 11.9, of 700 9.9 / 17; 64 of 250 22.9 / 18.4, of 1000 54 / 49, of 150 to 8000 200 / 241; 256
-// of 1 to 1000 138 / 107.)
-int share_wgs(long heads, long rows, long hd, long bound) {
-  const int cus = hn_device_cus();
-  if (rows > (hd == 256 ? 16 : kShareRows) || bound <= kGrain) return 0;
-  return heads >= 2 * cus && bound <= 1024 * (heads / cus) ? 0 : cus * resident(hd);
+// How a call runs, by its sizes alone: wgs workgroups that share the positions, or, with 0,
+// one per head; of runs of many rows, one per block and share of its positions, of `each`
+// stages.
+struct Way {
+  bool blocks;
+  int wgs, shares, each;
+  long entries, bytes;  // of workspace
+};
+
+// One per head needs no join, but its longest head is the last to end, and few heads leave
+// the chip idle.  (One token, 8 KV heads of 128, shared / per head, us: 1 sequence of 100 8.5
+// / 5.8, of 300 9.2 / 11.9, of 700 9.9 / 17; 64 of 250 22.9 / 18.4, of 1000 54 / 49, of 150 to
+// 8000 200 / 241; 256 of 1 to 1000 138 / 107.)
+Way way_of(long B, long nh, long nkv, long hd, long max_new, long bound) {
+  const long rows = nh / nkv * max_new, heads = B * nkv;
+  const int cus = hn_device_cus(), wgs = cus * resident(hd);
+  Way x = {rows > share_rows(hd), 0, 1, 1 << 30, 0, 0};
+  if (x.blocks) {
+    const long blocks = heads * hn_cdiv(rows, kBlock);
+    x.shares = (int)max(1l, min(wgs / blocks, bound / kShare));
+    if (x.shares > 1) {
+      x.each = hn_cdiv(hn_cdiv(bound, stage_of(hd)), x.shares);
+      x.entries = blocks * x.shares;
+      x.bytes = x.entries * kBlock * (hd + 2) * 4;
+    }
+  } else {
+    x.wgs = bound <= kGrain || (heads >= 2 * cus && bound <= 1024 * (heads / cus)) ? 0 : wgs;
+    x.bytes = 2l * x.wgs * rows * (hd + 2) * 4;
+  }
+  return x;
 }
-
-long part_bytes(long wgs, long rows, long hd) { return 2 * wgs * rows * (hd + 2) * 4; }
 
 template <class T, int HD, int NT>
 int attend_rows(const Attend<T>& A, int B, int nkv, hipStream_t stream) {
@@ -1050,27 +1160,31 @@ int attend_rows(const Attend<T>& A, int B, int nkv, hipStream_t stream) {
 }
 
 template <class T, int HD>
-int attend_hd(const Attend<T>& A, int B, int nkv, hipStream_t stream) {
-  if constexpr (HD != 256)
-    if (A.R > kShareRows) {
-      block_kernel<T, HD><<<dim3(nkv, hn_cdiv(A.R, kBlock), B), 256, 0, stream>>>(A);
-      HN_LAUNCH_CHECK("hn_paged_attention");
-      return 0;
-    }
+int attend_hd(const Attend<T>& A, bool by_blocks, int B, int nkv, hipStream_t stream) {
+  if (by_blocks) {
+    const int blocks = hn_cdiv(A.R, kBlock);
+    block_kernel<T, HD><<<dim3(nkv, blocks * A.shares, B), 256, 0, stream>>>(A);
+    HN_LAUNCH_CHECK("hn_paged_attention");
+    if (A.shares == 1) return 0;
+    join_blocks_kernel<T, HD><<<dim3(nkv, blocks * (HD / 8), B), 256, 0, stream>>>(A);
+    HN_LAUNCH_CHECK("hn_paged_attention");
+    return 0;
+  }
   if (A.R <= 16) return attend_rows<T, HD, 1>(A, B, nkv, stream);
   return attend_rows<T, HD, HD == 256 ? 1 : 2>(A, B, nkv, stream);
 }
 
 template <class T>
 int attend(const Step& P, const void* q, long ld_q, const void* k, const void* v, int nh, int hd,
-           int max_new, int wgs, float scale, void* out, long ld_o, void* work,
+           int max_new, const Way& way, float scale, void* out, long ld_o, void* work,
            hipStream_t stream) {
   const int rep = nh / P.nkv;
   const Attend<T> A = {P, (const T*)q, (const T*)k, (const T*)v, (T*)out, (float*)work, ld_q, ld_o,
-                       rep, max_new, rep * max_new, wgs, scale};
-  if (hd == 64) return attend_hd<T, 64>(A, P.B, P.nkv, stream);
-  if (hd == 128) return attend_hd<T, 128>(A, P.B, P.nkv, stream);
-  return attend_hd<T, 256>(A, P.B, P.nkv, stream);
+                       rep, max_new, rep * max_new, way.wgs, way.shares, way.each, way.entries,
+                       scale};
+  if (hd == 64) return attend_hd<T, 64>(A, way.blocks, P.B, P.nkv, stream);
+  if (hd == 128) return attend_hd<T, 128>(A, way.blocks, P.B, P.nkv, stream);
+  return attend_hd<T, 256>(A, way.blocks, P.B, P.nkv, stream);
 }
 
 }  // namespace
@@ -1100,8 +1214,7 @@ extern "C" long hn_paged_attention_workspace_bytes(const hn_paged_step* s) {
   if (!s || s->B <= 0 || s->T <= 0 || s->nkv <= 0 || s->nh < s->nkv || s->hd <= 0 ||
       s->max_new <= 0)
     return 0;
-  const long rows = s->nh / s->nkv * s->max_new;
-  return part_bytes(share_wgs(s->B * s->nkv, rows, s->hd, s->bound), rows, s->hd);
+  return way_of(s->B, s->nh, s->nkv, s->hd, s->max_new, s->bound).bytes;
 }
 
 extern "C" int hn_paged_attention(const hn_paged_step* step, const void* q, long ld_q, int dtype,
@@ -1123,14 +1236,12 @@ extern "C" int hn_paged_attention(const hn_paged_step* step, const void* q, long
                    ((uintptr_t)q | (uintptr_t)out) % 16 == 0,
                "hn_paged_attention: rows of %ld, strides of %ld and %ld: 16-byte aligned rows",
                nh * hd, ld_q, ld_o);
-  const long rows = nh / nkv * max_new;
-  const int wgs = share_wgs(P.B * nkv, rows, hd, step->bound);
-  HN_ARG_CHECK(wgs == 0 || (work && (uintptr_t)work % 16 == 0 &&
-                            work_bytes >= part_bytes(wgs, rows, hd)),
-               "hn_paged_attention: a workspace of %ld bytes, %ld given",
-               part_bytes(wgs, rows, hd), work ? work_bytes : 0);
+  const Way way = way_of(P.B, nh, nkv, hd, max_new, step->bound);
+  HN_ARG_CHECK(way.bytes == 0 || (work && (uintptr_t)work % 16 == 0 && work_bytes >= way.bytes),
+               "hn_paged_attention: a workspace of %ld bytes, %ld given", way.bytes,
+               work ? work_bytes : 0);
   return (dtype == 0 ? attend<h16> : attend<b16>)(P, q, ld_q, k, v, (int)nh, (int)hd,
-                                                  (int)max_new, wgs, scale, out, ld_o, work,
+                                                  (int)max_new, way, scale, out, ld_o, work,
                                                   (hipStream_t)stream);
 }
 
