@@ -13,6 +13,7 @@ import torch
 from .. import _lib
 
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+_I64, _I32, _F32 = torch.int64, torch.int32, torch.float32
 
 
 def _rows(x: torch.Tensor):
@@ -44,31 +45,37 @@ def adjust_logits(logits: torch.Tensor, text: Optional[torch.Tensor] = None,
     word, the lowest bit first) is zero become -inf.  repetition (above 0), presence and
     frequency: numbers, or fp32 [B].  out: logits itself, or another tensor of its
     shape, type and device that does not overlap it; None: a new one."""
-    dt, dev = logits.dtype, logits.device
+    dt, dev, at_dev = logits.dtype, logits.device, logits.get_device()
     assert logits.dim() == 2 and dt in _DTYPES and logits.shape[1] > 0, \
         "logits: fp16, bf16 or fp32 [B, V], V > 0"
     B, V = logits.shape
-    assert text is not None or (lens is None and prompt is None), "lens and prompt are of a text"
     if text is not None:
-        assert text.dtype == torch.int64 and text.dim() == 2 and text.shape[0] == B \
-            and text.device == dev, f"text: int64 [{B}, width] on {dev}"
-        lens, prompt = _each(lens, "lens", B, dev), _each(prompt, "prompt", B, dev)
-    rep, rep1 = _amount(repetition, "repetition", B, dev)
+        assert text.dtype is _I64 and text.dim() == 2 and text.shape[0] == B \
+            and text.get_device() == at_dev, f"text: int64 [{B}, width] on {dev}"
+        if lens is not None:
+            assert lens.dtype is _I64 and lens.shape == (B,) and lens.get_device() == at_dev, \
+                f"lens: int64 [{B}] on {dev}"
+        if prompt is not None:
+            assert prompt.dtype is _I64 and prompt.shape == (B,) \
+                and prompt.get_device() == at_dev, f"prompt: int64 [{B}] on {dev}"
+    else:
+        assert lens is None and prompt is None, "lens and prompt are of a text"
+    rep, rep1 = _amount(repetition, "repetition", B, at_dev)
     assert rep is not None or rep1 > 0.0, f"repetition {rep1}"
-    pres, pres1 = _amount(presence, "presence", B, dev)
-    freq, freq1 = _amount(frequency, "frequency", B, dev)
+    pres, pres1 = _amount(presence, "presence", B, at_dev)
+    freq, freq1 = _amount(frequency, "frequency", B, at_dev)
     ids, values = (None, None) if bias is None else bias
     if bias is not None:
-        assert ids.dtype == torch.int64 and ids.dim() == 2 and ids.shape[0] == B \
-            and values.dtype == torch.float32 and values.shape == ids.shape \
-            and ids.device == values.device == dev, \
+        assert ids.dtype is _I64 and ids.dim() == 2 and ids.shape[0] == B \
+            and values.dtype is _F32 and values.shape == ids.shape \
+            and ids.get_device() == values.get_device() == at_dev, \
             f"bias: (int64 [{B}, n], fp32 [{B}, n]) on {dev}"
     if allowed is not None:
-        assert allowed.dtype == torch.int32 and allowed.dim() == 2 and allowed.shape[0] == B \
-            and allowed.shape[1] >= -(-V // 32) and allowed.device == dev, \
+        assert allowed.dtype is _I32 and allowed.dim() == 2 and allowed.shape[0] == B \
+            and allowed.shape[1] >= -(-V // 32) and allowed.get_device() == at_dev, \
             f"allowed: int32 [{B}, {-(-V // 32)}] on {dev}"
     if out is not None:
-        assert out.shape == logits.shape and out.dtype == dt and out.device == dev \
+        assert out.shape == logits.shape and out.dtype is dt and out.device == dev \
             and out.stride(1) == 1 and (B <= 1 or out.stride(0) >= V), \
             "out: shape, type and device of logits, dense rows"
     if not logits.is_cuda:
@@ -76,15 +83,20 @@ def adjust_logits(logits: torch.Tensor, text: Optional[torch.Tensor] = None,
             torch.full((B,), n) if x is None else x
             for x, n in ((rep, rep1), (pres, pres1), (freq, freq1))], ids, values, allowed)
         return y if out is None else out.copy_(y)
-    src, ld = (logits, max(out.stride(0), V)) if out is logits else _rows(logits)
+    ld_o = V if out is None else max(out.stride(0), V)
+    src, ld = (logits, ld_o) if out is logits else _rows(logits)
     if out is None:
         out = src.new_empty((B, V))
     at = ld_t = width = at_lens = at_prompt = at_ids = ld_i = at_v = ld_v = n = at_a = ld_a = 0
     if text is not None:
         text, ld_t = _rows(text)
         at, width = text.data_ptr(), text.shape[1]
-        at_lens = 0 if lens is None else lens.data_ptr()
-        at_prompt = 0 if prompt is None else prompt.data_ptr()
+        if lens is not None:
+            lens = lens.contiguous()
+            at_lens = lens.data_ptr()
+        if prompt is not None:
+            prompt = prompt.contiguous()
+            at_prompt = prompt.data_ptr()
     if ids is not None:
         ids, ld_i = _rows(ids)
         values, ld_v = _rows(values)
@@ -96,25 +108,16 @@ def adjust_logits(logits: torch.Tensor, text: Optional[torch.Tensor] = None,
                  at_lens, at_prompt, 0 if rep is None else rep.data_ptr(),
                  0 if pres is None else pres.data_ptr(), 0 if freq is None else freq.data_ptr(),
                  rep1, pres1, freq1, at_ids, ld_i, at_v, ld_v, n, at_a, ld_a, B, V,
-                 out.data_ptr(), max(out.stride(0), V))
+                 out.data_ptr(), ld_o)
     return out
 
 
-def _each(x, name, B, dev):
-    """An int64 [B] or None."""
-    if x is None:
-        return None
-    assert x.dtype == torch.int64 and x.shape == (B,) and x.device == dev, \
-        f"{name}: int64 [{B}] on {dev}"
-    return x if x.stride(0) == 1 else x.contiguous()
-
-
-def _amount(x, name, B, dev):
+def _amount(x, name, B, at_dev):
     """(fp32 [B] or None, else the number)."""
     if isinstance(x, torch.Tensor):
-        assert x.dtype == torch.float32 and x.shape == (B,) and x.device == dev, \
-            f"{name}: a number or fp32 [{B}] on {dev}"
-        return (x if x.stride(0) == 1 else x.contiguous()), 0.0
+        assert x.dtype is _F32 and x.shape == (B,) and x.get_device() == at_dev, \
+            f"{name}: a number or fp32 [{B}] on the logits' device"
+        return x.contiguous(), 0.0
     x = float(x)
     assert math.isfinite(x), f"{name} {x}"
     return None, x
