@@ -1232,7 +1232,8 @@ extern "C" int hn_paged_attention(const hn_paged_step* step, const void* q, long
   Step P;
   if (int rc = check_step("hn_paged_attention", step, q, k, v, dtype, P)) return rc;
   const long nh = step->nh, nkv = step->nkv, hd = step->hd, max_new = step->max_new;
-  HN_ARG_CHECK(max_new >= 1 && step->bound >= 1 && max_new <= (1l << 24) / nh,
+  HN_ARG_CHECK(max_new >= 1 && step->bound >= 1 && max_new <= (1l << 24) / nh &&
+                   nh / nkv * max_new <= 65535l * kBlock,
                "hn_paged_attention: max_new %ld, bound %ld", max_new, step->bound);
   HN_ARG_CHECK(P.cols < 1l << 26 && P.cols * P.page < 1l << 30 &&
                    (double)P.B * nkv * (P.cols * P.page / kGrain + 1) < 2147483648.0,

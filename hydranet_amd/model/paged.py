@@ -110,6 +110,8 @@ class PagedKVCache:
         full, rest = divmod(length, self.page_size)
         assert 0 <= length and len(pages) >= full + (rest > 0), \
             f"{len(pages)} pages for {length} positions"
+        assert all(0 <= p < self.num_pages and self._users[p] > 0 for p in pages[:full + 1]), \
+            "only pages that are taken can be shared"
         mine = self.take(1) if rest else []
         self.share(pages[:full])
         if rest:
@@ -230,7 +232,10 @@ class PagedBatch:
                  starts: Optional[torch.Tensor] = None, rows: Optional[int] = None,
                  max_new: int = 1):
         dev = table.device
-        assert table.dtype == torch.int32 and table.dim() == 2, "table: int32 [B, columns]"
+        assert table.dtype == torch.int32 and table.dim() == 2 \
+            and (table.shape[1] <= 1 or table.stride(1) == 1) \
+            and (table.shape[0] <= 1 or table.stride(0) >= table.shape[1]), \
+            "table: int32 [B, columns], dense rows"
         B = table.shape[0]
         assert lens.dtype == torch.int64 and tuple(lens.shape) == (B,) and lens.device == dev \
             and lens.is_contiguous(), f"lens: int64 [{B}] on {dev}, contiguous"
@@ -241,12 +246,9 @@ class PagedBatch:
             assert starts.dtype == torch.int32 and tuple(starts.shape) == (B + 1,) \
                 and starts.device == dev and starts.is_contiguous(), \
                 f"starts: int32 [{B + 1}] on {dev}, contiguous"
-            assert rows is not None and rows >= 0 and max_new >= 1, \
-                "starts needs the step's rows and max_new"
+            assert rows is not None and rows >= 0 and max_new >= 1 and (B or not rows), \
+                "starts needs the step's rows and max_new, rows need a sequence"
         assert kv_bound >= 1, f"kv_bound {kv_bound}"
-        if table.stride(1) != 1 and table.shape[1] > 1 or table.stride(0) < table.shape[1] \
-                and B > 1:
-            table = table.contiguous()
         self.table, self.lens, self.starts = table, lens, starts
         self.size, self.rows, self.max_new, self.kv_bound = B, rows, max_new, kv_bound
         self.device = dev
@@ -270,7 +272,8 @@ class PagedBatch:
                            self.rows, num_heads, nkv, hd, cache.page_size, self.max_new,
                            self.kv_bound)
         at = ctypes.addressof(s)
-        made = (s, at, _lib.lib().hn_paged_attention_workspace_bytes(at))
+        with torch.cuda.device(self.device):  # (it goes by the device's CUs)
+            made = (s, at, _lib.lib().hn_paged_attention_workspace_bytes(at))
         self._made = (cache, num_heads, made)
         return made
 
@@ -384,7 +387,7 @@ def paged_attention(q: torch.Tensor, batch: PagedBatch, cache: PagedKVCache, lay
             q, ld = _lib.aligned_rows(q.contiguous()), columns
         out = q.new_empty((T, columns))
         _, step, n = batch._step(cache, nh)
-        work = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+        work = q.new_empty((n // 2,)) if n else None  # (two bytes each)
         _lib.call_on(q.device, "hn_paged_attention", step, q.data_ptr(), ld, _DTYPES[q.dtype],
                      k.data_ptr(), v.data_ptr(), scale, out.data_ptr(), columns,
                      None if work is None else work.data_ptr(), n)

@@ -116,19 +116,25 @@ def test_pages_that_are_not_named(counts, hint):
     assert got.isnan().all() and starts[-1] == s["rows"]
 
 
-@pytest.mark.parametrize("rep,hd", [(4, 128), (1, 64), (20, 64), (2, 256)])
-def test_values_that_are_no_numbers(rep, hd):
+@pytest.mark.parametrize("hint", [None, 5000])
+@pytest.mark.parametrize("rep,hd,n", [(4, 128, 50), (1, 64, 50), (20, 64, 50), (2, 256, 50),
+                                      (4, 128, 4), (4, 64, 8), (2, 256, 8)])
+def test_values_that_are_no_numbers(rep, hd, n, hint):
     """A value that is NaN or infinite reaches the rows that see it and no other."""
     from hydranet_amd.model.paged import paged_attention
-    C, n = 37, 50
+    C = 1037
     s = ref.make(6, [C, 5], [n, 8], 1, hd, 16, torch.float16, DEV, poison=True)
     q = torch.randn(s["rows"], rep * hd, generator=s["gen"]).half().to(DEV)
-    want = paged_attention(q, ref.batch(s, False), _cache(s), 0)
-    for at, d, x in ((C + 20, 3, math.nan), (C + 49, hd - 1, math.inf), (C + 1, 0, -math.inf)):
+
+    def run():
+        return paged_attention(q, ref.batch(s, False, hint), _cache(s), 0)
+    want = run()
+    for at, d, x in ((C + n // 2, 3, math.nan), (C + n - 1, hd - 1, math.inf),
+                     (C + 1, 0, -math.inf)):
         old = s["v"].clone()
         p = int(s["table"][0, at // 16])
         s["v"][p, 0, at % 16 // 8, d, at % 8] = x
-        got = paged_attention(q, ref.batch(s, False), _cache(s), 0).view(-1, rep, hd)
+        got = run().view(-1, rep, hd)
         s["v"].copy_(old)
         w = want.view(-1, rep, hd).clone()
         w[at - C:n, :, d] = x
@@ -138,11 +144,62 @@ def test_values_that_are_no_numbers(rep, hd):
         assert hit.isnan().all() if math.isnan(x) else (hit == x).all()
         assert torch.equal(got[other], w[other])
     # a key: its scores are no numbers, so neither are the rows that see it
-    at = C + 11
+    at = C + n // 2
     s["k"][int(s["table"][0, at // 16]), 0, at % 16, 1] = math.nan
-    got = paged_attention(q, ref.batch(s, False), _cache(s), 0)
-    assert got[11:n].isnan().all() and torch.equal(got[:11], want[:11])
+    got = run()
+    assert got[n // 2:n].isnan().all() and torch.equal(got[:n // 2], want[:n // 2])
     assert torch.equal(got[n:], want[n:])
+
+
+@pytest.mark.parametrize("hint", [None, 9000])
+@pytest.mark.parametrize("runs", [False, True])
+def test_many_sequences(runs, hint):
+    """Hundreds of sequences of ragged lengths, some without part, some without rows."""
+    from hydranet_amd.model.paged import RotaryTable, paged_append, paged_attention
+    g = torch.Generator().manual_seed(1)
+    B = 210
+    lens = (torch.rand(B, generator=g) ** 3 * 700).long().tolist()
+    counts = (torch.rand(B, generator=g) ** 4 * 30).long().tolist() if runs else None
+    for b in range(0, B, 7):
+        lens[b] = -1
+    s = ref.make(12, lens, counts, 1, 64, 16, torch.float16, DEV, poison=True)
+    one = ref.batch(s, not runs, hint)
+    q = torch.randn(s["rows"], 3 * 64, generator=s["gen"]).half()
+    want, bound = ref.attend(s, q, 3)
+    got = paged_attention(q.to(DEV), one, _cache(s), 0)
+    assert ((got.double().cpu() - want).abs() <= bound).all()
+    cos, sin = ref.tables(64, 800)
+    qkv = torch.randn(s["rows"], 5 * 64, generator=s["gen"]).half()
+    q = paged_append(qkv.to(DEV), RotaryTable.wrap(cos.to(DEV), sin.to(DEV)), one, _cache(s), 0, 3)
+    live = torch.zeros(s["rows"], dtype=torch.bool)
+    k, v, table = s["k"].cpu(), s["v"].cpu(), s["table"].cpu()
+    for row, b, pos in ref.tokens({n: s[n].cpu() for n in ("starts", "lens")}):
+        live[row] = True
+        x = qkv[row].view(5, 64)
+        y = ref.rotate(x[:4].double(), cos[pos], sin[pos], "half")
+        out = torch.cat((q[row].cpu().view(3, 64), k[table[b, pos // 16], :, pos % 16])).double()
+        assert ((out - y).abs() <= 2.0 ** -11 * y.abs() + 2.0 ** -20).all()
+        assert torch.equal(v[table[b, pos // 16], 0, pos % 16 // 8, :, pos % 8], x[4])
+    assert not q[~live.to(DEV)].any()
+
+
+def test_two_calls_at_once():
+    """Attention of two batches on two streams, each with its own workspace."""
+    from hydranet_amd.model.paged import paged_attention
+    work = []
+    for seed, lens in ((1, [9000, 100]), (2, [3000, 5000, 7000])):
+        s = ref.make(seed, lens, None, 2, 128, 64, torch.float16, DEV)
+        q = torch.randn(len(lens), 8 * 128, generator=s["gen"]).half().to(DEV)
+        work.append((q, ref.batch(s, True), _cache(s), torch.cuda.Stream()))
+    want = [paged_attention(q, one, cache, 0) for q, one, cache, _ in work]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(20):
+        for q, one, cache, stream in work:
+            with torch.cuda.stream(stream):
+                got.append(paged_attention(q, one, cache, 0))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[i % 2]) for i, x in enumerate(got))
 
 
 @pytest.mark.parametrize("layout", ["half", "interleaved"])

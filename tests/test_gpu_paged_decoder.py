@@ -73,6 +73,24 @@ def test_ragged_steps_equal_each_text_alone(model):
     assert at == [90, 7, 40, 130]
 
 
+def test_int4_projections():
+    """The same with the attention's projections in INT4, stacked into one launch."""
+    from hydranet_amd.model.decoder import (MixtralDecoderConfig, build_synthetic_decoder,
+                                            convert_dense_to_int4)
+    from hydranet_amd.model.paged import PagedBatch, PagedKVCache
+    cfg = MixtralDecoderConfig(num_layers=2, hidden_dim=512, intermediate_dim=1024,
+                               num_attention_heads=8, num_kv_heads=2, head_dim=128, vocab_size=V,
+                               num_experts=8, experts_per_token=2, max_position_embeddings=256)
+    m = convert_dense_to_int4(build_synthetic_decoder(cfg, DEV, decode_top_k=2, seed=4))
+    texts = _prompts([30, 12])
+    cache = PagedKVCache(2, 8, 2, 128, 16, DEV)
+    table = cache.table([cache.take(2), cache.take(1)])
+    starts = torch.tensor([0, 30, 42], dtype=torch.int32, device=DEV)
+    one = PagedBatch(table, torch.zeros(2, dtype=torch.int64, device=DEV), 30, starts, 42, 30)
+    got = m.forward_paged(torch.tensor(sum(texts, []), device=DEV), one, cache, 2)
+    _close(got, torch.cat([_alone(m, t) for t in texts]))
+
+
 def test_logits_of_chosen_rows(model):
     from hydranet_amd.model.paged import PagedBatch, PagedKVCache
     texts = _prompts([20, 33])

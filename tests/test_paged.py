@@ -140,6 +140,9 @@ def test_pages():
     assert c.free_pages == 10
     with pytest.raises(AssertionError, match="taken"):
         c.share([0])
+    with pytest.raises(AssertionError, match="taken"):
+        c.fork([0, 1], 20)
+    assert c.free_pages == 10
     assert c.table([[1, 2], [], [3]]).tolist() == [[1, 2], [-1, -1], [3, -1]]
     assert c.table([[1]], 3).tolist() == [[1, -1, -1]]
     for src, dst in (([0], [0]), ([0, 1], [1, 2]), ([0, 0], [3, 3]), ([10], [1]), ([0], [-1]),
@@ -229,6 +232,9 @@ def test_refusals():
     starts = torch.tensor([0, 1, 2], dtype=torch.int32)
     _refused("table", PagedBatch, t.long(), lens, 9)
     _refused("table", PagedBatch, t[0], lens, 9)
+    _refused("table", PagedBatch, torch.zeros(3, 2, dtype=torch.int32).t(), lens, 9)
+    _refused("table", PagedBatch, torch.zeros(1, 3, dtype=torch.int32).expand(2, 3), lens, 9)
+    _refused("sequence", PagedBatch, t[:0], lens[:0], 9, starts[:1], 4)
     _refused("lens", PagedBatch, t, lens.int(), 9)
     _refused("lens", PagedBatch, t, lens[:1], 9)
     _refused("kv_bound", PagedBatch, t, lens, 0)
@@ -317,7 +323,8 @@ def test_library_refusals():
                        dict(scale=math.nan), dict(scale=3e38), dict(new=0), dict(bound=0),
                        dict(n=0), dict(cols=1 << 26, ldt=1 << 26), long,
                        dict(long, work=16, bytes_=need - 1), dict(long, work=8, bytes_=need),
-                       dict(new=1 << 23)):
+                       dict(new=1 << 23),
+                       dict(nh=1, ld=512, new=1 << 24)):
         with pytest.raises(RuntimeError, match="hn_paged_attention"):
             attend(**kw)
 
