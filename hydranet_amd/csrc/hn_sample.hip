@@ -40,7 +40,8 @@ __device__ __forceinline__ Some<T, N> read(const T* p) {
 template <class T, int N>
 __global__ __launch_bounds__(kThreads) void adjust_kernel(Adjust A, const T* logits, long ld,
                                                           T* out, long ld_o) {
-  extern __shared__ uint32_t s_count[];
+  extern __shared__ __align__(16) uint32_t s_count[];
+  typedef uint32_t Words __attribute__((ext_vector_type(N)));
   constexpr int kChunk = kThreads * N;
   int* s_bias = reinterpret_cast<int*>(s_count + kChunk);
   const int b = blockIdx.y, tid = threadIdx.x;
@@ -62,11 +63,8 @@ __global__ __launch_bounds__(kThreads) void adjust_kernel(Adjust A, const T* log
   const float freq = A.freq ? A.freq[b] : A.freq1;
   const bool counts = A.text != nullptr, biases = A.n > 0;
   if (counts || biases) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      s_count[tid + i * kThreads] = 0;
-      if (biases) s_bias[tid + i * kThreads] = -1;
-    }
+    *reinterpret_cast<Words*>(s_count + tid * N) = Words{};
+    if (biases) *reinterpret_cast<Words*>(s_bias + tid * N) = Words{} - 1;
     __syncthreads();
     if (counts) {
       long n = A.lens ? A.lens[b] : A.width;
@@ -101,16 +99,19 @@ __global__ __launch_bounds__(kThreads) void adjust_kernel(Adjust A, const T* log
     }
     __syncthreads();
   }
+  Words many = Words{}, last = Words{} - 1;
+  if (counts) many = *reinterpret_cast<const Words*>(s_count + tid * N);
+  if (biases) last = *reinterpret_cast<const Words*>(s_bias + tid * N);
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     float y = (float)x[i];
-    const uint32_t c = counts ? s_count[tid * N + i] : 0u;
+    const uint32_t c = many[i];
     if (c) {
       y = y > 0.f ? y / r : y * r;
       const uint32_t n = c & ~kSeen;
       if (n) y = y - freq * (float)n - pres;
     }
-    const int at = biases ? s_bias[tid * N + i] : -1;
+    const int at = (int)last[i];
     if (at >= 0) y += A.bias[b * A.ld_bias + at];
     if (!((word >> ((v + i) & 31)) & 1u)) y = -__builtin_inff();
     x[i] = (T)y;
