@@ -35,8 +35,12 @@ struct Vec<b16> {
 };
 
 // ---------------------------------------------------------------------------
-// The append.  One thread per element, grid (T, nh + 2 nkv): rows and rotated parts of any
-// alignment.
+// The append.  Bytes are all there is: projections read, queries and pages written, 54 to 57
+// us for prompts of 9520 tokens, 32 heads over 8 of 128 (239 MB, 4.2 to 4.4 TB/s; a large copy
+// moves 5.1), 4.9 us for 64 single tokens, where the latency of lengths, tables and angles
+// after each other counts.
+//
+// One thread per element, grid (T, nh + 2 nkv): rows and rotated parts of any alignment.
 template <class T>
 __global__ __launch_bounds__(256) void append_kernel(Step P, const T* __restrict__ qkv, long ld,
                                                      const float* __restrict__ cos_t,
@@ -222,6 +226,12 @@ __global__ __launch_bounds__(256) void append_rows_kernel(
 // dimensions are consecutive, and so are 8 positions of a value's dimension.  Block t's
 // row 4 c + i is position 8 c + 4 t + i, so that a lane's scores of both blocks are the 8
 // consecutive positions that its lane of the value operand holds.
+//
+// One token per sequence is bound by the cache's bytes, 8 KV heads of 128 and 4 query heads
+// each: 64 sequences of 150 to 8000 197 to 231 us (1.07 GB, 4.6 to 5.4 TB/s; a large copy moves
+// 5.1), 64 of 2000 91 us (5.8), and, of few positions, by memory's latency: one text of 701
+// 9.3 us in two launches.  A wave's products are 13 times as fast as its bytes come, so the
+// 4 rows of 16 that it uses cost nothing.
 constexpr int kTile = 32;
 constexpr int NW = 4;  // waves of a workgroup
 // Workgroups that a CU's registers hold at once.  (Three of 128 dimensions spill: one text of
@@ -244,7 +254,9 @@ struct Attend {
   Step P;
   const T *q, *k, *v;
   T* out;
-  float* part;  // entries of R rows of HD sums, then of R (maximum, sum)
+  // entries of the workspace: R (of blocks: 128) rows of HD sums each, then of as many
+  // (maximum, sum)
+  float* part;
   long ld_q, ld_o;
   int rep, max_new, R, wgs;
   int shares, each;  // of a block's positions, and the stages of one
@@ -268,8 +280,8 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 
 // A sequence's rows [row, row + n) of the step, its cached positions C and the end L of
 // those that are read.  Positions past the table's are all one to a row that sees them,
-// so neither C nor L exceeds the first of them by more than 1.  n < 0: rows that are
-// zero (no part), or NaN (more than max_new).
+// so neither C nor L exceeds the first of them by more than 1.  none: rows that are zero
+// (no part); nan: NaN (more than max_new).
 struct Run {
   int row, n, C, L;
   bool none, nan;
@@ -601,8 +613,18 @@ __device__ __forceinline__ void finish(const Attend<T>& A, const Sums<T, HD, NT>
 // a wave, and walks the positions in stages that all four read from LDS; the next stage
 // goes from memory to LDS (buffer_load ... lds) meanwhile.  A stage lies there as in the
 // pages, but that a key's 16-byte chunks are at chunk ^ key(position), so that the 16
-// positions that a read takes cover the banks once.  Two workgroups per CU: one's loads
-// and softmax under the other's products.
+// positions that a read takes cover the banks once (the counter of conflicts stays at 0).
+// Two workgroups per CU: one's loads and softmax under the other's products.
+//
+// Bounds: where there are several workgroups for each place, the matrix units beside the
+// exponentials and the LDS reads (4000 rows after 4000 positions: 391 us, 1.0 PFLOP/s, a large
+// product reaches 1.17); where each has about one, the longest block's stages after each
+// other (1.9 us each alone on a CU) while others are done: runs of 1000, 688 and 376 after
+// 900 to 4000 128 to 146 us, 0.66 to 0.75 PFLOP/s, the CUs busy in 64 % of the time.
+// Measured and not taken: all blocks' stages dealt evenly to the workgroups (they then walk
+// different positions at once, out of L2: 4000 after 4000 462 us, with a plan and joins of 23
+// us); five smaller stages in LDS, four of them on their way, and scores made a stage ahead
+// beside the exponentials (no difference); more shares than places (146 to 201).
 constexpr int kBlock = 128;
 constexpr int stage_of(int hd) { return hd == 256 ? 32 : 64; }
 
@@ -834,7 +856,9 @@ __device__ __forceinline__ void block_range(const Attend<T>& A, const Run& r, in
 }
 
 // A workgroup per (KV head, block and share of its positions, sequence), the longest blocks
-// of a run first.  A block's A.each stages a share (the rest in the last); its entry of the
+// of a run first.  A head's blocks side by side walk the same positions at once, so all but
+// the first find them in the XCD's L2: with the sequences side by side instead, 8 of 1000
+// rows after 3000 take 392 us, as it is 299.  A block's A.each stages a share (the rest in the last); its entry of the
 // workspace goes by the block and the share.
 template <class T, int HD>
 __global__ __launch_bounds__(256, resident(HD)) void block_kernel(Attend<T> A) {
