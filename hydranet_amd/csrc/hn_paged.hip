@@ -246,7 +246,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kUp = 8.f, kLag = 6.f;
 // Positions that workgroups share out as one.
 constexpr int kGrain = 128;
-// Positions that a share of a block's has at least.
+// Positions that a share of a block's has at least.  (80 rows of one sequence of 1020: 16.5
+// us, of 1024 or one share 30.)
 constexpr long kShare = 256;
 
 template <class T>
@@ -1104,8 +1105,10 @@ int check_step(const char* who, const hn_paged_step* s, const void* x, const voi
   return 0;
 }
 
-// Rows from which a thread takes four heads of a token, so that it reads the angles once.
-constexpr int kManyRows = 1024;
+// Rows from which a thread takes four heads of a token, so that it reads the angles once
+// (9520 rows 54 us, with one head a thread 77; 500 7.3 / 8.1, 100 5.2 / 5.2, 64 single tokens
+// 5.7 / 5.0).
+constexpr int kManyRows = 256;
 
 template <class T, int HD>
 void append_rows(const Step& P, const T* qkv, long ld, const float* cos_t, const float* sin_t,
@@ -1143,8 +1146,9 @@ int append(const Step& P, const void* qkv_, long ld, const float* cos_t, const f
 }
 
 // Rows of one (sequence, KV head) up to which a workgroup takes all of them for a share of
-// the positions; more go by blocks.
-constexpr int share_rows(long hd) { return hd == 256 ? 16 : 32; }
+// the positions; more go by blocks.  (Shared / by blocks, us: 20 rows of 1 sequence of 3000
+// 12.4 / 14.7, of 8 30.8 / 31.7; 32 rows of 8 33.1 / 31.3, of 64 180 / 166.)
+constexpr int share_rows(long hd) { return hd == 256 ? 16 : 24; }
 
 // How a call runs, by its sizes alone: wgs workgroups that share the positions, or, with 0,
 // one per head; of runs of many rows, one per block and share of its positions, of `each`
@@ -1161,6 +1165,7 @@ struct Way {
 // 8000 200 / 241; 256 of 1 to 1000 138 / 107.)
 Way way_of(long B, long nh, long nkv, long hd, long max_new, long bound) {
   const long rows = nh / nkv * max_new, heads = B * nkv;
+  bound = min(bound, 1l << 30);  // (no table has more positions)
   const int cus = hn_device_cus(), wgs = cus * resident(hd);
   Way x = {rows > share_rows(hd), 0, 1, 1 << 30, 0, 0};
   if (x.blocks) {

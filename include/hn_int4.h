@@ -560,7 +560,8 @@ typedef struct hn_paged_step {
  *   [T][nh * hd], keys and values to their pages.  Rows of a sequence with a
  *   negative length write no page and zero queries; a row whose position is past
  *   cos_t, or whose page the table does not name (past its columns, or an id
- *   outside [0, num_pages)), writes no page and NaN queries. */
+ *   outside [0, num_pages)), writes no page and NaN queries.  q_out overlaps
+ *   nothing that is read. */
 int hn_paged_append(const hn_paged_step* step, const void* qkv, long ld_qkv, int dtype,
                     const float* cos_t, const float* sin_t, long table_rows, long rotary,
                     int interleaved, void* q_out, void* k, void* v, void* stream);
@@ -573,8 +574,8 @@ int hn_paged_append(const hn_paged_step* step, const void* qkv, long ld_qkv, int
  *   of a sequence with more than max_new of them.  A position that a row does not
  *   see has no effect on it, whatever it holds.  scale above 0 and finite, also
  *   times log2(e); 16-byte aligned operands, ld_q and ld_o multiples of 8; cols *
- *   page < 2^30.  work: hn_paged_attention_workspace_bytes(step) bytes, 16-byte
- *   aligned, any contents. */
+ *   page < 2^30; out overlaps nothing that is read.  work:
+ *   hn_paged_attention_workspace_bytes(step) bytes, 16-byte aligned, any contents. */
 long hn_paged_attention_workspace_bytes(const hn_paged_step* step);
 int hn_paged_attention(const hn_paged_step* step, const void* q, long ld_q, int dtype,
                        const void* k, const void* v, float scale, void* out, long ld_o,

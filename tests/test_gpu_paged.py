@@ -48,7 +48,7 @@ def test_attention(i, dt):
     # bounds are hints, and rows may have a stride
     wide = torch.randn(s["rows"], nkv * rep * hd + 8, device=DEV).to(q.dtype)
     wide[:, :q.shape[1]] = q
-    for hint in (1, 100, 5000):
+    for hint in (1, 100, 5000, 2 ** 40):
         two = paged_attention(wide[:, :q.shape[1]], ref.batch(s, counts is None, hint), _cache(s),
                               0)
         assert ((two.double().cpu() - want).abs() <= bound).all()
