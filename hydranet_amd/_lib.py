@@ -128,21 +128,27 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+def _failed(name: str, rc: int) -> None:
+    msg = lib().hn_last_error_string().decode(errors="replace")
+    raise RuntimeError(f"{name} failed (rc={rc}): {msg}")
+
+
 def call(name: str, *args) -> None:
     rc = getattr(lib(), name)(*args)
     if rc != 0:
-        msg = lib().hn_last_error_string().decode(errors="replace")
-        raise RuntimeError(f"{name} failed (rc={rc}): {msg}")
+        _failed(name, rc)
 
 
 def call_on(device: torch.device, name: str, *args) -> None:
     """call() on the current stream of `device`, added as the last argument, with it
     as the current device."""
-    at = torch.cuda.current_device()
+    at = torch._C._cuda_getDevice()
     index = at if device.index is None else device.index
     stream_ = torch._C._cuda_getCurrentRawStream(index)
     if index == at:
-        call(name, *args, stream_)
+        rc = getattr(_lib or lib(), name)(*args, stream_)
+        if rc != 0:
+            _failed(name, rc)
     else:
         with torch.cuda.device(device):
             call(name, *args, stream_)

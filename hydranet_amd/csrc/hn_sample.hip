@@ -135,7 +135,9 @@ __global__ __launch_bounds__(kThreads) void adjust_kernel(Adjust A, const T* log
 }
 
 // As few tokens a thread as give about two workgroups per CU, 8 at most: every workgroup
-// reads the whole text.
+// reads the whole text.  (1, 4 and 8 a thread, us: one row of 32000 3.1, 3.6, 4.5; 64 rows of
+// 32000, texts to 8000, 18.1, 9.4, 9.2, without texts 9.0, 4.8, 5.1; 256 rows 34, 15.6, 12.8; 64
+// of 130001 51, 23.2, 21.3.)
 template <class T>
 int adjust(const Adjust& A, const void* logits, long ld, void* out, long ld_o, long B,
            hipStream_t stream) {

@@ -211,8 +211,7 @@ class RotaryTable:
         self.cos, self.sin, self.layout = cos.contiguous(), sin.contiguous(), layout
         self.dim, self.device = 2 * cos.shape[1], cos.device
 
-    @property
-    def args(self):
+    def _args(self):
         """The angles' arguments of a library call."""
         return (self.cos.data_ptr(), self.sin.data_ptr(), self.cos.shape[0], self.dim,
                 self.layout == "interleaved")
@@ -251,7 +250,7 @@ class PagedBatch:
         assert kv_bound >= 1, f"kv_bound {kv_bound}"
         self.table, self.lens, self.starts = table, lens, starts
         self.size, self.rows, self.max_new, self.kv_bound = B, rows, max_new, kv_bound
-        self.device = dev
+        self.device, self.index = dev, table.get_device()
         self._made = None
 
     def _step(self, cache: PagedKVCache, num_heads: int):
@@ -305,9 +304,10 @@ def _check(batch: PagedBatch, cache: PagedKVCache, layer: int, x: torch.Tensor,
     k = cache.k[layer]
     assert x.shape == (batch.rows, columns), \
         f"{name} {tuple(x.shape)} vs {batch.rows} rows of {columns}"
-    assert x.device == batch.device == k.device, \
+    at = x.get_device()
+    assert at == batch.index and at == k.get_device(), \
         f"{name} on {x.device}, the batch on {batch.device}, the cache on {k.device}"
-    assert x.dtype == k.dtype, f"{name} {x.dtype}, the cache {k.dtype}"
+    assert x.dtype is k.dtype, f"{name} {x.dtype}, the cache {k.dtype}"
     return k
 
 
@@ -333,7 +333,7 @@ def paged_append(qkv: torch.Tensor, rope: RotaryTable, batch: PagedBatch, cache:
             qkv, ld = qkv.contiguous(), columns
         q = qkv.new_empty((T, num_heads * hd))
         _lib.call_on(qkv.device, "hn_paged_append", batch._step(cache, num_heads)[1],
-                     qkv.data_ptr(), ld, _DTYPES[qkv.dtype], *rope.args, q.data_ptr(),
+                     qkv.data_ptr(), ld, _DTYPES[qkv.dtype], *rope._args(), q.data_ptr(),
                      k.data_ptr(), v.data_ptr())
         return q
     wide = torch.float64 if qkv.dtype == torch.float64 else torch.float32
