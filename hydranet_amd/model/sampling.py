@@ -18,6 +18,8 @@ _I64, _I32, _F32 = torch.int64, torch.int32, torch.float32
 
 def _rows(x: torch.Tensor):
     """x with its last axis dense and rows that do not overlap, and their stride."""
+    if x.is_contiguous():
+        return x, x.shape[1]
     ld, last = x.stride()
     if last != 1 or ld < x.shape[1]:
         x = x.contiguous()
