@@ -370,10 +370,19 @@ __device__ __forceinline__ int grains_below(const Attend<T>& A, int to) {
   return __builtin_amdgcn_readlane(lane_scan(n), 63);
 }
 
-// Of 8 positions from `at` on, the values that must not reach a product: at positions past
-// hi, which no row sees (their probabilities are zero, but what lies there may be
-// anything), and, at those past lo, which only some rows see, NaN and infinities, as 0
-// times them would reach the others.  Returns whether there was such a one.
+// Values that are no numbers.  A row has the infinities and NaN of the positions that it
+// sees in their dimensions, whatever their weights: a softmax's are above 0.  A product
+// would make NaN of an infinity where the probability was rounded to 0, or with what its
+// rounding left (of either sign, or 0), and give it to the rows that do not see it, too.
+// So at positions that only some rows see (past lo) they are taken out of the products and
+// added afterwards; among the others a first walk looks for none, its sums tell whether
+// there was one, and if so a second takes them out everywhere (lo = -1).  The joins keep
+// them from weights of 0 (weight).
+//
+// Of 8 positions from `at` on, the values that must not reach a product: those at positions
+// past hi, which no row sees (their probabilities are zero, but what lies there may be
+// anything), and those past lo that are no numbers.  Returns whether there was one of the
+// latter.
 template <class T, int E>
 __device__ __forceinline__ uint32_t clean(typename Vec<T>::t (&v)[E], int at, int lo, int hi) {
   uint32_t odd = 0;
@@ -394,14 +403,14 @@ __device__ __forceinline__ uint32_t clean(typename Vec<T>::t (&v)[E], int at, in
   return odd;
 }
 
-// Those values, added to the rows that see them.  mine(p): whether this wave had position p.
-template <class T, int HD, int NT, class F>
+// Those of positions [from, to], added to the rows that see them.
+template <class T, int HD, int NT>
 __device__ __forceinline__ void add_odd(const Attend<T>& A, float4v (&o)[NT][HD / 16],
-                                        const int (&lim)[NT], int b, int g, int lo, int hi, int kg,
-                                        F mine) {
+                                        const int (&lim)[NT], int b, int g, int from, int to,
+                                        int kg) {
   const Step& P = A.P;
-  for (int p = lo + 1; p <= hi; ++p) {
-    const long id = mine(p) ? page_of(P, b, p) : -1;
+  for (int p = from; p <= to; ++p) {
+    const long id = page_of(P, b, p);
     if (id < 0) continue;
     const int slot = p & (P.page - 1);
     const T* v = A.v + ((id * P.nkv + g) * P.page + (slot & ~7)) * HD + (slot & 7);
@@ -417,11 +426,34 @@ __device__ __forceinline__ void add_odd(const Attend<T>& A, float4v (&o)[NT][HD 
   }
 }
 
+// NaN if one of a row's sums is no number (else 0).
+template <int N>
+__device__ __forceinline__ float probe(const float4v (&o)[N]) {
+  float4v x = (float4v)(0.f);
+#pragma unroll
+  for (int e = 0; e < N; ++e)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) x[c] = __builtin_fmaf(o[e][c], 0.f, x[c]);
+  return (x[0] + x[1]) + (x[2] + x[3]);
+}
+
+// The weight 2^x of sums in a join: above 0, so that an infinity stays one.  (2^-149 times any
+// finite sum is below 2^-21.)
+__device__ __forceinline__ float weight(float x) {
+  return fmaxf(__builtin_amdgcn_exp2f(x), 0x1p-149f);
+}
+
 // The sums of NT x 16 rows over a wave's positions.
 template <class T, int HD, int NT>
 struct Sums {
   float4v o[NT][HD / 16], l[NT];
   float mx[NT];
+  __device__ __forceinline__ void start(int t) {
+    mx[t] = -__builtin_inff();
+    l[t] = (float4v)(0.f);
+#pragma unroll
+    for (int e = 0; e < HD / 16; ++e) o[t][e] = (float4v)(0.f);
+  }
 };
 
 // A wave's tiles `wave`, `wave` + NW, .. of [first, end) of a run, for rows row0 on of KV
@@ -449,10 +481,7 @@ __device__ __forceinline__ void walk(const Attend<T>& A, Sums<T, HD, NT>& W, con
       q[t][u] = __builtin_bit_cast(V8, w);
     }
     lim[t] = in ? r.C + tok : lo;
-    W.mx[t] = -__builtin_inff();
-    W.l[t] = (float4v)(0.f);
-#pragma unroll
-    for (int e = 0; e < HD / 16; ++e) W.o[t][e] = (float4v)(0.f);
+    W.start(t);
   }
   const int tiles = (min(end, hi + 1) - first + kTile - 1) / kTile;
   const int mine = (tiles - wave + NW - 1) / NW;
@@ -492,77 +521,93 @@ __device__ __forceinline__ void walk(const Attend<T>& A, Sums<T, HD, NT>& W, con
 #pragma unroll
   for (int i = 0; i < 8; ++i) ones[i] = (T)1.f;
 
-  uint32_t odd = 0;
-  Ids id = ids(0), next = ids(1);
-  keys(0, id.k);
-  values(0, id.v);
-  for (int i = 0; i < mine; ++i) {
-    const Ids after = ids(i + 2);
-    const int p0 = start(i), at = p0 + 8 * kg;  // this lane's 8 positions
-    const bool bad = !named(id.v);              // they lie on no page
-    const bool edge = p0 + kTile - 1 > lo || __any(bad);
-    float4v s[NT][2];
+  // apart: values that are no numbers are taken out at every position
+  for (bool apart = false;; apart = true) {
+    const int all = apart ? -1 : lo;
+    int odd_from = mine, odd_to = -1;  // the tiles that had some of those
+    Ids id = ids(0), next = ids(1);
+    keys(0, id.k);
+    values(0, id.v);
+    for (int i = 0; i < mine; ++i) {
+      const Ids after = ids(i + 2);
+      const int p0 = start(i), at = p0 + 8 * kg;  // this lane's 8 positions
+      const bool bad = !named(id.v);              // they lie on no page
+      const bool edge = p0 + kTile - 1 > all || __any(bad);
+      float4v s[NT][2];
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        s[t][j] = (float4v)(0.f);
+        for (int j = 0; j < 2; ++j) {
+          s[t][j] = (float4v)(0.f);
 #pragma unroll
-        for (int u = 0; u < HD / 32; ++u) s[t][j] = Vec<T>::mfma(k[j][u], q[t][u], s[t][j]);
-      }
-    keys(i + 1, next.k);
-    V8 p[NT], rest[NT];
+          for (int u = 0; u < HD / 32; ++u) s[t][j] = Vec<T>::mfma(k[j][u], q[t][u], s[t][j]);
+        }
+      keys(i + 1, next.k);
+      V8 p[NT], rest[NT];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      if (edge)
+      for (int t = 0; t < NT; ++t) {
+        if (edge)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              if (bad) s[t][j][c] = __builtin_nanf("");
+              if (at + 4 * j + c > lim[t]) s[t][j][c] = -__builtin_inff();
+            }
+        float tm = s[t][0][0];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tm = fmaxf(tm, s[t][j][c]);
+        if (__any(tm * scale > W.mx[t] + kLag)) {
+          const float nm = fmaxf(W.mx[t], row_max(tm) * scale);
+          const float al = nm == W.mx[t] ? 1.f : __builtin_amdgcn_exp2f(W.mx[t] - nm);
+          W.l[t] *= al;
+#pragma unroll
+          for (int e = 0; e < HD / 16; ++e) W.o[t][e] *= al;
+          W.mx[t] = nm;
+        }
+        const float ref = W.mx[t] == -__builtin_inff() ? 0.f : W.mx[t] - kUp;
 #pragma unroll
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            if (bad) s[t][j][c] = __builtin_nanf("");
-            if (at + 4 * j + c > lim[t]) s[t][j][c] = -__builtin_inff();
+            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j][c], scale, -ref));
+            p[t][4 * j + c] = (T)x;
+            if constexpr (NT == 1) rest[t][4 * j + c] = (T)(x - (float)p[t][4 * j + c]);
           }
-      float tm = s[t][0][0];
-#pragma unroll
-      for (int j = 0; j < 2; ++j)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tm = fmaxf(tm, s[t][j][c]);
-      if (__any(tm * scale > W.mx[t] + kLag)) {
-        const float nm = fmaxf(W.mx[t], row_max(tm) * scale);
-        const float al = nm == W.mx[t] ? 1.f : __builtin_amdgcn_exp2f(W.mx[t] - nm);
-        W.l[t] *= al;
-#pragma unroll
-        for (int e = 0; e < HD / 16; ++e) W.o[t][e] *= al;
-        W.mx[t] = nm;
+        W.l[t] = Vec<T>::mfma(ones, p[t], W.l[t]);
+        if constexpr (NT == 1) W.l[t] = Vec<T>::mfma(ones, rest[t], W.l[t]);
       }
-      const float ref = W.mx[t] == -__builtin_inff() ? 0.f : W.mx[t] - kUp;
+      // (values on no page were read from another one: no row gets a number that it sees)
+      if (edge && __any(clean<T>(v, bad ? hi + 1 : at, all, hi)))
+        odd_from = min(odd_from, i), odd_to = i;
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int e = 0; e < HD / 16; ++e)
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j][c], scale, -ref));
-          p[t][4 * j + c] = (T)x;
-          if constexpr (NT == 1) rest[t][4 * j + c] = (T)(x - (float)p[t][4 * j + c]);
+        for (int t = 0; t < NT; ++t) {
+          W.o[t][e] = Vec<T>::mfma(v[e], p[t], W.o[t][e]);
+          if constexpr (NT == 1) W.o[t][e] = Vec<T>::mfma(v[e], rest[t], W.o[t][e]);
         }
-      W.l[t] = Vec<T>::mfma(ones, p[t], W.l[t]);
-      if constexpr (NT == 1) W.l[t] = Vec<T>::mfma(ones, rest[t], W.l[t]);
+      values(i + 1, next.v);
+      id = next, next = after;
     }
-    // (values on no page were read from another one: no row gets a number that it sees)
-    if (edge) odd |= clean<T>(v, bad ? hi + 1 : at, lo, hi);
+    bool odd = false;
 #pragma unroll
-    for (int e = 0; e < HD / 16; ++e)
+    for (int t = 0; t < NT; ++t) {
+      const float x = probe(W.o[t]);
+      odd |= row0 + 16 * t + n < A.rep * r.n && x != x;
+    }
+    if (!apart && __any(odd)) {
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        W.o[t][e] = Vec<T>::mfma(v[e], p[t], W.o[t][e]);
-        if constexpr (NT == 1) W.o[t][e] = Vec<T>::mfma(v[e], rest[t], W.o[t][e]);
-      }
-    values(i + 1, next.v);
-    id = next, next = after;
+      for (int t = 0; t < NT; ++t) W.start(t);
+      continue;
+    }
+    for (int i = odd_from; i <= odd_to; ++i)
+      add_odd<T, HD, NT>(A, W.o, lim, b, g, max(start(i), all + 1), min(start(i) + kTile - 1, hi),
+                         kg);
+    return;
   }
-  if (lo < hi && __any(odd))
-    add_odd<T, HD, NT>(A, W.o, lim, b, g, lo, hi, kg, [&](int p) {
-      return p >= first && p < first + kTile * tiles && (p - first) / kTile % NW == wave;
-    });
 }
 
 // The waves' sums of 16 rows joined, then the rows themselves, or the range's entry of
@@ -593,8 +638,8 @@ __device__ __forceinline__ void finish(const Attend<T>& A, const Sums<T, HD, NT>
       float sum = 0.f, x[8] = {};
 #pragma unroll
       for (int w = 0; w < NW; ++w) {
-        // a wave without tiles has sums of zero and weight exp2(-inf) = 0
-        const float al = __builtin_amdgcn_exp2f(s_m[(w * 16 + rr) * 2] - ref);
+        // (a wave without tiles has sums of zero)
+        const float al = weight(s_m[(w * 16 + rr) * 2] - ref);
         sum += al * s_m[(w * 16 + rr) * 2 + 1];
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[j] += al * s_o[(w * 16 + rr) * kPad + d + j];
@@ -672,8 +717,6 @@ __device__ __forceinline__ void block_range(const Attend<T>& A, const Run& r, in
   // positions that all of this wave's rows see, and past which none sees any
   const int lo = r.C + row0 / A.rep;
   const int hi = min(r.C + min((row0 + 31) / A.rep, r.n - 1), r.L - 1);
-  float4v o[NT][HD / 16], l[NT];
-  float mx[NT];
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int row = row0 + 16 * t + n, tok = row / A.rep, head = row - tok * A.rep;
@@ -686,10 +729,6 @@ __device__ __forceinline__ void block_range(const Attend<T>& A, const Run& r, in
       q[t][u] = __builtin_bit_cast(V8, w);
     }
     lim[t] = in ? r.C + tok : lo;
-    mx[t] = -__builtin_inff();
-    l[t] = (float4v)(0.f);
-#pragma unroll
-    for (int e = 0; e < HD / 16; ++e) o[t][e] = (float4v)(0.f);
   }
 
   const int shift = __builtin_ctz(P.page);
@@ -753,94 +792,116 @@ __device__ __forceinline__ void block_range(const Attend<T>& A, const Run& r, in
 #pragma unroll
   for (int i = 0; i < 8; ++i) ones[i] = (T)1.f;
 
-  uint32_t odd = 0;
-  Ids id = pages(from), next = pages(from + 1);
-  issue(from, id);
-  for (int st = from; st < to; ++st) {
-    wait_vmcnt<0>();  // this wave's part of the stage has landed
-    stage_barrier();  // everyone's, and the stage before is used
-    if (st + 1 < to) issue(st + 1, next);
-    uint32_t bad = 0;
+  __shared__ int s_again;  // (set and read between the stages' barriers and the one behind them)
+  if (tid == 0) s_again = 0;
+  Sums<T, HD, NT> W;
+  for (bool apart = false;; apart = true) {
+    const int all = apart ? -1 : lo;
+    int odd_from = to, odd_to = -1;  // the stages that had values which are no numbers
 #pragma unroll
-    for (int i = 0; i < SP / 16; ++i) bad |= id.id[i] < 0 ? 1u << i : 0u;
-    id = next, next = pages(st + 2);
-    const uint32_t here = (uint32_t)(st & 1) * 2 * kBytes;
-    // (Waves without rows, or past the last position that theirs see, go along.)
-    const bool edge = st * SP + SP - 1 > lo || bad;
-    const int p0 = st * SP;
-    float4v s[NT][SP / 16];  // block 2 h + j of half h
+    for (int t = 0; t < NT; ++t) W.start(t);
+    Ids id = pages(from), next = pages(from + 1);
+    issue(from, id);
+    for (int st = from; st < to; ++st) {
+      wait_vmcnt<0>();  // this wave's part of the stage has landed
+      stage_barrier();  // everyone's, and the stage before is used
+      if (st + 1 < to) issue(st + 1, next);
+      uint32_t bad = 0;
 #pragma unroll
-    for (int x = 0; x < SP / 16; ++x) {
-      V8 k[HD / 32];
+      for (int i = 0; i < SP / 16; ++i) bad |= id.id[i] < 0 ? 1u << i : 0u;
+      id = next, next = pages(st + 2);
+      const uint32_t here = (uint32_t)(st & 1) * 2 * kBytes;
+      // (Waves without rows, or past the last position that theirs see, go along.)
+      const bool edge = st * SP + SP - 1 > all || bad;
+      const int p0 = st * SP;
+      float4v s[NT][SP / 16];  // block 2 h + j of half h
 #pragma unroll
-      for (int u = 0; u < HD / 32; ++u)
-        k[u] = lds_read<V8>(k_at[u] + here + (32 * (x >> 1) + 4 * (x & 1)) * HD * 2);
+      for (int x = 0; x < SP / 16; ++x) {
+        V8 k[HD / 32];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) s[t][x] = (float4v)(0.f);
+        for (int u = 0; u < HD / 32; ++u)
+          k[u] = lds_read<V8>(k_at[u] + here + (32 * (x >> 1) + 4 * (x & 1)) * HD * 2);
 #pragma unroll
-      for (int u = 0; u < HD / 32; ++u)
+        for (int t = 0; t < NT; ++t) s[t][x] = (float4v)(0.f);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) s[t][x] = Vec<T>::mfma(k[u], q[t][u], s[t][x]);
-    }
-    V8 p[NT][SP / 32];
+        for (int u = 0; u < HD / 32; ++u)
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      if (edge) {
-        int see = lim[t] - p0 - 8 * kg;
-        asm volatile("" : "+v"(see));  // (else as many differences from it stay in registers)
+          for (int t = 0; t < NT; ++t) s[t][x] = Vec<T>::mfma(k[u], q[t][u], s[t][x]);
+      }
+      V8 p[NT][SP / 32];
 #pragma unroll
-        for (int x = 0; x < SP / 16; ++x) {
-          const bool none = bad >> (2 * (x >> 1) + (kg >> 1)) & 1;
+      for (int t = 0; t < NT; ++t) {
+        if (edge) {
+          int see = lim[t] - p0 - 8 * kg;
+          asm volatile("" : "+v"(see));  // (else as many differences from it stay in registers)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            if (none) s[t][x][c] = __builtin_nanf("");
-            if (32 * (x >> 1) + 4 * (x & 1) + c > see) s[t][x][c] = -__builtin_inff();
+          for (int x = 0; x < SP / 16; ++x) {
+            const bool none = bad >> (2 * (x >> 1) + (kg >> 1)) & 1;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              if (none) s[t][x][c] = __builtin_nanf("");
+              if (32 * (x >> 1) + 4 * (x & 1) + c > see) s[t][x][c] = -__builtin_inff();
+            }
           }
         }
+        float tm = s[t][0][0];
+#pragma unroll
+        for (int x = 0; x < SP / 16; ++x)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tm = fmaxf(tm, s[t][x][c]);
+        if (__any(tm * scale > W.mx[t] + kLag)) {
+          const float nm = fmaxf(W.mx[t], row_max(tm) * scale);
+          const float al = nm == W.mx[t] ? 1.f : __builtin_amdgcn_exp2f(W.mx[t] - nm);
+          W.l[t] *= al;
+#pragma unroll
+          for (int e = 0; e < HD / 16; ++e) W.o[t][e] *= al;
+          W.mx[t] = nm;
+        }
+        const float ref = W.mx[t] == -__builtin_inff() ? 0.f : W.mx[t] - kUp;
+#pragma unroll
+        for (int x = 0; x < SP / 16; ++x)
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            p[t][x >> 1][4 * (x & 1) + c] =
+                (T)__builtin_amdgcn_exp2f(__builtin_fmaf(s[t][x][c], scale, -ref));
       }
-      float tm = s[t][0][0];
 #pragma unroll
-      for (int x = 0; x < SP / 16; ++x)
+      for (int h = 0; h < SP / 32; ++h) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) tm = fmaxf(tm, s[t][x][c]);
-      if (__any(tm * scale > mx[t] + kLag)) {
-        const float nm = fmaxf(mx[t], row_max(tm) * scale);
-        const float al = nm == mx[t] ? 1.f : __builtin_amdgcn_exp2f(mx[t] - nm);
-        l[t] *= al;
+        for (int t = 0; t < NT; ++t) W.l[t] = Vec<T>::mfma(ones, p[t][h], W.l[t]);
 #pragma unroll
-        for (int e = 0; e < HD / 16; ++e) o[t][e] *= al;
-        mx[t] = nm;
+        for (int e0 = 0; e0 < HD / 16; e0 += 4) {
+          V8 v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            v[e] = lds_read<V8>(v_at + here + h * HD * 64 + (e0 + e) * 256);
+          if (edge && __any(clean<T>(v, p0 + 32 * h + 8 * kg, all, hi)))
+            odd_from = min(odd_from, st), odd_to = st;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+              W.o[t][e0 + e] = Vec<T>::mfma(v[e], p[t][h], W.o[t][e0 + e]);
+        }
       }
-      const float ref = mx[t] == -__builtin_inff() ? 0.f : mx[t] - kUp;
-#pragma unroll
-      for (int x = 0; x < SP / 16; ++x)
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          p[t][x >> 1][4 * (x & 1) + c] =
-              (T)__builtin_amdgcn_exp2f(__builtin_fmaf(s[t][x][c], scale, -ref));
     }
+    if (!apart) {
+      bool odd = false;
 #pragma unroll
-    for (int h = 0; h < SP / 32; ++h) {
-#pragma unroll
-      for (int t = 0; t < NT; ++t) l[t] = Vec<T>::mfma(ones, p[t][h], l[t]);
-#pragma unroll
-      for (int e0 = 0; e0 < HD / 16; e0 += 4) {
-        V8 v[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          v[e] = lds_read<V8>(v_at + here + h * HD * 64 + (e0 + e) * 256);
-        if (edge) odd |= clean<T>(v, p0 + 32 * h + 8 * kg, lo, hi);
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-#pragma unroll
-          for (int t = 0; t < NT; ++t) o[t][e0 + e] = Vec<T>::mfma(v[e], p[t][h], o[t][e0 + e]);
+      for (int t = 0; t < NT; ++t) {
+        const float x = probe(W.o[t]);
+        odd |= row0 + 16 * t + n < rows && x != x;
       }
+      if (__any(odd)) s_again = 1;
+      __syncthreads();  // (also: the last stage is used, before the first of a second walk)
+      if (s_again) continue;
     }
+    if (busy)
+      add_odd<T, HD, NT>(A, W.o, lim, b, g, max(odd_from * SP, all + 1),
+                         min(odd_to * SP + SP - 1, hi), kg);
+    break;
   }
   if (!busy) return;
-  if (__any(odd))
-    add_odd<T, HD, NT>(A, o, lim, b, g, lo, hi, kg,
-                       [&](int p) { return p / SP >= from && p / SP < to; });
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int row = row0 + 16 * t + n, tok = row / A.rep, head = row - tok * A.rep;
@@ -849,19 +910,19 @@ __device__ __forceinline__ void block_range(const Attend<T>& A, const Run& r, in
       const long at = entry * kBlock + (row - block * kBlock);
       float* dst = A.part + at * HD + 4 * kg;
 #pragma unroll
-      for (int e = 0; e < HD / 16; ++e) *reinterpret_cast<float4v*>(dst + 16 * e) = o[t][e];
+      for (int e = 0; e < HD / 16; ++e) *reinterpret_cast<float4v*>(dst + 16 * e) = W.o[t][e];
       float* pm = A.part + A.entries * kBlock * HD + at * 2;
-      if (kg == 0) pm[0] = mx[t], pm[1] = l[t][0];
+      if (kg == 0) pm[0] = W.mx[t], pm[1] = W.l[t][0];
       continue;
     }
-    const float is = 1.f / l[t][0];
+    const float is = 1.f / W.l[t][0];
     T* dst = A.out + (long)(r.row + tok) * A.ld_o + (long)(g * A.rep + head) * HD + 4 * kg;
 #pragma unroll
     for (int e = 0; e < HD / 16; ++e) {
       typedef T V4 __attribute__((ext_vector_type(4)));
       V4 y;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) y[c] = (T)(o[t][e][c] * is);
+      for (int c = 0; c < 4; ++c) y[c] = (T)(W.o[t][e][c] * is);
       *reinterpret_cast<V4*>(dst + 16 * e) = y;
     }
   }
@@ -918,12 +979,12 @@ __global__ __launch_bounds__(256) void join_blocks_kernel(Attend<T> A) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) nm = fmaxf(nm, em[j]);
     const float ref = nm == -__builtin_inff() ? 0.f : nm;
-    const float a = __builtin_amdgcn_exp2f(m - ref);
+    const float a = weight(m - ref);
     o *= a, sum *= a, m = nm;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       if (i + j >= n) continue;
-      const float z = __builtin_amdgcn_exp2f(em[j] - ref);
+      const float z = weight(em[j] - ref);
       o += eo[j] * z, sum += el[j] * z;
     }
   }
@@ -1048,12 +1109,12 @@ __global__ __launch_bounds__(256) void join_kernel(Attend<T> A) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) nm = fmaxf(nm, em[i]);
     const float ref = nm == -__builtin_inff() ? 0.f : nm;
-    const float a = __builtin_amdgcn_exp2f(m - ref);
+    const float a = weight(m - ref);
     o *= a, sum *= a, m = nm;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (w + i * kAt > w1) continue;
-      const float z = __builtin_amdgcn_exp2f(em[i] - ref);
+      const float z = weight(em[i] - ref);
       o += eo[i] * z, sum += el[i] * z;
     }
   }
@@ -1067,7 +1128,7 @@ __global__ __launch_bounds__(256) void join_kernel(Attend<T> A) {
   o = (float4v)(0.f), sum = 0.f;
 #pragma unroll
   for (int i = 0; i < kAt; ++i) {
-    const float a = __builtin_amdgcn_exp2f(s_m[i] - ref);
+    const float a = weight(s_m[i] - ref);
     o += s_o[i][c] * a, sum += s_l[i] * a;
   }
   const int tok = row / A.rep, head = row - tok * A.rep;
