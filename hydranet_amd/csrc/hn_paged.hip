@@ -372,12 +372,13 @@ __device__ __forceinline__ int grains_below(const Attend<T>& A, int to) {
 
 // Values that are no numbers.  A row has the infinities and NaN of the positions that it
 // sees in their dimensions, whatever their weights: a softmax's are above 0.  A product
-// would make NaN of an infinity where the probability was rounded to 0, or with what its
-// rounding left (of either sign, or 0), and give it to the rows that do not see it, too.
-// So at positions that only some rows see (past lo) they are taken out of the products and
-// added afterwards; among the others a first walk looks for none, its sums tell whether
-// there was one, and if so a second takes them out everywhere (lo = -1).  The joins keep
-// them from weights of 0 (weight).
+// makes NaN of an infinity where the probability was rounded to 0, or with what its rounding
+// left (of either sign, or 0), also for the rows that do not see it.  So at positions that
+// only some rows see (past lo) they are taken out of the products and added to the rows
+// afterwards.  Among the positions that all rows see a first walk looks for none: its sums
+// tell whether there was one, and then a second walk takes them out everywhere (lo = -1).
+// The joins' weights are not 0 either (weight).  (The look at the sums costs 0.2 to 0.3 us of
+// a launch, 2 to 3 % of prompts by blocks.)
 //
 // Of 8 positions from `at` on, the values that must not reach a product: those at positions
 // past hi, which no row sees (their probabilities are zero, but what lies there may be

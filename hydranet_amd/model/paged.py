@@ -371,7 +371,8 @@ def paged_attention(q: torch.Tensor, batch: PagedBatch, cache: PagedKVCache, lay
     and values in the pages) over the positions up to their own -> [rows, heads * hd].
     scale: of the scores, 1 / sqrt(hd) by default.  Rows of a sequence that takes no
     part and of no sequence are zero; a row that sees a position whose page is not named
-    is NaN, and so are the rows of a run of more than the batch's max_new."""
+    is NaN, and so are the rows of a run of more than the batch's max_new.  An infinite or
+    NaN value is in its dimension of the rows that see it, whatever its weight."""
     nkv, hd, T = cache.kv_heads, cache.head_dim, batch.rows
     assert q.dim() == 2 and q.shape[1] % hd == 0, f"q [rows, heads * {hd}]"
     columns = q.shape[1]

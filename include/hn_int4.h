@@ -572,7 +572,9 @@ int hn_paged_append(const hn_paged_step* step, const void* qkv, long ld_qkv, int
  *   [T][ld_q].  Rows of a sequence with a negative length are zero; a row that
  *   sees a position whose page the table does not name is NaN, and so are the rows
  *   of a sequence with more than max_new of them.  A position that a row does not
- *   see has no effect on it, whatever it holds.  scale above 0 and finite, also
+ *   see has no effect on it, whatever it holds; a value that is infinite or NaN is
+ *   in its dimension of the rows that see it, whatever its weight (infinities of both
+ *   signs: NaN).  scale above 0 and finite, also
  *   times log2(e); 16-byte aligned operands, ld_q and ld_o multiples of 8; cols *
  *   page < 2^30; out overlaps nothing that is read.  work:
  *   hn_paged_attention_workspace_bytes(step) bytes, 16-byte aligned, any contents. */
