@@ -228,30 +228,33 @@ __global__ __launch_bounds__(256) void append_rows_kernel(
 // consecutive positions that its lane of the value operand holds.
 //
 // One token per sequence is bound by the cache's bytes, 8 KV heads of 128 and 4 query heads
-// each: 64 sequences of 150 to 8000 197 to 231 us (1.07 GB, 4.6 to 5.4 TB/s; a large copy moves
-// 5.1), 64 of 2000 91 us (5.8), and, of few positions, by memory's latency: one text of 701
-// 9.3 us in two launches.  A wave's products are 13 times as fast as its bytes come, so the
-// 4 rows of 16 that it uses cost nothing.
+// each: 64 sequences of 150 to 8000 196 to 203 us (1.07 GB, 5.3 to 5.5 TB/s; a large read
+// reaches 6.2), 64 of 2000 91 us (5.8), and, of few positions, by memory's latency: one text
+// of 701 9.8 us in two launches.  A wave's products are 6 times as fast as its bytes come, so
+// the 4 rows of 16 that it uses cost nothing.
 constexpr int kTile = 32;
 constexpr int NW = 4;  // waves of a workgroup
-// Workgroups that a CU's registers hold at once.  (Three of 128 dimensions spill: one text of
-// 31777 43 us, two 33.)
+// Workgroups per CU that the positions are shared out to, and that the registers hold at
+// least.  (Three of 128 dimensions spill: one text of 31777 43 us, two 33.)
 constexpr int resident(long hd) { return hd == 256 ? 1 : 2; }
+// The same of runs by blocks.  (Of 64 dimensions, two / three: 8 of 1000 rows after 3000 261 /
+// 245 us.)
+constexpr int resident_blocks(long hd) { return hd == 64 ? 3 : resident(hd); }
 constexpr float kLog2e = 1.4426950408889634f;
 // Probabilities are 2^8 times the softmax's, relative to a maximum that follows the true
 // one only when it lags by 2^6: below 2^14, so fp16 holds them, and those down to 2^-22
-// of the largest are normal numbers.  They are rounded to the cache's type because that
-// is what the matrix instruction multiplies with the values; a row's sum is of the
-// same numbers, so that their weights still add up to 1.  Up to 16 rows a KV head, which
-// the bytes bound, what the rounding left is multiplied as well, in the same time
-// (relative error 2.6e-4 without it and 2.1e-4 with it in fp16, 2.1e-3 and 1.7e-3 in
-// bf16); two tiles of 16 would spill (20 heads a KV head 28 us, 31 with it), and runs
-// by blocks are bound by the products.
+// of the largest are normal numbers.  The matrix instruction multiplies numbers of the
+// cache's type with the values, so a probability goes in as two: itself rounded, and what
+// that left (in all 2^-22 of it is lost in fp16, 2^-16 in bf16).  The second product costs
+// nothing where the bytes are the bound, and runs by blocks a third (chunks of prompts 147 us
+// without it, 191 with it); without it they would be off by more than the result's own
+// rounding (relative to 64 bits 2.7e-4, 2.1e-4 with it, in fp16; 2.1e-3 and 1.7e-3 in bf16).
+// A row's sum is of the probabilities as they are, in fp32.
 constexpr float kUp = 8.f, kLag = 6.f;
 // Positions that workgroups share out as one.
 constexpr int kGrain = 128;
-// Positions that a share of a block's has at least.  (80 rows of one sequence of 1020: 16.5
-// us, of 1024 or one share 30.)
+// Positions that a share of a block's has at least.  (80 rows of one sequence of 1020: 19.6
+// us, in one share 43.)
 constexpr long kShare = 256;
 
 template <class T>
@@ -269,16 +272,23 @@ struct Attend {
   float scale;
 };
 
-// max over the four lanes, 16 apart, that hold one row
-__device__ __forceinline__ float row_max(float x) {
+// f over the four lanes, 16 apart, that hold one row
+template <class F>
+__device__ __forceinline__ float over_row(float x, F f) {
   const uint32_t w = __builtin_bit_cast(uint32_t, x);
   const auto a = __builtin_amdgcn_permlane16_swap(w, w, false, false);
   const uint32_t a0 = a[0], a1 = a[1];
-  x = fmaxf(__builtin_bit_cast(float, a0), __builtin_bit_cast(float, a1));
+  x = f(__builtin_bit_cast(float, a0), __builtin_bit_cast(float, a1));
   const uint32_t v = __builtin_bit_cast(uint32_t, x);
   const auto b = __builtin_amdgcn_permlane32_swap(v, v, false, false);
   const uint32_t b0 = b[0], b1 = b[1];
-  return fmaxf(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
+  return f(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
+}
+__device__ __forceinline__ float row_max(float x) {
+  return over_row(x, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float row_sum(float x) {
+  return over_row(x, [](float a, float b) { return a + b; });
 }
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -447,11 +457,11 @@ __device__ __forceinline__ float weight(float x) {
 // The sums of NT x 16 rows over a wave's positions.
 template <class T, int HD, int NT>
 struct Sums {
-  float4v o[NT][HD / 16], l[NT];
-  float mx[NT];
+  float4v o[NT][HD / 16];
+  float mx[NT], l[NT];  // (l while a walk runs: of the lane's positions)
   __device__ __forceinline__ void start(int t) {
     mx[t] = -__builtin_inff();
-    l[t] = (float4v)(0.f);
+    l[t] = 0.f;
 #pragma unroll
     for (int e = 0; e < HD / 16; ++e) o[t][e] = (float4v)(0.f);
   }
@@ -518,12 +528,10 @@ __device__ __forceinline__ void walk(const Attend<T>& A, Sums<T, HD, NT>& W, con
     for (int e = 0; e < HD / 16; ++e) v[e] = *reinterpret_cast<const V8*>(x + 128 * e);
   };
   const float scale = A.scale * kLog2e;
-  V8 ones;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) ones[i] = (T)1.f;
 
   // apart: values that are no numbers are taken out at every position
   for (bool apart = false;; apart = true) {
+    asm volatile("" : "+s"(first), "+s"(g));  // (else what both walks begin with stays in registers)
     const int all = apart ? -1 : lo;
     int odd_from = mine, odd_to = -1;  // the tiles that had some of those
     Ids id = ids(0), next = ids(1);
@@ -574,11 +582,10 @@ __device__ __forceinline__ void walk(const Attend<T>& A, Sums<T, HD, NT>& W, con
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j][c], scale, -ref));
+            W.l[t] += x;
             p[t][4 * j + c] = (T)x;
-            if constexpr (NT == 1) rest[t][4 * j + c] = (T)(x - (float)p[t][4 * j + c]);
+            rest[t][4 * j + c] = (T)(x - (float)p[t][4 * j + c]);
           }
-        W.l[t] = Vec<T>::mfma(ones, p[t], W.l[t]);
-        if constexpr (NT == 1) W.l[t] = Vec<T>::mfma(ones, rest[t], W.l[t]);
       }
       // (values on no page were read from another one: no row gets a number that it sees)
       if (edge && __any(clean<T>(v, bad ? hi + 1 : at, all, hi)))
@@ -588,7 +595,7 @@ __device__ __forceinline__ void walk(const Attend<T>& A, Sums<T, HD, NT>& W, con
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
           W.o[t][e] = Vec<T>::mfma(v[e], p[t], W.o[t][e]);
-          if constexpr (NT == 1) W.o[t][e] = Vec<T>::mfma(v[e], rest[t], W.o[t][e]);
+          W.o[t][e] = Vec<T>::mfma(v[e], rest[t], W.o[t][e]);
         }
       values(i + 1, next.v);
       id = next, next = after;
@@ -607,8 +614,10 @@ __device__ __forceinline__ void walk(const Attend<T>& A, Sums<T, HD, NT>& W, con
     for (int i = odd_from; i <= odd_to; ++i)
       add_odd<T, HD, NT>(A, W.o, lim, b, g, max(start(i), all + 1), min(start(i) + kTile - 1, hi),
                          kg);
-    return;
+    break;
   }
+#pragma unroll
+  for (int t = 0; t < NT; ++t) W.l[t] = row_sum(W.l[t]);
 }
 
 // The waves' sums of 16 rows joined, then the rows themselves, or the range's entry of
@@ -623,7 +632,7 @@ __device__ __forceinline__ void finish(const Attend<T>& A, const Sums<T, HD, NT>
   for (int t = 0; t < NT; ++t) {
     __syncthreads();  // (the last use of the buffers)
     if (row0 + 16 * t + n < rows) {
-      if (kg == 0) s_m[(wave * 16 + n) * 2] = W.mx[t], s_m[(wave * 16 + n) * 2 + 1] = W.l[t][0];
+      if (kg == 0) s_m[(wave * 16 + n) * 2] = W.mx[t], s_m[(wave * 16 + n) * 2 + 1] = W.l[t];
 #pragma unroll
       for (int e = 0; e < HD / 16; ++e)
         *reinterpret_cast<float4v*>(s_o + (wave * 16 + n) * kPad + 16 * e + 4 * kg) = W.o[t][e];
@@ -674,15 +683,17 @@ __device__ __forceinline__ void finish(const Attend<T>& A, const Sums<T, HD, NT>
 // positions that a read takes cover the banks once (the counter of conflicts stays at 0).
 // Two workgroups per CU: one's loads and softmax under the other's products.
 //
-// Bounds: where there are several workgroups for each place, the matrix units beside the
-// exponentials and the LDS reads (4000 rows after 4000 positions: 391 us, 1.0 PFLOP/s, a large
-// product reaches 1.17); where each has about one, the longest block's stages after each
-// other (1.9 us each alone on a CU) while others are done: runs of 1000, 688 and 376 after
-// 900 to 4000 128 to 146 us, 0.66 to 0.75 PFLOP/s, the CUs busy in 64 % of the time.
-// Measured and not taken: all blocks' stages dealt evenly to the workgroups (they then walk
-// different positions at once, out of L2: 4000 after 4000 462 us, with a plan and joins of 23
-// us); five smaller stages in LDS, four of them on their way, and scores made a stage ahead
-// beside the exponentials (no difference); more shares than places (146 to 201).
+// Bounds: where there are several workgroups for each place, the matrix units, which make a
+// half more products than the formula has, the second one for what a probability's rounding
+// left (4000 rows after 4000 positions: 530 to 550 us, 0.72 to 0.74 PFLOP/s of the formula's
+// and 1.1 in all, a large product reaches 1.14 to 1.17); where each has about one, the longest
+// block's stages after each other while others are done: runs of 1000, 688 and 376 after 900
+// to 4000 187 to 192 us.
+// Measured without the second product (391 and 146 us then) and not taken: all blocks' stages
+// dealt evenly to the workgroups (they then walk different positions at once, out of L2: 462
+// us, with a plan and joins of 23); five smaller stages in LDS, four of them on their way, and
+// scores made a stage ahead beside the exponentials (no difference); more shares than places
+// (146 to 201).
 constexpr int kBlock = 128;
 constexpr int stage_of(int hd) { return hd == 256 ? 32 : 64; }
 
@@ -789,14 +800,12 @@ __device__ __forceinline__ void block_range(const Attend<T>& A, const Run& r, in
     k_at[u] = lds0 + (8 * (n >> 2) + (n & 3)) * HD * 2 + 16 * ((4 * u + kg) ^ mine);
   const uint32_t v_at = lds0 + kBytes + kg * HD * 16 + n * 16;
   const float scale = A.scale * kLog2e;
-  V8 ones;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) ones[i] = (T)1.f;
 
   __shared__ int s_again;  // (set and read between the stages' barriers and the one behind them)
   if (tid == 0) s_again = 0;
   Sums<T, HD, NT> W;
   for (bool apart = false;; apart = true) {
+    asm volatile("" : "+s"(from));  // (as in walk)
     const int all = apart ? -1 : lo;
     int odd_from = to, odd_to = -1;  // the stages that had values which are no numbers
 #pragma unroll
@@ -829,7 +838,7 @@ __device__ __forceinline__ void block_range(const Attend<T>& A, const Run& r, in
 #pragma unroll
           for (int t = 0; t < NT; ++t) s[t][x] = Vec<T>::mfma(k[u], q[t][u], s[t][x]);
       }
-      V8 p[NT][SP / 32];
+      V8 p[NT][SP / 32], rest[NT][SP / 32];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         if (edge) {
@@ -862,14 +871,16 @@ __device__ __forceinline__ void block_range(const Attend<T>& A, const Run& r, in
 #pragma unroll
         for (int x = 0; x < SP / 16; ++x)
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-            p[t][x >> 1][4 * (x & 1) + c] =
-                (T)__builtin_amdgcn_exp2f(__builtin_fmaf(s[t][x][c], scale, -ref));
+          for (int c = 0; c < 4; ++c) {
+            const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][x][c], scale, -ref));
+            const int i = 4 * (x & 1) + c;
+            W.l[t] += y;
+            p[t][x >> 1][i] = (T)y;
+            rest[t][x >> 1][i] = (T)(y - (float)p[t][x >> 1][i]);
+          }
       }
 #pragma unroll
       for (int h = 0; h < SP / 32; ++h) {
-#pragma unroll
-        for (int t = 0; t < NT; ++t) W.l[t] = Vec<T>::mfma(ones, p[t][h], W.l[t]);
 #pragma unroll
         for (int e0 = 0; e0 < HD / 16; e0 += 4) {
           V8 v[4];
@@ -883,6 +894,11 @@ __device__ __forceinline__ void block_range(const Attend<T>& A, const Run& r, in
 #pragma unroll
             for (int t = 0; t < NT; ++t)
               W.o[t][e0 + e] = Vec<T>::mfma(v[e], p[t][h], W.o[t][e0 + e]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+              W.o[t][e0 + e] = Vec<T>::mfma(v[e], rest[t][h], W.o[t][e0 + e]);
         }
       }
     }
@@ -904,6 +920,8 @@ __device__ __forceinline__ void block_range(const Attend<T>& A, const Run& r, in
   }
   if (!busy) return;
 #pragma unroll
+  for (int t = 0; t < NT; ++t) W.l[t] = row_sum(W.l[t]);
+#pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int row = row0 + 16 * t + n, tok = row / A.rep, head = row - tok * A.rep;
     if (row >= rows) continue;
@@ -913,10 +931,10 @@ __device__ __forceinline__ void block_range(const Attend<T>& A, const Run& r, in
 #pragma unroll
       for (int e = 0; e < HD / 16; ++e) *reinterpret_cast<float4v*>(dst + 16 * e) = W.o[t][e];
       float* pm = A.part + A.entries * kBlock * HD + at * 2;
-      if (kg == 0) pm[0] = W.mx[t], pm[1] = W.l[t][0];
+      if (kg == 0) pm[0] = W.mx[t], pm[1] = W.l[t];
       continue;
     }
-    const float is = 1.f / W.l[t][0];
+    const float is = 1.f / W.l[t];
     T* dst = A.out + (long)(r.row + tok) * A.ld_o + (long)(g * A.rep + head) * HD + 4 * kg;
 #pragma unroll
     for (int e = 0; e < HD / 16; ++e) {
@@ -932,10 +950,10 @@ __device__ __forceinline__ void block_range(const Attend<T>& A, const Run& r, in
 // A workgroup per (KV head, block and share of its positions, sequence), the longest blocks
 // of a run first.  A head's blocks side by side walk the same positions at once, so all but
 // the first find them in the XCD's L2: with the sequences side by side instead, 8 of 1000
-// rows after 3000 take 392 us, as it is 299.  A block's A.each stages a share (the rest in the last); its entry of the
-// workspace goes by the block and the share.
+// rows after 3000 take 635 us, as it is 390.  A block's A.each stages a share (the rest in
+// the last); its entry of the workspace goes by the block and the share.
 template <class T, int HD>
-__global__ __launch_bounds__(256, resident(HD)) void block_kernel(Attend<T> A) {
+__global__ __launch_bounds__(256, resident_blocks(HD)) void block_kernel(Attend<T> A) {
   __shared__ __align__(1024) unsigned char s_buf[8 * stage_of(HD) * HD];
   const int g = blockIdx.x, b = blockIdx.z, part = gridDim.y - 1 - blockIdx.y;
   const int block = part / A.shares, share = part - block * A.shares;
@@ -1219,9 +1237,10 @@ int append(const Step& P, const void* qkv_, long ld, const float* cos_t, const f
 }
 
 // Rows of one (sequence, KV head) up to which a workgroup takes all of them for a share of
-// the positions; more go by blocks.  (Shared / by blocks, us: 20 rows of 1 sequence of 3000
-// 12.4 / 14.7, of 8 30.8 / 31.7; 32 rows of 8 33.1 / 31.3, of 64 180 / 166.)
-constexpr int share_rows(long hd) { return hd == 256 ? 16 : 24; }
+// the positions, as many as its waves' registers hold; more go by blocks.  (Shared / by
+// blocks, us, 8 KV heads of 128: 20 rows of 1 sequence of 3000 13.0 / 17.4, of 8 28.2 / 33.4, of
+// 64 149 / 163; 32 rows 15.3 / 18.0, 30.9 / 32.5, 156 / 164, of 64 of 150 to 8000 230 / 322.)
+constexpr int share_rows(long hd) { return hd == 256 ? 16 : 32; }
 
 // How a call runs, by its sizes alone: wgs workgroups that share the positions, or, with 0,
 // one per head; of runs of many rows, one per block and share of its positions, of `each`
