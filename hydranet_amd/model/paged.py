@@ -332,9 +332,9 @@ def paged_append(qkv: torch.Tensor, rope: RotaryTable, batch: PagedBatch, cache:
         if last != 1 or ld < columns:
             qkv, ld = qkv.contiguous(), columns
         q = qkv.new_empty((T, num_heads * hd))
-        _lib.call_on(qkv.device, "hn_paged_append", batch._step(cache, num_heads)[1],
-                     qkv.data_ptr(), ld, _DTYPES[qkv.dtype], *rope._args(), q.data_ptr(),
-                     k.data_ptr(), v.data_ptr())
+        held, step, _ = batch._step(cache, num_heads)  # (held: until the call has read it)
+        _lib.call_on(qkv.device, "hn_paged_append", step, qkv.data_ptr(), ld,
+                     _DTYPES[qkv.dtype], *rope._args(), q.data_ptr(), k.data_ptr(), v.data_ptr())
         return q
     wide = torch.float64 if qkv.dtype == torch.float64 else torch.float32
     q = torch.zeros((T, num_heads, hd), dtype=qkv.dtype)
@@ -387,7 +387,7 @@ def paged_attention(q: torch.Tensor, batch: PagedBatch, cache: PagedKVCache, lay
         if last != 1 or ld % 8 or ld < columns or q.data_ptr() % 16:
             q, ld = _lib.aligned_rows(q.contiguous()), columns
         out = q.new_empty((T, columns))
-        _, step, n = batch._step(cache, nh)
+        held, step, n = batch._step(cache, nh)  # (held: until the call has read it)
         work = q.new_empty((n // 2,)) if n else None  # (two bytes each)
         _lib.call_on(q.device, "hn_paged_attention", step, q.data_ptr(), ld, _DTYPES[q.dtype],
                      k.data_ptr(), v.data_ptr(), scale, out.data_ptr(), columns,
