@@ -230,7 +230,7 @@ __global__ __launch_bounds__(256) void append_rows_kernel(
 // One token per sequence is bound by the cache's bytes, 8 KV heads of 128 and 4 query heads
 // each: 64 sequences of 150 to 8000 196 to 203 us (1.07 GB, 5.3 to 5.5 TB/s; a large read
 // reaches 6.2), 64 of 2000 91 us (5.8), and, of few positions, by memory's latency: one text
-// of 701 9.8 us in two launches.  A wave's products are 6 times as fast as its bytes come, so
+// of 701 9.8 us in two launches.  A wave's products are 8 times as fast as its bytes come, so
 // the 4 rows of 16 that it uses cost nothing.
 constexpr int kTile = 32;
 constexpr int NW = 4;  // waves of a workgroup
