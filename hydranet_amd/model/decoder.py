@@ -67,6 +67,11 @@ class RMSNorm(nn.Module):
         return (self.weight * x).to(dt)
 
 
+def _capturing(t: torch.Tensor) -> bool:
+    """Whether work on t is being captured into a graph."""
+    return t.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
 class RotaryEmbedding(nn.Module):
     def __init__(self, dim: int, max_positions: int, base: float, device=None):
         super().__init__()
@@ -275,25 +280,29 @@ class Attention(nn.Module):
         weights stacked into one matrix (one GEMM), or, for Int4Linear
         projections (convert_dense_to_int4), their packed weights and scales
         stacked into one hn_int4_linear launch.  The stack is rebuilt when a
-        weight is replaced or modified."""
+        weight is replaced or modified.  One made inside a capture is the
+        graph's alone: it is filled when the graph is replayed."""
         from ..kernels.int4_linear import Int4Linear, stacked_int4
         projs = (self.q_proj, self.k_proj, self.v_proj)
         int4 = all(isinstance(m, Int4Linear) for m in projs)
         ts = [t for m in projs for t in ((m.weight_packed, m.weight_scale) if int4 else
                                          (m.weight,))]
         key = (int4,) + tuple((t.data_ptr(), t._version) for t in ts)
-        if getattr(self, "_qkv_key", None) != key:
+        if getattr(self, "_qkv_key", None) == key:
+            w = self._qkv_w
+        else:
             if int4:
                 assert all(m.bias is None for m in projs), "q/k/v projections carry no bias"
-                self._qkv_w = stacked_int4(projs)
+                w = stacked_int4(projs)
             else:
-                self._qkv_w = torch.cat([m.weight.detach() for m in projs], 0)
-            self._qkv_key = key
+                w = torch.cat([m.weight.detach() for m in projs], 0)
+            if not _capturing(x2):
+                self._qkv_w, self._qkv_key = w, key
         if int4:
             from ..kernels.int4_gemm import int4_linear
-            packed, scale, g = self._qkv_w
+            packed, scale, g = w
             return int4_linear(x2, packed, scale, g)
-        return F.linear(x2, self._qkv_w)
+        return F.linear(x2, w)
 
     def forward(self, x: torch.Tensor, rope: "RotaryEmbedding", pos: torch.Tensor,
                 cache: KVCache, layer: int, kv_len: int,
@@ -622,7 +631,8 @@ class MixtralDecoder(nn.Module):
                          self.decode_top_k if top_k is None else top_k, tree)
 
     def _rope_table(self):
-        """The decoder's angles as a RotaryTable, made again when the module's are others."""
+        """The decoder's angles as a RotaryTable, made again when the module's are others.
+        One made inside a capture is the graph's alone (see Attention._qkv)."""
         from .paged import RotaryTable
         cos, sin = self.rotary.cos_cached, self.rotary.sin_cached
         old = getattr(self, "_rope", None)
@@ -630,6 +640,8 @@ class MixtralDecoder(nn.Module):
                 or old[2] != (cos._version, sin._version):
             half = cos.shape[1] // 2
             table = RotaryTable.wrap(cos[:, :half].float(), sin[:, :half].float())
+            if _capturing(cos):
+                return table
             old = self._rope = (cos, sin, (cos._version, sin._version), table)
         return old[3]
 
