@@ -631,19 +631,27 @@ class MixtralDecoder(nn.Module):
                          self.decode_top_k if top_k is None else top_k, tree)
 
     def _rope_table(self):
-        """The decoder's angles as a RotaryTable, made again when the module's are others.
-        One made inside a capture is the graph's alone (see Attention._qkv)."""
+        """The decoder's angles as a RotaryTable, made again when the module's are others:
+        in the same memory while it fits, so that captured steps follow.  One made inside a
+        capture is the graph's alone (see Attention._qkv)."""
         from .paged import RotaryTable
         cos, sin = self.rotary.cos_cached, self.rotary.sin_cached
-        old = getattr(self, "_rope", None)
-        if old is None or old[0] is not cos or old[1] is not sin \
-                or old[2] != (cos._version, sin._version):
-            half = cos.shape[1] // 2
-            table = RotaryTable.wrap(cos[:, :half].float(), sin[:, :half].float())
+        old, changes = getattr(self, "_rope", None), (cos._version, sin._version)
+        if old is not None and old[0] is cos and old[1] is sin and old[2] == changes:
+            return old[3]
+        half = cos.shape[1] // 2
+        with torch.inference_mode(False):  # (the copies may be written again)
+            cos_h, sin_h = cos[:, :half].float(), sin[:, :half].float()
             if _capturing(cos):
-                return table
-            old = self._rope = (cos, sin, (cos._version, sin._version), table)
-        return old[3]
+                return RotaryTable.wrap(cos_h, sin_h)
+            table = None if old is None else old[3]
+            if table is not None and table.cos.shape == cos_h.shape and table.device == cos.device:
+                table.cos.copy_(cos_h)
+                table.sin.copy_(sin_h)
+            else:
+                table = RotaryTable.wrap(cos_h.clone(), sin_h.clone())
+        self._rope = (cos, sin, changes, table)
+        return table
 
     @torch.no_grad()
     def forward_paged(self, tokens: torch.Tensor, batch, cache, top_k: Optional[int] = None,

@@ -46,6 +46,25 @@ def test_first_step_inside_a_capture():
         assert torch.equal(held, want) and torch.equal(step(), want)
 
 
+def test_angles_changed_after_a_capture():
+    model = _model()
+    step = _step(model)
+    first = step().clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    with torch.no_grad():
+        model.rotary.cos_cached.copy_(model.rotary.cos_cached.flip(0))
+        model.rotary.sin_cached.copy_(model.rotary.sin_cached.flip(0))
+    other = step().clone()
+    assert not torch.equal(other, first)
+    junk = [torch.full((256, 64), 9.0, device=DEV) for _ in range(8)]  # (where a table was)
+    for _ in range(3):
+        graph.replay()
+        assert torch.equal(held, other) and torch.equal(step(), other)
+    del junk
+
+
 def test_a_model_used_inside_and_outside_of_inference_mode():
     model = _model()
     with torch.inference_mode():
