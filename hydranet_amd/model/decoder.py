@@ -72,6 +72,12 @@ def _capturing(t: torch.Tensor) -> bool:
     return t.is_cuda and torch.cuda.is_current_stream_capturing()
 
 
+def _changes(*ts: torch.Tensor):
+    """How often each was changed in place; None if one does not say (made in inference
+    mode): what is made of such tensors is not kept."""
+    return None if any(t.is_inference() for t in ts) else tuple(t._version for t in ts)
+
+
 class RotaryEmbedding(nn.Module):
     def __init__(self, dim: int, max_positions: int, base: float, device=None):
         super().__init__()
@@ -287,8 +293,9 @@ class Attention(nn.Module):
         int4 = all(isinstance(m, Int4Linear) for m in projs)
         ts = [t for m in projs for t in ((m.weight_packed, m.weight_scale) if int4 else
                                          (m.weight,))]
-        key = (int4,) + tuple((t.data_ptr(), t._version) for t in ts)
-        if getattr(self, "_qkv_key", None) == key:
+        changes = _changes(*ts)
+        key = (int4, changes) + tuple(t.data_ptr() for t in ts)
+        if changes is not None and getattr(self, "_qkv_key", None) == key:
             w = self._qkv_w
         else:
             if int4:
@@ -296,7 +303,7 @@ class Attention(nn.Module):
                 w = stacked_int4(projs)
             else:
                 w = torch.cat([m.weight.detach() for m in projs], 0)
-            if not _capturing(x2):
+            if changes is not None and not _capturing(x2):
                 self._qkv_w, self._qkv_key = w, key
         if int4:
             from ..kernels.int4_gemm import int4_linear
@@ -636,8 +643,9 @@ class MixtralDecoder(nn.Module):
         capture is the graph's alone (see Attention._qkv)."""
         from .paged import RotaryTable
         cos, sin = self.rotary.cos_cached, self.rotary.sin_cached
-        old, changes = getattr(self, "_rope", None), (cos._version, sin._version)
-        if old is not None and old[0] is cos and old[1] is sin and old[2] == changes:
+        old, changes = getattr(self, "_rope", None), _changes(cos, sin)
+        if old is not None and changes is not None and old[0] is cos and old[1] is sin \
+                and old[2] == changes:
             return old[3]
         half = cos.shape[1] // 2
         with torch.inference_mode(False):  # (the copies may be written again)

@@ -65,6 +65,21 @@ def test_angles_changed_after_a_capture():
     del junk
 
 
+@pytest.mark.parametrize("inside", [True, False])
+def test_weights_made_in_inference_mode(inside):
+    """Tensors that record no changes: nothing made of them is kept."""
+    want = _step(_model())()
+    with torch.inference_mode():
+        model = _model()
+    with torch.inference_mode(inside):
+        step = _step(model)
+        assert torch.equal(step(), want) and torch.equal(step(), want)
+    with torch.inference_mode():
+        model.rotary.cos_cached.neg_()
+        other = _step(model)()
+    assert not torch.equal(other, want)
+
+
 def test_a_model_used_inside_and_outside_of_inference_mode():
     model = _model()
     with torch.inference_mode():
