@@ -1175,13 +1175,22 @@ bool fits(long hd, long page) {
          (page & (page - 1)) == 0;
 }
 
+bool heads_fit(const hn_paged_step* s) {
+  return s->nkv > 0 && s->nh > 0 && s->nh % s->nkv == 0 && s->nh < 1 << 16;
+}
+
+// Whether the attention's launches hold the rows of a sequence.  (The heads fit.)
+bool rows_fit(const hn_paged_step* s) {
+  return s->max_new >= 1 && s->bound >= 1 && s->max_new <= (1l << 24) / s->nh &&
+         s->nh / s->nkv * s->max_new <= 65535l * kBlock;
+}
+
 // Checks a step, and fills what the kernels take of it.
 int check_step(const char* who, const hn_paged_step* s, const void* x, const void* k,
                const void* v, int dtype, Step& P) {
   HN_ARG_CHECK(s, "%s: null step", who);
   HN_ARG_CHECK(dtype == 0 || dtype == 1, "%s: dtype %d (0 fp16, 1 bf16)", who, dtype);
-  HN_ARG_CHECK(s->nkv > 0 && s->nh > 0 && s->nh % s->nkv == 0 && s->nh < 1 << 16,
-               "%s: %ld heads over %ld KV heads", who, s->nh, s->nkv);
+  HN_ARG_CHECK(heads_fit(s), "%s: %ld heads over %ld KV heads", who, s->nh, s->nkv);
   HN_ARG_CHECK(fits(s->hd, s->page), "%s: heads of 64, 128 or 256 (got %ld), pages of 16 to 1024 "
                "positions, a power of two (got %ld)", who, s->hd, s->page);
   HN_ARG_CHECK(s->B >= 0 && s->B < 65536 && s->T >= 0 && s->T < 1 << 30 && s->num_pages >= 0 &&
@@ -1341,8 +1350,9 @@ extern "C" int hn_paged_append(const hn_paged_step* step, const void* qkv, long 
 }
 
 extern "C" long hn_paged_attention_workspace_bytes(const hn_paged_step* s) {
-  if (!s || s->B <= 0 || s->T <= 0 || s->nkv <= 0 || s->nh < s->nkv || s->hd <= 0 ||
-      s->max_new <= 0)
+  // (0 too for what the call refuses)
+  if (!s || s->B <= 0 || s->B >= 65536 || s->T <= 0 || !heads_fit(s) || !fits(s->hd, s->page) ||
+      !rows_fit(s))
     return 0;
   return way_of(s->B, s->nh, s->nkv, s->hd, s->max_new, s->bound).bytes;
 }
@@ -1353,9 +1363,8 @@ extern "C" int hn_paged_attention(const hn_paged_step* step, const void* q, long
   Step P;
   if (int rc = check_step("hn_paged_attention", step, q, k, v, dtype, P)) return rc;
   const long nh = step->nh, nkv = step->nkv, hd = step->hd, max_new = step->max_new;
-  HN_ARG_CHECK(max_new >= 1 && step->bound >= 1 && max_new <= (1l << 24) / nh &&
-                   nh / nkv * max_new <= 65535l * kBlock,
-               "hn_paged_attention: max_new %ld, bound %ld", max_new, step->bound);
+  HN_ARG_CHECK(rows_fit(step), "hn_paged_attention: max_new %ld, bound %ld", max_new,
+               step->bound);
   HN_ARG_CHECK(P.cols < 1l << 26 && P.cols * P.page < 1l << 30 &&
                    (double)P.B * nkv * (P.cols * P.page / kGrain + 1) < 2147483648.0,
                "hn_paged_attention: %d sequences of %ld pages", P.B, P.cols);

@@ -577,7 +577,8 @@ int hn_paged_append(const hn_paged_step* step, const void* qkv, long ld_qkv, int
  *   signs: NaN).  scale above 0 and finite, also
  *   times log2(e); 16-byte aligned operands, ld_q and ld_o multiples of 8; cols *
  *   page < 2^30; out overlaps nothing that is read.  work:
- *   hn_paged_attention_workspace_bytes(step) bytes, 16-byte aligned, any contents. */
+ *   hn_paged_attention_workspace_bytes(step) bytes (0 for sizes that the call
+ *   refuses), 16-byte aligned, any contents. */
 long hn_paged_attention_workspace_bytes(const hn_paged_step* step);
 int hn_paged_attention(const hn_paged_step* step, const void* q, long ld_q, int dtype,
                        const void* k, const void* v, float scale, void* out, long ld_o,
