@@ -14,6 +14,7 @@ from .. import _lib
 
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
 _I64, _I32, _F32 = torch.int64, torch.int32, torch.float32
+_MOST = torch.finfo(torch.float32).max
 
 
 def _rows(x: torch.Tensor):
@@ -45,7 +46,7 @@ def adjust_logits(logits: torch.Tensor, text: Optional[torch.Tensor] = None,
     a token that is named twice, the last entry's; ids outside the vocabulary, such as
     -1, are padding); tokens whose bit of allowed int32 [B, ceil(V / 32)] (32 tokens to a
     word, the lowest bit first) is zero become -inf.  repetition (above 0), presence and
-    frequency: numbers, or fp32 [B].  out: logits itself, or another tensor of its
+    frequency: numbers that fp32 holds, or fp32 [B].  out: logits itself, or another tensor of its
     shape, type and device that does not overlap it; None: a new one."""
     dt, dev, at_dev = logits.dtype, logits.device, logits.get_device()
     assert logits.dim() == 2 and dt in _DTYPES and logits.shape[1] > 0, \
@@ -63,7 +64,7 @@ def adjust_logits(logits: torch.Tensor, text: Optional[torch.Tensor] = None,
     else:
         assert lens is None and prompt is None, "lens and prompt are of a text"
     rep, rep1 = _amount(repetition, "repetition", B, at_dev)
-    assert rep is not None or rep1 > 0.0, f"repetition {rep1}"
+    assert rep is not None or rep1 >= 2.0 ** -126, f"repetition {rep1}"
     pres, pres1 = _amount(presence, "presence", B, at_dev)
     freq, freq1 = _amount(frequency, "frequency", B, at_dev)
     ids, values = (None, None) if bias is None else bias
@@ -121,7 +122,7 @@ def _amount(x, name, B, at_dev):
             f"{name}: a number or fp32 [{B}] on the logits' device"
         return x.contiguous(), 0.0
     x = float(x)
-    assert math.isfinite(x), f"{name} {x}"
+    assert -_MOST <= x <= _MOST, f"{name} {x}: finite in fp32"
     return None, x
 
 
