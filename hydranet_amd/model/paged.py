@@ -448,7 +448,7 @@ class _Slots:
                 self._body()  # warm-up (allocator, library handles): no slot takes part
             torch.cuda.current_stream(dev).wait_stream(s)
             self.graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(self.graph):
+            with torch.cuda.device(dev), torch.cuda.graph(self.graph):  # (on the current device)
                 self._body()
 
     def draw(self, logits, text, lens, prompt, allowed, uniforms):
