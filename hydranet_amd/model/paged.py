@@ -108,9 +108,10 @@ class PagedKVCache:
         """The pages of a further sequence with the same first `length` positions: the
         full ones shared, the last one, which either may go on writing, copied."""
         full, rest = divmod(length, self.page_size)
-        assert 0 <= length and len(pages) >= full + (rest > 0), \
+        used = pages[:full + (rest > 0)]
+        assert 0 <= length and len(used) == full + (rest > 0), \
             f"{len(pages)} pages for {length} positions"
-        assert all(0 <= p < self.num_pages and self._users[p] > 0 for p in pages[:full + 1]), \
+        assert all(0 <= p < self.num_pages and self._users[p] > 0 for p in used), \
             "only pages that are taken can be shared"
         mine = self.take(1) if rest else []
         self.share(pages[:full])
