@@ -538,7 +538,9 @@ def generate(model, prompts, max_new_tokens: int, temperature: float = 0.0, samp
 
     def bits(text):
         w = allowed(text)
-        return every if w is None else torch.as_tensor(w, dtype=torch.int32).cpu()
+        w = every if w is None else torch.as_tensor(w, dtype=torch.int32).cpu()
+        assert tuple(w.shape) == (words,), f"allowed: {words} words (got {tuple(w.shape)})"
+        return w
 
     out: List[List[int]] = [[] for _ in range(B * samples)]
     texts = {}                    # slot -> (entry of out, prompt, pages)

@@ -92,6 +92,20 @@ def test_every_token_index(model, graph, samples, options):
         for i in range(n):
             _few(int(missed[s, i]), 24, f"sample {s}, token {i}")
 
+@pytest.mark.parametrize("shape", [(1,), (1, V // 32), (V // 32 + 1,)])
+@pytest.mark.parametrize("first", [True, False])
+def test_words_of_another_number_are_refused(model, shape, first):
+    """Of the first token and of a later one (where one word stood for all the others)."""
+    from hydranet_amd.model.paged import PagedKVCache
+    cache = PagedKVCache(2, 6, 2, 128, 16, DEV)
+    prompt = _prompts([9])[0]
+
+    def allowed(text):
+        return None if not first and text == prompt else torch.full(shape, -1, dtype=torch.int32)
+    with pytest.raises(AssertionError, match="allowed"):
+        model.generate_paged([prompt], 5, allowed=allowed, cache=cache)
+    assert cache.free_pages == 6
+
 
 @pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
 def test_a_model_on_another_device_than_the_current_one():
