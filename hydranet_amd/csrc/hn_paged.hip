@@ -21,6 +21,7 @@ template <>
 struct Vec<h16> {
   typedef half8_t t;
   static constexpr uint32_t inf = 0x7c00u;
+  static constexpr float less = 1.f;  // a second walk's probabilities, to a first's
   static __device__ __forceinline__ float4v mfma(t a, t b, float4v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
   }
@@ -29,6 +30,7 @@ template <>
 struct Vec<b16> {
   typedef bf8 t;
   static constexpr uint32_t inf = 0x7f80u;
+  static constexpr float less = 0x1p-40f;
   static __device__ __forceinline__ float4v mfma(t a, t b, float4v c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
   }
@@ -386,9 +388,14 @@ __device__ __forceinline__ int grains_below(const Attend<T>& A, int to) {
 // left (of either sign, or 0), also for the rows that do not see it.  So at positions that
 // only some rows see (past lo) they are taken out of the products and added to the rows
 // afterwards.  Among the positions that all rows see a first walk looks for none: its sums
-// tell whether there was one, and then a second walk takes them out everywhere (lo = -1).
-// The joins' weights are not 0 either (weight).  (The look at the sums costs 0.2 to 0.3 us of
-// a launch, 2 to 3 % of prompts by blocks.)
+// tell whether there was one (far), and then a second walk takes them out everywhere (lo =
+// -1).  The joins' weights are not 0 either (weight).  The look at the sums costs 0.2 to 0.3
+// us of a launch, 2 to 3 % of prompts by blocks.
+//
+// Values near bf16's largest: 2^14 times one is no number of fp32.  Their sums are found in the
+// same way, and the second walk's probabilities are 2^40 times smaller (Vec::less; a factor
+// behind the exponential, so that other rows' sums come out as they were; in bf16 3 % of
+// prompts by blocks).
 //
 // Of 8 positions from `at` on, the values that must not reach a product: those at positions
 // past hi, which no row sees (their probabilities are zero, but what lies there may be
@@ -437,15 +444,16 @@ __device__ __forceinline__ void add_odd(const Attend<T>& A, float4v (&o)[NT][HD 
   }
 }
 
-// NaN if one of a row's sums is no number (else 0).
+// Whether one of a row's sums is no number, or past about kFar, so that a join might overflow.
+constexpr float kFar = 0x1p100f;
 template <int N>
-__device__ __forceinline__ float probe(const float4v (&o)[N]) {
+__device__ __forceinline__ bool far(const float4v (&o)[N]) {
   float4v x = (float4v)(0.f);
 #pragma unroll
   for (int e = 0; e < N; ++e)
 #pragma unroll
-    for (int c = 0; c < 4; ++c) x[c] = __builtin_fmaf(o[e][c], 0.f, x[c]);
-  return (x[0] + x[1]) + (x[2] + x[3]);
+    for (int c = 0; c < 4; ++c) x[c] = __builtin_fmaf(o[e][c], 0x1p127f / kFar, x[c]);
+  return !(__builtin_fabsf((x[0] + x[1]) + (x[2] + x[3])) < __builtin_inff());
 }
 
 // The weight 2^x of sums in a join: above 0, so that an infinity stays one.  (2^-149 times any
@@ -464,6 +472,31 @@ struct Sums {
     l[t] = 0.f;
 #pragma unroll
     for (int e = 0; e < HD / 16; ++e) o[t][e] = (float4v)(0.f);
+  }
+  // The sums so far are `less` times what they are: a row's are brought back, or, where one
+  // is past kFar, they are what they are to a larger maximum.
+  __device__ __forceinline__ void end(float less) {
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      l[t] = row_sum(l[t]);
+      if (less == 1.f) continue;
+      const float up = 1.f / less, most = kFar * less;
+      float over = 0.f;
+#pragma unroll
+      for (int e = 0; e < HD / 16; ++e)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float x = __builtin_fabsf(o[t][e][c]);
+          if (x >= most && x < __builtin_inff()) over = 1.f;
+        }
+      if (row_max(over) > 0.f) {
+        mx[t] += __builtin_log2f(up);
+      } else {
+        l[t] *= up;
+#pragma unroll
+        for (int e = 0; e < HD / 16; ++e) o[t][e] *= up;
+      }
+    }
   }
 };
 
@@ -533,6 +566,7 @@ __device__ __forceinline__ void walk(const Attend<T>& A, Sums<T, HD, NT>& W, con
   for (bool apart = false;; apart = true) {
     asm volatile("" : "+s"(first), "+s"(g));  // (else what both walks begin with stays in registers)
     const int all = apart ? -1 : lo;
+    const float less = apart ? Vec<T>::less : 1.f;
     int odd_from = mine, odd_to = -1;  // the tiles that had some of those
     Ids id = ids(0), next = ids(1);
     keys(0, id.k);
@@ -581,7 +615,8 @@ __device__ __forceinline__ void walk(const Attend<T>& A, Sums<T, HD, NT>& W, con
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j][c], scale, -ref));
+            float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][j][c], scale, -ref));
+            if (Vec<T>::less != 1.f) x *= less;
             W.l[t] += x;
             p[t][4 * j + c] = (T)x;
             rest[t][4 * j + c] = (T)(x - (float)p[t][4 * j + c]);
@@ -603,8 +638,7 @@ __device__ __forceinline__ void walk(const Attend<T>& A, Sums<T, HD, NT>& W, con
     bool odd = false;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-      const float x = probe(W.o[t]);
-      odd |= row0 + 16 * t + n < A.rep * r.n && x != x;
+      odd |= row0 + 16 * t + n < A.rep * r.n && far(W.o[t]);
     }
     if (!apart && __any(odd)) {
 #pragma unroll
@@ -614,10 +648,9 @@ __device__ __forceinline__ void walk(const Attend<T>& A, Sums<T, HD, NT>& W, con
     for (int i = odd_from; i <= odd_to; ++i)
       add_odd<T, HD, NT>(A, W.o, lim, b, g, max(start(i), all + 1), min(start(i) + kTile - 1, hi),
                          kg);
+    W.end(less);
     break;
   }
-#pragma unroll
-  for (int t = 0; t < NT; ++t) W.l[t] = row_sum(W.l[t]);
 }
 
 // The waves' sums of 16 rows joined, then the rows themselves, or the range's entry of
@@ -807,6 +840,7 @@ __device__ __forceinline__ void block_range(const Attend<T>& A, const Run& r, in
   for (bool apart = false;; apart = true) {
     asm volatile("" : "+s"(from));  // (as in walk)
     const int all = apart ? -1 : lo;
+    const float less = apart ? Vec<T>::less : 1.f;
     int odd_from = to, odd_to = -1;  // the stages that had values which are no numbers
 #pragma unroll
     for (int t = 0; t < NT; ++t) W.start(t);
@@ -872,7 +906,8 @@ __device__ __forceinline__ void block_range(const Attend<T>& A, const Run& r, in
         for (int x = 0; x < SP / 16; ++x)
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][x][c], scale, -ref));
+            float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][x][c], scale, -ref));
+            if (Vec<T>::less != 1.f) y *= less;
             const int i = 4 * (x & 1) + c;
             W.l[t] += y;
             p[t][x >> 1][i] = (T)y;
@@ -906,8 +941,7 @@ __device__ __forceinline__ void block_range(const Attend<T>& A, const Run& r, in
       bool odd = false;
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const float x = probe(W.o[t]);
-        odd |= row0 + 16 * t + n < rows && x != x;
+        odd |= row0 + 16 * t + n < rows && far(W.o[t]);
       }
       if (__any(odd)) s_again = 1;
       __syncthreads();  // (also: the last stage is used, before the first of a second walk)
@@ -916,11 +950,10 @@ __device__ __forceinline__ void block_range(const Attend<T>& A, const Run& r, in
     if (busy)
       add_odd<T, HD, NT>(A, W.o, lim, b, g, max(odd_from * SP, all + 1),
                          min(odd_to * SP + SP - 1, hi), kg);
+    W.end(less);
     break;
   }
   if (!busy) return;
-#pragma unroll
-  for (int t = 0; t < NT; ++t) W.l[t] = row_sum(W.l[t]);
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     const int row = row0 + 16 * t + n, tok = row / A.rep, head = row - tok * A.rep;
