@@ -37,12 +37,13 @@ struct Vec<b16> {
 };
 
 // ---------------------------------------------------------------------------
-// The append.  Bytes are all there is: projections read, queries and pages written, 54 to 57
-// us for prompts of 9520 tokens, 32 heads over 8 of 128 (239 MB, 4.2 to 4.4 TB/s; a large copy
-// moves 5.1), 4.9 us for 64 single tokens, where the latency of lengths, tables and angles
+// The append.  Bytes are all there is: projections read, queries and pages written, 55 to 57
+// us for prompts of 8928 tokens, 32 heads over 8 of 128 (224 MB, 3.9 to 4.1 TB/s; a large copy
+// moves 5.2), 4.9 us for 64 single tokens, where the latency of lengths, tables and angles
 // after each other counts.
 //
-// One thread per element, grid (T, nh + 2 nkv): rows and rotated parts of any alignment.
+// One thread per element, grid (T, nh + 2 nkv): rows and rotated parts of any alignment (the
+// prompts 283 us, 64 single tokens 5.0).
 template <class T>
 __global__ __launch_bounds__(256) void append_kernel(Step P, const T* __restrict__ qkv, long ld,
                                                      const float* __restrict__ cos_t,
@@ -80,7 +81,7 @@ __global__ __launch_bounds__(256) void append_kernel(Step P, const T* __restrict
 }
 
 // 16 bytes; those of many rows past the caches, which keep the queries and pages instead
-// (prompts of 9520 tokens 57 -> 54 us).
+// (the prompts 57 -> 54 us).
 template <bool MANY, class T>
 __device__ __forceinline__ typename Vec<T>::t once(const T* p) {
   const auto* v = reinterpret_cast<const typename Vec<T>::t*>(p);
@@ -1190,7 +1191,8 @@ __global__ __launch_bounds__(256) void join_kernel(Attend<T> A) {
   for (int i = 0; i < 4; ++i) dst[i] = (T)(o[i] * is);
 }
 
-// Pages src[i] to dst[i] of every layer; the addresses and pairs go in the arguments.
+// Pages src[i] to dst[i] of every layer; the addresses and pairs go in the arguments.  (64
+// pages of 32 layers, 8 heads of 128 and 64 positions, 215 us, 5.0 TB/s; one page 11.6.)
 constexpr int kLayers = 64, kPairs = 64;
 struct Copies {
   void *k[kLayers], *v[kLayers];
@@ -1239,7 +1241,7 @@ int check_step(const char* who, const hn_paged_step* s, const void* x, const voi
 }
 
 // Rows from which a thread takes four heads of a token, so that it reads the angles once
-// (9520 rows 54 us, with one head a thread 77; 500 7.3 / 8.1, 100 5.2 / 5.2, 64 single tokens
+// (8928 rows 54 us, with one head a thread 77; 500 7.3 / 8.1, 100 5.2 / 5.2, 64 single tokens
 // 5.7 / 5.0).
 constexpr int kManyRows = 256;
 

@@ -200,7 +200,7 @@ class RotaryTable:
 
     @classmethod
     def wrap(cls, cos: torch.Tensor, sin: torch.Tensor, layout: str = "half") -> "RotaryTable":
-        """Over given tables [positions, dim / 2] fp32."""
+        """Over given tables [positions, dim / 2] fp32 (copies, if they are not contiguous)."""
         r = cls.__new__(cls)
         r._set(cos, sin, layout)
         return r
@@ -224,9 +224,10 @@ class PagedBatch:
     cached positions before the step, negative: it takes no part.  starts int32 [B + 1]
     (not decreasing, from 0): sequence b's new tokens are rows starts[b] to starts[b +
     1] - 1 of the step's `rows`, at most max_new each; None: one row each.  kv_bound: about
-    the most positions of a sequence (with the new ones), for the launches' sizes; the
-    results do not go by it.  The tensors are read when the kernels run,
-    so a captured step may be replayed after they were changed in place."""
+    the most positions of a sequence (with the new ones), for the launches' sizes, and so
+    the order in which sums are added; the results do not go by it otherwise.  The tensors
+    are read when the kernels run, so a captured step may be replayed after they were
+    changed in place."""
 
     def __init__(self, table: torch.Tensor, lens: torch.Tensor, kv_bound: int,
                  starts: Optional[torch.Tensor] = None, rows: Optional[int] = None,

@@ -544,7 +544,7 @@ int hn_kv_fork(void* const* kt, void* const* v, long layers, long max_len, long 
  * C_b on.  Rows of no sequence write no page and are zero in the outputs.
  * Sequences may share pages that neither writes.  nh query heads over nkv KV heads.
  * max_new: the most rows of a sequence; bound: about the most positions (C_b +
- * rows), which chooses the launch, not the result. */
+ * rows), which chooses the launch, and so the order of sums, nothing else. */
 typedef struct hn_paged_step {
   const int* table;
   long ld_table, cols, num_pages;
